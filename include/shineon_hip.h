@@ -27,6 +27,10 @@ extern "C" {
 #define SO_ERR_SHAPE (-2) /* unsupported shape combination */
 #define SO_NOT_APPLICABLE (-3) /* a specialised entry point declines this problem: nothing was launched, use the general one */
 
+/* element types of the token operators (everything else is fp32) */
+#define SO_F32 0
+#define SO_BF16 1
+
 /* activation codes (models/networks/cpvton/unet.py:132-135,201-211; models/networks/activation.py) */
 #define SO_ACT_NONE_ 0
 #define SO_ACT_RELU_ 1
@@ -506,6 +510,77 @@ int so_gan_loss_fwd(const float* x, int ldx, long long rows, int C, int mode, in
                     float* out, float* ws, void* stream);
 int so_gan_loss_bwd(const float* x, int ldx, long long rows, int C, int mode, int target_is_real, int for_discriminator,
                     const float* gout, float* dx, int lddx, void* stream);
+
+/* ---- token operators (csrc/dropout.hip, csrc/qkrope.hip) ----------------------------------------
+ * nn.Dropout of the U-Net blocks (models/networks/cpvton/unet.py, use_dropout) and of token blocks, and what an attention over
+ * tokens applies to its queries and keys.  Elements are SO_F32 or SO_BF16 (`dtype`), all arithmetic is fp32. */
+
+/* state = {seed, offset} (int64, device): out <- state, then offset += blocks.  One node per draw: a captured graph replays with
+ * new numbers. */
+int so_rng_draw(void* state, void* out, long long blocks, void* stream);
+
+/* y = residual + keep(e) * x * scale over rows x C elements (residual may be NULL), e = row * C + column;
+ * keep(e) = word (e % 4) of Philox4x32-10 with key rng[0] and counter rng[1] + e / 4 is >= threshold (= round(p * 2^32)).
+ * A dropped element is 0 whatever x holds.  The backward pass is the same call on dy. */
+int so_dropout(int dtype, const void* x, long long ldx, const void* residual, long long ldr, void* y, long long ldy, long long rows,
+               long long C, const void* rng, long long threshold, float scale, void* stream);
+
+/* Per-head RMS norm of q [B][L][Hq][D] and k [B][L][Hk][D] (strides in elements, channels contiguous, D even and <= 128; weights
+ * [D] fp32) followed by the rotation of the first R channels (pairs i, i + R/2) by row pos of the [P][R/2] tables; pos: int32 /
+ * int64 with strides, or NULL = start + token index.  A position outside the table gives NaN.  yq, yk: dense.
+ * _bwd: dy, dq, dk dense; dwq, dwk [D]; ws: so_qk_norm_rotary_ws_floats(D) floats. */
+int so_qk_norm_rotary_fwd(int dtype, const void* q, long long sqb, long long sql, long long sqh, int Hq, const void* k, long long skb,
+                          long long skl, long long skh, int Hk, const float* wq, const float* wk, const float* cosv,
+                          const float* sinv, long long P, const void* pos, int pos64, long long pos_sb, long long pos_sl,
+                          long long start, void* yq, void* yk, int B, int L, int D, int R, float eps, void* stream);
+long long so_qk_norm_rotary_ws_floats(int D);
+int so_qk_norm_rotary_bwd(int dtype, const void* q, long long sqb, long long sql, long long sqh, int Hq, const void* k, long long skb,
+                          long long skl, long long skh, int Hk, const float* wq, const float* wk, const float* cosv,
+                          const float* sinv, long long P, const void* pos, int pos64, long long pos_sb, long long pos_sl,
+                          long long start, const void* dyq, const void* dyk, void* dq, void* dk, float* dwq, float* dwk, int B, int L,
+                          int D, int R, float eps, float* ws, long long ws_floats, void* stream);
+
+/* ---- multi-head attention with a learned relative position bias (csrc/mha_fwd.hip, csrc/mha_bwd.hip) -----------------
+ * The form of models/networks/attention/sagan.py:29-54 with heads, a scale, a key mask and positions:
+ *   o[b][i][h] = sum_j softmax_j(scale q[b][i][h] . k[b][j][h / (Hq / Hk)] + table[lut[code[j] - code[q_start + i] + code_max]][h]) v[b][j][..]
+ * over the visible keys j; a row without any gives 0.  q [B][Lq][Hq][D], k / v [B][Lk][Hk][D] (strides in elements, channels
+ * contiguous, multiples of 16 bytes), o / dout / dq / dk / dv dense in the same order, D <= 128 and D * element size a multiple of 16.
+ * code: one non-decreasing int per token of a sequence (t) or map (y (2 W - 1) + x), padded with the last value to at least 128 past
+ * the next multiple of 128; linear = 1 where code[t] = t.  bias: so_mha_prep's expansion of the table, [Hq][V], readable 128 floats
+ * in front and behind.  words: so_mha_prep's mask bits [B][nwords], nwords = ceil(Lk / 64). */
+typedef struct so_mha_desc {
+  const void *q, *k, *v;
+  void* o;
+  void* o_lo;                  /* bf16, training: what o's rounding left of the result; NULL otherwise */
+  float* lse;                  /* training: [B][Hq][Lq], log2 of the softmax denominators (+inf: empty row); or NULL */
+  const float* bias;
+  const int* code;
+  const void* words;
+  float *part_o, *part_ml;     /* so_mha_parts > 1: B * Hq * Lq * parts * D and * 2 floats */
+  const void* dout;            /* backward */
+  void *dq, *dk, *dv;
+  float* delta;                /* backward: [B][Hq][Lq] scratch */
+  float* strips;               /* backward, gradient of the bias: so_mha_strip_floats */
+  long long sqb, sql, sqh, skb, skl, skh, svb, svl, svh;
+  int dtype, B, Hq, Hk, Lq, Lk, D, V, code_max, tokens, q_start, linear, nwords;
+  int two;                     /* bf16 forward: probabilities as a pair of bf16 products (the bias gradient needs o to fp32 accuracy) */
+  int width;                   /* tokens of a map row (a sequence: its length) */
+  float scale;
+} so_mha_desc;
+int so_mha_desc_bytes(void);
+
+/* bias[h * V + v] = table[lut[v]][h] / scale (finite entries kept within +-2^30 / log2(e)); words[b][w] = bits of the B x Lk mask bytes (row pitch
+ * mask_sb).  table or mask may be NULL. */
+int so_mha_prep(const float* table, const void* lut, int V, int H, float scale, float* bias, const void* mask, long long mask_sb, int B,
+                int Lk, void* words, void* stream);
+/* parts of the key axis that so_mha_fwd will use for this problem (>= 1), or an error */
+int so_mha_parts(const void* desc);
+int so_mha_fwd(const void* desc, void* stream);
+/* dq, dk, dv from dout; with strips also the per-block sums of the bias gradient over equal offsets, which so_mha_dtable adds up:
+ * dtable[r][h] = sum over offsets v of row r (order[start[r]] .. order[start[r + 1] - 1]).  dvec: Hq * V floats of scratch. */
+long long so_mha_strip_floats(const void* desc);
+int so_mha_bwd(const void* desc, void* stream);
+int so_mha_dtable(const void* desc, const void* order, const void* start, int rows, float* dvec, float* dtable, void* stream);
 
 #ifdef __cplusplus
 }

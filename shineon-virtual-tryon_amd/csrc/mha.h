@@ -1,0 +1,157 @@
+// Shared pieces of the multi-head attention kernels (mha_fwd.hip, mha_bwd.hip), gfx950.
+//
+// One 16-byte fragment per lane is the unit of all products: bf16 holds 8 values of it (one v_mfma_f32_32x32x16_bf16: lane (row l %
+// 32, half l / 32) supplies k = 8 half + e), fp32 holds 4 (four v_mfma_f32_32x32x2_f32: MFMA e takes k = 4 half + e).  Either way a
+// product step covers 32 bytes of the k axis and the byte addresses are the same for both types.
+//
+// A 32 x 32 accumulator holds, in lane (column l % 32, half), register r: row (r & 3) + 8 (r >> 2) + 4 half.  The kernels compute
+// scores TRANSPOSED against what they multiply them with next (rows = the axis that the next product sums over), so accumulator
+// registers 4 c .. 4 c + 3 (fp32) or 8 c .. 8 c + 7 (bf16) are already the B fragment of that product's step c, with
+//     k(step c, element e) = 8 c + 4 half + e (fp32)  or  16 c + (e & 3) + 8 (e >> 2) + 4 half (bf16);
+// the A fragment is read to match: single dwords (fp32) or two ds_read_b64_tr_b16 (bf16), which transpose on the way.
+#pragma once
+#include <hip/hip_runtime.h>
+#include "common.h"
+#include "../../include/shineon_hip.h"
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));   // four floats at any float's address
+
+namespace mha {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <typename T> struct Elem;
+template <> struct Elem<float> {
+  static constexpr int E = 4;          // elements of a 16-byte fragment
+  typedef f32x4 frag;
+};
+template <> struct Elem<__bf16> {
+  static constexpr int E = 8;
+  typedef bf16x8 frag;
+};
+
+__device__ __forceinline__ f32x16 mma(f32x4 a, f32x4 b, f32x16 acc) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], acc, 0, 0, 0);
+  return acc;
+}
+__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 acc) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0);
+}
+
+__device__ __forceinline__ int acc_row(int r, int half) { return (r & 3) + 8 * (r >> 2) + 4 * half; }
+
+template <int N> struct Log2 { static constexpr int v = 1 + Log2<N / 2>::v; };
+template <> struct Log2<1> { static constexpr int v = 0; };
+
+// A tile of rows in LDS: DP channels of T per row as 16-byte chunks, chunk c of row r at position c ^ f(r).  Rows are a power of two
+// chunks long; f spreads eight consecutive rows (the lanes of one ds_read_b128 phase) over all banks.
+template <typename T, int DP>
+struct Tile {
+  static constexpr int E = Elem<T>::E, NC = DP / E;                      // chunks that hold data
+  static constexpr int NP = NC <= 4 ? 4 : NC <= 8 ? 8 : NC <= 16 ? 16 : 32;   // chunks of a row in LDS
+  static constexpr int kRowBytes = NP * 16;
+  __device__ static __forceinline__ int swz(int row) { return NP == 4 ? (row >> 1) & 3 : row & 7; }
+  __device__ static __forceinline__ int at(int row, int chunk) { return row * kRowBytes + ((chunk ^ swz(row)) << 4); }
+
+  // A / B fragment "row, step m of the channel axis"
+  __device__ static __forceinline__ typename Elem<T>::frag row_frag(const char* t, int row, int m, int half) {
+    return *reinterpret_cast<const typename Elem<T>::frag*>(t + at(row, 2 * m + half));
+  }
+  // A fragment "column 32 t + lane, step c of the ROW axis" of the 32 rows from row0 (a multiple of 32)
+  __device__ static __forceinline__ typename Elem<T>::frag col_frag(const char* tile, int row0, int t, int c, int lane);
+};
+
+template <int DP>
+__device__ __forceinline__ f32x4 col_frag_f32(const char* tile, int row0, int t, int c, int lane) {
+  typedef Tile<float, DP> TL;
+  const int half = lane >> 5, col = 32 * t + (lane & 31);
+  f32x4 f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int row = row0 + 8 * c + 4 * half + e;
+    f[e] = *reinterpret_cast<const float*>(tile + TL::at(row, col >> 2) + 4 * (col & 3));
+  }
+  return f;
+}
+template <int DP>
+__device__ __forceinline__ bf16x8 col_frag_bf16(const char* tile, int row0, int t, int c, int lane) {
+  typedef Tile<__bf16, DP> TL;
+  const int half = lane >> 5, row = row0 + 16 * c + 4 * half + ((lane & 15) >> 2);
+  const int chunk = 4 * t + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), in = 8 * (lane & 1);
+  typedef __attribute__((address_space(3))) s16x4* lds_p;
+  union { s16x4 s[2]; bf16x8 f; } u;
+  u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(tile + TL::at(row, chunk) + in));
+  u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(tile + TL::at(row + 8, chunk) + in));
+  return u.f;
+}
+template <typename T, int DP> struct ColFrag;
+template <int DP> struct ColFrag<float, DP> {
+  __device__ static __forceinline__ f32x4 get(const char* t, int r0, int tt, int c, int lane) { return col_frag_f32<DP>(t, r0, tt, c, lane); }
+};
+template <int DP> struct ColFrag<__bf16, DP> {
+  __device__ static __forceinline__ bf16x8 get(const char* t, int r0, int tt, int c, int lane) { return col_frag_bf16<DP>(t, r0, tt, c, lane); }
+};
+
+// accumulator registers of step c as a B fragment; bf16 rounds here (half a step, 2^-8 of the value: the products run at the rate of
+// 16-bit operands; sums, statistics and accumulators stay fp32)
+__device__ __forceinline__ void to_frag(const f32x16& a, int c, f32x4& f) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f[e] = a[4 * c + e];
+}
+__device__ __forceinline__ void to_frag(const f32x16& a, int c, bf16x8& f) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = (__bf16)a[8 * c + e];
+}
+
+// 16-byte chunk of a row in global memory, zero when `on` is false (the address is then not formed)
+template <typename T>
+__device__ __forceinline__ f32x4 load_chunk(const T* row, int chunk, bool on) {
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  if (on) v = *reinterpret_cast<const f32x4*>(row + chunk * Elem<T>::E);
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ typename Elem<T>::frag as_frag(f32x4 v) {
+  union { f32x4 v; typename Elem<T>::frag f; } u;
+  u.v = v;
+  return u.f;
+}
+
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+
+// visible keys [64 w, 64 w + 64) of a sample as bits; keys behind the last are invisible
+__device__ __forceinline__ unsigned long long key_word(const unsigned long long* words, int w, int Lk) {
+  const int left = Lk - 64 * w;
+  unsigned long long m = left >= 64 ? ~0ULL : left <= 0 ? 0ULL : (1ULL << left) - 1;
+  return words ? m & words[w] : m;
+}
+
+// first and one-past-last word with a visible key (the whole wave calls it)
+__device__ __forceinline__ void word_range(const unsigned long long* words, int Lk, int lane, int& lo, int& hi) {
+  const int n = (Lk + 63) >> 6;
+  lo = 0;
+  hi = n;
+  if (!words) return;
+  lo = n;
+  hi = 0;
+  for (int w0 = 0; w0 < n; w0 += 64) {
+    const int w = w0 + lane;
+    const unsigned long long any = __ballot(w < n && words[w < n ? w : 0] != 0);
+    if (any) {
+      if (lo == n) lo = w0 + __builtin_ctzll(any);
+      hi = w0 + 64 - __builtin_clzll(any);
+    }
+  }
+}
+
+// 2^x for the softmax: v_exp_f32 (1 ulp); x <= 0 here up to rounding, results below 2^-126 vanish
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+}  // namespace mha
+
+int so_mha_check(const so_mha_desc* d);   // shape, type and alignment rules that all entry points share

@@ -1,0 +1,528 @@
+// Multi-head attention with a learned relative position bias, backward, gfx950.
+//
+//   P = exp2(c s - lse),  delta_i = sum_c do_ic o_ic,  dS = P (do v^T - delta),
+//   dq = scale dS k,  dk = scale dS^T q,  dv = P^T do,  dtable[r][h] = sum of dS_h over the pairs of bucket r
+//
+// Two passes over the score matrix, each rebuilding P from q, k and the saved row statistics, so that every sum has one owner and a
+// fixed order (no atomics on global memory): mha_dq_k owns query rows and walks the keys, mha_dkv_k owns keys and walks the query
+// rows of all heads that share them.  7 products instead of the 5 of a single pass whose dq would be added up by atomics.
+//
+// The bias gradient.  In mha_dq_k a lane holds one query and its registers hold keys, so dS for one register are 64 pairs: 32 different
+// offsets for each half of the wave.  Each half adds into a ring of its own in LDS (ds_add_f32; the 32 lanes hit 32 different words,
+// one wave's LDS operations stay in order, so the sum's order is fixed), indexed by offset modulo the ring.  As the walk moves on,
+// offsets that no later key can reach are summed over the eight rings and written to the block's strip; mha_dvec_k and mha_drow_k then
+// add strips over blocks and offsets over buckets.
+#include "mha.h"
+
+using namespace mha;
+
+namespace {
+
+struct BwdP {
+  so_mha_desc d;
+  float c;            // scale * log2 e
+  int ring, strip;    // floats of one LDS ring (a power of two) and of one block's strip
+  int stages, qtiles;
+};
+
+constexpr int BK = 64;          // keys (mha_dq_k) or query rows (mha_dkv_k) of a tile
+
+// most codes between the first and last of n consecutive tokens
+__host__ __device__ inline int code_span(int n, int width) {
+  return n < 2 ? 0 : (n - 1) + ((n - 2) / width + 1) * (width - 1);
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void mha_dq_k(const BwdP P) {
+  typedef Tile<T, DP> TL;
+  typedef typename Elem<T>::frag frag;
+  constexpr int E = Elem<T>::E, KM = 2 * E, NM = DP / KM, NT = DP / 32, NCS = 32 / KM;
+  constexpr int TILE = BK * TL::kRowBytes, CH = BK * TL::NC / 256;
+  static_assert(BK * TL::NC % 256 == 0, "staging");
+  extern __shared__ __attribute__((aligned(16))) char sm[];          // [stages][K tile | V tile] | [4 waves][2 halves][ring]
+  const so_mha_desc& D = P.d;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
+  const int bh = blockIdx.x, b = bh / D.Hq, head = bh - b * D.Hq, hk = head / (D.Hq / D.Hk);
+  const int q0 = blockIdx.y * 128, qlast = (q0 + 128 < D.Lq ? q0 + 128 : D.Lq) - 1;
+  const int row = q0 + 32 * wave + li;
+  const bool rowv = row < D.Lq;
+  const int qi = rowv ? row : qlast;
+
+  const unsigned long long* words = D.words ? (const unsigned long long*)D.words + (size_t)b * D.nwords : nullptr;
+  int t0, t1;
+  word_range(words, D.Lk, lane, t0, t1);
+
+  frag q[NM], go[NM];
+  float delta = 0.f;
+  {
+    const T* qr = (const T*)D.q + (size_t)b * D.sqb + (size_t)qi * D.sql + (size_t)head * D.sqh;
+    const size_t orow = (((size_t)b * D.Lq + qi) * D.Hq + head) * D.D;
+#pragma unroll
+    for (int m = 0; m < NM; ++m) {
+      const int ch = 2 * m + half;
+      const bool on = rowv && ch * E < D.D;
+      q[m] = as_frag<T>(load_chunk<T>(qr, ch, on));
+      go[m] = as_frag<T>(load_chunk<T>((const T*)D.dout + orow, ch, on));
+      const frag ov = as_frag<T>(load_chunk<T>((const T*)D.o + orow, ch, on));
+#pragma unroll
+      for (int e = 0; e < E; ++e) delta += (float)go[m][e] * (float)ov[e];
+      if (D.o_lo) {
+        const frag lv = as_frag<T>(load_chunk<T>((const T*)D.o_lo + orow, ch, on));
+#pragma unroll
+        for (int e = 0; e < E; ++e) delta += (float)go[m][e] * (float)lv[e];
+      }
+    }
+    delta += other_half(delta);
+  }
+  const size_t stat = ((size_t)b * D.Hq + head) * D.Lq + qi;
+  const float lse = rowv ? D.lse[stat] : INFINITY;
+  if (rowv && half == 0) D.delta[stat] = delta;
+  const int cq = D.bias ? D.code[D.q_start + qi] : 0;
+  const float* bias = D.bias ? D.bias + (size_t)head * D.V + D.code_max - cq : nullptr;
+
+  // bias gradient: rings cleared, strip filled with zeros up to the first offset that the walk can reach
+  const bool want = D.strips != nullptr;
+  float* rings = reinterpret_cast<float*>(sm + P.stages * 2 * TILE);
+  float* mine = rings + (2 * wave + half) * P.ring;
+  const int rmask = P.ring - 1;
+  const int cqf = D.bias ? D.code[D.q_start + q0] : 0, cql = D.bias ? D.code[D.q_start + qlast] : 0;
+  const int v0 = -cql;                                                 // code[0] = 0
+  float* strip = want ? D.strips + ((size_t)bh * P.qtiles + blockIdx.y) * P.strip : nullptr;
+  int flushed = v0;
+  if (want) {
+    for (int i = tid; i < 8 * P.ring; i += 256) rings[i] = 0.f;
+    const int first = t0 < t1 ? D.code[t0 * BK] - cql : v0;
+    for (int v = v0 + tid; v < first; v += 256) strip[v - v0] = 0.f;
+    flushed = first;
+  }
+  auto flush = [&](int upto) {
+    for (int v = flushed + tid; v < upto; v += 256) {
+      float x = 0.f;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        float* at = rings + r * P.ring + (v & rmask);
+        x += *at;
+        *at = 0.f;
+      }
+      strip[v - v0] = x;
+    }
+    flushed = upto;
+  };
+
+  f32x4 kreg[CH], vreg[CH];
+  const T* kb = (const T*)D.k + (size_t)b * D.skb + (size_t)hk * D.skh;
+  const T* vb = (const T*)D.v + (size_t)b * D.svb + (size_t)hk * D.svh;
+  auto fetch = [&](int t) {
+    const unsigned long long w = key_word(words, t, D.Lk);
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+      const int idx = tid + 256 * u, r = idx / TL::NC, ch = idx % TL::NC, key = t * BK + r;
+      const bool on = ((w >> r) & 1) && ch * E < D.D;
+      kreg[u] = load_chunk<T>(kb + (size_t)(on ? key : 0) * D.skl, ch, on);
+      vreg[u] = load_chunk<T>(vb + (size_t)(on ? key : 0) * D.svl, ch, on);
+    }
+  };
+  auto store = [&](int st) {
+    char* kt = sm + st * 2 * TILE;
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+      const int idx = tid + 256 * u, r = idx / TL::NC, ch = idx % TL::NC;
+      *reinterpret_cast<f32x4*>(kt + TL::at(r, ch)) = kreg[u];
+      *reinterpret_cast<f32x4*>(kt + TILE + TL::at(r, ch)) = vreg[u];
+    }
+  };
+
+  f32x16 dq[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dq[t][r] = 0.f;
+  if (t0 < t1) {
+    fetch(t0);
+    store(0);
+  }
+  __syncthreads();
+  for (int t = t0; t < t1; ++t) {
+    const int st = P.stages == 2 ? (t - t0) & 1 : 0;
+    const char* kt = sm + st * 2 * TILE;
+    const char* vt = kt + TILE;
+    if (t + 1 < t1) fetch(t + 1);
+    if (want && t > t0) flush(D.code[t * BK] - cql);      // offsets below this tile's: final, and no wave adds to them any more
+    const unsigned long long w64 = key_word(words, t, D.Lk);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int key0 = t * BK + 32 * u;
+      f32x16 s, dp;
+      if (bias) {
+        if (D.linear) {
+          const float* bp = bias + key0 + 4 * half;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const f32x4u v = *reinterpret_cast<const f32x4u*>(bp + 8 * g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * g + e] = v[e];
+          }
+        } else {
+          const int* cp = D.code + key0 + 4 * half;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const i32x4 v = *reinterpret_cast<const i32x4*>(cp + 8 * g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * g + e] = bias[v[e]];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dp[r] = 0.f;
+#pragma unroll
+      for (int k = 0; k < NM; ++k) s = mma(TL::row_frag(kt, 32 * u + li, k, half), q[k], s);
+#pragma unroll
+      for (int k = 0; k < NM; ++k) dp = mma(TL::row_frag(vt, 32 * u + li, k, half), go[k], dp);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = exp2_(__builtin_fmaf(s[r], P.c, -lse)) * (dp[r] - delta);      // dS
+      const unsigned w = (unsigned)(w64 >> (32 * u));
+      if (w != ~0u) {
+        const unsigned my = w >> (4 * half);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = (my >> acc_row(r, 0)) & 1 ? s[r] : 0.f;
+      }
+      if (want) {
+        if (D.linear) {
+          const int base = key0 + 4 * half - cq;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) atomicAdd(mine + ((base + acc_row(r, 0)) & rmask), s[r]);
+        } else {
+          const int* cp = D.code + key0 + 4 * half;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const i32x4 v = *reinterpret_cast<const i32x4*>(cp + 8 * g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) atomicAdd(mine + ((v[e] - cq) & rmask), s[4 * g + e]);
+          }
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < NCS; ++c) {
+        frag f;
+        to_frag(s, c, f);
+#pragma unroll
+        for (int v = 0; v < NT; ++v) dq[v] = mma(ColFrag<T, DP>::get(kt, 32 * u, v, c, lane), f, dq[v]);
+      }
+    }
+    if (P.stages == 1) __syncthreads();
+    if (t + 1 < t1) store(P.stages == 2 ? st ^ 1 : 0);
+    __syncthreads();
+  }
+  if (want) {
+    if (t0 < t1) {
+      const int kl = (t1 * BK < D.Lk ? t1 * BK : D.Lk) - 1;
+      flush(D.code[kl] - cqf + 1);
+    }
+    for (int v = flushed + tid; v < v0 + P.strip; v += 256) strip[v - v0] = 0.f;
+  }
+  if (!rowv) return;
+  T* out = (T*)D.dq + (((size_t)b * D.Lq + qi) * D.Hq + head) * D.D;
+#pragma unroll
+  for (int v = 0; v < NT; ++v)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = 32 * v + 8 * g + 4 * half;
+      if (c < D.D) {
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        t4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = (T)(dq[v][4 * g + e] * D.scale);
+        *reinterpret_cast<t4*>(out + c) = x;
+      }
+    }
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void mha_dkv_k(const BwdP P) {
+  typedef Tile<T, DP> TL;
+  typedef typename Elem<T>::frag frag;
+  constexpr int E = Elem<T>::E, KM = 2 * E, NM = DP / KM, NT = DP / 32, NCS = 32 / KM;
+  constexpr int TILE = BK * TL::kRowBytes, CH = BK * TL::NC / 256;
+  extern __shared__ __attribute__((aligned(16))) char sm[];          // [2][Q tile | dO tile | lse | delta]
+  constexpr int STAGE = 2 * TILE + 2 * BK * 4;
+  const so_mha_desc& D = P.d;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
+  const int bh = blockIdx.x, b = bh / D.Hk, hk = bh - b * D.Hk, G = D.Hq / D.Hk;
+  const int key = blockIdx.y * 128 + 32 * wave + li;
+  const unsigned long long* words = D.words ? (const unsigned long long*)D.words + (size_t)b * D.nwords : nullptr;
+  const int w0 = 2 * blockIdx.y;
+  const unsigned long long wa = key_word(words, w0, D.Lk), wb = w0 + 1 < D.nwords ? key_word(words, w0 + 1, D.Lk) : 0ULL;
+  const bool keyv = key < D.Lk, vis = ((wave < 2 ? wa : wb) >> (key & 63)) & 1;
+
+  frag k[NM], v[NM];
+  {
+    const T* kr = (const T*)D.k + (size_t)b * D.skb + (size_t)(keyv ? key : 0) * D.skl + (size_t)hk * D.skh;
+    const T* vr = (const T*)D.v + (size_t)b * D.svb + (size_t)(keyv ? key : 0) * D.svl + (size_t)hk * D.svh;
+#pragma unroll
+    for (int m = 0; m < NM; ++m) {
+      const int ch = 2 * m + half;
+      k[m] = as_frag<T>(load_chunk<T>(kr, ch, vis && ch * E < D.D));
+      v[m] = as_frag<T>(load_chunk<T>(vr, ch, vis && ch * E < D.D));
+    }
+  }
+  const float* bias0 = D.bias ? D.bias + D.code_max + D.code[keyv ? key : D.Lk - 1] : nullptr;
+
+  const int qt = (D.Lq + BK - 1) / BK, n = (wa | wb) ? G * qt : 0;    // a block without a visible key writes zeros
+  f32x4 qreg[CH], greg[CH];
+  float sreg = 0.f;
+  auto fetch = [&](int t) {
+    const int head = hk * G + t / qt, q0 = (t % qt) * BK;
+    const T* qb = (const T*)D.q + (size_t)b * D.sqb + (size_t)head * D.sqh;
+    const T* gb = (const T*)D.dout + ((size_t)b * D.Lq * D.Hq + head) * D.D;
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+      const int idx = tid + 256 * u, r = idx / TL::NC, ch = idx % TL::NC, i = q0 + r;
+      const bool on = i < D.Lq && ch * E < D.D;
+      qreg[u] = load_chunk<T>(qb + (size_t)(on ? i : 0) * D.sql, ch, on);
+      greg[u] = load_chunk<T>(gb + (size_t)(on ? i : 0) * D.Hq * D.D, ch, on);
+    }
+    if (tid < 2 * BK) {
+      const int i = q0 + (tid & (BK - 1));
+      const float* src = (tid < BK ? D.lse : D.delta) + ((size_t)b * D.Hq + head) * D.Lq;
+      sreg = i < D.Lq ? src[i] : tid < BK ? INFINITY : 0.f;
+    }
+  };
+  auto store = [&](int st) {
+    char* qtile = sm + st * STAGE;
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+      const int idx = tid + 256 * u, r = idx / TL::NC, ch = idx % TL::NC;
+      *reinterpret_cast<f32x4*>(qtile + TL::at(r, ch)) = qreg[u];
+      *reinterpret_cast<f32x4*>(qtile + TILE + TL::at(r, ch)) = greg[u];
+    }
+    if (tid < 2 * BK) reinterpret_cast<float*>(qtile + 2 * TILE)[tid] = sreg;
+  };
+
+  f32x16 dk[NT], dv[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dk[t][r] = dv[t][r] = 0.f;
+  if (n) {
+    fetch(0);
+    store(0);
+  }
+  __syncthreads();
+  for (int t = 0; t < n; ++t) {
+    const int st = P.stages == 2 ? t & 1 : 0;
+    const char* qtile = sm + st * STAGE;
+    const char* gtile = qtile + TILE;
+    const float* stats = reinterpret_cast<const float*>(qtile + 2 * TILE);
+    if (t + 1 < n) fetch(t + 1);
+    const int head = hk * G + t / qt, q0 = (t % qt) * BK;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      f32x16 s, dp;
+      if (bias0) {
+        const float* bias = bias0 + (size_t)head * D.V;
+        if (D.linear) {      // four consecutive rows are four floats downwards
+          const float* bp = bias - (D.q_start + q0 + 32 * u + 4 * half) - 3;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const f32x4u x = *reinterpret_cast<const f32x4u*>(bp - 8 * g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * g + e] = x[3 - e];
+          }
+        } else {
+          const int* cp = D.code + D.q_start + q0 + 32 * u + 4 * half;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = bias[-cp[acc_row(r, 0)]];
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dp[r] = 0.f;
+#pragma unroll
+      for (int m = 0; m < NM; ++m) s = mma(TL::row_frag(qtile, 32 * u + li, m, half), k[m], s);
+#pragma unroll
+      for (int m = 0; m < NM; ++m) dp = mma(TL::row_frag(gtile, 32 * u + li, m, half), v[m], dp);
+      const int rows_left = D.Lq - q0 - 32 * u;
+      if (rows_left < 32) {      // rows behind the last query: their bias was read from whatever lies in front of the expanded table
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = acc_row(r, half) < rows_left ? s[r] : -INFINITY;
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(stats + 32 * u + 8 * g + 4 * half);
+        const f32x4 de = *reinterpret_cast<const f32x4*>(stats + BK + 32 * u + 8 * g + 4 * half);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * g + e;
+          s[r] = vis ? exp2_(__builtin_fmaf(s[r], P.c, -ls[e])) : 0.f;
+          dp[r] = s[r] * (dp[r] - de[e]);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < NCS; ++c) {
+        frag f, g;
+        to_frag(s, c, f);
+        to_frag(dp, c, g);
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+          dv[x] = mma(ColFrag<T, DP>::get(gtile, 32 * u, x, c, lane), f, dv[x]);
+          dk[x] = mma(ColFrag<T, DP>::get(qtile, 32 * u, x, c, lane), g, dk[x]);
+        }
+      }
+    }
+    if (P.stages == 1) __syncthreads();
+    if (t + 1 < n) store(P.stages == 2 ? st ^ 1 : 0);
+    __syncthreads();
+  }
+  if (!keyv) return;
+  const size_t at = (((size_t)b * D.Lk + key) * D.Hk + hk) * D.D;
+#pragma unroll
+  for (int x = 0; x < NT; ++x)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = 32 * x + 8 * g + 4 * half;
+      if (c < D.D) {
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        t4 a, bb;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          a[e] = vis ? (T)(dk[x][4 * g + e] * D.scale) : (T)0.f;
+          bb[e] = vis ? (T)dv[x][4 * g + e] : (T)0.f;
+        }
+        *reinterpret_cast<t4*>((T*)D.dk + at + c) = a;
+        *reinterpret_cast<t4*>((T*)D.dv + at + c) = bb;
+      }
+    }
+}
+
+// dvec[h][code_max + v] = sum over samples and query blocks of their strips
+__global__ __launch_bounds__(256) void mha_dvec_k(const BwdP P, float* dvec) {
+  const so_mha_desc& D = P.d;
+  const int i = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
+  if (i >= D.V) return;
+  const int v = i - D.code_max;
+  float x = 0.f;
+  for (int t = 0; t < P.qtiles; ++t) {
+    const int ql = (128 * t + 128 < D.Lq ? 128 * t + 128 : D.Lq) - 1, at = v + D.code[D.q_start + ql];
+    if (at < 0 || at >= P.strip) continue;
+    for (int b = 0; b < D.B; ++b) x += D.strips[(((size_t)b * D.Hq + h) * P.qtiles + t) * P.strip + at];
+  }
+  dvec[(size_t)h * D.V + i] = x;
+}
+
+// dtable[r][h] = sum of dvec over the offsets of bucket r; one wave per entry
+__global__ __launch_bounds__(256) void mha_drow_k(const float* dvec, const int* order, const int* start, int rows, int H, int V,
+                                                  float* dtable) {
+  const int lane = threadIdx.x & 63, i = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= rows * H) return;
+  const int r = i / H, h = i - r * H;
+  float x = 0.f;
+  for (int j = start[r] + lane; j < start[r + 1]; j += 64) x += dvec[(size_t)h * V + order[j]];
+  x = so_wave_sum(x);
+  if (lane == 0) dtable[i] = x;
+}
+
+constexpr int kLds = 160 * 1024;
+
+int make(const so_mha_desc* d, BwdP& p) {
+  const int err = so_mha_check(d);
+  if (err) return err;
+  p = BwdP{};
+  p.d = *d;
+  p.c = d->scale * kLog2e;
+  p.qtiles = (d->Lq + 127) / 128;
+  p.stages = 2;
+  if (d->strips) {
+    if (!d->bias || d->width < 1) return SO_ERR_SHAPE;
+    const int w = d->linear ? 1 : d->width;
+    // the offsets that one tile of keys can reach from the block's rows, and those of the tile before still being written out
+    const int need = code_span(128, w) + code_span(BK, w) + code_span(BK + 1, w) + 1;
+    p.ring = 256;
+    while (p.ring < need) p.ring <<= 1;
+    if (p.ring > 2048) return SO_ERR_SHAPE;
+    const long long all = (long long)(d->linear ? d->Lk : (d->Lk - 1) / d->width * (2LL * d->width - 1) + d->width) + code_span(128, w) + 1;
+    p.strip = (int)all;
+  }
+  return 0;
+}
+
+template <typename K>
+int lds_limit(K k, size_t lds) {
+  if (lds <= 64 * 1024) return 0;
+  return (int)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+}
+
+template <typename T, int DP>
+int launch(BwdP p, hipStream_t st) {
+  typedef Tile<T, DP> TL;
+  constexpr size_t tile = (size_t)BK * TL::kRowBytes;
+  const size_t rings = p.d.strips ? (size_t)8 * p.ring * 4 : 0;
+  p.stages = 4 * tile + rings <= kLds ? 2 : 1;
+  size_t lds = p.stages * 2 * tile + rings;
+  if (lds > kLds) return SO_ERR_SHAPE;
+  int err = lds_limit(mha_dq_k<T, DP>, lds);
+  if (err) return err;
+  hipLaunchKernelGGL((mha_dq_k<T, DP>), dim3(p.d.B * p.d.Hq, p.qtiles), dim3(256), lds, st, p);
+  err = SO_LAUNCH_CHECK();
+  if (err) return err;
+  constexpr size_t stage = 2 * tile + 2 * BK * 4;
+  p.stages = 2 * stage <= kLds ? 2 : 1;
+  lds = p.stages * stage;
+  err = lds_limit(mha_dkv_k<T, DP>, lds);
+  if (err) return err;
+  hipLaunchKernelGGL((mha_dkv_k<T, DP>), dim3(p.d.B * p.d.Hk, (p.d.Lk + 127) / 128), dim3(256), lds, st, p);
+  return SO_LAUNCH_CHECK();
+}
+template <typename T>
+int launch_d(const BwdP& p, hipStream_t st) {
+  if (p.d.D <= 32) return launch<T, 32>(p, st);
+  if (p.d.D <= 64) return launch<T, 64>(p, st);
+  if (p.d.D <= 96) return launch<T, 96>(p, st);
+  return launch<T, 128>(p, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+long long so_mha_strip_floats(const void* desc) {
+  so_mha_desc d = *(const so_mha_desc*)desc;
+  float one;
+  d.strips = &one;       // only asked whether it is wanted
+  BwdP p;
+  const int err = make(&d, p);
+  return err ? err : (long long)d.B * d.Hq * p.qtiles * p.strip;
+}
+
+int so_mha_bwd(const void* desc, void* stream) {
+  const so_mha_desc* d = (const so_mha_desc*)desc;
+  BwdP p;
+  const int err = make(d, p);
+  if (err) return err;
+  if (!d->q || !d->k || !d->v || !d->o || !d->dout || !d->dq || !d->dk || !d->dv || !d->lse || !d->delta) return SO_ERR_SHAPE;
+  if ((((uintptr_t)d->dout) | ((uintptr_t)d->dq) | ((uintptr_t)d->dk) | ((uintptr_t)d->dv)) & 15) return SO_ERR_ALIGN;
+  if ((long long)d->B * d->Hq > 0x7fffffffLL || p.qtiles > 65535) return SO_ERR_SHAPE;
+  return d->dtype == SO_F32 ? launch_d<float>(p, (hipStream_t)stream) : launch_d<__bf16>(p, (hipStream_t)stream);
+}
+
+int so_mha_dtable(const void* desc, const void* order, const void* start, int rows, float* dvec, float* dtable, void* stream) {
+  const so_mha_desc* d = (const so_mha_desc*)desc;
+  BwdP p;
+  const int err = make(d, p);
+  if (err) return err;
+  if (!d->strips || !order || !start || rows < 1 || !dvec || !dtable || d->Hq > 65535 || (long long)rows * d->Hq > 0x7fffff00LL)
+    return SO_ERR_SHAPE;
+  hipStream_t st = (hipStream_t)stream;
+  hipLaunchKernelGGL(mha_dvec_k, dim3((d->V + 255) / 256, d->Hq), dim3(256), 0, st, p, dvec);
+  int e = SO_LAUNCH_CHECK();
+  if (e) return e;
+  hipLaunchKernelGGL(mha_drow_k, dim3((rows * d->Hq + 3) / 4), dim3(256), 0, st, dvec, (const int*)order, (const int*)start, rows, d->Hq,
+                     d->V, dtable);
+  return SO_LAUNCH_CHECK();
+}
+
+}  // extern "C"

@@ -1,0 +1,448 @@
+// Multi-head attention with a learned relative position bias, forward, gfx950.
+//
+//   o_i = sum_j softmax_j(scale q_i . k_j + bias_h[code_j - code_i]) v_j,   j over the visible keys; a row without any gives 0
+//
+// One pass over the keys per row of queries: running maximum m, running sum l and o unnormalised in registers (fp32), rescaled when m
+// moves.  The bias is the learned table expanded over offsets (so_mha_prep: one float per head and offset, divided by scale) and
+// ENTERS AS THE INITIAL ACCUMULATOR of the q k^T product, so adding it costs no vector instruction beyond its load: the scores in
+// log2 units are acc * (scale log2 e) in one multiply-add with -m.
+//
+// A block is four waves.  Query heads that share a key head are consecutive rows of one problem (row = head in group * Lq + i), so a
+// single token's heads fill one tile.
+//   SPLIT = false: 128 rows per block, 32 per wave; all waves walk the same 64-key tiles.
+//   SPLIT = true (rows of a key head <= 32): 32 rows per block; each wave takes 32 of the 128 keys of a tile and the four running
+//   softmaxes are merged through LDS at the end - with few rows the kernel is bound by reading keys and values, and this puts the
+//   four waves on different ones.
+// When there are too few blocks to fill the chip the keys are cut into gridDim.z parts, each leaves (o, m, l) in fp32 and
+// so_mha_join merges them.
+#include "mha.h"
+
+using namespace mha;
+
+namespace {
+
+struct FwdP {
+  so_mha_desc d;
+  int parts, tiles_per_part, tile_keys;
+  float c;              // scale * log2 e
+};
+
+template <typename T, int DP, bool SPLIT, bool TWO>   // TWO: the probabilities as hi + lo pair of bf16 products
+__global__ __launch_bounds__(256) void mha_fwd_k(const FwdP P) {
+  typedef Tile<T, DP> TL;
+  typedef typename Elem<T>::frag frag;
+  constexpr int E = Elem<T>::E, KM = 2 * E, NM = DP / KM, NT = DP / 32, NCS = 32 / KM;
+  constexpr int TK = SPLIT ? 128 : 64, SUBS = SPLIT ? 1 : 2;       // keys of a tile; 32-key pieces of it that one wave takes
+  constexpr int TILE = TK * TL::kRowBytes, STAGES = 4 * TILE <= 150 * 1024 ? 2 : 1;
+  constexpr int CH = TK * TL::NC / 256;                             // chunks each thread stages of K and of V
+  static_assert(TK * TL::NC % 256 == 0, "staging");
+  extern __shared__ __attribute__((aligned(16))) char sm[];         // [STAGES][K tile | V tile]
+  const so_mha_desc& D = P.d;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
+  const int bh = blockIdx.x, b = bh / D.Hk, hk = bh - b * D.Hk, G = D.Hq / D.Hk, part = blockIdx.z;
+  const int rows = G * D.Lq;
+  const int row = blockIdx.y * (SPLIT ? 32 : 128) + (SPLIT ? 0 : 32 * wave) + li;
+  const bool rowv = row < rows;
+  const int head = hk * G + (rowv ? row / D.Lq : 0), qi = rowv ? row % D.Lq : 0;
+
+  // keys of this part
+  const unsigned long long* words = D.words ? (const unsigned long long*)D.words + (size_t)b * D.nwords : nullptr;
+  int wlo, whi;
+  word_range(words, D.Lk, lane, wlo, whi);
+  constexpr int WPT = TK / 64;
+  int t0 = wlo / WPT, t1 = (whi + WPT - 1) / WPT;                   // visible tiles
+  if (P.parts > 1) {
+    const int n = t1 > t0 ? t1 - t0 : 0, per = (n + P.parts - 1) / P.parts;
+    t0 += part * per;
+    t1 = t0 + per < t1 ? t0 + per : t1;
+  }
+
+  frag q[NM];
+  {
+    const T* qr = (const T*)D.q + (size_t)b * D.sqb + (size_t)qi * D.sql + (size_t)head * D.sqh;
+#pragma unroll
+    for (int m = 0; m < NM; ++m) q[m] = as_frag<T>(load_chunk<T>(qr, 2 * m + half, rowv && (2 * m + half) * E < D.D));
+  }
+  const float* bias = nullptr;
+  if (D.bias) bias = D.bias + (size_t)head * D.V + D.code_max - D.code[D.q_start + qi];
+
+  f32x4 kreg[CH], vreg[CH];
+  const T* kb = (const T*)D.k + (size_t)b * D.skb + (size_t)hk * D.skh;
+  const T* vb = (const T*)D.v + (size_t)b * D.svb + (size_t)hk * D.svh;
+  auto fetch = [&](int t) {
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+      const int idx = tid + 256 * u, r = idx / TL::NC, ch = idx % TL::NC, key = t * TK + r;
+      const unsigned long long w = key_word(words, key >> 6 < D.nwords ? key >> 6 : 0, D.Lk);
+      const bool on = key < D.Lk && ((w >> (key & 63)) & 1) && ch * E < D.D;
+      kreg[u] = load_chunk<T>(kb + (size_t)(on ? key : 0) * D.skl, ch, on);
+      vreg[u] = load_chunk<T>(vb + (size_t)(on ? key : 0) * D.svl, ch, on);
+    }
+  };
+  auto store = [&](int st) {
+    char* kt = sm + st * 2 * TILE;
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+      const int idx = tid + 256 * u, r = idx / TL::NC, ch = idx % TL::NC;
+      *reinterpret_cast<f32x4*>(kt + TL::at(r, ch)) = kreg[u];
+      *reinterpret_cast<f32x4*>(kt + TILE + TL::at(r, ch)) = vreg[u];
+    }
+  };
+
+  f32x16 o[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
+  float m = -INFINITY, l = 0.f;
+
+  if (t0 < t1) {
+    fetch(t0);
+    store(0);
+  }
+  __syncthreads();
+  for (int t = t0; t < t1; ++t) {
+    const int st = STAGES == 2 ? (t - t0) & 1 : 0;
+    const char* kt = sm + st * 2 * TILE;
+    const char* vt = kt + TILE;
+    if (t + 1 < t1) fetch(t + 1);
+    // scores of this wave's keys
+    f32x16 s[SUBS];
+    float mx = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u) {
+      const int r0 = SPLIT ? 32 * wave : 32 * u, key0 = t * TK + r0;
+      if (bias) {
+        if (D.linear) {
+          const float* bp = bias + key0 + 4 * half;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const f32x4u v = *reinterpret_cast<const f32x4u*>(bp + 8 * g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[u][4 * g + e] = v[e];
+          }
+        } else {
+          const int* cp = D.code + key0 + 4 * half;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const i32x4 v = *reinterpret_cast<const i32x4*>(cp + 8 * g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[u][4 * g + e] = bias[v[e]];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < NM; ++k) s[u] = mma(TL::row_frag(kt, r0 + li, k, half), q[k], s[u]);
+      const unsigned long long w64 = key_word(words, key0 >> 6 < D.nwords ? key0 >> 6 : 0, D.Lk);
+      const unsigned w = key0 >= D.Lk ? 0u : (unsigned)(w64 >> (key0 & 32));
+      if (w != ~0u) {
+        const unsigned mine = w >> (4 * half);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[u][r] = (mine >> acc_row(r, 0)) & 1 ? s[u][r] : -INFINITY;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[u][r]);
+    }
+    mx = fmaxf(mx, other_half(mx)) * P.c;
+    const float mn = fmaxf(m, mx), ms = mn == -INFINITY ? 0.f : mn;
+    const float alpha = exp2_(m - ms);
+    m = mn;
+    float sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[u][r] = exp2_(__builtin_fmaf(s[u][r], P.c, -ms));
+        sum += s[u][r];
+      }
+    l = l * alpha + sum;
+    if (__any(alpha != 1.f)) {
+#pragma unroll
+      for (int v = 0; v < NT; ++v)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[v][r] *= alpha;
+    }
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u) {
+      const int r0 = SPLIT ? 32 * wave : 32 * u;
+#pragma unroll
+      for (int c = 0; c < NCS; ++c) {
+        frag p, lo;
+        to_frag(s[u], c, p);
+        if constexpr (TWO) {
+          f32x16 rest;
+#pragma unroll
+          for (int e = 0; e < E; ++e) rest[E * c + e] = s[u][E * c + e] - (float)p[e];
+          to_frag(rest, c, lo);
+        }
+#pragma unroll
+        for (int v = 0; v < NT; ++v) {
+          const frag a = ColFrag<T, DP>::get(vt, r0, v, c, lane);
+          o[v] = mma(a, p, o[v]);
+          if constexpr (TWO) o[v] = mma(a, lo, o[v]);
+        }
+      }
+    }
+    if (STAGES == 1) __syncthreads();
+    if (t + 1 < t1) store(STAGES == 2 ? st ^ 1 : 0);
+    __syncthreads();
+  }
+  l += other_half(l);
+
+  if constexpr (SPLIT) {
+    // merge the four waves' softmaxes: statistics first, then each wave adds its scaled rows in turn
+    float* st = reinterpret_cast<float*>(sm);                       // [4][32] m | [4][32] l | [32][DP + 1] o
+    if (half == 0) {
+      st[32 * wave + li] = m;
+      st[128 + 32 * wave + li] = l;
+    }
+    __syncthreads();
+    float mn = -INFINITY, ln = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mn = fmaxf(mn, st[32 * w + li]);
+    const float ms = mn == -INFINITY ? 0.f : mn;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) ln += st[128 + 32 * w + li] * exp2_(st[32 * w + li] - ms);
+    const float f = exp2_(m - ms);
+    float* os = st + 256;
+    for (int w = 0; w < 4; ++w) {
+      if (wave == w) {
+#pragma unroll
+        for (int v = 0; v < NT; ++v)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            float* at = os + li * (DP + 1) + 32 * v + acc_row(r, half);
+            const float x = o[v][r] * f;
+            *at = w == 0 ? x : *at + x;
+          }
+      }
+      __syncthreads();
+    }
+    if (wave != 0) return;
+    m = mn;
+    l = ln;
+#pragma unroll
+    for (int v = 0; v < NT; ++v)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[v][r] = os[li * (DP + 1) + 32 * v + acc_row(r, half)];
+  }
+  if (!rowv) return;
+  if (P.parts > 1) {      // unnormalised rows and statistics for so_mha_join: [b][Hk][rows][parts]
+    const size_t at = ((size_t)bh * rows + row) * P.parts + part;
+    if (half == 0) {
+      D.part_ml[2 * at] = m;
+      D.part_ml[2 * at + 1] = l;
+    }
+    float* po = D.part_o + at * D.D;
+#pragma unroll
+    for (int v = 0; v < NT; ++v)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int c = 32 * v + 8 * g + 4 * half;
+        if (c < D.D) *reinterpret_cast<f32x4*>(po + c) = f32x4{o[v][4 * g], o[v][4 * g + 1], o[v][4 * g + 2], o[v][4 * g + 3]};
+      }
+    return;
+  }
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;        // an empty row gives zeros, NaN stays NaN
+  const size_t orow = ((size_t)b * D.Lq + qi) * D.Hq + head;
+  T* op = (T*)D.o + orow * D.D;
+  T* lp = D.o_lo ? (T*)D.o_lo + orow * D.D : nullptr;
+#pragma unroll
+  for (int v = 0; v < NT; ++v)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = 32 * v + 8 * g + 4 * half;
+      if (c < D.D) {
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        t4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = o[v][4 * g + e] * inv;
+          hi[e] = (T)x;
+          lo[e] = (T)(x - (float)hi[e]);
+        }
+        *reinterpret_cast<t4*>(op + c) = hi;
+        if (lp) *reinterpret_cast<t4*>(lp + c) = lo;
+      }
+    }
+  if (D.lse && half == 0) D.lse[((size_t)b * D.Hq + head) * D.Lq + qi] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
+// joins the parts of a row: weights 2^(m_p - max m), fixed order.  One wave per row.
+template <typename T>
+__global__ __launch_bounds__(256) void mha_join_k(const FwdP P) {
+  const so_mha_desc& D = P.d;
+  const int G = D.Hq / D.Hk, rows = G * D.Lq, lane = threadIdx.x & 63;
+  const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= (long long)D.B * D.Hk * rows) return;
+  const int bh = (int)(at / rows), row = (int)(at - (long long)bh * rows), b = bh / D.Hk, hk = bh - b * D.Hk;
+  const float* ml = D.part_ml + 2 * at * P.parts;
+  float mn = -INFINITY, l = 0.f;
+  for (int p = 0; p < P.parts; ++p) mn = fmaxf(mn, ml[2 * p]);
+  const float ms = mn == -INFINITY ? 0.f : mn;
+  float x[2] = {0.f, 0.f};
+  for (int p = 0; p < P.parts; ++p) {
+    const float w = exp2_(ml[2 * p] - ms);
+    l += ml[2 * p + 1] * w;
+    const float* po = D.part_o + (at * P.parts + p) * D.D;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (lane + 64 * u < D.D) x[u] += po[lane + 64 * u] * w;
+  }
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+  const int head = hk * G + row / D.Lq, qi = row % D.Lq;
+  const size_t orow = ((size_t)b * D.Lq + qi) * D.Hq + head;
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    if (lane + 64 * u < D.D) {
+      const float v = x[u] * inv;
+      const T hi = (T)v;
+      ((T*)D.o)[orow * D.D + lane + 64 * u] = hi;
+      if (D.o_lo) ((T*)D.o_lo)[orow * D.D + lane + 64 * u] = (T)(v - (float)hi);
+    }
+  if (D.lse && lane == 0) D.lse[((size_t)b * D.Hq + head) * D.Lq + qi] = l == 0.f ? INFINITY : mn + __builtin_amdgcn_logf(l);
+}
+
+// bias[h][v] = table[lut[v]][h] / scale, finite values kept finite; words[b][w] = bits of the mask bytes
+struct PrepP {
+  const float* table;
+  const int* lut;
+  const unsigned char* mask;
+  float* bias;
+  unsigned long long* words;
+  long long mask_sb;
+  int V, H, B, Lk, nwords, bias_blocks;
+  float inv_scale, top;
+};
+__global__ __launch_bounds__(256) void mha_prep_k(const PrepP p) {
+  if ((int)blockIdx.x < p.bias_blocks) {
+    const int v = blockIdx.x * 256 + threadIdx.x;
+    if (v >= p.V) return;
+    const float* row = p.table + (size_t)p.lut[v] * p.H;
+    for (int h = blockIdx.y; h < p.H; h += gridDim.y) {
+      float x = row[h];
+      if (x > -INFINITY && x < INFINITY) x = fminf(fmaxf(x * p.inv_scale, -p.top), p.top);
+      p.bias[(size_t)h * p.V + v] = x;
+    }
+    return;
+  }
+  if (blockIdx.y) return;
+  const int lane = threadIdx.x & 63;
+  const long long i = (long long)(blockIdx.x - p.bias_blocks) * 4 + (threadIdx.x >> 6);
+  if (i >= (long long)p.B * p.nwords) return;
+  const int b = (int)(i / p.nwords), w = (int)(i - (long long)b * p.nwords), key = 64 * w + lane;
+  const unsigned long long bits = __ballot(key < p.Lk && p.mask[b * p.mask_sb + key] != 0);
+  if (lane == 0) p.words[i] = bits;
+}
+
+template <typename T, int DP, bool SPLIT, bool TWO>
+int launch(const FwdP& p, hipStream_t st) {
+  typedef Tile<T, DP> TL;
+  constexpr int TK = SPLIT ? 128 : 64, TILE = TK * TL::kRowBytes, STAGES = 4 * TILE <= 150 * 1024 ? 2 : 1;
+  constexpr int merge = (256 + 32 * (DP + 1)) * 4;
+  constexpr int lds = SPLIT && merge > STAGES * 2 * TILE ? merge : STAGES * 2 * TILE;
+  const int rows = p.d.Hq / p.d.Hk * p.d.Lq, per = SPLIT ? 32 : 128;
+  auto k = mha_fwd_k<T, DP, SPLIT, TWO>;
+  if (lds > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return (int)e;
+  }
+  hipLaunchKernelGGL(k, dim3(p.d.B * p.d.Hk, (rows + per - 1) / per, p.parts), dim3(256), lds, st, p);
+  return SO_LAUNCH_CHECK();
+}
+template <typename T, int DP>
+int launch_mode(const FwdP& p, bool split, hipStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (p.d.two) return split ? launch<T, DP, true, true>(p, st) : launch<T, DP, false, true>(p, st);
+  }
+  return split ? launch<T, DP, true, false>(p, st) : launch<T, DP, false, false>(p, st);
+}
+template <typename T>
+int launch_d(const FwdP& p, bool split, hipStream_t st) {
+  if (p.d.D <= 32) return launch_mode<T, 32>(p, split, st);
+  if (p.d.D <= 64) return launch_mode<T, 64>(p, split, st);
+  if (p.d.D <= 96) return launch_mode<T, 96>(p, split, st);
+  return launch_mode<T, 128>(p, split, st);
+}
+
+}  // namespace
+
+// shape, type and alignment rules that all entry points share
+int so_mha_check(const so_mha_desc* d) {
+  if (!d || (d->dtype != SO_F32 && d->dtype != SO_BF16)) return SO_ERR_SHAPE;
+  if (d->B < 1 || d->Hq < 1 || d->Hk < 1 || d->Hq % d->Hk || d->Lq < 1 || d->Lk < 1 || d->D < 1 || d->D > 128) return SO_ERR_SHAPE;
+  if ((long long)d->B * d->Hk > 0x7fffffffLL || (long long)(d->Hq / d->Hk) * d->Lq > 0x7fffff00LL || d->Lk > 0x7fffff00) return SO_ERR_SHAPE;
+  if (((long long)(d->Hq / d->Hk) * d->Lq + 127) / 128 > 65535 || ((long long)d->Lk + 127) / 128 > 65535) return SO_ERR_SHAPE;   // grid.y
+  if (!(d->scale > 0.f) || d->nwords != (d->Lk + 63) / 64) return SO_ERR_SHAPE;
+  const int E = d->dtype == SO_F32 ? 4 : 8;
+  if (d->D % E) return SO_ERR_ALIGN;
+  const long long s[] = {d->sqb, d->sql, d->sqh, d->skb, d->skl, d->skh, d->svb, d->svl, d->svh};
+  for (long long x : s)
+    if (x % E) return SO_ERR_ALIGN;
+  if ((((uintptr_t)d->q) | ((uintptr_t)d->k) | ((uintptr_t)d->v) | ((uintptr_t)d->o) | ((uintptr_t)d->o_lo)) & 15) return SO_ERR_ALIGN;
+  if (d->bias && (!d->code || (((uintptr_t)d->code) & 15) || d->V != 2 * d->code_max + 1 || d->q_start < 0)) return SO_ERR_SHAPE;
+  if (d->bias && (d->q_start + (long long)d->Lq > d->tokens || d->Lk > d->tokens)) return SO_ERR_SHAPE;
+  return 0;
+}
+
+extern "C" {
+
+int so_mha_desc_bytes(void) { return (int)sizeof(so_mha_desc); }
+
+int so_mha_prep(const float* table, const void* lut, int V, int H, float scale, float* bias, const void* mask, long long mask_sb, int B,
+                int Lk, void* words, void* stream) {
+  if ((table && (V < 1 || H < 1 || !lut || !bias)) || (mask && (B < 1 || Lk < 1 || !words)) || !(scale > 0.f)) return SO_ERR_SHAPE;
+  PrepP p = {};
+  p.table = table; p.lut = (const int*)lut; p.mask = (const unsigned char*)mask; p.bias = bias; p.words = (unsigned long long*)words;
+  p.mask_sb = mask_sb; p.V = V; p.H = H; p.B = B; p.Lk = Lk; p.nwords = (Lk + 63) / 64;
+  p.bias_blocks = table ? (V + 255) / 256 : 0;
+  p.inv_scale = 1.f / scale;
+  // Finite entries are kept within +-2^30 in the kernels' log2 units: exp2(fma(acc, c, -m)) sees the rounding of m = max(acc c), at most
+  // 2^-24 of it, as a common factor of a row - at 2^30 that is 2^64, still far from overflow.
+  p.top = 1073741824.f / (scale * kLog2e);
+  const long long mb = mask ? ((long long)B * p.nwords + 3) / 4 : 0;
+  if (p.bias_blocks + mb == 0) return 0;
+  if (p.bias_blocks + mb > 0x7fffffffLL) return SO_ERR_SHAPE;
+  hipLaunchKernelGGL(mha_prep_k, dim3((unsigned)(p.bias_blocks + mb), table ? (H < 16 ? H : 16) : 1), dim3(256), 0, (hipStream_t)stream, p);
+  return SO_LAUNCH_CHECK();
+}
+
+// parts of the key axis: enough blocks to give every CU two, at least two tiles of keys to a part
+int so_mha_parts(const void* desc) {
+  const so_mha_desc* d = (const so_mha_desc*)desc;
+  const int err = so_mha_check(d);
+  if (err) return err;
+  const int rows = d->Hq / d->Hk * d->Lq;
+  const bool split = rows <= 32;
+  const long long blocks = (long long)d->B * d->Hk * (split ? 1 : (rows + 127) / 128);
+  const int tiles = (d->Lk + (split ? 127 : 63)) / (split ? 128 : 64);
+  long long parts = (512 + blocks - 1) / blocks;
+  if (parts > tiles / 2) parts = tiles / 2;
+  return parts < 2 ? 1 : (int)(parts > 256 ? 256 : parts);
+}
+
+int so_mha_fwd(const void* desc, void* stream) {
+  const so_mha_desc* d = (const so_mha_desc*)desc;
+  const int parts = so_mha_parts(d);
+  if (parts < 0) return parts;
+  if (!d->q || !d->k || !d->v || !d->o || (parts > 1 && (!d->part_o || !d->part_ml || (((uintptr_t)d->part_o) & 15)))) return SO_ERR_SHAPE;
+  FwdP p = {};
+  p.d = *d;
+  p.parts = parts;
+  p.c = d->scale * kLog2e;
+  const int rows = d->Hq / d->Hk * d->Lq;
+  const bool split = rows <= 32;
+  hipStream_t st = (hipStream_t)stream;
+  int err = d->dtype == SO_F32 ? launch_d<float>(p, split, st) : launch_d<__bf16>(p, split, st);
+  if (err || parts == 1) return err;
+  const long long n = ((long long)d->B * d->Hk * rows + 3) / 4;
+  if (n > 0x7fffffffLL) return SO_ERR_SHAPE;
+  if (d->dtype == SO_F32) hipLaunchKernelGGL(mha_join_k<float>, dim3((unsigned)n), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL(mha_join_k<__bf16>, dim3((unsigned)n), dim3(256), 0, st, p);
+  return SO_LAUNCH_CHECK();
+}
+
+}  // extern "C"

@@ -1,0 +1,502 @@
+"""Autograd operators over tokens - what an attention layer with heads and positions is made of, beside the SAGAN core of ops.py:
+
+  dropout             mask from a counter-based generator, never stored              (csrc/dropout.hip)
+  qk_norm_rotary      per-head RMS norm of queries and keys + position rotation       (csrc/qkrope.hip)
+  attention           softmax attention with heads shared by groups, a key mask and a learned relative position bias by buckets
+                      (csrc/mha_fwd.hip, csrc/mha_bwd.hip)
+
+Same contract as ops.py: torch supplies device memory, the current stream and the autograd tape; the arithmetic is in
+libshineon_hip.so, there is no CPU fallback, everything may be captured into a hipGraph.  Two differences: operands may be float32 or
+bfloat16 (arithmetic and statistics are fp32 either way), and every call runs on the device of its operands, on that device's current
+stream, whatever the current device is."""
+import ctypes
+import math
+
+import torch
+
+from ._lib import check, lib
+from .ops import _require_cuda
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _dtype(*ts):
+    for t in ts:
+        _require_cuda(t)
+        if t.dtype not in _DTYPES:
+            raise TypeError(f"float32 or bfloat16 only (got {t.dtype})")
+        if t.dtype != ts[0].dtype:
+            raise TypeError(f"operands of one type only (got {ts[0].dtype} and {t.dtype})")
+        if t.device != ts[0].device:
+            raise ValueError(f"operands on one device only (got {ts[0].device} and {t.device})")
+    return _DTYPES[ts[0].dtype]
+
+
+def _fp32_param(t, shape, device, what):
+    if t.dtype != torch.float32:
+        raise TypeError(f"{what}: float32 only (got {t.dtype})")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{what}: expected on {device}, got {t.device}")
+    return t.detach().contiguous()
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+# ------------------------------------------------------------------------------------------------
+# dropout
+# ------------------------------------------------------------------------------------------------
+def rng_state(seed, device, offset=0):
+    """State of the counter-based generator: int64 {seed, offset} on the device."""
+    return torch.tensor([_int64(seed), _int64(offset)], dtype=torch.int64, device=device)
+
+
+def _int64(v):
+    v = int(v) & 0xFFFFFFFFFFFFFFFF
+    return v - (1 << 64) if v >> 63 else v
+
+
+def _check_rng(rng, device):
+    if rng.dtype != torch.int64 or rng.numel() != 2 or not rng.is_contiguous() or rng.device != device:
+        raise ValueError(f"the generator's state is two contiguous int64 values on {device} (rng_state)")
+
+
+def rng_draw(state, numel):
+    """{seed, offset} for one dropout over `numel` elements; the state moves on past the counters it uses (one per four elements).
+    Runs on the device, so a captured graph draws anew at every replay."""
+    _require_cuda(state)
+    _check_rng(state, state.device)
+    out = torch.empty_like(state)
+    with torch.cuda.device(state.device):
+        check(lib().so_rng_draw(state.data_ptr(), out.data_ptr(), (int(numel) + 3) // 4, _stream(state.device)), "rng_draw")
+    return out
+
+
+def _pitch_rows(t):
+    """(rows, C, pitch) of a tensor whose elements lie in counting order - channels innermost for a 4-D map - with at most a constant
+    gap behind each row; None when they do not."""
+    if t.dim() == 4:
+        t = t.permute(0, 2, 3, 1)
+    if t.is_contiguous():
+        return 1, t.numel(), t.numel()
+    c = t.shape[-1]
+    if t.dim() < 2 or (c > 1 and t.stride(-1) != 1):
+        return None
+    dims = [(s, st) for s, st in zip(t.shape[:-1], t.stride()[:-1]) if s > 1]
+    if not dims or dims[-1][1] < c or any(a[1] != b[0] * b[1] for a, b in zip(dims[:-1], dims[1:])):
+        return None
+    return t.numel() // c, c, dims[-1][1]
+
+
+def _like_rows(x):
+    """An empty dense tensor of x's shape, elements in counting order."""
+    if x.dim() == 4:
+        n, c, h, w = x.shape
+        return torch.empty((n, h, w, c), dtype=x.dtype, device=x.device).permute(0, 3, 1, 2)
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+def _in_order(t):
+    rows = _pitch_rows(t)
+    if rows is None:
+        t = _like_rows(t).copy_(t)
+        rows = _pitch_rows(t)
+    return t, rows
+
+
+def _dropout_launch(x, p, rng, residual):
+    dt = _dtype(x) if residual is None else _dtype(x, residual)
+    y = _like_rows(x)
+    if x.numel() == 0:
+        return y
+    x, (rows, c, ldx) = _in_order(x)
+    ldr = 0
+    if residual is not None:
+        residual, (rr, rc, ldr) = _in_order(residual)
+        if rr != rows:      # one of the two is dense, the other has a pitch: both as rows
+            c = c if rows > 1 else rc
+            rows = x.numel() // c
+            ldx, ldr = (ldx if ldx < x.numel() else c), (ldr if ldr < x.numel() else c)
+    with torch.cuda.device(x.device):
+        check(lib().so_dropout(dt, x.data_ptr(), ldx, None if residual is None else residual.data_ptr(), ldr, y.data_ptr(),
+                               c, rows, c, rng.data_ptr(), int(round(p * 2.0 ** 32)), 1.0 / (1.0 - p) if p < 1.0 else 0.0,
+                               _stream(x.device)), "dropout")
+    return y
+
+
+class _DropoutFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, rng):
+        ctx.p = p
+        ctx.save_for_backward(rng)
+        return _dropout_launch(x, p, rng, residual)
+
+    @staticmethod
+    def backward(ctx, dy):
+        (rng,) = ctx.saved_tensors
+        dx = _dropout_launch(dy, ctx.p, rng, None) if ctx.needs_input_grad[0] else None
+        return dx, dy if ctx.needs_input_grad[1] else None, None, None
+
+
+def dropout(x, p, rng, residual=None):
+    """residual + x * keep / (1 - p).  keep of element e (row-major; channels innermost for a 4-D map) is word e % 4 of Philox4x32-10
+    with key rng[0] at counter rng[1] + e / 4, compared with p; the mask is recomputed in the backward pass.  `rng`: one draw
+    (rng_draw), which must not be written to before the backward pass has run.  A dropped element counts as 0 whatever it holds;
+    p = 1 drops everything."""
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout probability outside [0, 1]: {p}")
+    _dtype(x)
+    _check_rng(rng, x.device)
+    if residual is not None:
+        _dtype(x, residual)
+        if residual.shape != x.shape:
+            raise ValueError(f"residual of shape {tuple(residual.shape)} for x of shape {tuple(x.shape)}")
+    return _DropoutFn.apply(x, residual, p, rng)
+
+
+# ------------------------------------------------------------------------------------------------
+# query / key norm + rotation
+# ------------------------------------------------------------------------------------------------
+def rotary_table(shape, rot_dim, base=10000.0, device="cuda"):
+    """(cos, sin), float32 [tokens, rot_dim / 2], angles computed in double.  shape: a length, or (H, W) for the tokens of a map in row
+    order - the first rot_dim // 4 pairs then turn with the row, the others with the column."""
+    if rot_dim < 0 or rot_dim % 2:
+        raise ValueError(f"rot_dim must be even (got {rot_dim})")
+    half = rot_dim // 2
+
+    def axis(n, pairs):
+        f = base ** (-torch.arange(pairs, dtype=torch.float64) / max(pairs, 1))
+        return torch.arange(n, dtype=torch.float64)[:, None] * f
+
+    if isinstance(shape, int):
+        angle = axis(shape, half)
+    else:
+        h, w = shape
+        ny = rot_dim // 4
+        y, x = axis(h, ny), axis(w, half - ny)
+        angle = torch.cat([y[:, None].expand(h, w, ny), x[None].expand(h, w, half - ny)], -1).reshape(h * w, half)
+    return angle.cos().float().to(device), angle.sin().float().to(device)
+
+
+def _heads(t, what):
+    """[B, L, H, D] with contiguous channels (copied otherwise)."""
+    if t.dim() != 4:
+        raise ValueError(f"{what}: expected [B, L, H, D], got {tuple(t.shape)}")
+    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
+
+
+class _QkNormRotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, cos, sin, positions, start, eps):
+        dt = _dtype(q, k)
+        q, k = _heads(q, "q"), _heads(k, "k")
+        b, n, hq, d = q.shape
+        yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        ctx.save_for_backward(q, k, wq, wk, cos, sin, positions)
+        ctx.cfg = (dt, start, eps)
+        if q.numel():
+            with torch.cuda.device(q.device):
+                check(lib().so_qk_norm_rotary_fwd(*_QkNormRotaryFn._common(dt, q, k, wq, wk, cos, sin, positions, start),
+                                                  yq.data_ptr(), yk.data_ptr(), b, n, d, 2 * cos.shape[1], eps, _stream(q.device)),
+                      "qk_norm_rotary_fwd")
+        return yq, yk
+
+    @staticmethod
+    def _common(dt, q, k, wq, wk, cos, sin, positions, start):
+        psb = psl = 0
+        if positions is not None:
+            psl = positions.stride(-1)
+            psb = positions.stride(0) if positions.dim() == 2 else 0
+        return (dt, q.data_ptr(), *q.stride()[:3], q.shape[2], k.data_ptr(), *k.stride()[:3], k.shape[2], wq.data_ptr(), wk.data_ptr(),
+                cos.data_ptr(), sin.data_ptr(), cos.shape[0], None if positions is None else positions.data_ptr(),
+                int(positions is not None and positions.dtype == torch.int64), psb, psl, start)
+
+    @staticmethod
+    def backward(ctx, dyq, dyk):
+        q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
+        dt, start, eps = ctx.cfg
+        b, n, hq, d = q.shape
+        dev = q.device
+        dyq, dyk = dyq.contiguous(), dyk.contiguous()
+        dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        dk = torch.empty(k.shape, dtype=k.dtype, device=dev)
+        if not q.numel():
+            return dq, dk, torch.zeros_like(wq), torch.zeros_like(wk), None, None, None, None, None
+        dwq, dwk = torch.empty_like(wq), torch.empty_like(wk)
+        L = lib()
+        ws = torch.empty(L.so_qk_norm_rotary_ws_floats(d), dtype=torch.float32, device=dev)
+        with torch.cuda.device(dev):
+            check(L.so_qk_norm_rotary_bwd(*_QkNormRotaryFn._common(dt, q, k, wq, wk, cos, sin, positions, start), dyq.data_ptr(),
+                                          dyk.data_ptr(), dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(), dwk.data_ptr(), b, n, d,
+                                          2 * cos.shape[1], eps, ws.data_ptr(), ws.numel(), _stream(dev)), "qk_norm_rotary_bwd")
+        return dq, dk, dwq, dwk, None, None, None, None, None
+
+
+def qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions=None, start=0, eps=1e-6):
+    """RMS norm over the channels of every head of q [B, L, Hq, D] and k [B, L, Hk, D] (weights [D], float32), then the rotation of
+    channel pairs (i, i + R/2) by the token's row of cos / sin [P, R/2] (rotary_table); channels R .. D - 1 are not rotated.
+    positions: int32 / int64, [L] or [B, L]; without it token l has position start + l.  q and k may be slices of one projection.  D
+    even, at most 128.  A position outside the table makes that token's outputs NaN (its position is only known on the device).
+    Returns dense (q', k')."""
+    _dtype(q, k)
+    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"q [B, L, Hq, D] and k [B, L, Hk, D] expected, got {tuple(q.shape)} and {tuple(k.shape)}")
+    b, n, _, d = q.shape
+    if d < 2 or d % 2 or d > 128 or q.shape[2] < 1 or k.shape[2] < 1:
+        raise ValueError(f"head size must be even and at most 128, at least one head each (got {tuple(q.shape)}, {tuple(k.shape)})")
+    if cos.dim() != 2 or 2 * cos.shape[1] > d:
+        raise ValueError(f"cos / sin of shape [P, R/2] with R <= {d} expected, got {tuple(cos.shape)}")
+    cos, sin = _fp32_param(cos, cos.shape, q.device, "cos"), _fp32_param(sin, cos.shape, q.device, "sin")
+    if positions is None:
+        if start < 0 or start + n > cos.shape[0]:
+            raise ValueError(f"positions {start} .. {start + n - 1} outside a table of {cos.shape[0]} rows")
+    else:
+        if start:
+            raise ValueError("positions and start exclude each other")
+        if positions.dtype not in (torch.int32, torch.int64) or positions.device != q.device:
+            raise TypeError(f"positions: int32 or int64 on {q.device}")
+        if tuple(positions.shape) not in ((n,), (b, n)):
+            raise ValueError(f"positions of shape ({n},) or ({b}, {n}) expected, got {tuple(positions.shape)}")
+    for t, what in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        _fp32_param(t, (d,), q.device, what)
+    return _QkNormRotaryFn.apply(q, k, q_weight.contiguous(), k_weight.contiguous(), cos, sin, positions, int(start), float(eps))
+
+
+# ------------------------------------------------------------------------------------------------
+# attention
+# ------------------------------------------------------------------------------------------------
+class _Desc(ctypes.Structure):
+    """so_mha_desc of include/shineon_hip.h."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "o", "o_lo", "lse", "bias", "code", "words", "part_o", "part_ml", "dout",
+                                                "dq", "dk", "dv", "delta", "strips")]
+                + [(n, ctypes.c_longlong) for n in ("sqb", "sql", "sqh", "skb", "skl", "skh", "svb", "svl", "svh")]
+                + [(n, ctypes.c_int) for n in ("dtype", "B", "Hq", "Hk", "Lq", "Lk", "D", "V", "code_max", "tokens", "q_start", "linear",
+                                               "nwords", "two", "width")]
+                + [("scale", ctypes.c_float)])
+
+
+def bucket_bounds(num_buckets, max_distance):
+    """Distances at which the buckets of one direction start: one bucket per distance below half of `num_buckets`, then logarithmically
+    spaced ones up to `max_distance`.  Step t of the m logarithmic ones starts at the first whole distance d with
+    d >= exact (max_distance / exact)^(t / m), decided in whole numbers."""
+    exact = num_buckets // 2
+    m = num_buckets - exact
+    bounds, d = list(range(1, exact + 1)), exact
+    for t in range(1, m):
+        while d ** m * exact ** t < exact ** m * max_distance ** t:
+            d += 1
+        bounds.append(d)
+    return bounds
+
+
+class RelativePositions:
+    """Which pairs of tokens share an entry of a learned bias table.
+
+    shape: a length, or (H, W) for the tokens of a map in row order.  Along one axis the signed distance key - query falls into one of
+    `num_buckets` buckets: with `bidirectional` half of them for keys behind the query and half for keys in front (key > query), else
+    all of them for keys at or before the query, keys after it counting as distance 0.  A map has num_buckets^2 buckets, row bucket *
+    num_buckets + column bucket.  `rows` is the number of table entries per head.  Built once per shape; immutable."""
+
+    def __init__(self, shape, num_buckets=32, max_distance=128, bidirectional=True, device="cuda"):
+        h, w = (1, int(shape)) if isinstance(shape, int) else (int(shape[0]), int(shape[1]))
+        if h < 1 or w < 1:
+            raise ValueError(f"empty shape {shape}")
+        half = num_buckets // 2 if bidirectional else num_buckets
+        if half < 2 or (bidirectional and num_buckets % 2):
+            raise ValueError(f"at least 2 buckets per direction, an even number for both directions (got {num_buckets})")
+        if max_distance <= half // 2:
+            raise ValueError(f"max_distance must exceed the {half // 2} distances that have buckets of their own (got {max_distance})")
+        if h > 1 and w > 512:
+            raise ValueError(f"map rows of at most 512 tokens (got {w})")
+        self.shape, self.tokens, self.width = (h, w), h * w, w
+        self.num_buckets, self.max_distance, self.bidirectional = num_buckets, max_distance, bidirectional
+        self.linear = int(h == 1)
+        self.code_max = (h - 1) * (2 * w - 1) + w - 1
+        if 2 * self.code_max + 1 > 1 << 28:
+            raise ValueError(f"shape {shape} has too many offsets")
+        bounds = torch.tensor(bucket_bounds(half, max_distance), dtype=torch.int64)
+
+        def axis(n):
+            d = torch.arange(-(n - 1), n)
+            if bidirectional:
+                return torch.bucketize(d.abs(), bounds, right=True) + half * (d > 0)
+            return torch.bucketize((-d).clamp(min=0), bounds, right=True)
+
+        lut = axis(w) if h == 1 else (axis(h)[:, None] * num_buckets + axis(w)[None, :]).reshape(-1)
+        self.rows = num_buckets if h == 1 else num_buckets * num_buckets
+        token = torch.arange(self.tokens)
+        code = token if h == 1 else (token // w) * (2 * w - 1) + token % w
+        pad = (self.tokens + 127) // 128 * 128 + 128 - self.tokens
+        code = torch.cat([code, code[-1:].expand(pad)])
+        order = torch.argsort(lut, stable=True)
+        start = torch.searchsorted(lut[order].contiguous(), torch.arange(self.rows + 1))
+        self.device = torch.empty(0, device=device).device
+        # a map's offset is (dy) (2 W - 1) + dx: every value of the range is one (dy, dx), so the lookup is dense
+        self.lut, self.code, self.order, self.start = (t.to(torch.int32).to(self.device) for t in (lut, code, order, start))
+
+
+def _rows16(t, what):
+    """[B, L, H, D] as the kernels read it: channels contiguous, everything else a multiple of 16 bytes - zero channels appended to D and
+    a dense copy made where it is not."""
+    t = _heads(t, what)
+    e = 16 // t.element_size()
+    d = t.shape[3]
+    if d % e:
+        t = torch.nn.functional.pad(t, (0, e - d % e))
+    if t.data_ptr() % 16 or any(s % e for s, n in zip(t.stride()[:3], t.shape[:3]) if n > 1):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _strides(t):
+    """Strides of the first three axes; an axis of one entry counts as stride 0."""
+    return [s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3])]
+
+
+class _AttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, mask, rel, q_start, scale, train):
+        d_true = q.shape[3]
+        q, k, v = _rows16(q, "q"), _rows16(k, "k"), _rows16(v, "v")
+        b, lq, hq, d = q.shape
+        lk, hk = k.shape[1], k.shape[2]
+        dev, L = q.device, lib()
+        o = torch.empty((b, lq, hq, d), dtype=q.dtype, device=dev)
+        ctx.dims = (d_true, q_start, scale)
+        ctx.rel = rel
+        if not q.numel() or not lk:
+            ctx.save_for_backward(q, k, v, table)
+            ctx.empty = True
+            return o.zero_()[..., :d_true]
+        ctx.empty = False
+        f = lambda *s: torch.empty(s, dtype=torch.float32, device=dev)  # noqa: E731
+        x = _Desc(dtype=_DTYPES[q.dtype], B=b, Hq=hq, Hk=hk, Lq=lq, Lk=lk, D=d, nwords=(lk + 63) // 64, scale=scale, q=q.data_ptr(),
+                  k=k.data_ptr(), v=v.data_ptr(), o=o.data_ptr())
+        (x.sqb, x.sql, x.sqh), (x.skb, x.skl, x.skh), (x.svb, x.svl, x.svh) = _strides(q), _strides(k), _strides(v)
+        words = bias = lse = o_lo = None
+        with torch.cuda.device(dev):
+            st = _stream(dev)
+            if mask is not None:
+                words = torch.empty((b, x.nwords), dtype=torch.int64, device=dev)
+                x.words = words.data_ptr()
+            if table is not None:
+                x.V, x.code_max, x.tokens, x.q_start, x.linear, x.width = (2 * rel.code_max + 1, rel.code_max, rel.tokens, q_start,
+                                                                           rel.linear, rel.width)
+                bias = f(hq * x.V + 256)      # readable on both sides: 128 floats
+                x.bias, x.code = bias.data_ptr() + 512, rel.code.data_ptr()
+            if table is not None or mask is not None:
+                check(L.so_mha_prep(None if table is None else table.data_ptr(), None if table is None else rel.lut.data_ptr(), x.V, hq,
+                                    scale, x.bias, None if mask is None else mask.data_ptr(), 0 if mask is None else mask.stride(0), b,
+                                    lk, x.words, st), "mha_prep")
+            if train:
+                lse = f(b, hq, lq)
+                x.lse = lse.data_ptr()
+                if q.dtype == torch.bfloat16:
+                    o_lo = torch.empty_like(o)
+                    x.o_lo = o_lo.data_ptr()
+                    x.two = int(table is not None and ctx.needs_input_grad[3])
+            parts = L.so_mha_parts(ctypes.addressof(x))
+            if parts < 0:
+                check(parts, "mha_parts")
+            if parts > 1:
+                po, pml = f(b * hq * lq * parts * d), f(b * hq * lq * parts * 2)
+                x.part_o, x.part_ml = po.data_ptr(), pml.data_ptr()
+            check(L.so_mha_fwd(ctypes.addressof(x), st), "mha_fwd")
+        if train:
+            ctx.save_for_backward(q, k, v, table, o, o_lo, lse, bias, words)
+        return o if d == d_true else o[..., :d_true].contiguous()
+
+    @staticmethod
+    def backward(ctx, dout):
+        d_true, q_start, scale = ctx.dims
+        if ctx.empty:
+            q, k, v, table = ctx.saved_tensors
+            return (*(torch.zeros_like(t[..., :d_true]) for t in (q, k, v)), None if table is None else torch.zeros_like(table), None,
+                    None, None, None, None)
+        q, k, v, table, o, o_lo, lse, bias, words = ctx.saved_tensors
+        rel = ctx.rel
+        b, lq, hq, d = q.shape
+        lk, hk = k.shape[1], k.shape[2]
+        dev, L = q.device, lib()
+        dout = dout if d == d_true else torch.nn.functional.pad(dout, (0, d - d_true))
+        dout = dout.contiguous()
+        if dout.data_ptr() % 16:
+            dout = dout.clone()
+        dq, dk, dv = torch.empty_like(o), torch.empty((b, lk, hk, d), dtype=k.dtype, device=dev), torch.empty((b, lk, hk, d), dtype=k.dtype, device=dev)
+        f = lambda *s: torch.empty(s, dtype=torch.float32, device=dev)  # noqa: E731
+        delta, dtable = f(b, hq, lq), None
+        x = _Desc(dtype=_DTYPES[q.dtype], B=b, Hq=hq, Hk=hk, Lq=lq, Lk=lk, D=d, nwords=(lk + 63) // 64, scale=scale, q=q.data_ptr(),
+                  k=k.data_ptr(), v=v.data_ptr(), o=o.data_ptr(), o_lo=None if o_lo is None else o_lo.data_ptr(), lse=lse.data_ptr(),
+                  words=None if words is None else words.data_ptr(), dout=dout.data_ptr(), dq=dq.data_ptr(), dk=dk.data_ptr(),
+                  dv=dv.data_ptr(), delta=delta.data_ptr())
+        (x.sqb, x.sql, x.sqh), (x.skb, x.skl, x.skh), (x.svb, x.svl, x.svh) = _strides(q), _strides(k), _strides(v)
+        if bias is not None:
+            x.V, x.code_max, x.tokens, x.q_start, x.linear, x.width = (2 * rel.code_max + 1, rel.code_max, rel.tokens, q_start, rel.linear,
+                                                                       rel.width)
+            x.bias, x.code = bias.data_ptr() + 512, rel.code.data_ptr()
+        with torch.cuda.device(dev):
+            st = _stream(dev)
+            if bias is not None and ctx.needs_input_grad[3]:
+                n = L.so_mha_strip_floats(ctypes.addressof(x))
+                if n < 0:
+                    check(int(n), "mha_strip_floats")
+                strips, dvec, dtable = f(n), f(hq * x.V), f(rel.rows, hq)
+                x.strips = strips.data_ptr()
+            check(L.so_mha_bwd(ctypes.addressof(x), st), "mha_bwd")
+            if dtable is not None:
+                check(L.so_mha_dtable(ctypes.addressof(x), rel.order.data_ptr(), rel.start.data_ptr(), rel.rows, dvec.data_ptr(),
+                                      dtable.data_ptr(), st), "mha_dtable")
+        if d != d_true:
+            dq, dk, dv = (t[..., :d_true] for t in (dq, dk, dv))
+        return dq, dk, dv, dtable, None, None, None, None, None
+
+
+def attention(q, k, v, scale=None, key_mask=None, relative=None, bias_table=None, q_start=0):
+    """softmax(scale q k^T + bias) v over the visible keys, per head.
+
+    q [B, Lq, Hq, D]; k, v [B, Lk, Hk, D]; Hq a multiple of Hk (query heads h * Hq / Hk .. share key head h); float32 or bfloat16,
+    D <= 128.  Any strides: operands whose rows do not start at multiples of 16 bytes, or whose channels are not contiguous, are copied
+    first.  scale: default D^-1/2, must be positive.
+
+    key_mask: bool [B, Lk], True = visible.  Hidden keys and values may hold anything (inf and NaN included) and get zero gradients; a
+    sample without visible keys gives zeros.
+
+    relative + bias_table: a RelativePositions plan and its learned table [plan.rows, Hq] (float32).  Key j against query i adds the
+    entry of the bucket of token j against token q_start + i.  An entry may be -inf; finite ones beyond +-7.4e8 count as that.
+
+    One or a few queries over long keys (a new token against what came before) are split over the keys.  Returns [B, Lq, Hq, D];
+    differentiable in q, k, v and bias_table.  The order of all sums is fixed: the same inputs give the same bits."""
+    _dtype(q, k, v)
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"q [B, Lq, Hq, D], k and v [B, Lk, Hk, D] expected, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    b, lq, hq, d = q.shape
+    lk, hk = k.shape[1], k.shape[2]
+    if hk < 1 or hq < 1 or hq % hk:
+        raise ValueError(f"{hq} query heads cannot share {hk} key heads evenly")
+    if d < 1 or d > 128:
+        raise ValueError(f"head size 1 .. 128 (got {d})")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not (0.0 < scale < math.inf):
+        raise ValueError(f"scale must be positive and finite (got {scale})")
+    if key_mask is not None:
+        if key_mask.dtype != torch.bool or tuple(key_mask.shape) != (b, lk) or key_mask.device != q.device:
+            raise ValueError(f"key_mask: bool of shape ({b}, {lk}) on {q.device} expected, got {key_mask.dtype} {tuple(key_mask.shape)}")
+        key_mask = key_mask if lk <= 1 or key_mask.stride(1) == 1 else key_mask.contiguous()
+    if (relative is None) != (bias_table is None):
+        raise ValueError("relative and bias_table belong together")
+    if relative is not None:
+        if relative.device != q.device:
+            raise ValueError(f"the plan is on {relative.device}, q on {q.device}")
+        if q_start < 0 or q_start + lq > relative.tokens or lk > relative.tokens:
+            raise ValueError(f"queries {q_start} .. {q_start + lq - 1} and {lk} keys do not fit a plan of {relative.tokens} tokens")
+        _fp32_param(bias_table, (relative.rows, hq), q.device, "bias_table")
+        bias_table = bias_table.contiguous()
+    elif q_start:
+        raise ValueError("q_start without relative positions")
+    train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias_table))
+    return _AttentionFn.apply(q, k, v, bias_table, key_mask, relative, int(q_start), scale, train)

@@ -1,0 +1,96 @@
+"""Token operators, host side: the generator's published vectors, bucket plans, rotation tables, refusals before any launch."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import tokens_ref as ref
+from shineon_virtual_tryon_amd import _lib, ops_tokens as tok
+
+
+def test_oracle_generator_known_answers():
+    """The published Philox4x32-10 vectors (zeros, ones, digits of pi)."""
+    f = 0xFFFFFFFF
+    cases = [([0] * 4, [0] * 2, "6627e8d5 e169c58d bc57ac4c 9b00dbd8"), ([f] * 4, [f] * 2, "408f276d 41c83b0e a20bc7c6 6d5451fd"),
+             ([0x243f6a88, 0x85a308d3, 0x13198a2e, 0x03707344], [0xa4093822, 0x299f31d0], "d16cfe09 94fdcceb 5001e420 24126ea1")]
+    for ctr, key, want in cases:
+        got = ref.philox4x32_full([np.array([c], np.uint64) for c in ctr], key)[0]
+        assert " ".join("%08x" % int(w) for w in got) == want
+
+
+@pytest.mark.parametrize("both", [True, False])
+@pytest.mark.parametrize("num,far", [(4, 3), (8, 20), (32, 128), (16, 32), (6, 100), (10, 7)])
+@pytest.mark.parametrize("shape", [1, 2, 300, (3, 5), (1, 9), (9, 1), (20, 40)], ids=str)
+def test_plan_buckets(shape, num, far, both):
+    p = tok.RelativePositions(shape, num, far, both, device="cpu")
+    n = p.tokens
+    code = p.code[:n].long()
+    got = p.lut.long()[code[None] - code[:, None] + p.code_max]
+    assert torch.equal(got, ref.pair_buckets(shape, n, n, 0, num, far, both))
+    assert (p.code[n:] == p.code[n - 1]).all() and len(p.code) >= (n + 127) // 128 * 128 + 128
+    for r in range(p.rows):
+        assert (p.lut[p.order[p.start[r]:p.start[r + 1]].long()] == r).all()
+    assert int(p.start[-1]) == len(p.lut) == 2 * p.code_max + 1
+
+
+def test_plan_refusals():
+    for kw in (dict(shape=0), dict(shape=(3, 0)), dict(shape=5, num_buckets=3), dict(shape=5, num_buckets=2), dict(shape=5, num_buckets=32, max_distance=8),
+               dict(shape=(2, 513)), dict(shape=1 << 29)):
+        with pytest.raises(ValueError):
+            tok.RelativePositions(device="cpu", **kw)
+    with pytest.raises(ValueError):
+        tok.rotary_table(4, 3, device="cpu")
+
+
+def test_rotary_table_angles():
+    cos, sin = tok.rotary_table(70000, 8, device="cpu")
+    a = 69999 * 10000.0 ** (-2 / 8)
+    assert abs(cos[69999, 1].item() - np.cos(a)) <= 2.0 ** -24 and abs(sin[69999, 1].item() - np.sin(a)) <= 2.0 ** -24
+    cos, sin = tok.rotary_table((3, 4), 8, device="cpu")
+    assert cos.shape == (12, 4)
+    assert torch.equal(cos[4:8, :2], cos[4:5, :2].expand(4, 2)) and torch.equal(cos[1::4, 2:], cos[1:2, 2:].expand(3, 2))
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(1, 2, 1, 8)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        tok.dropout(x, 0.5, tok.rng_state(1, "cpu"))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        tok.rng_draw(tok.rng_state(1, "cpu"), 4)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        tok.qk_norm_rotary(x, x, torch.ones(8), torch.ones(8), *tok.rotary_table(2, 8, device="cpu"))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        tok.attention(x, x, x)
+
+
+def _desc(**kw):
+    base = dict(q=256, k=256, v=256, o=256, dtype=0, B=1, Hq=4, Hk=2, Lq=8, Lk=8, D=64, nwords=1, scale=0.125, sqb=2048, sql=256, sqh=64, skb=1024,
+                skl=128, skh=64, svb=1024, svl=128, svh=64)
+    return tok._Desc(**{**base, **kw})
+
+
+def test_c_entry_points_refuse_before_launching():
+    """Wrong descriptors come back as error codes from the host side of the C ABI."""
+    L = _lib.lib()
+    assert L.so_mha_desc_bytes() == ctypes.sizeof(tok._Desc)
+    assert L.so_mha_parts(ctypes.addressof(_desc())) >= 1
+    shape, align = -2, -1
+    for kw, want in ((dict(dtype=2), shape), (dict(Hq=3), shape), (dict(D=132), shape), (dict(D=0), shape), (dict(Lk=0), shape), (dict(scale=0.0), shape),
+                     (dict(scale=float("nan")), shape), (dict(nwords=2), shape), (dict(D=62), align), (dict(sql=254), align), (dict(q=260), align),
+                     (dict(dtype=1, D=60), align), (dict(bias=256, code=None, V=15, code_max=7, tokens=8), shape),
+                     (dict(bias=256, code=256, V=15, code_max=7, tokens=8, q_start=1), shape), (dict(bias=256, code=256, V=14, code_max=7, tokens=8), shape),
+                     (dict(q=None), shape)):
+        assert L.so_mha_fwd(ctypes.addressof(_desc(**kw)), None) == want, kw
+    assert L.so_mha_bwd(ctypes.addressof(_desc()), None) == shape          # no dout
+    assert L.so_mha_strip_floats(ctypes.addressof(_desc())) == shape       # no bias
+    assert L.so_mha_prep(None, None, 0, 0, 0.0, None, None, 0, 0, 0, None, None) == shape
+    assert L.so_dropout(2, None, 4, None, 0, None, 4, 1, 4, None, 0, 1.0, None) == shape
+    assert L.so_dropout(0, None, 3, None, 0, None, 4, 1, 4, None, 0, 1.0, None) == shape
+    assert L.so_dropout(0, None, 4, None, 0, None, 4, 1, 4, None, 2 ** 32 + 1, 1.0, None) == shape
+    assert L.so_dropout(0, None, 4, None, 0, None, 4, 0, 4, None, 0, 1.0, None) == 0
+    assert L.so_rng_draw(None, None, 1, None) == shape
+    qk = (0, 256, 64, 64, 64, 1, 256, 64, 64, 64, 1, 256, 256, 256, 256)
+    assert L.so_qk_norm_rotary_fwd(*qk, 4, None, 0, 0, 0, 0, 256, 256, 1, 5, 64, 64, 1e-6, None) == shape      # five tokens, four rows of angles
+    assert L.so_qk_norm_rotary_fwd(*qk, 8, None, 0, 0, 0, 0, 256, 256, 1, 5, 63, 62, 1e-6, None) == shape
+    assert L.so_qk_norm_rotary_bwd(*qk, 8, None, 0, 0, 0, 0, 256, 256, 256, 256, 256, 256, 1, 5, 64, 64, 1e-6, 256, 10, None) == shape

@@ -1,0 +1,542 @@
+"""Token operators (ops_tokens: dropout, qk_norm_rotary, attention) on the GPU against plain 64-bit forms.  Every tolerance is a bound
+computed from the operands (tokens_ref): half a step of the type for each rounding the kernels make."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import tokens_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+TYPES = pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+
+
+@pytest.fixture(scope="module")
+def tok():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    from shineon_virtual_tryon_amd import ops_tokens
+
+    return ops_tokens
+
+
+def normal(seed, *shape, dtype=F32, std=1.0):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * std).to(dtype).cuda()
+
+
+def d64(t):
+    return t.detach().double().cpu()
+
+
+# ------------------------------------------------------------------------------------------------------------------- dropout
+@TYPES
+@pytest.mark.parametrize("shape", [(1,), (3,), (8,), (2047,), (5, 1023), (2, 3, 129), (2, 7, 5, 3), (2, 64, 16, 12), (3, 1, 1, 2)], ids=str)
+@pytest.mark.parametrize("p,seed,offset", [(0.1, 12345, 0), (0.5, -1, 2 ** 32 - 3), (0.73, 2 ** 63 + 11, 2 ** 64 - 2)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_dropout_matches_the_generator(tok, dtype, shape, p, seed, offset, residual):
+    x = normal(1, *shape, dtype=dtype)
+    if x.dim() == 4:
+        x = x.contiguous(memory_format=torch.channels_last)
+    x.requires_grad_()
+    r = normal(2, *shape, dtype=dtype).requires_grad_() if residual else None
+    y = tok.dropout(x, p, tok.rng_state(seed, "cuda", offset), residual=r)
+    keep = ref.keep_mask(shape, p, seed & (2 ** 64 - 1), offset)
+    u = ref.HALF_STEP[dtype]
+
+    def expect(v, res):
+        a = torch.where(keep, v / (1 - p), 0.0)
+        want = a + (res if res is not None else 0.0)
+        return want, 3 * ref.U32 * a.abs() + (u + ref.U32) * want.abs()
+
+    ref.check(y, *expect(d64(x), d64(r) if residual else None), "y")
+    dy = normal(3, *shape, dtype=dtype)
+    grads = torch.autograd.grad(y, [x] + ([r] if residual else []), dy)
+    ref.check(grads[0], *expect(d64(dy), None), "dx")
+    if residual:
+        assert torch.equal(grads[1], dy)
+
+
+@TYPES
+def test_dropout_reads_slices_in_counting_order(tok, dtype):
+    """A channel slice of a wider map, an offset (unaligned) view, a transposed tensor: the mask belongs to the element, not to the
+    memory."""
+    p, rng = 0.4, tok.rng_state(7, "cuda", 100)
+    wide = normal(1, 2, 12, 5, 4, dtype=dtype).contiguous(memory_format=torch.channels_last)
+    flat = normal(2, 1001, dtype=dtype)
+    cases = [wide[:, 3:10], flat[1:], normal(3, 6, 40, dtype=dtype)[:, 5:18], normal(4, 9, 7, dtype=dtype).t(), normal(5, 4, 3, 8, dtype=dtype)[:, 1]]
+    for x in cases:
+        y, dense = tok.dropout(x, p, rng), tok.dropout(x.contiguous(), p, rng)
+        assert torch.equal(y, dense) and y.shape == x.shape
+        assert torch.equal(tok.dropout(x, p, rng, residual=x.contiguous()), tok.dropout(x.contiguous(), p, rng, residual=x))
+
+
+@TYPES
+def test_dropout_limits(tok, dtype):
+    rng = tok.rng_state(3, "cuda")
+    x = normal(1, 333, dtype=dtype)
+    assert torch.equal(tok.dropout(x, 0.0, rng), x)
+    assert torch.equal(tok.dropout(torch.full_like(x, float("nan")), 1.0, rng, residual=x), x)
+    bad = torch.full_like(x, float("inf"))
+    y = tok.dropout(bad, 0.5, rng)
+    keep = ref.keep_mask((333,), 0.5, 3, 0).cuda()
+    assert (y[~keep] == 0).all() and y[keep].isinf().all()
+    assert tok.dropout(x[:0], 0.3, rng).shape == (0,)
+
+
+def test_dropout_state_moves_on_and_replays_draw_anew(tok):
+    x = torch.ones(4096, device="cuda")
+    state = tok.rng_state(11, "cuda")
+    eager = []
+    for _ in range(4):
+        eager.append(tok.dropout(x, 0.5, tok.rng_draw(state, x.numel())))
+    assert state.tolist() == [11, 4 * 1024]
+    assert all(not torch.equal(a, b) for a, b in zip(eager[:-1], eager[1:]))
+    state.copy_(tok.rng_state(11, "cuda"))
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = tok.dropout(x, 0.5, tok.rng_draw(state, x.numel()))
+    for want in eager:
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+        torch.randn(1000, device="cuda").sum().item()
+
+
+# ------------------------------------------------------------------------------------------------------------------- q / k norm
+def _qk_bound(x, w, cos, sin, eps, dy=None, dtype=F32):
+    """(value, bound) of y and, given dy, of dx and dw: r carries (D + 6) half steps, each product two more."""
+    d, u = x.shape[-1], ref.HALF_STEP[dtype]
+    y = ref.norm_rotary(x, w, cos, sin, eps)
+    n = x * (x.square().mean(-1, keepdim=True) + eps).rsqrt()
+    mag = ref.rotate((n * w).abs(), cos.abs()[..., None, :], -sin.abs()[..., None, :])
+    mag = torch.maximum(mag, (n * w).abs())
+    h = cos.shape[-1]
+    both = (n * w).abs()
+    mag[..., :h] = both[..., :h] + both[..., h:2 * h]
+    mag[..., h:2 * h] = mag[..., :h]
+    out = {"y": (y, (d + 12) * ref.U32 * mag + u * (y.abs() + (d + 12) * ref.U32 * mag))}
+    if dy is not None:
+        r = (x.square().mean(-1, keepdim=True) + eps).rsqrt()
+        dn = ref.rotate(dy, cos[..., None, :], -sin[..., None, :])
+        a = dy.abs().clone()
+        a[..., :h] = a[..., h:2 * h] = dy.abs()[..., :h] + dy.abs()[..., h:2 * h]
+        gn, ga = dn * w, a * w.abs()
+        dx = r * (gn - n * (gn * n).mean(-1, keepdim=True))
+        e = (3 * d + 30) * ref.U32 * r * (ga + n.abs() * (ga * n.abs()).mean(-1, keepdim=True))
+        rows = x[..., 0].numel()
+        out["dx"] = (dx, e + u * (dx.abs() + e))
+        out["dw"] = ((dn * n).sum((0, 1, 2)), ref.U32 * (d + 24 + rows / 8) * (a * n.abs()).sum((0, 1, 2)))
+    return out
+
+
+@TYPES
+@pytest.mark.parametrize("b,l,hq,hk,d,r", [(1, 1, 1, 1, 2, 2), (2, 5, 3, 1, 64, 64), (1, 33, 8, 2, 128, 128), (2, 7, 4, 4, 72, 36), (3, 4, 2, 1, 40, 24),
+                                           (1, 9, 5, 5, 96, 0), (2, 3, 2, 2, 6, 4), (2, 300, 16, 4, 128, 64), (1, 4100, 2, 1, 32, 32)], ids=str)
+@pytest.mark.parametrize("positions", ["none", "start", "1d", "2d"])
+def test_qk_norm_rotary(tok, dtype, b, l, hq, hk, d, r, positions):
+    qkv = normal(1, b, l, (hq + 2 * hk) * d, dtype=dtype, std=1.7)
+    q = qkv[..., :hq * d].unflatten(-1, (hq, d)).detach().requires_grad_()
+    k = qkv[..., hq * d:(hq + hk) * d].unflatten(-1, (hk, d)).detach().requires_grad_()
+    wq, wk = ((1 + normal(s, d, std=0.2)).requires_grad_() for s in (2, 3))
+    cos, sin = tok.rotary_table(l + 50, r)
+    pos, start, rows = None, 0, torch.arange(l)[None].expand(b, l)
+    if positions == "start":
+        start, rows = 13, rows + 13
+    elif positions == "1d":
+        pos = torch.randint(0, l + 50, (l,), generator=torch.Generator().manual_seed(4), dtype=torch.int32).cuda()
+        rows = pos.cpu().long()[None].expand(b, l)
+    elif positions == "2d":
+        pos = torch.randint(0, l + 50, (l, b), generator=torch.Generator().manual_seed(4)).cuda().t()
+        rows = pos.cpu()
+    yq, yk = tok.qk_norm_rotary(q, k, wq, wk, cos, sin, positions=pos, start=start, eps=1e-5)
+    dyq, dyk = normal(5, b, l, hq, d, dtype=dtype), normal(6, b, l, hk, d, dtype=dtype)
+    grads = torch.autograd.grad([yq, yk], [q, k, wq, wk], [dyq, dyk])
+    c64, s64 = d64(cos)[rows], d64(sin)[rows]
+    for name, x, w, y, dy, dx, dw in (("q", q, wq, yq, dyq, grads[0], grads[2]), ("k", k, wk, yk, dyk, grads[1], grads[3])):
+        want = _qk_bound(d64(x), d64(w), c64, s64, 1e-5, d64(dy), dtype)
+        for got, key in ((y, "y"), (dx, "dx"), (dw, "dw")):
+            ref.check(got, *want[key], f"{name}: {key}")
+
+
+def test_qk_norm_rotary_gradients_match_differences(tok):
+    q, k = normal(1, 1, 3, 2, 8).requires_grad_(), normal(2, 1, 3, 1, 8).requires_grad_()
+    wq, wk = normal(3, 8).requires_grad_(), normal(4, 8).requires_grad_()
+    cos, sin = tok.rotary_table(3, 8)
+    gq, gk = normal(5, 1, 3, 2, 8), normal(6, 1, 3, 1, 8)
+    f = lambda *a: sum((d64(y) * d64(g)).sum() for y, g in zip(tok.qk_norm_rotary(*a, cos, sin), (gq, gk)))  # noqa: E731
+    grads = torch.autograd.grad(tok.qk_norm_rotary(q, k, wq, wk, cos, sin), [q, k, wq, wk], [gq, gk])
+    _differences(f, [q, k, wq, wk], grads)
+
+
+def _differences(f, args, grads, step=2.0 ** -6):
+    """Central differences along the gradient of one argument at a time: error step^2 / 6 f''' + rounding of f (2^-22 |f| / step)."""
+    args = [a.detach() for a in args]
+    for i, g in enumerate(grads):
+        direction = g / g.norm()
+        moved = [f(*(a + s * step * direction if j == i else a for j, a in enumerate(args))) for s in (1, -1)]
+        slope = (moved[0] - moved[1]).item() / (2 * step)
+        assert abs(slope - g.norm().item()) <= 5e-3 * g.norm().item() + 1e-3, (i, slope, g.norm().item())
+
+
+@TYPES
+def test_qk_norm_rotary_outside_the_table_is_nan(tok, dtype):
+    q, k = normal(1, 2, 3, 2, 16, dtype=dtype), normal(2, 2, 3, 1, 16, dtype=dtype)
+    w = torch.ones(16, device="cuda")
+    cos, sin = tok.rotary_table(4, 8)
+    pos = torch.tensor([[0, 4, 1], [2 ** 40, 3, -1]], device="cuda")
+    yq, yk = tok.qk_norm_rotary(q, k, w, w, cos, sin, positions=pos)
+    bad = (pos < 0) | (pos >= 4)
+    for y in (yq, yk):
+        assert y[bad][..., :8].isnan().all() and y[~bad].isfinite().all() and y[..., 8:].isfinite().all()
+
+
+# ------------------------------------------------------------------------------------------------------------------- attention
+def _attention_case(tok, dtype, b, lq, lk, hq, hk, d, shape=None, mask=None, q_start=0, num=8, far=20, both=True, train=True, seed=0, table=None):
+    q, k, v = (normal(seed + i, b, n, h, d, dtype=dtype).requires_grad_(train) for i, (n, h) in enumerate(((lq, hq), (lk, hk), (lk, hk))))
+    rel = bias = buckets = None
+    if shape is not None:
+        rel = tok.RelativePositions(shape, num, far, both)
+        if table is None:
+            table = normal(seed + 4, rel.rows, hq, std=0.7)
+        table = table.requires_grad_(train)
+        buckets = ref.pair_buckets(shape, lq, lk, q_start, num, far, both)
+        bias = d64(table).T[:, buckets]
+    o = tok.attention(q, k, v, key_mask=mask, relative=rel, bias_table=table if rel is not None else None, q_start=q_start)
+    do = normal(seed + 5, b, lq, hq, d, dtype=dtype)
+    want = ref.attention(d64(q), d64(k), d64(v), d ** -0.5, None if mask is None else mask.cpu(), bias, d64(do) if train else None, dtype,
+                         two=rel is not None and train)
+    ref.check(o, *want["o"], "o")
+    if not train:
+        return o
+    leaves = [q, k, v] + ([table] if rel is not None else [])
+    grads = torch.autograd.grad(o, leaves, do)
+    for name, g in zip(("dq", "dk", "dv"), grads):
+        ref.check(g, *want[name], name)
+    if rel is not None:
+        ref.check(grads[3], *ref.table_grad(*want["ds"], buckets, rel.rows), "dtable")
+    return o
+
+
+def _mask(b, lk, kind, seed=9):
+    if kind is None:
+        return None
+    if kind == "ragged":
+        lens = torch.tensor([max(0, lk - 1 - (37 * i) % (lk + 1)) for i in range(b)])
+        return (torch.arange(lk)[None] < lens[:, None]).cuda()
+    if kind == "holes":
+        return (torch.rand(b, lk, generator=torch.Generator().manual_seed(seed)) < 0.6).cuda()
+    if kind == "tail":
+        return (torch.arange(lk)[None] >= lk - 3).expand(b, lk).cuda()
+    m = torch.zeros(b, lk, dtype=torch.bool)       # "empty": the first sample sees nothing
+    m[1:] = True
+    return m.cuda()
+
+
+@TYPES
+@pytest.mark.parametrize("lq,lk", [(1, 1), (1, 64), (2, 63), (33, 65), (64, 64), (129, 130), (200, 31), (5, 300)])
+@pytest.mark.parametrize("hq,hk,d", [(1, 1, 64), (4, 2, 32), (3, 1, 128), (2, 2, 96)])
+def test_attention_sizes(tok, dtype, lq, lk, hq, hk, d):
+    _attention_case(tok, dtype, 2, lq, lk, hq, hk, d)
+
+
+@TYPES
+@pytest.mark.parametrize("shape", [1, 2, 63, 64, 130, 321, (5, 7), (16, 12), (1, 40), (70, 1), (2, 130), (9, 64)], ids=str)
+@pytest.mark.parametrize("mask", [None, "ragged", "holes"])
+@pytest.mark.parametrize("d", [64, 40])
+def test_attention_relative(tok, dtype, shape, mask, d):
+    n = shape if isinstance(shape, int) else shape[0] * shape[1]
+    _attention_case(tok, dtype, 2, n, n, 4, 2, d, shape=shape, mask=_mask(2, n, mask))
+
+
+@TYPES
+@pytest.mark.parametrize("mask", ["ragged", "holes", "tail", "empty"])
+@pytest.mark.parametrize("lq,lk", [(3, 700), (150, 700), (70, 70)])
+def test_attention_masks(tok, dtype, mask, lq, lk):
+    _attention_case(tok, dtype, 3, lq, lk, 2, 1, 64, mask=_mask(3, lk, mask))
+
+
+@TYPES
+@pytest.mark.parametrize("hq,hk,d", [(1, 1, 64), (8, 2, 128), (16, 1, 64), (40, 1, 32)])
+@pytest.mark.parametrize("lq,lk,start", [(1, 4099, 4098), (1, 2500, 0), (2, 1537, 1300), (7, 3001, 5)])
+def test_attention_few_queries_over_long_keys(tok, dtype, hq, hk, d, lq, lk, start):
+    mask = torch.arange(lk)[None].cuda() < torch.tensor([[lk], [lk // 3]]).cuda()
+    for train in (False, True):
+        _attention_case(tok, dtype, 2, lq, lk, hq, hk, d, shape=max(lk, start + lq) + 1, q_start=start, mask=mask, num=32, far=128, train=train)
+
+
+@TYPES
+@pytest.mark.parametrize("shape,q_start,lq,lk", [((12, 9), 20, 50, 108), ((30, 33), 1, 7, 600), (500, 100, 129, 333)], ids=str)
+def test_attention_part_of_the_plan(tok, dtype, shape, q_start, lq, lk):
+    _attention_case(tok, dtype, 1, lq, lk, 2, 2, 64, shape=shape, q_start=q_start)
+
+
+@TYPES
+@pytest.mark.parametrize("shape", [257, (6, 21)], ids=str)
+def test_attention_one_direction(tok, dtype, shape):
+    n = shape if isinstance(shape, int) else shape[0] * shape[1]
+    _attention_case(tok, dtype, 1, n, n, 2, 1, 64, shape=shape, both=False, num=16, far=64)
+
+
+@TYPES
+def test_attention_wide_maps(tok, dtype):
+    """The widest rows a plan takes: the largest rings of the bias gradient."""
+    for shape, d in (((2, 512), 128), ((3, 257), 64)):
+        _attention_case(tok, dtype, 1, shape[0] * shape[1], shape[0] * shape[1], 1, 1, d, shape=shape, num=8, far=100)
+
+
+@TYPES
+def test_attention_blocking_entries(tok, dtype):
+    """Table entries of -inf hide pairs, finite ones at the type's lowest value leave the row a softmax over what they are added to."""
+    rel_rows = 8
+    table = normal(3, rel_rows, 2, std=0.5)
+    table[1], table[6, 0] = -math.inf, -math.inf
+    _attention_case(tok, dtype, 2, 90, 90, 2, 1, 64, shape=90, table=table.clone())
+    q, k, v = (normal(i, 1, 50, 1, 32, dtype=dtype) for i in range(3))
+    rel = tok.RelativePositions(50, 8, 20)
+    low = torch.full((8, 1), torch.finfo(F32).min, device="cuda")
+    o = tok.attention(q, k, v, relative=rel, bias_table=low)
+    mean = d64(v).mean(1, keepdim=True).expand(1, 50, 1, 32)      # the scores vanish against the entry: all keys weigh the same
+    ref.check(o, mean, (ref.HALF_STEP[dtype] * 2 + 64 * ref.U32) * d64(v).abs().mean(1, keepdim=True).expand_as(mean), "lowest entries")
+    none = torch.full((8, 1), -math.inf, device="cuda").requires_grad_()
+    qq, kk, vv = (t.clone().requires_grad_() for t in (q, k, v))
+    o = tok.attention(qq, kk, vv, relative=rel, bias_table=none)
+    assert (o == 0).all()
+    for g in torch.autograd.grad(o, [qq, kk, vv, none], torch.ones_like(o)):
+        assert (g == 0).all()
+
+
+@TYPES
+@pytest.mark.parametrize("lq,lk", [(40, 150), (2, 900)])
+def test_attention_hidden_keys_may_hold_anything(tok, dtype, lq, lk):
+    mask = _mask(2, lk, "holes")
+    q, k, v = normal(1, 2, lq, 2, 64, dtype=dtype), normal(2, 2, lk, 1, 64, dtype=dtype), normal(3, 2, lk, 1, 64, dtype=dtype)
+    rel = tok.RelativePositions(lk, 8, 20)
+    table = normal(4, 8, 2)
+    do = normal(5, 2, lq, 2, 64, dtype=dtype)
+    results = []
+    for fill in (0.0, float("nan"), float("inf"), -float("inf")):
+        kk, vv = (torch.where(mask[:, :, None, None], t, torch.full_like(t, fill)).requires_grad_() for t in (k, v))
+        qq, tt = q.clone().requires_grad_(), table.clone().requires_grad_()
+        o = tok.attention(qq, kk, vv, key_mask=mask, relative=rel, bias_table=tt)
+        results.append([o.detach(), *torch.autograd.grad(o, [qq, kk, vv, tt], do)])
+    for other in results[1:]:
+        for a, b in zip(results[0], other):
+            assert torch.equal(a, b)
+    assert (results[0][2][~mask] == 0).all() and (results[0][3][~mask] == 0).all()
+
+
+@TYPES
+@pytest.mark.parametrize("d", [1, 3, 20, 33, 72, 100, 127])
+def test_attention_any_head_size(tok, dtype, d):
+    _attention_case(tok, dtype, 1, 45, 70, 2, 1, d, shape=70)
+
+
+@TYPES
+def test_attention_strides(tok, dtype):
+    """Slices of one projection, head-major tensors, unaligned views, broadcast keys: the same values as dense operands."""
+    b, n, h, d = 2, 77, 2, 64
+    qkv = normal(1, b, n, 3 * h * d, dtype=dtype)
+    q, k, v = (t.unflatten(-1, (h, d)) for t in qkv.chunk(3, -1))
+    rel = tok.RelativePositions((7, 11), 8, 20)
+    table = normal(2, 64, h)
+    f = lambda *a: tok.attention(*a, relative=rel, bias_table=table)  # noqa: E731
+    dense = f(q.contiguous(), k.contiguous(), v.contiguous())
+    assert torch.equal(f(q, k, v), dense)
+    major = [t.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3) for t in (q, k, v)]
+    assert torch.equal(f(*major), dense)
+    odd = [torch.cat([t.reshape(-1)[:1], t.reshape(-1)])[1:].view(b, n, h, d) for t in (q, k, v)]
+    assert odd[0].data_ptr() % 16 and torch.equal(f(*odd), dense)
+    last = [t.transpose(-1, -2).contiguous().transpose(-1, -2) for t in (q, k, v)]
+    assert torch.equal(f(*last), dense)
+    one = k[:1, :, :1].contiguous()
+    leaf = one.clone().requires_grad_()
+    o = f(q, leaf.expand(b, n, h, d), v)
+    full = leaf.detach().expand(b, n, h, d).contiguous().requires_grad_()
+    o2 = f(q, full, v)
+    assert torch.equal(o, o2)
+    do = normal(3, b, n, h, d, dtype=dtype)
+    (g,), (g2,) = torch.autograd.grad(o, leaf, do), torch.autograd.grad(o2, full, do)
+    assert torch.allclose(g.float(), g2.float().sum((0, 2), keepdim=True).to(dtype).float(), rtol=2.0 ** -6, atol=1e-6 if dtype == F32 else 2.0 ** -6)
+
+
+def test_attention_empty(tok):
+    q, k, v = (torch.randn(2, n, 2, 16, device="cuda", requires_grad=True) for n in (3, 0, 0))
+    o = tok.attention(q, k, v)
+    assert o.shape == (2, 3, 2, 16) and (o == 0).all()
+    assert all((g == 0).all() for g in torch.autograd.grad(o.sum(), [q, k, v]))
+    assert tok.attention(q[:, :0], q, q).shape == (2, 0, 2, 16) and tok.attention(q[:0], q[:0], q[:0]).shape == (0, 3, 2, 16)
+
+
+def test_attention_gradients_match_differences(tok):
+    rel = tok.RelativePositions((4, 5), 8, 20)
+    q, k, v = (normal(i, 1, 20, 2, 16) for i in range(3))
+    table = normal(4, 64, 2, std=0.5)
+    g = normal(5, 1, 20, 2, 16)
+    leaves = [t.requires_grad_() for t in (q, k, v, table)]
+    f = lambda q, k, v, t: (d64(tok.attention(q, k, v, relative=rel, bias_table=t)) * d64(g)).sum()  # noqa: E731
+    grads = torch.autograd.grad(tok.attention(q, k, v, relative=rel, bias_table=table), leaves, g)
+    _differences(f, leaves, grads)
+
+
+@TYPES
+def test_attention_scale_and_single_gradients(tok, dtype):
+    """A scale of its own; gradients asked of one operand at a time are the ones that all together give."""
+    q, k, v = (normal(i, 1, 70, 2, 32, dtype=dtype) for i in range(3))
+    table, rel = normal(4, 8, 2), tok.RelativePositions(70, 8, 20)
+    do = normal(5, 1, 70, 2, 32, dtype=dtype)
+    want = ref.attention(d64(q), d64(k), d64(v), 0.03, None, d64(table).T[:, ref.pair_buckets(70, 70, 70, 0, 8, 20)], dtype=dtype)
+    ref.check(tok.attention(q, k, v, scale=0.03, relative=rel, bias_table=table), *want["o"], "o")
+    full = [t.clone().requires_grad_() for t in (q, k, v, table)]
+    g = torch.autograd.grad(tok.attention(full[0], full[1], full[2], relative=rel, bias_table=full[3]), full, do)
+    for i in (0, 1, 2, 3):
+        only = [t.clone().requires_grad_(j == i) for j, t in enumerate((q, k, v, table))]
+        (gi,) = torch.autograd.grad(tok.attention(only[0], only[1], only[2], relative=rel, bias_table=only[3]), [only[i]], do)
+        if dtype == F32 or i == 3:
+            assert torch.equal(gi, g[i])
+        else:      # without the table's gradient the probabilities are rounded once more: compare through the operand's type
+            assert torch.allclose(gi.float(), g[i].float(), rtol=2.0 ** -6, atol=2.0 ** -6 * g[i].float().abs().max().item())
+
+
+# ------------------------------------------------------------------------------------------------------------------- together
+def _layer(tok, x, state, p):
+    """Projection slices -> norm + rotation -> attention with a bias -> dropout on the residual: what a layer does."""
+    q, k, v = (t.unflatten(-1, (n, 32)) for t, n in zip(x["qkv"].split([128, 64, 64], -1), (4, 2, 2)))
+    q, k = tok.qk_norm_rotary(q, k, x["wq"], x["wk"], x["cos"], x["sin"])
+    o = tok.attention(q, k, v, key_mask=x["mask"], relative=x["rel"], bias_table=x["table"])
+    return tok.dropout(o.flatten(2), p, tok.rng_draw(state, o.numel()), residual=x["res"])
+
+
+def _layer_inputs(tok, dtype):
+    n = 12 * 9
+    cos, sin = tok.rotary_table((12, 9), 32)
+    leaves = dict(qkv=normal(1, 2, n, 256, dtype=dtype), wq=normal(2, 32, std=0.2) + 1, wk=normal(3, 32, std=0.2) + 1,
+                  table=normal(4, 64, 4, std=0.5), res=normal(5, 2, n, 128, dtype=dtype))
+    leaves = {k: v.requires_grad_() for k, v in leaves.items()}
+    return leaves, dict(leaves, cos=cos, sin=sin, mask=_mask(2, n, "ragged"), rel=tok.RelativePositions((12, 9), 8, 20))
+
+
+@TYPES
+def test_layer_streams_repeats_and_graphs(tok, dtype):
+    """The three operators as a layer uses them: the same bits on another stream, in a second run and in every replay of a captured
+    forward and backward pass, with eager work between the replays."""
+    leaves, x = _layer_inputs(tok, dtype)
+    dy = normal(7, 2, 108, 128, dtype=dtype)
+    state = tok.rng_state(5, "cuda")
+
+    def step():
+        y = _layer(tok, x, state, 0.3)
+        return [y.detach(), *torch.autograd.grad(y, list(leaves.values()), dy)]
+
+    runs = []
+    for _ in range(3):
+        runs.append(step())
+    state.copy_(tok.rng_state(5, "cuda"))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = step()
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(runs[0], other):
+        assert torch.equal(a, b)
+    assert not torch.equal(runs[0][0], runs[1][0])
+    state.copy_(tok.rng_state(5, "cuda"))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for want in runs:
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(captured, want):
+            assert torch.equal(a, b)
+        normal(1, 100, 100) @ normal(2, 100, 100)
+
+
+def test_layer_against_64_bits(tok):
+    """The chain in fp32 against the same chain in 64 bits: outputs and all gradients."""
+    leaves, x = _layer_inputs(tok, F32)
+    dy = normal(7, 2, 108, 128)
+    state = tok.rng_state(5, "cuda")
+    y = _layer(tok, x, state, 0.3)
+    grads = torch.autograd.grad(y, list(leaves.values()), dy)
+    z = {k: d64(v).requires_grad_() for k, v in leaves.items()}
+    q, k, v = (t.unflatten(-1, (n, 32)) for t, n in zip(z["qkv"].split([128, 64, 64], -1), (4, 2, 2)))
+    q, k = (ref.norm_rotary(t, z[w], d64(x["cos"])[None], d64(x["sin"])[None], 1e-6) for t, w in ((q, "wq"), (k, "wk")))
+    s = torch.einsum("bihd,bjhd->bhij", q, k.repeat_interleave(2, 2)) * 32 ** -0.5
+    s = s + z["table"].T[:, ref.pair_buckets((12, 9), 108, 108, 0, 8, 20)]
+    mask = x["mask"].cpu()
+    p = s.masked_fill(~mask[:, None, None, :], -1e300).softmax(-1) * mask.any(1)[:, None, None, None]
+    o = torch.einsum("bhij,bjhd->bihd", p, torch.where(mask[:, :, None, None], v, 0.0).repeat_interleave(2, 2)).flatten(2)
+    keep = ref.keep_mask((2, 108, 128), 0.3, 5, 0)
+    want = z["res"] + torch.where(keep, o / 0.7, 0.0)
+    wgrads = torch.autograd.grad(want, list(z.values()), d64(dy))
+    # fp32 throughout: (D + Lk) half steps relative to the largest entry cover the sums of the chain
+    for a, b, name in zip((y, *grads), (want, *wgrads), ("y", *leaves)):
+        ref.check(a, b.detach(), torch.full_like(b, 300 * ref.U32 * b.abs().max().item()).detach(), name)
+
+
+# ------------------------------------------------------------------------------------------------------------------- refusals
+def test_refusals(tok):
+    x = torch.zeros(2, 5, 4, 16, device="cuda")
+    rng = tok.rng_state(1, "cuda")
+    w, table = torch.ones(16, device="cuda"), torch.zeros(8, 4, device="cuda")
+    rel = tok.RelativePositions(5, 8, 20)
+    cos, sin = tok.rotary_table(5, 16)
+    mask = torch.ones(2, 5, dtype=torch.bool, device="cuda")
+    with pytest.raises(ValueError, match="probability"):
+        tok.dropout(x, 1.5, rng)
+    with pytest.raises(ValueError, match="probability"):
+        tok.dropout(x, float("nan"), rng)
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        tok.dropout(x.half(), 0.5, rng)
+    with pytest.raises(ValueError, match="state"):
+        tok.dropout(x, 0.5, rng.int())
+    with pytest.raises(ValueError, match="state"):
+        tok.dropout(x, 0.5, rng.cpu())
+    with pytest.raises(ValueError, match="residual"):
+        tok.dropout(x, 0.5, rng, residual=x[:1])
+    with pytest.raises(TypeError, match="one type"):
+        tok.dropout(x, 0.5, rng, residual=x.bfloat16())
+    with pytest.raises(ValueError, match="outside a table"):
+        tok.qk_norm_rotary(x, x, w, w, cos, sin, start=1)
+    with pytest.raises(ValueError, match="exclude"):
+        tok.qk_norm_rotary(x, x, w, w, cos, sin, positions=torch.zeros(5, dtype=torch.int64, device="cuda"), start=1)
+    with pytest.raises(TypeError, match="positions"):
+        tok.qk_norm_rotary(x, x, w, w, cos, sin, positions=torch.zeros(5, device="cuda"))
+    with pytest.raises(ValueError, match="positions"):
+        tok.qk_norm_rotary(x, x, w, w, cos, sin, positions=torch.zeros(4, dtype=torch.int32, device="cuda"))
+    with pytest.raises(ValueError, match="R <="):
+        tok.qk_norm_rotary(x, x, w, w, *tok.rotary_table(5, 18))
+    with pytest.raises(ValueError, match="q_weight"):
+        tok.qk_norm_rotary(x, x, w[:8], w, cos, sin)
+    with pytest.raises(TypeError, match="k_weight"):
+        tok.qk_norm_rotary(x, x, w, w.bfloat16(), cos, sin)
+    big = torch.zeros(1, 2, 1, 130, device="cuda")
+    with pytest.raises(ValueError, match="at most 128"):
+        tok.qk_norm_rotary(big, big, torch.ones(130, device="cuda"), torch.ones(130, device="cuda"), cos, sin)
+    with pytest.raises(ValueError, match="head size"):
+        tok.attention(big, big, big)
+    with pytest.raises(ValueError, match="share"):
+        tok.attention(x, x[:, :, :3], x[:, :, :3])
+    with pytest.raises(ValueError, match="expected"):
+        tok.attention(x, x, x[:, :4])
+    with pytest.raises(ValueError, match="scale"):
+        tok.attention(x, x, x, scale=0.0)
+    with pytest.raises(ValueError, match="key_mask"):
+        tok.attention(x, x, x, key_mask=mask.float())
+    with pytest.raises(ValueError, match="key_mask"):
+        tok.attention(x, x, x, key_mask=mask[:, :4])
+    with pytest.raises(ValueError, match="together"):
+        tok.attention(x, x, x, relative=rel)
+    with pytest.raises(ValueError, match="bias_table"):
+        tok.attention(x, x, x, relative=rel, bias_table=table[:7])
+    with pytest.raises(ValueError, match="do not fit"):
+        tok.attention(x, x, x, relative=rel, bias_table=table, q_start=1)
+    with pytest.raises(ValueError, match="q_start"):
+        tok.attention(x, x, x, q_start=1)
+    with pytest.raises(ValueError, match="plan is on"):
+        tok.attention(x, x, x, relative=tok.RelativePositions(5, 8, 20, device="cpu"), bias_table=table)
