@@ -4,11 +4,13 @@
 // 32, half l / 32) supplies k = 8 half + e), fp32 holds 4 (four v_mfma_f32_32x32x2_f32: MFMA e takes k = 4 half + e).  Either way a
 // product step covers 32 bytes of the k axis and the byte addresses are the same for both types.
 //
-// A 32 x 32 accumulator holds, in lane (column l % 32, half), register r: row (r & 3) + 8 (r >> 2) + 4 half.  The kernels compute
-// scores TRANSPOSED against what they multiply them with next (rows = the axis that the next product sums over), so accumulator
-// registers 4 c .. 4 c + 3 (fp32) or 8 c .. 8 c + 7 (bf16) are already the B fragment of that product's step c, with
-//     k(step c, element e) = 8 c + 4 half + e (fp32)  or  16 c + (e & 3) + 8 (e >> 2) + 4 half (bf16);
-// the A fragment is read to match: single dwords (fp32) or two ds_read_b64_tr_b16 (bf16), which transpose on the way.
+// A 32 x 32 accumulator holds, in lane (column l % 32, half), register r: row (r & 3) + 8 (r >> 2) + 4 half.  The rows of a score
+// product are dealt out so that this is tile row 16 half + r (tile_row: lane l of the A fragment reads tile row tile_row(l)): a lane
+// then holds sixteen CONSECUTIVE rows.  Scores are computed TRANSPOSED against what they multiply next (rows = the axis that the next
+// product sums over), so registers 4 c .. 4 c + 3 (fp32) or 8 c .. 8 c + 7 (bf16) are already the B fragment of that product's step c:
+//     row(step c, element e) = 16 half + 4 c + e (fp32)  or  16 half + 8 c + e (bf16);
+// its A fragment is read to match: single dwords (fp32) or two ds_read_b64_tr_b16 (bf16), which transpose on the way.  The products
+// whose rows are channels keep the plain order.
 #pragma once
 #include <hip/hip_runtime.h>
 #include "common.h"
@@ -44,28 +46,28 @@ __device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 acc) {
 }
 
 __device__ __forceinline__ int acc_row(int r, int half) { return (r & 3) + 8 * (r >> 2) + 4 * half; }
+__device__ __forceinline__ int tile_row(int l) { return 16 * ((l >> 2) & 1) + 4 * (l >> 3) + (l & 3); }
 
 template <int N> struct Log2 { static constexpr int v = 1 + Log2<N / 2>::v; };
 template <> struct Log2<1> { static constexpr int v = 0; };
 
 // A tile of rows in LDS: DP channels of T per row as 16-byte chunks, chunk c of row r at position c ^ f(r).  Rows are a power of two
-// chunks long; f spreads eight consecutive rows (the lanes of one ds_read_b128 phase) over all banks.
+// chunks long; f spreads the eight rows that one phase of a ds_read_b128 touches (4 n .. 4 n + 3 and the same 16 further) over all banks.
 template <typename T, int DP>
 struct Tile {
   static constexpr int E = Elem<T>::E, NC = DP / E;                      // chunks that hold data
   static constexpr int NP = NC <= 4 ? 4 : NC <= 8 ? 8 : NC <= 16 ? 16 : 32;   // chunks of a row in LDS
   static constexpr int kRowBytes = NP * 16;
-  __device__ static __forceinline__ int swz(int row) { return NP == 4 ? (row >> 1) & 3 : row & 7; }
+  __device__ static __forceinline__ int swz(int row) { return NP == 4 ? ((row >> 1) & 1) | ((row >> 3) & 2) : (row & 3) | ((row >> 2) & 4); }
   __device__ static __forceinline__ int at(int row, int chunk) { return row * kRowBytes + ((chunk ^ swz(row)) << 4); }
 
-  // A / B fragment "row, step m of the channel axis"
+  // A fragment "row, step m of the channel axis"
   __device__ static __forceinline__ typename Elem<T>::frag row_frag(const char* t, int row, int m, int half) {
     return *reinterpret_cast<const typename Elem<T>::frag*>(t + at(row, 2 * m + half));
   }
-  // A fragment "column 32 t + lane, step c of the ROW axis" of the 32 rows from row0 (a multiple of 32)
-  __device__ static __forceinline__ typename Elem<T>::frag col_frag(const char* tile, int row0, int t, int c, int lane);
 };
 
+// A fragment "column 32 t + lane, step c of the ROW axis" of the 32 rows from row0
 template <int DP>
 __device__ __forceinline__ f32x4 col_frag_f32(const char* tile, int row0, int t, int c, int lane) {
   typedef Tile<float, DP> TL;
@@ -73,7 +75,7 @@ __device__ __forceinline__ f32x4 col_frag_f32(const char* tile, int row0, int t,
   f32x4 f;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const int row = row0 + 8 * c + 4 * half + e;
+    const int row = row0 + 16 * half + 4 * c + e;
     f[e] = *reinterpret_cast<const float*>(tile + TL::at(row, col >> 2) + 4 * (col & 3));
   }
   return f;
@@ -81,12 +83,12 @@ __device__ __forceinline__ f32x4 col_frag_f32(const char* tile, int row0, int t,
 template <int DP>
 __device__ __forceinline__ bf16x8 col_frag_bf16(const char* tile, int row0, int t, int c, int lane) {
   typedef Tile<__bf16, DP> TL;
-  const int half = lane >> 5, row = row0 + 16 * c + 4 * half + ((lane & 15) >> 2);
+  const int half = lane >> 5, row = row0 + 16 * half + 8 * c + ((lane & 15) >> 2);
   const int chunk = 4 * t + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), in = 8 * (lane & 1);
   typedef __attribute__((address_space(3))) s16x4* lds_p;
   union { s16x4 s[2]; bf16x8 f; } u;
   u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(tile + TL::at(row, chunk) + in));
-  u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(tile + TL::at(row + 8, chunk) + in));
+  u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(tile + TL::at(row + 4, chunk) + in));
   return u.f;
 }
 template <typename T, int DP> struct ColFrag;

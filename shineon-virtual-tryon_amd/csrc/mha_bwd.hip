@@ -7,11 +7,11 @@
 // fixed order (no atomics on global memory): mha_dq_k owns query rows and walks the keys, mha_dkv_k owns keys and walks the query
 // rows of all heads that share them.  7 products instead of the 5 of a single pass whose dq would be added up by atomics.
 //
-// The bias gradient.  In mha_dq_k a lane holds one query and its registers hold keys, so dS for one register are 64 pairs: 32 different
-// offsets for each half of the wave.  Each half adds into a ring of its own in LDS (ds_add_f32; the 32 lanes hit 32 different words,
-// one wave's LDS operations stay in order, so the sum's order is fixed), indexed by offset modulo the ring.  As the walk moves on,
-// offsets that no later key can reach are summed over the eight rings and written to the block's strip; mha_dvec_k and mha_drow_k then
-// add strips over blocks and offsets over buckets.
+// The bias gradient needs dS summed along the diagonals of equal offset.  In mha_dq_k a wave adds the sums of each 32 x 32 piece into
+// rings of its own in LDS, indexed by offset modulo the ring (plain read, add, write: one wave's LDS operations stay in order, so the
+// sums have a fixed order).  As the walk over the keys moves on, offsets that no later key can reach are summed over the block's rings
+// and written to the block's strip; mha_dvec_k and mha_drow_k add strips over blocks and offsets over buckets.  (LDS float atomics, one
+// ds_add_f32 per register, were the first form: 300 cycles each, two thirds of the whole backward pass.)
 #include "mha.h"
 
 using namespace mha;
@@ -23,6 +23,7 @@ struct BwdP {
   float c;            // scale * log2 e
   int ring, strip;    // floats of one LDS ring (a power of two) and of one block's strip
   int stages, qtiles;
+  int per_wave;       // LDS rings of one wave: one for each half (sequences) or one (maps)
 };
 
 constexpr int BK = 64;          // keys (mha_dq_k) or query rows (mha_dkv_k) of a tile
@@ -30,6 +31,61 @@ constexpr int BK = 64;          // keys (mha_dq_k) or query rows (mha_dkv_k) of 
 // most codes between the first and last of n consecutive tokens
 __host__ __device__ inline int code_span(int n, int width) {
   return n < 2 ? 0 : (n - 1) + ((n - 2) / width + 1) * (width - 1);
+}
+
+template <int CTRL, bool ZERO>
+__device__ __forceinline__ float dpp(float old, float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), CTRL, 0xF, 0xF, ZERO));
+}
+
+// Diagonal sums of a 16 x 16 piece per row of 16 lanes: lane j holds query j, s[r] key r.  The running sums move one lane up per key
+// (lane j then holds diagonal r - j); what leaves lane 15 is finished and enters lane 0 of the second register, which moves along.
+// run: diagonal 15 - j;  fin: diagonal -1 - j (lane 15: zero).  46 vector instructions, no LDS.
+__device__ __forceinline__ void diagonals(const f32x16& s, float& run, float& fin) {
+  constexpr int kShr1 = 0x111, kRor1 = 0x121;
+  run = s[0];
+  fin = 0.f;
+#pragma unroll
+  for (int r = 1; r < 16; ++r) {
+    fin = dpp<kShr1, false>(dpp<kRor1, true>(0.f, run), fin);
+    run = s[r] + dpp<kShr1, true>(0.f, run);
+  }
+}
+
+// The same for a piece of a map, where 32 consecutive keys or queries may lie in several map rows and equal token distances are equal
+// offsets only inside one (key row, query row) rectangle: the piece goes through LDS and for every rectangle lane l walks diagonal
+// l - (queries - 1).  Different lanes of a rectangle add to different words of the ring.
+constexpr int kSkewPitch = 33, kSkew = 32 * kSkewPitch;
+__device__ __forceinline__ void rectangles(const f32x16& s, float* skew, float* ring, int rmask, int key0, int q0, int width, int lane) {
+  const int li = lane & 31, half = lane >> 5;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) skew[(16 * half + r) * kSkewPitch + li] = s[r];
+  __builtin_amdgcn_wave_barrier();      // one wave's LDS operations complete in order
+  int ky = key0 / width, kx = key0 - ky * width;
+  for (int ka = 0; ka < 32;) {
+    const int nk = width - kx < 32 - ka ? width - kx : 32 - ka;
+    int qy = q0 / width, qx = q0 - qy * width;
+    for (int qa = 0; qa < 32;) {
+      const int nq = width - qx < 32 - qa ? width - qx : 32 - qa;
+      const int d = lane - (nq - 1);
+      float x = 0.f;
+#pragma unroll 8
+      for (int k = 0; k < nk; ++k) {
+        const int q = k - d;
+        const bool on = q >= 0 && q < nq;
+        const float y = skew[(ka + k) * kSkewPitch + qa + (on ? q : 0)];
+        x += on ? y : 0.f;
+      }
+      if (d < nk) ring[((ky - qy) * (2 * width - 1) + kx - qx + d) & rmask] += x;
+      __builtin_amdgcn_wave_barrier();
+      qa += nq;
+      qx = 0;
+      ++qy;
+    }
+    ka += nk;
+    kx = 0;
+    ++ky;
+  }
 }
 
 template <typename T, int DP>
@@ -83,14 +139,16 @@ __global__ __launch_bounds__(256) void mha_dq_k(const BwdP P) {
   // bias gradient: rings cleared, strip filled with zeros up to the first offset that the walk can reach
   const bool want = D.strips != nullptr;
   float* rings = reinterpret_cast<float*>(sm + P.stages * 2 * TILE);
-  float* mine = rings + (2 * wave + half) * P.ring;
+  float* mine = rings + wave * P.per_wave * P.ring;
+  float* skew = rings + 4 * P.per_wave * P.ring + wave * kSkew;      // maps only
+  const int qw = D.q_start + q0 + 32 * wave, cqw = qw;               // first token of the wave's rows; its code in a sequence
   const int rmask = P.ring - 1;
   const int cqf = D.bias ? D.code[D.q_start + q0] : 0, cql = D.bias ? D.code[D.q_start + qlast] : 0;
   const int v0 = -cql;                                                 // code[0] = 0
   float* strip = want ? D.strips + ((size_t)bh * P.qtiles + blockIdx.y) * P.strip : nullptr;
   int flushed = v0;
   if (want) {
-    for (int i = tid; i < 8 * P.ring; i += 256) rings[i] = 0.f;
+    for (int i = tid; i < 4 * P.per_wave * P.ring; i += 256) rings[i] = 0.f;
     const int first = t0 < t1 ? D.code[t0 * BK] - cql : v0;
     for (int v = v0 + tid; v < first; v += 256) strip[v - v0] = 0.f;
     flushed = first;
@@ -98,8 +156,7 @@ __global__ __launch_bounds__(256) void mha_dq_k(const BwdP P) {
   auto flush = [&](int upto) {
     for (int v = flushed + tid; v < upto; v += 256) {
       float x = 0.f;
-#pragma unroll
-      for (int r = 0; r < 8; ++r) {
+      for (int r = 0; r < 4 * P.per_wave; ++r) {
         float* at = rings + r * P.ring + (v & rmask);
         x += *at;
         *at = 0.f;
@@ -155,18 +212,18 @@ __global__ __launch_bounds__(256) void mha_dq_k(const BwdP P) {
       f32x16 s, dp;
       if (bias) {
         if (D.linear) {
-          const float* bp = bias + key0 + 4 * half;
+          const float* bp = bias + key0 + 16 * half;
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            const f32x4u v = *reinterpret_cast<const f32x4u*>(bp + 8 * g);
+            const f32x4u v = *reinterpret_cast<const f32x4u*>(bp + 4 * g);
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[4 * g + e] = v[e];
           }
         } else {
-          const int* cp = D.code + key0 + 4 * half;
+          const int* cp = D.code + key0 + 16 * half;
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            const i32x4 v = *reinterpret_cast<const i32x4*>(cp + 8 * g);
+            const i32x4 v = *reinterpret_cast<const i32x4*>(cp + 4 * g);
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[4 * g + e] = bias[v[e]];
           }
@@ -178,30 +235,26 @@ __global__ __launch_bounds__(256) void mha_dq_k(const BwdP P) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] = 0.f;
 #pragma unroll
-      for (int k = 0; k < NM; ++k) s = mma(TL::row_frag(kt, 32 * u + li, k, half), q[k], s);
+      for (int k = 0; k < NM; ++k) s = mma(TL::row_frag(kt, 32 * u + tile_row(li), k, half), q[k], s);
 #pragma unroll
-      for (int k = 0; k < NM; ++k) dp = mma(TL::row_frag(vt, 32 * u + li, k, half), go[k], dp);
+      for (int k = 0; k < NM; ++k) dp = mma(TL::row_frag(vt, 32 * u + tile_row(li), k, half), go[k], dp);
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = exp2_(__builtin_fmaf(s[r], P.c, -lse)) * (dp[r] - delta);      // dS
       const unsigned w = (unsigned)(w64 >> (32 * u));
       if (w != ~0u) {
-        const unsigned my = w >> (4 * half);
+        const unsigned my = w >> (16 * half);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = (my >> acc_row(r, 0)) & 1 ? s[r] : 0.f;
+        for (int r = 0; r < 16; ++r) s[r] = (my >> r) & 1 ? s[r] : 0.f;
       }
       if (want) {
         if (D.linear) {
-          const int base = key0 + 4 * half - cq;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) atomicAdd(mine + ((base + acc_row(r, 0)) & rmask), s[r]);
+          float fin, run;
+          diagonals(s, run, fin);
+          const int v = key0 + 16 * half - cqw - 16 * (li >> 4) + 15 - (li & 15);
+          mine[half * P.ring + (v & rmask)] += run;
+          mine[half * P.ring + ((v - 16) & rmask)] += fin;
         } else {
-          const int* cp = D.code + key0 + 4 * half;
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const i32x4 v = *reinterpret_cast<const i32x4*>(cp + 8 * g);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) atomicAdd(mine + ((v[e] - cq) & rmask), s[4 * g + e]);
-          }
+          rectangles(s, skew, mine, rmask, key0, qw, D.width, lane);
         }
       }
 #pragma unroll
@@ -323,18 +376,18 @@ __global__ __launch_bounds__(256) void mha_dkv_k(const BwdP P) {
       f32x16 s, dp;
       if (bias0) {
         const float* bias = bias0 + (size_t)head * D.V;
-        if (D.linear) {      // four consecutive rows are four floats downwards
-          const float* bp = bias - (D.q_start + q0 + 32 * u + 4 * half) - 3;
+        if (D.linear) {      // consecutive rows are floats downwards
+          const float* bp = bias - (D.q_start + q0 + 32 * u + 16 * half) - 3;
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            const f32x4u x = *reinterpret_cast<const f32x4u*>(bp - 8 * g);
+            const f32x4u x = *reinterpret_cast<const f32x4u*>(bp - 4 * g);
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[4 * g + e] = x[3 - e];
           }
         } else {
-          const int* cp = D.code + D.q_start + q0 + 32 * u + 4 * half;
+          const int* cp = D.code + D.q_start + q0 + 32 * u + 16 * half;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = bias[-cp[acc_row(r, 0)]];
+          for (int r = 0; r < 16; ++r) s[r] = bias[-cp[r]];
         }
       } else {
 #pragma unroll
@@ -343,18 +396,18 @@ __global__ __launch_bounds__(256) void mha_dkv_k(const BwdP P) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] = 0.f;
 #pragma unroll
-      for (int m = 0; m < NM; ++m) s = mma(TL::row_frag(qtile, 32 * u + li, m, half), k[m], s);
+      for (int m = 0; m < NM; ++m) s = mma(TL::row_frag(qtile, 32 * u + tile_row(li), m, half), k[m], s);
 #pragma unroll
-      for (int m = 0; m < NM; ++m) dp = mma(TL::row_frag(gtile, 32 * u + li, m, half), v[m], dp);
+      for (int m = 0; m < NM; ++m) dp = mma(TL::row_frag(gtile, 32 * u + tile_row(li), m, half), v[m], dp);
       const int rows_left = D.Lq - q0 - 32 * u;
       if (rows_left < 32) {      // rows behind the last query: their bias was read from whatever lies in front of the expanded table
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = acc_row(r, half) < rows_left ? s[r] : -INFINITY;
+        for (int r = 0; r < 16; ++r) s[r] = 16 * half + r < rows_left ? s[r] : -INFINITY;
       }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const f32x4 ls = *reinterpret_cast<const f32x4*>(stats + 32 * u + 8 * g + 4 * half);
-        const f32x4 de = *reinterpret_cast<const f32x4*>(stats + BK + 32 * u + 8 * g + 4 * half);
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(stats + 32 * u + 16 * half + 4 * g);
+        const f32x4 de = *reinterpret_cast<const f32x4*>(stats + BK + 32 * u + 16 * half + 4 * g);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = 4 * g + e;
@@ -436,6 +489,7 @@ int make(const so_mha_desc* d, BwdP& p) {
   p.c = d->scale * kLog2e;
   p.qtiles = (d->Lq + 127) / 128;
   p.stages = 2;
+  p.per_wave = d->linear ? 2 : 1;
   if (d->strips) {
     if (!d->bias || d->width < 1) return SO_ERR_SHAPE;
     const int w = d->linear ? 1 : d->width;
@@ -460,7 +514,7 @@ template <typename T, int DP>
 int launch(BwdP p, hipStream_t st) {
   typedef Tile<T, DP> TL;
   constexpr size_t tile = (size_t)BK * TL::kRowBytes;
-  const size_t rings = p.d.strips ? (size_t)8 * p.ring * 4 : 0;
+  const size_t rings = p.d.strips ? ((size_t)4 * p.per_wave * p.ring + (p.d.linear ? 0 : 4 * kSkew)) * 4 : 0;
   p.stages = 4 * tile + rings <= kLds ? 2 : 1;
   size_t lds = p.stages * 2 * tile + rings;
   if (lds > kLds) return SO_ERR_SHAPE;

@@ -114,18 +114,18 @@ __global__ __launch_bounds__(256) void mha_fwd_k(const FwdP P) {
       const int r0 = SPLIT ? 32 * wave : 32 * u, key0 = t * TK + r0;
       if (bias) {
         if (D.linear) {
-          const float* bp = bias + key0 + 4 * half;
+          const float* bp = bias + key0 + 16 * half;
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            const f32x4u v = *reinterpret_cast<const f32x4u*>(bp + 8 * g);
+            const f32x4u v = *reinterpret_cast<const f32x4u*>(bp + 4 * g);
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[u][4 * g + e] = v[e];
           }
         } else {
-          const int* cp = D.code + key0 + 4 * half;
+          const int* cp = D.code + key0 + 16 * half;
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            const i32x4 v = *reinterpret_cast<const i32x4*>(cp + 8 * g);
+            const i32x4 v = *reinterpret_cast<const i32x4*>(cp + 4 * g);
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[u][4 * g + e] = bias[v[e]];
           }
@@ -135,13 +135,13 @@ __global__ __launch_bounds__(256) void mha_fwd_k(const FwdP P) {
         for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
       }
 #pragma unroll
-      for (int k = 0; k < NM; ++k) s[u] = mma(TL::row_frag(kt, r0 + li, k, half), q[k], s[u]);
+      for (int k = 0; k < NM; ++k) s[u] = mma(TL::row_frag(kt, r0 + tile_row(li), k, half), q[k], s[u]);
       const unsigned long long w64 = key_word(words, key0 >> 6 < D.nwords ? key0 >> 6 : 0, D.Lk);
       const unsigned w = key0 >= D.Lk ? 0u : (unsigned)(w64 >> (key0 & 32));
       if (w != ~0u) {
-        const unsigned mine = w >> (4 * half);
+        const unsigned mine = w >> (16 * half);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[u][r] = (mine >> acc_row(r, 0)) & 1 ? s[u][r] : -INFINITY;
+        for (int r = 0; r < 16; ++r) s[u][r] = (mine >> r) & 1 ? s[u][r] : -INFINITY;
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[u][r]);
