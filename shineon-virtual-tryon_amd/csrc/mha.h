@@ -124,14 +124,68 @@ __device__ __forceinline__ typename Elem<T>::frag as_frag(f32x4 v) {
   return u.f;
 }
 
+// Fills a tile of ROWS rows in LDS from rows `stride` bytes apart, by LDS-DMA (no registers, no ds_write).  A fill writes lane after
+// lane, so the chunk swizzle is applied on the source side.  Rows whose bit is clear and channels behind D are requested at an offset
+// outside the descriptor and arrive as zeros; nothing outside the operand is read.  The caller drains (SO_DMA_DRAIN) before the barrier
+// that publishes the tile.
+typedef __attribute__((address_space(3))) void* lds_ptr;
+template <typename T, int DP, int ROWS, int WAVES>
+struct Filler {
+  typedef Tile<T, DP> TL;
+  static constexpr int N = ROWS * TL::NP / (64 * WAVES), RPF = 64 * WAVES / TL::NP;   // fills per thread; rows per round of fills
+  static_assert(N * 64 * WAVES == ROWS * TL::NP, "whole fills");
+  unsigned off[N];
+  int row0;
+  __device__ __forceinline__ Filler(int D, unsigned stride, int tid) {
+    row0 = tid / TL::NP;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int row = row0 + j * RPF, ch = (tid & (TL::NP - 1)) ^ TL::swz(row);
+      off[j] = ch * TL::E < D ? row * stride + ch * 16 : 0x80000000u;
+    }
+  }
+  // rows [base_row, base_row + ROWS) of the tile at `src`; bits: one per row (64 rows from base_row 0, further ones in `more`)
+  __device__ __forceinline__ void fill(char* tile, const void* src, unsigned long long bits, unsigned long long more, int wave) const {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(src), 0, 0x7FFFFFFF, 0x00020000);
+    const bool all = bits == ~0ULL && (ROWS <= 64 || more == ~0ULL);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      unsigned o = off[j];
+      if (!all) {
+        const int row = row0 + j * RPF;
+        const unsigned long long w = ROWS > 64 && row >= 64 ? more : bits;
+        o = (w >> (row & 63)) & 1 ? o : 0x80000000u;
+      }
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(tile + (j * WAVES + wave) * 1024), 16, (int)o, 0, 0, 0);
+    }
+  }
+};
+
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
 
 // visible keys [64 w, 64 w + 64) of a sample as bits; keys behind the last are invisible
-__device__ __forceinline__ unsigned long long key_word(const unsigned long long* words, int w, int Lk) {
+__device__ __forceinline__ unsigned long long tail_word(int w, int Lk) {
   const int left = Lk - 64 * w;
-  unsigned long long m = left >= 64 ? ~0ULL : left <= 0 ? 0ULL : (1ULL << left) - 1;
-  return words ? m & words[w] : m;
+  return left >= 64 ? ~0ULL : left <= 0 ? 0ULL : (1ULL << left) - 1;
 }
+// Mask words of an ascending walk: the wave holds 64 of them, one per lane, and hands them out as scalars.
+struct KeyWords {
+  const unsigned long long* words;
+  int n, Lk, first, lane;
+  unsigned long long mine;
+  __device__ __forceinline__ KeyWords(const unsigned long long* words, int n, int Lk, int lane)
+      : words(words), n(n), Lk(Lk), first(-64), lane(lane), mine(0) {}
+  __device__ __forceinline__ unsigned long long get(int w) {
+    const unsigned long long tail = tail_word(w, Lk);
+    if (!words) return tail;
+    if (w < first || w >= first + 64) {
+      first = w;
+      mine = w + lane < n ? words[w + lane] : 0ULL;
+    }
+    const unsigned lo = __builtin_amdgcn_readlane((int)(unsigned)mine, w - first), hi = __builtin_amdgcn_readlane((int)(unsigned)(mine >> 32), w - first);
+    return tail & (((unsigned long long)hi << 32) | lo);
+  }
+};
 
 // first and one-past-last word with a visible key (the whole wave calls it)
 __device__ __forceinline__ void word_range(const unsigned long long* words, int Lk, int lane, int& lo, int& hi) {

@@ -89,16 +89,15 @@ __device__ __forceinline__ void rectangles(const f32x16& s, float* skew, float* 
 }
 
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void mha_dq_k(const BwdP P) {
+__global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha_dq_k(const BwdP P) {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::frag frag;
   constexpr int E = Elem<T>::E, KM = 2 * E, NM = DP / KM, NT = DP / 32, NCS = 32 / KM;
-  constexpr int TILE = BK * TL::kRowBytes, CH = BK * TL::NC / 256;
-  static_assert(BK * TL::NC % 256 == 0, "staging");
+  constexpr int TILE = BK * TL::kRowBytes;
   extern __shared__ __attribute__((aligned(16))) char sm[];          // [stages][K tile | V tile] | [4 waves][2 halves][ring]
   const so_mha_desc& D = P.d;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
-  const int bh = blockIdx.x, b = bh / D.Hq, head = bh - b * D.Hq, hk = head / (D.Hq / D.Hk);
+  const int bh = (int)((blockIdx.x + blockIdx.y) % gridDim.x), b = bh / D.Hq, head = bh - b * D.Hq, hk = head / (D.Hq / D.Hk);
   const int q0 = blockIdx.y * 128, qlast = (q0 + 128 < D.Lq ? q0 + 128 : D.Lq) - 1;
   const int row = q0 + 32 * wave + li;
   const bool rowv = row < D.Lq;
@@ -166,27 +165,17 @@ __global__ __launch_bounds__(256) void mha_dq_k(const BwdP P) {
     flushed = upto;
   };
 
-  f32x4 kreg[CH], vreg[CH];
   const T* kb = (const T*)D.k + (size_t)b * D.skb + (size_t)hk * D.skh;
   const T* vb = (const T*)D.v + (size_t)b * D.svb + (size_t)hk * D.svh;
-  auto fetch = [&](int t) {
-    const unsigned long long w = key_word(words, t, D.Lk);
-#pragma unroll
-    for (int u = 0; u < CH; ++u) {
-      const int idx = tid + 256 * u, r = idx / TL::NC, ch = idx % TL::NC, key = t * BK + r;
-      const bool on = ((w >> r) & 1) && ch * E < D.D;
-      kreg[u] = load_chunk<T>(kb + (size_t)(on ? key : 0) * D.skl, ch, on);
-      vreg[u] = load_chunk<T>(vb + (size_t)(on ? key : 0) * D.svl, ch, on);
-    }
-  };
-  auto store = [&](int st) {
+  const int wave_u = __builtin_amdgcn_readfirstlane(wave);
+  const Filler<T, DP, BK, 4> fk(D.D, (unsigned)(D.skl * sizeof(T)), tid), fv(D.D, (unsigned)(D.svl * sizeof(T)), tid);
+  KeyWords kw(words, D.nwords, D.Lk, lane);
+  unsigned long long next = 0;
+  auto fetch = [&](int t, int st) {
+    next = kw.get(t);
     char* kt = sm + st * 2 * TILE;
-#pragma unroll
-    for (int u = 0; u < CH; ++u) {
-      const int idx = tid + 256 * u, r = idx / TL::NC, ch = idx % TL::NC;
-      *reinterpret_cast<f32x4*>(kt + TL::at(r, ch)) = kreg[u];
-      *reinterpret_cast<f32x4*>(kt + TILE + TL::at(r, ch)) = vreg[u];
-    }
+    fk.fill(kt, kb + (size_t)t * BK * D.skl, next, 0, wave_u);
+    fv.fill(kt + TILE, vb + (size_t)t * BK * D.svl, next, 0, wave_u);
   };
 
   f32x16 dq[NT];
@@ -194,18 +183,16 @@ __global__ __launch_bounds__(256) void mha_dq_k(const BwdP P) {
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dq[t][r] = 0.f;
-  if (t0 < t1) {
-    fetch(t0);
-    store(0);
-  }
+  if (t0 < t1) fetch(t0, 0);
+  SO_DMA_DRAIN();
   __syncthreads();
   for (int t = t0; t < t1; ++t) {
     const int st = P.stages == 2 ? (t - t0) & 1 : 0;
     const char* kt = sm + st * 2 * TILE;
     const char* vt = kt + TILE;
-    if (t + 1 < t1) fetch(t + 1);
+    const unsigned long long w64 = next;
+    if (P.stages == 2 && t + 1 < t1) fetch(t + 1, st ^ 1);
     if (want && t > t0) flush(D.code[t * BK] - cql);      // offsets below this tile's: final, and no wave adds to them any more
-    const unsigned long long w64 = key_word(words, t, D.Lk);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int key0 = t * BK + 32 * u;
@@ -265,8 +252,11 @@ __global__ __launch_bounds__(256) void mha_dq_k(const BwdP P) {
         for (int v = 0; v < NT; ++v) dq[v] = mma(ColFrag<T, DP>::get(kt, 32 * u, v, c, lane), f, dq[v]);
       }
     }
-    if (P.stages == 1) __syncthreads();
-    if (t + 1 < t1) store(P.stages == 2 ? st ^ 1 : 0);
+    if (P.stages == 1) {
+      __syncthreads();
+      if (t + 1 < t1) fetch(t + 1, 0);
+    }
+    SO_DMA_DRAIN();
     __syncthreads();
   }
   if (want) {
@@ -294,20 +284,21 @@ __global__ __launch_bounds__(256) void mha_dq_k(const BwdP P) {
 }
 
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void mha_dkv_k(const BwdP P) {
+__global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha_dkv_k(const BwdP P) {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::frag frag;
   constexpr int E = Elem<T>::E, KM = 2 * E, NM = DP / KM, NT = DP / 32, NCS = 32 / KM;
-  constexpr int TILE = BK * TL::kRowBytes, CH = BK * TL::NC / 256;
+  constexpr int TILE = BK * TL::kRowBytes;
   extern __shared__ __attribute__((aligned(16))) char sm[];          // [2][Q tile | dO tile | lse | delta]
   constexpr int STAGE = 2 * TILE + 2 * BK * 4;
   const so_mha_desc& D = P.d;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
-  const int bh = blockIdx.x, b = bh / D.Hk, hk = bh - b * D.Hk, G = D.Hq / D.Hk;
+  const int bh = (int)((blockIdx.x + blockIdx.y) % gridDim.x), b = bh / D.Hk, hk = bh - b * D.Hk, G = D.Hq / D.Hk;
   const int key = blockIdx.y * 128 + 32 * wave + li;
   const unsigned long long* words = D.words ? (const unsigned long long*)D.words + (size_t)b * D.nwords : nullptr;
   const int w0 = 2 * blockIdx.y;
-  const unsigned long long wa = key_word(words, w0, D.Lk), wb = w0 + 1 < D.nwords ? key_word(words, w0 + 1, D.Lk) : 0ULL;
+  const unsigned long long wa = tail_word(w0, D.Lk) & (words ? words[w0] : ~0ULL);
+  const unsigned long long wb = w0 + 1 < D.nwords ? tail_word(w0 + 1, D.Lk) & (words ? words[w0 + 1] : ~0ULL) : 0ULL;
   const bool keyv = key < D.Lk, vis = ((wave < 2 ? wa : wb) >> (key & 63)) & 1;
 
   frag k[NM], v[NM];
@@ -324,19 +315,15 @@ __global__ __launch_bounds__(256) void mha_dkv_k(const BwdP P) {
   const float* bias0 = D.bias ? D.bias + D.code_max + D.code[keyv ? key : D.Lk - 1] : nullptr;
 
   const int qt = (D.Lq + BK - 1) / BK, n = (wa | wb) ? G * qt : 0;    // a block without a visible key writes zeros
-  f32x4 qreg[CH], greg[CH];
+  const int wave_u = __builtin_amdgcn_readfirstlane(wave);
+  const Filler<T, DP, BK, 4> fq(D.D, (unsigned)(D.sql * sizeof(T)), tid), fg(D.D, (unsigned)((size_t)D.Hq * D.D * sizeof(T)), tid);
   float sreg = 0.f;
-  auto fetch = [&](int t) {
+  auto fetch = [&](int t, int st) {
     const int head = hk * G + t / qt, q0 = (t % qt) * BK;
-    const T* qb = (const T*)D.q + (size_t)b * D.sqb + (size_t)head * D.sqh;
-    const T* gb = (const T*)D.dout + ((size_t)b * D.Lq * D.Hq + head) * D.D;
-#pragma unroll
-    for (int u = 0; u < CH; ++u) {
-      const int idx = tid + 256 * u, r = idx / TL::NC, ch = idx % TL::NC, i = q0 + r;
-      const bool on = i < D.Lq && ch * E < D.D;
-      qreg[u] = load_chunk<T>(qb + (size_t)(on ? i : 0) * D.sql, ch, on);
-      greg[u] = load_chunk<T>(gb + (size_t)(on ? i : 0) * D.Hq * D.D, ch, on);
-    }
+    const unsigned long long rows = tail_word(t % qt, D.Lq);
+    char* qtile = sm + st * STAGE;
+    fq.fill(qtile, (const T*)D.q + (size_t)b * D.sqb + (size_t)head * D.sqh + (size_t)q0 * D.sql, rows, 0, wave_u);
+    fg.fill(qtile + TILE, (const T*)D.dout + (((size_t)b * D.Lq + q0) * D.Hq + head) * D.D, rows, 0, wave_u);
     if (tid < 2 * BK) {
       const int i = q0 + (tid & (BK - 1));
       const float* src = (tid < BK ? D.lse : D.delta) + ((size_t)b * D.Hq + head) * D.Lq;
@@ -344,14 +331,7 @@ __global__ __launch_bounds__(256) void mha_dkv_k(const BwdP P) {
     }
   };
   auto store = [&](int st) {
-    char* qtile = sm + st * STAGE;
-#pragma unroll
-    for (int u = 0; u < CH; ++u) {
-      const int idx = tid + 256 * u, r = idx / TL::NC, ch = idx % TL::NC;
-      *reinterpret_cast<f32x4*>(qtile + TL::at(r, ch)) = qreg[u];
-      *reinterpret_cast<f32x4*>(qtile + TILE + TL::at(r, ch)) = greg[u];
-    }
-    if (tid < 2 * BK) reinterpret_cast<float*>(qtile + 2 * TILE)[tid] = sreg;
+    if (tid < 2 * BK) reinterpret_cast<float*>(sm + st * STAGE + 2 * TILE)[tid] = sreg;
   };
 
   f32x16 dk[NT], dv[NT];
@@ -360,16 +340,17 @@ __global__ __launch_bounds__(256) void mha_dkv_k(const BwdP P) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[t][r] = dv[t][r] = 0.f;
   if (n) {
-    fetch(0);
+    fetch(0, 0);
     store(0);
   }
+  SO_DMA_DRAIN();
   __syncthreads();
   for (int t = 0; t < n; ++t) {
     const int st = P.stages == 2 ? t & 1 : 0;
     const char* qtile = sm + st * STAGE;
     const char* gtile = qtile + TILE;
     const float* stats = reinterpret_cast<const float*>(qtile + 2 * TILE);
-    if (t + 1 < n) fetch(t + 1);
+    if (P.stages == 2 && t + 1 < n) fetch(t + 1, st ^ 1);
     const int head = hk * G + t / qt, q0 = (t % qt) * BK;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -427,8 +408,12 @@ __global__ __launch_bounds__(256) void mha_dkv_k(const BwdP P) {
         }
       }
     }
-    if (P.stages == 1) __syncthreads();
+    if (P.stages == 1) {
+      __syncthreads();
+      if (t + 1 < n) fetch(t + 1, 0);
+    }
     if (t + 1 < n) store(P.stages == 2 ? st ^ 1 : 0);
+    SO_DMA_DRAIN();
     __syncthreads();
   }
   if (!keyv) return;

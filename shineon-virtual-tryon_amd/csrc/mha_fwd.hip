@@ -28,18 +28,16 @@ struct FwdP {
 };
 
 template <typename T, int DP, bool SPLIT, bool TWO>   // TWO: the probabilities as hi + lo pair of bf16 products
-__global__ __launch_bounds__(256) void mha_fwd_k(const FwdP P) {
+__global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 96 ? 2 : 1))) void mha_fwd_k(const FwdP P) {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::frag frag;
   constexpr int E = Elem<T>::E, KM = 2 * E, NM = DP / KM, NT = DP / 32, NCS = 32 / KM;
   constexpr int TK = SPLIT ? 128 : 64, SUBS = SPLIT ? 1 : 2;       // keys of a tile; 32-key pieces of it that one wave takes
   constexpr int TILE = TK * TL::kRowBytes, STAGES = 4 * TILE <= 150 * 1024 ? 2 : 1;
-  constexpr int CH = TK * TL::NC / 256;                             // chunks each thread stages of K and of V
-  static_assert(TK * TL::NC % 256 == 0, "staging");
   extern __shared__ __attribute__((aligned(16))) char sm[];         // [STAGES][K tile | V tile]
   const so_mha_desc& D = P.d;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
-  const int bh = blockIdx.x, b = bh / D.Hk, hk = bh - b * D.Hk, G = D.Hq / D.Hk, part = blockIdx.z;
+  const int bh = (int)((blockIdx.x + blockIdx.y) % gridDim.x), b = bh / D.Hk, hk = bh - b * D.Hk, G = D.Hq / D.Hk, part = blockIdx.z;
   const int rows = G * D.Lq;
   const int row = blockIdx.y * (SPLIT ? 32 : 128) + (SPLIT ? 0 : 32 * wave) + li;
   const bool rowv = row < rows;
@@ -66,27 +64,18 @@ __global__ __launch_bounds__(256) void mha_fwd_k(const FwdP P) {
   const float* bias = nullptr;
   if (D.bias) bias = D.bias + (size_t)head * D.V + D.code_max - D.code[D.q_start + qi];
 
-  f32x4 kreg[CH], vreg[CH];
   const T* kb = (const T*)D.k + (size_t)b * D.skb + (size_t)hk * D.skh;
   const T* vb = (const T*)D.v + (size_t)b * D.svb + (size_t)hk * D.svh;
-  auto fetch = [&](int t) {
-#pragma unroll
-    for (int u = 0; u < CH; ++u) {
-      const int idx = tid + 256 * u, r = idx / TL::NC, ch = idx % TL::NC, key = t * TK + r;
-      const unsigned long long w = key_word(words, key >> 6 < D.nwords ? key >> 6 : 0, D.Lk);
-      const bool on = key < D.Lk && ((w >> (key & 63)) & 1) && ch * E < D.D;
-      kreg[u] = load_chunk<T>(kb + (size_t)(on ? key : 0) * D.skl, ch, on);
-      vreg[u] = load_chunk<T>(vb + (size_t)(on ? key : 0) * D.svl, ch, on);
-    }
-  };
-  auto store = [&](int st) {
+  const int wave_u = __builtin_amdgcn_readfirstlane(wave);
+  const Filler<T, DP, TK, 4> fk(D.D, (unsigned)(D.skl * sizeof(T)), tid), fv(D.D, (unsigned)(D.svl * sizeof(T)), tid);
+  KeyWords kw(words, D.nwords, D.Lk, lane);
+  unsigned long long bits[2] = {0, 0}, next[2] = {0, 0};
+  auto fetch = [&](int t, int st) {      // tile t -> stage st; its mask words -> next
+    next[0] = kw.get(WPT * t);
+    if (WPT == 2) next[1] = kw.get(WPT * t + 1);
     char* kt = sm + st * 2 * TILE;
-#pragma unroll
-    for (int u = 0; u < CH; ++u) {
-      const int idx = tid + 256 * u, r = idx / TL::NC, ch = idx % TL::NC;
-      *reinterpret_cast<f32x4*>(kt + TL::at(r, ch)) = kreg[u];
-      *reinterpret_cast<f32x4*>(kt + TILE + TL::at(r, ch)) = vreg[u];
-    }
+    fk.fill(kt, kb + (size_t)t * TK * D.skl, next[0], next[1], wave_u);
+    fv.fill(kt + TILE, vb + (size_t)t * TK * D.svl, next[0], next[1], wave_u);
   };
 
   f32x16 o[NT];
@@ -96,16 +85,16 @@ __global__ __launch_bounds__(256) void mha_fwd_k(const FwdP P) {
     for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
   float m = -INFINITY, l = 0.f;
 
-  if (t0 < t1) {
-    fetch(t0);
-    store(0);
-  }
+  if (t0 < t1) fetch(t0, 0);
+  SO_DMA_DRAIN();
   __syncthreads();
   for (int t = t0; t < t1; ++t) {
     const int st = STAGES == 2 ? (t - t0) & 1 : 0;
     const char* kt = sm + st * 2 * TILE;
     const char* vt = kt + TILE;
-    if (t + 1 < t1) fetch(t + 1);
+    bits[0] = next[0];
+    bits[1] = next[1];
+    if (STAGES == 2 && t + 1 < t1) fetch(t + 1, st ^ 1);
     // scores of this wave's keys
     f32x16 s[SUBS];
     float mx = -INFINITY;
@@ -136,8 +125,7 @@ __global__ __launch_bounds__(256) void mha_fwd_k(const FwdP P) {
       }
 #pragma unroll
       for (int k = 0; k < NM; ++k) s[u] = mma(TL::row_frag(kt, r0 + tile_row(li), k, half), q[k], s[u]);
-      const unsigned long long w64 = key_word(words, key0 >> 6 < D.nwords ? key0 >> 6 : 0, D.Lk);
-      const unsigned w = key0 >= D.Lk ? 0u : (unsigned)(w64 >> (key0 & 32));
+      const unsigned w = (unsigned)(bits[r0 >> 6] >> (r0 & 32));
       if (w != ~0u) {
         const unsigned mine = w >> (16 * half);
 #pragma unroll
@@ -186,8 +174,11 @@ __global__ __launch_bounds__(256) void mha_fwd_k(const FwdP P) {
         }
       }
     }
-    if (STAGES == 1) __syncthreads();
-    if (t + 1 < t1) store(STAGES == 2 ? st ^ 1 : 0);
+    if (STAGES == 1) {
+      __syncthreads();
+      if (t + 1 < t1) fetch(t + 1, 0);
+    }
+    SO_DMA_DRAIN();
     __syncthreads();
   }
   l += other_half(l);
@@ -379,6 +370,9 @@ int so_mha_check(const so_mha_desc* d) {
   if (!(d->scale > 0.f) || d->nwords != (d->Lk + 63) / 64) return SO_ERR_SHAPE;
   const int E = d->dtype == SO_F32 ? 4 : 8;
   if (d->D % E) return SO_ERR_ALIGN;
+  // a tile's rows lie within 2^31 bytes of its first
+  if (d->skl < 0 || d->svl < 0 || d->sql < 0 || d->skl * 4 * 128 >= (1LL << 31) || d->svl * 4 * 128 >= (1LL << 31) || d->sql * 4 * 128 >= (1LL << 31) ||
+      (long long)d->Hq * d->D * 4 * 128 >= (1LL << 31)) return SO_ERR_SHAPE;
   const long long s[] = {d->sqb, d->sql, d->sqh, d->skb, d->skl, d->skh, d->svb, d->svl, d->svh};
   for (long long x : s)
     if (x % E) return SO_ERR_ALIGN;
