@@ -8,8 +8,7 @@
 // rows of all heads that share them.  7 products instead of the 5 of a single pass whose dq would be added up by atomics.
 //
 // The bias gradient needs dS summed along the diagonals of equal offset.  In mha_dq_k a wave adds the sums of each 32 x 32 piece into
-// rings of its own in LDS, indexed by offset modulo the ring (plain read, add, write: one wave's LDS operations stay in order, so the
-// sums have a fixed order).  As the walk over the keys moves on, offsets that no later key can reach are summed over the block's rings
+// rings of its own in LDS, indexed by offset modulo the ring, in a fixed order.  As the walk over the keys moves on, offsets that no later key can reach are summed over the block's rings
 // and written to the block's strip; mha_dvec_k and mha_drow_k add strips over blocks and offsets over buckets.  (LDS float atomics, one
 // ds_add_f32 per register, were the first form: 300 cycles each, two thirds of the whole backward pass.)
 #include "mha.h"
@@ -38,18 +37,25 @@ __device__ __forceinline__ float dpp(float old, float v) {
   return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), CTRL, 0xF, 0xF, ZERO));
 }
 
-// Diagonal sums of a 16 x 16 piece per row of 16 lanes: lane j holds query j, s[r] key r.  The running sums move one lane up per key
-// (lane j then holds diagonal r - j); what leaves lane 15 is finished and enters lane 0 of the second register, which moves along.
-// run: diagonal 15 - j;  fin: diagonal -1 - j (lane 15: zero).  46 vector instructions, no LDS.
-__device__ __forceinline__ void diagonals(const f32x16& s, float& run, float& fin) {
+// Diagonal sums of 16 keys x 32 queries of a sequence, in vector instructions.  Per row of 16 lanes, lane j holds query j, s[r] key r:
+// the running sums move one lane up per key (lane j then holds diagonal r - j); what leaves lane 15 is finished and enters lane 0 of a
+// second register, which moves along.  At the end run = diagonal 15 - j, fin = diagonal -1 - j (lane 15: zero), against the row's first
+// query.  The diagonals of the second row's run are those of the first row's fin, and the first row's run (pend, kept in the second
+// row's lanes) are those of the second row's fin 32 keys further on, where this half of the wave works next.  So every call finishes
+// the 32 diagonals in front of its keys: lane l returns diagonal -1 - l against the half's first key and the wave's first query.
+__device__ __forceinline__ float diagonals(const f32x16& s, float& pend, int li) {
   constexpr int kShr1 = 0x111, kRor1 = 0x121;
-  run = s[0];
-  fin = 0.f;
+  float run = s[0], fin = 0.f;
 #pragma unroll
   for (int r = 1; r < 16; ++r) {
     fin = dpp<kShr1, false>(dpp<kRor1, true>(0.f, run), fin);
     run = s[r] + dpp<kShr1, true>(0.f, run);
   }
+  // rows 0 1 2 3 -> first: 0 0 2 2, second: 1 1 3 3
+  const auto rows = __builtin_amdgcn_permlane16_swap(__float_as_uint(run), __float_as_uint(run), false, false);
+  const float x = fin + (li < 16 ? __uint_as_float(rows[1]) : pend);
+  pend = __uint_as_float(rows[0]);
+  return x;
 }
 
 // The same for a piece of a map, where 32 consecutive keys or queries may lie in several map rows and equal token distances are equal
@@ -140,7 +146,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
   float* rings = reinterpret_cast<float*>(sm + P.stages * 2 * TILE);
   float* mine = rings + wave * P.per_wave * P.ring;
   float* skew = rings + 4 * P.per_wave * P.ring + wave * kSkew;      // maps only
-  const int qw = D.q_start + q0 + 32 * wave, cqw = qw;               // first token of the wave's rows; its code in a sequence
+  const int qw = D.q_start + q0 + 32 * wave;                         // first token of the wave's rows
   const int rmask = P.ring - 1;
   const int cqf = D.bias ? D.code[D.q_start + q0] : 0, cql = D.bias ? D.code[D.q_start + qlast] : 0;
   const int v0 = -cql;                                                 // code[0] = 0
@@ -152,6 +158,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
     for (int v = v0 + tid; v < first; v += 256) strip[v - v0] = 0.f;
     flushed = first;
   }
+  float pend = 0.f;      // sequences: see diagonals()
+  int base = 0;
   auto flush = [&](int upto) {
     for (int v = flushed + tid; v < upto; v += 256) {
       float x = 0.f;
@@ -162,7 +170,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
       }
       strip[v - v0] = x;
     }
-    flushed = upto;
+    if (upto > flushed) flushed = upto;
   };
 
   const T* kb = (const T*)D.k + (size_t)b * D.skb + (size_t)hk * D.skh;
@@ -192,7 +200,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
     const char* vt = kt + TILE;
     const unsigned long long w64 = next;
     if (P.stages == 2 && t + 1 < t1) fetch(t + 1, st ^ 1);
-    if (want && t > t0) flush(D.code[t * BK] - cql);      // offsets below this tile's: final, and no wave adds to them any more
+    // offsets below those of this tile are final, and nothing adds to them any more (a sequence's rings are written up to the last
+    // row's first key exclusively)
+    if (want && t > t0) flush(D.linear ? t * BK - D.q_start - q0 - 128 : D.code[t * BK] - cql);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int key0 = t * BK + 32 * u;
@@ -221,10 +231,11 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] = 0.f;
-#pragma unroll
-      for (int k = 0; k < NM; ++k) s = mma(TL::row_frag(kt, 32 * u + tile_row(li), k, half), q[k], s);
+      // do v^T first: it needs nothing from global memory and hides the latency of the bias
 #pragma unroll
       for (int k = 0; k < NM; ++k) dp = mma(TL::row_frag(vt, 32 * u + tile_row(li), k, half), go[k], dp);
+#pragma unroll
+      for (int k = 0; k < NM; ++k) s = mma(TL::row_frag(kt, 32 * u + tile_row(li), k, half), q[k], s);
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = exp2_(__builtin_fmaf(s[r], P.c, -lse)) * (dp[r] - delta);      // dS
       const unsigned w = (unsigned)(w64 >> (32 * u));
@@ -235,11 +246,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
       }
       if (want) {
         if (D.linear) {
-          float fin, run;
-          diagonals(s, run, fin);
-          const int v = key0 + 16 * half - cqw - 16 * (li >> 4) + 15 - (li & 15);
-          mine[half * P.ring + (v & rmask)] += run;
-          mine[half * P.ring + ((v - 16) & rmask)] += fin;
+          base = key0 + 16 * half - qw;
+          mine[half * P.ring + ((base - 1 - li) & rmask)] = diagonals(s, pend, li);
         } else {
           rectangles(s, skew, mine, rmask, key0, qw, D.width, lane);
         }
@@ -261,6 +269,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
   }
   if (want) {
     if (t0 < t1) {
+      if (D.linear) {
+        if (li >= 16) mine[half * P.ring + ((base + 31 - li) & rmask)] = pend;
+        __syncthreads();
+      }
       const int kl = (t1 * BK < D.Lk ? t1 * BK : D.Lk) - 1;
       flush(D.code[kl] - cqf + 1);
     }
@@ -377,9 +389,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] = 0.f;
 #pragma unroll
-      for (int m = 0; m < NM; ++m) s = mma(TL::row_frag(qtile, 32 * u + tile_row(li), m, half), k[m], s);
-#pragma unroll
       for (int m = 0; m < NM; ++m) dp = mma(TL::row_frag(gtile, 32 * u + tile_row(li), m, half), v[m], dp);
+#pragma unroll
+      for (int m = 0; m < NM; ++m) s = mma(TL::row_frag(qtile, 32 * u + tile_row(li), m, half), k[m], s);
       const int rows_left = D.Lq - q0 - 32 * u;
       if (rows_left < 32) {      // rows behind the last query: their bias was read from whatever lies in front of the expanded table
 #pragma unroll
@@ -437,31 +449,35 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
     }
 }
 
-// dvec[h][code_max + v] = sum over samples and query blocks of their strips
+// dvec[h][code_max + v] = sum over samples and query blocks of their strips; 64 offsets x 4 runs of blocks, joined in order
 __global__ __launch_bounds__(256) void mha_dvec_k(const BwdP P, float* dvec) {
+  __shared__ float red[4][64];
   const so_mha_desc& D = P.d;
-  const int i = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
-  if (i >= D.V) return;
-  const int v = i - D.code_max;
+  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6, i = blockIdx.x * 64 + tx, h = blockIdx.y, v = i - D.code_max;
   float x = 0.f;
-  for (int t = 0; t < P.qtiles; ++t) {
+  for (int t = ty; t < P.qtiles; t += 4) {
     const int ql = (128 * t + 128 < D.Lq ? 128 * t + 128 : D.Lq) - 1, at = v + D.code[D.q_start + ql];
-    if (at < 0 || at >= P.strip) continue;
-    for (int b = 0; b < D.B; ++b) x += D.strips[(((size_t)b * D.Hq + h) * P.qtiles + t) * P.strip + at];
+    if (i >= D.V || at < 0 || at >= P.strip) continue;
+    const float* p = D.strips + ((size_t)h * P.qtiles + t) * P.strip + at;
+#pragma unroll 4
+    for (int b = 0; b < D.B; ++b) x += p[(size_t)b * D.Hq * P.qtiles * P.strip];
   }
-  dvec[(size_t)h * D.V + i] = x;
+  red[ty][tx] = x;
+  __syncthreads();
+  if (ty == 0 && i < D.V) dvec[(size_t)h * D.V + i] = ((red[0][tx] + red[1][tx]) + red[2][tx]) + red[3][tx];
 }
 
-// dtable[r][h] = sum of dvec over the offsets of bucket r; one wave per entry
+// dtable[r][h] = sum of dvec over the offsets of bucket r; one block per entry
 __global__ __launch_bounds__(256) void mha_drow_k(const float* dvec, const int* order, const int* start, int rows, int H, int V,
                                                   float* dtable) {
-  const int lane = threadIdx.x & 63, i = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= rows * H) return;
-  const int r = i / H, h = i - r * H;
+  __shared__ float red[4];
+  const int r = blockIdx.x / H, h = blockIdx.x - r * H;
+  const float* dv = dvec + (size_t)h * V;
   float x = 0.f;
-  for (int j = start[r] + lane; j < start[r + 1]; j += 64) x += dvec[(size_t)h * V + order[j]];
-  x = so_wave_sum(x);
-  if (lane == 0) dtable[i] = x;
+#pragma unroll 4
+  for (int j = start[r] + threadIdx.x; j < start[r + 1]; j += 256) x += dv[order[j]];
+  x = so_block_sum256(x, red);
+  if (threadIdx.x == 0) dtable[blockIdx.x] = x;
 }
 
 constexpr int kLds = 160 * 1024;
@@ -478,7 +494,8 @@ int make(const so_mha_desc* d, BwdP& p) {
   if (d->strips) {
     if (!d->bias || d->width < 1) return SO_ERR_SHAPE;
     const int w = d->linear ? 1 : d->width;
-    // the offsets that one tile of keys can reach from the block's rows, and those of the tile before still being written out
+    // the offsets that one tile of keys can reach from the block's rows, and those of the tile before still being written out (256
+    // cover a sequence: 47 in front of the tile's first key, 128 rows behind it, 64 of the tile before)
     const int need = code_span(128, w) + code_span(BK, w) + code_span(BK + 1, w) + 1;
     p.ring = 256;
     while (p.ring < need) p.ring <<= 1;
@@ -556,10 +573,10 @@ int so_mha_dtable(const void* desc, const void* order, const void* start, int ro
   if (!d->strips || !order || !start || rows < 1 || !dvec || !dtable || d->Hq > 65535 || (long long)rows * d->Hq > 0x7fffff00LL)
     return SO_ERR_SHAPE;
   hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(mha_dvec_k, dim3((d->V + 255) / 256, d->Hq), dim3(256), 0, st, p, dvec);
+  hipLaunchKernelGGL(mha_dvec_k, dim3((d->V + 63) / 64, d->Hq), dim3(256), 0, st, p, dvec);
   int e = SO_LAUNCH_CHECK();
   if (e) return e;
-  hipLaunchKernelGGL(mha_drow_k, dim3((rows * d->Hq + 3) / 4), dim3(256), 0, st, dvec, (const int*)order, (const int*)start, rows, d->Hq,
+  hipLaunchKernelGGL(mha_drow_k, dim3(rows * d->Hq), dim3(256), 0, st, dvec, (const int*)order, (const int*)start, rows, d->Hq,
                      d->V, dtable);
   return SO_LAUNCH_CHECK();
 }

@@ -85,22 +85,12 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
     for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
   float m = -INFINITY, l = 0.f;
 
-  if (t0 < t1) fetch(t0, 0);
-  SO_DMA_DRAIN();
-  __syncthreads();
-  for (int t = t0; t < t1; ++t) {
-    const int st = STAGES == 2 ? (t - t0) & 1 : 0;
-    const char* kt = sm + st * 2 * TILE;
-    const char* vt = kt + TILE;
-    bits[0] = next[0];
-    bits[1] = next[1];
-    if (STAGES == 2 && t + 1 < t1) fetch(t + 1, st ^ 1);
-    // scores of this wave's keys
-    f32x16 s[SUBS];
-    float mx = -INFINITY;
+  // initial accumulators of tile t: the bias.  Requested in front of the wait that ends the tile before.
+  f32x16 s[SUBS];
+  auto init = [&](int t) {
 #pragma unroll
     for (int u = 0; u < SUBS; ++u) {
-      const int r0 = SPLIT ? 32 * wave : 32 * u, key0 = t * TK + r0;
+      const int key0 = t * TK + (SPLIT ? 32 * wave : 32 * u);
       if (bias) {
         if (D.linear) {
           const float* bp = bias + key0 + 16 * half;
@@ -123,6 +113,27 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
       }
+    }
+  };
+
+  if (t0 < t1) {
+    fetch(t0, 0);
+    init(t0);
+  }
+  SO_DMA_DRAIN();
+  __syncthreads();
+  for (int t = t0; t < t1; ++t) {
+    const int st = STAGES == 2 ? (t - t0) & 1 : 0;
+    const char* kt = sm + st * 2 * TILE;
+    const char* vt = kt + TILE;
+    bits[0] = next[0];
+    bits[1] = next[1];
+    if (STAGES == 2 && t + 1 < t1) fetch(t + 1, st ^ 1);
+    // scores of this wave's keys
+    float mx = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u) {
+      const int r0 = SPLIT ? 32 * wave : 32 * u;
 #pragma unroll
       for (int k = 0; k < NM; ++k) s[u] = mma(TL::row_frag(kt, r0 + tile_row(li), k, half), q[k], s[u]);
       const unsigned w = (unsigned)(bits[r0 >> 6] >> (r0 & 32));
@@ -174,6 +185,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
         }
       }
     }
+    if (t + 1 < t1) init(t + 1);
     if (STAGES == 1) {
       __syncthreads();
       if (t + 1 < t1) fetch(t + 1, 0);
@@ -270,18 +282,37 @@ __global__ __launch_bounds__(256) void mha_join_k(const FwdP P) {
   const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (at >= (long long)D.B * D.Hk * rows) return;
   const int bh = (int)(at / rows), row = (int)(at - (long long)bh * rows), b = bh / D.Hk, hk = bh - b * D.Hk;
+  // lane p holds the statistics of part p (and of p + 64, ...: at most 256)
   const float* ml = D.part_ml + 2 * at * P.parts;
-  float mn = -INFINITY, l = 0.f;
-  for (int p = 0; p < P.parts; ++p) mn = fmaxf(mn, ml[2 * p]);
-  const float ms = mn == -INFINITY ? 0.f : mn;
-  float x[2] = {0.f, 0.f};
-  for (int p = 0; p < P.parts; ++p) {
-    const float w = exp2_(ml[2 * p] - ms);
-    l += ml[2 * p + 1] * w;
-    const float* po = D.part_o + (at * P.parts + p) * D.D;
+  float mp[4], w[4], mn = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (lane + 64 * u < D.D) x[u] += po[lane + 64 * u] * w;
+  for (int i = 0; i < 4; ++i) {
+    const int p = lane + 64 * i;
+    mp[i] = p < P.parts ? ml[2 * p] : -INFINITY;
+    w[i] = p < P.parts ? ml[2 * p + 1] : 0.f;
+    mn = fmaxf(mn, mp[i]);
+  }
+  mn = so_wave_max(mn);
+  const float ms = mn == -INFINITY ? 0.f : mn;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    mp[i] = exp2_(mp[i] - ms);
+    l += w[i] * mp[i];
+  }
+  l = so_wave_sum(l);
+  float x[2] = {0.f, 0.f};
+  const float* po = D.part_o + at * P.parts * D.D;
+  const bool c0 = lane < D.D, c1 = lane + 64 < D.D;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int n = P.parts - 64 * i < 64 ? P.parts - 64 * i : 64;
+#pragma unroll 8
+    for (int p = 0; p < n; ++p) {
+      const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mp[i]), p));
+      const float* row = po + (size_t)(64 * i + p) * D.D;
+      x[0] += c0 ? row[lane] * f : 0.f;
+      x[1] += c1 ? row[lane + 64] * f : 0.f;
+    }
   }
   const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
   const int head = hk * G + row / D.Lq, qi = row % D.Lq;
