@@ -51,14 +51,19 @@ __device__ __forceinline__ int tile_row(int l) { return 16 * ((l >> 2) & 1) + 4 
 template <int N> struct Log2 { static constexpr int v = 1 + Log2<N / 2>::v; };
 template <> struct Log2<1> { static constexpr int v = 0; };
 
-// A tile of rows in LDS: DP channels of T per row as 16-byte chunks, chunk c of row r at position c ^ f(r).  Rows are a power of two
-// chunks long; f spreads the eight rows that one phase of a ds_read_b128 touches (4 n .. 4 n + 3 and the same 16 further) over all banks.
+// A tile of rows in LDS: DP channels of T per row as 16-byte chunks, chunk c of row r at position c ^ f(r); rows are a power of two
+// chunks long.  f makes both ways of reading free of bank conflicts (64 banks; 16 lanes of a ds_read_b128 go together, those whose lane
+// bits 2, 3, 4 have the same parity): in row_frag these 16 lanes hold all values of row bits 0 - 3, in col_frag four rows of row bits
+// 0 - 1 are read in four neighbouring chunks, and an fp32 dword read takes two rows 16 apart.
 template <typename T, int DP>
 struct Tile {
   static constexpr int E = Elem<T>::E, NC = DP / E;                      // chunks that hold data
   static constexpr int NP = NC <= 4 ? 4 : NC <= 8 ? 8 : NC <= 16 ? 16 : 32;   // chunks of a row in LDS
   static constexpr int kRowBytes = NP * 16;
-  __device__ static __forceinline__ int swz(int row) { return NP == 4 ? ((row >> 1) & 1) | ((row >> 3) & 2) : (row & 3) | ((row >> 2) & 4); }
+  __device__ static __forceinline__ int swz(int row) {
+    const int hi = (row >> 2) & 3;
+    return NP == 4 ? hi : NP == 8 ? hi | ((row & 2) << 1) : (hi | ((row & 3) << 2)) ^ ((row >> 1) & 8);
+  }
   __device__ static __forceinline__ int at(int row, int chunk) { return row * kRowBytes + ((chunk ^ swz(row)) << 4); }
 
   // A fragment "row, step m of the channel axis"
