@@ -166,6 +166,15 @@ struct Filler {
   }
 };
 
+// n dwords of global memory -> LDS, by LDS-DMA; wave w of `WAVES` takes the 64-dword pieces w, w + WAVES, ...  `bytes` bounds the source
+// (what lies behind arrives as zeros).  LDS is written in whole pieces.
+template <int WAVES>
+__device__ __forceinline__ void fill_dwords(void* dst, const void* src, int n, unsigned bytes, int wave, int lane) {
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(src), 0, (int)bytes, 0x00020000);
+  for (int i = 64 * wave; i < n; i += 64 * WAVES)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)((char*)dst + 4 * i), 4, 4 * (i + lane), 0, 0, 0);
+}
+
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
 
 // visible keys [64 w, 64 w + 64) of a sample as bits; keys behind the last are invisible
@@ -212,6 +221,28 @@ __device__ __forceinline__ void word_range(const unsigned long long* words, int 
 
 // 2^x for the softmax: v_exp_f32 (1 ulp); x <= 0 here up to rounding, results below 2^-126 vanish
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Block -> (sample, key head, block of that group).  A one-dimensional grid; XCD x = id % 8 gets the x-th contiguous eighth of an order
+// in which the blocks of a (sample, key head), which read the same keys and values, follow each other: they stay in that XCD's L2
+// (4 MB: 8192 keys and values of 128 bf16 channels).  The order goes through half of every group's blocks and then through the other
+// half, samples innermost, so that an XCD meets several samples of a ragged batch.
+struct BlockOf { int b, hk, idx; };
+__device__ __forceinline__ BlockOf block_of(int B, int Hk, int per) {
+  const unsigned total = gridDim.x, x = blockIdx.x & 7, each = total >> 3, rest = total & 7;
+  unsigned v = x * each + (x < rest ? x : rest) + (blockIdx.x >> 3);
+  const unsigned groups = B * Hk, first = (per + 1) >> 1;
+  unsigned g, idx;
+  if (v < groups * first) {
+    g = v / first;
+    idx = v - g * first;
+  } else {
+    v -= groups * first;
+    const unsigned second = per - first;
+    g = v / second;
+    idx = first + v - g * second;
+  }
+  return BlockOf{(int)(g % B), (int)(g / B), (int)idx};
+}
 
 }  // namespace mha
 

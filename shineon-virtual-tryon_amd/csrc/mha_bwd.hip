@@ -21,8 +21,8 @@ struct BwdP {
   so_mha_desc d;
   float c;            // scale * log2 e
   int ring, strip;    // floats of one LDS ring (a power of two) and of one block's strip
-  int stages, qtiles;
-  int per_wave;       // LDS rings of one wave: one for each half (sequences) or one (maps)
+  int stages, qtiles, ktiles;
+  int seg;            // floats of the bias that a tile of 64 and a block of 128 tokens can meet, in whole 64s
 };
 
 constexpr int BK = 64;          // keys (mha_dq_k) or query rows (mha_dkv_k) of a tile
@@ -94,17 +94,22 @@ __device__ __forceinline__ void rectangles(const f32x16& s, float* skew, float* 
   }
 }
 
-template <typename T, int DP>
+// BIAS: 0 none, 1 tokens of a sequence (offset = key - query), 2 tokens of a map.  Everything a tile needs travels by LDS-DMA: K, V,
+// the piece of the expanded bias that its offsets lie in and (maps) the keys' codes; nothing in the loop waits for global memory
+// except the one drain per tile.
+template <typename T, int DP, int BIAS>
 __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha_dq_k(const BwdP P) {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::frag frag;
   constexpr int E = Elem<T>::E, KM = 2 * E, NM = DP / KM, NT = DP / 32, NCS = 32 / KM;
   constexpr int TILE = BK * TL::kRowBytes;
-  extern __shared__ __attribute__((aligned(16))) char sm[];          // [stages][K tile | V tile] | [4 waves][2 halves][ring]
+  extern __shared__ __attribute__((aligned(16))) char sm[];          // [stages][K tile | V tile | bias | codes] | rings | skew
   const so_mha_desc& D = P.d;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
-  const int bh = (int)((blockIdx.x + blockIdx.y) % gridDim.x), b = bh / D.Hq, head = bh - b * D.Hq, hk = head / (D.Hq / D.Hk);
-  const int q0 = blockIdx.y * 128, qlast = (q0 + 128 < D.Lq ? q0 + 128 : D.Lq) - 1;
+  const int G = D.Hq / D.Hk;
+  const BlockOf blk = block_of(D.B, D.Hk, G * P.qtiles);
+  const int b = blk.b, hk = blk.hk, head = hk * G + blk.idx / P.qtiles, qtile = blk.idx % P.qtiles, bh = b * D.Hq + head;
+  const int q0 = qtile * 128, qlast = (q0 + 128 < D.Lq ? q0 + 128 : D.Lq) - 1;
   const int row = q0 + 32 * wave + li;
   const bool rowv = row < D.Lq;
   const int qi = rowv ? row : qlast;
@@ -138,37 +143,46 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
   const size_t stat = ((size_t)b * D.Hq + head) * D.Lq + qi;
   const float lse = rowv ? D.lse[stat] : INFINITY;
   if (rowv && half == 0) D.delta[stat] = delta;
-  const int cq = D.bias ? D.code[D.q_start + qi] : 0;
-  const float* bias = D.bias ? D.bias + (size_t)head * D.V + D.code_max - cq : nullptr;
+
+  // codes of the block's first and last row; the first offset of tile t's piece of the bias is code(first key) - code(last row).  In a
+  // sequence rows behind the last count as well.
+  const int STAGE = 2 * TILE + (BIAS ? 4 * (P.seg + (BIAS == 2 ? BK : 0)) : 0);
+  const int cqf = BIAS == 0 ? 0 : BIAS == 1 ? D.q_start + q0 : D.code[D.q_start + q0];
+  const int cql = BIAS == 0 ? 0 : BIAS == 1 ? D.q_start + qlast : D.code[D.q_start + qlast];
+  const int cqe = BIAS == 1 ? D.q_start + q0 + 127 : cql;
+  const int mine_q = BIAS == 0 ? 0 : BIAS == 1 ? cqe - (D.q_start + row) : cqe - D.code[D.q_start + qi];   // this lane's place in a piece
+  const float* bias = BIAS ? D.bias + (size_t)head * D.V + D.code_max - cqe : nullptr;
 
   // bias gradient: rings cleared, strip filled with zeros up to the first offset that the walk can reach
-  const bool want = D.strips != nullptr;
-  float* rings = reinterpret_cast<float*>(sm + P.stages * 2 * TILE);
-  float* mine = rings + wave * P.per_wave * P.ring;
-  float* skew = rings + 4 * P.per_wave * P.ring + wave * kSkew;      // maps only
+  constexpr int RINGS = BIAS == 1 ? 8 : 4;
+  const bool want = BIAS && D.strips != nullptr;
+  float* rings = reinterpret_cast<float*>(sm + P.stages * STAGE);
+  float* mine = rings + wave * (RINGS / 4) * P.ring;
+  float* skew = rings + RINGS * P.ring + wave * kSkew;               // maps only
   const int qw = D.q_start + q0 + 32 * wave;                         // first token of the wave's rows
   const int rmask = P.ring - 1;
-  const int cqf = D.bias ? D.code[D.q_start + q0] : 0, cql = D.bias ? D.code[D.q_start + qlast] : 0;
   const int v0 = -cql;                                                 // code[0] = 0
-  float* strip = want ? D.strips + ((size_t)bh * P.qtiles + blockIdx.y) * P.strip : nullptr;
+  float* strip = want ? D.strips + ((size_t)bh * P.qtiles + qtile) * P.strip : nullptr;
   int flushed = v0;
   if (want) {
-    for (int i = tid; i < 4 * P.per_wave * P.ring; i += 256) rings[i] = 0.f;
-    const int first = t0 < t1 ? D.code[t0 * BK] - cql : v0;
+    for (int i = tid; i < RINGS * P.ring; i += 256) rings[i] = 0.f;
+    const int first = t0 < t1 ? (BIAS == 1 ? t0 * BK : D.code[t0 * BK]) - cql : v0;
     for (int v = v0 + tid; v < first; v += 256) strip[v - v0] = 0.f;
     flushed = first;
   }
   float pend = 0.f;      // sequences: see diagonals()
   int base = 0;
-  auto flush = [&](int upto) {
-    for (int v = flushed + tid; v < upto; v += 256) {
-      float x = 0.f;
-      for (int r = 0; r < 4 * P.per_wave; ++r) {
-        float* at = rings + r * P.ring + (v & rmask);
-        x += *at;
-        *at = 0.f;
+  auto flush = [&](int upto, int turn) {      // one wave's worth at a time, another wave first every time
+    for (int v = flushed + ((tid + 64 * turn) & 255); v < upto; v += 256) {
+      float x[RINGS], sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < RINGS; ++r) x[r] = rings[r * P.ring + (v & rmask)];
+#pragma unroll
+      for (int r = 0; r < RINGS; ++r) {
+        sum += x[r];
+        rings[r * P.ring + (v & rmask)] = 0.f;
       }
-      strip[v - v0] = x;
+      strip[v - v0] = sum;
     }
     if (upto > flushed) flushed = upto;
   };
@@ -181,9 +195,15 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
   unsigned long long next = 0;
   auto fetch = [&](int t, int st) {
     next = kw.get(t);
-    char* kt = sm + st * 2 * TILE;
+    char* kt = sm + st * STAGE;
     fk.fill(kt, kb + (size_t)t * BK * D.skl, next, 0, wave_u);
     fv.fill(kt + TILE, vb + (size_t)t * BK * D.svl, next, 0, wave_u);
+    if constexpr (BIAS == 1) fill_dwords<4>(kt + 2 * TILE, bias + t * BK, BK + 127, 0x7FFFFFFFu, wave_u, lane);
+    if constexpr (BIAS == 2) {
+      const int c0 = D.code[t * BK];
+      fill_dwords<4>(kt + 2 * TILE, bias + c0, D.code[t * BK + BK - 1] - cqf - (c0 - cqe) + 1, 0x7FFFFFFFu, wave_u, lane);
+      fill_dwords<4>(kt + 2 * TILE + 4 * P.seg, D.code + t * BK, BK, 0x7FFFFFFFu, (wave_u + 1) & 3, lane);
+    }
   };
 
   f32x16 dq[NT];
@@ -196,34 +216,30 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
   __syncthreads();
   for (int t = t0; t < t1; ++t) {
     const int st = P.stages == 2 ? (t - t0) & 1 : 0;
-    const char* kt = sm + st * 2 * TILE;
+    const char* kt = sm + st * STAGE;
     const char* vt = kt + TILE;
+    const float* seg = reinterpret_cast<const float*>(kt + 2 * TILE);
+    const int* codes = reinterpret_cast<const int*>(seg + P.seg);
     const unsigned long long w64 = next;
     if (P.stages == 2 && t + 1 < t1) fetch(t + 1, st ^ 1);
     // offsets below those of this tile are final, and nothing adds to them any more (a sequence's rings are written up to the last
     // row's first key exclusively)
-    if (want && t > t0) flush(D.linear ? t * BK - D.q_start - q0 - 128 : D.code[t * BK] - cql);
+    if (want && t > t0) flush(BIAS == 1 ? t * BK - D.q_start - q0 - 128 : codes[0] - cql, t & 3);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int key0 = t * BK + 32 * u;
       f32x16 s, dp;
-      if (bias) {
-        if (D.linear) {
-          const float* bp = bias + key0 + 16 * half;
+      if constexpr (BIAS == 1) {
+        const float* at = seg + 32 * u + 16 * half + mine_q;
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const f32x4u v = *reinterpret_cast<const f32x4u*>(bp + 4 * g);
+        for (int r = 0; r < 16; ++r) s[r] = at[r];
+      } else if constexpr (BIAS == 2) {
+        const float* at = seg + mine_q - codes[0];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[4 * g + e] = v[e];
-          }
-        } else {
-          const int* cp = D.code + key0 + 16 * half;
+        for (int g = 0; g < 4; ++g) {
+          const i32x4 c = *reinterpret_cast<const i32x4*>(codes + 32 * u + 16 * half + 4 * g);
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const i32x4 v = *reinterpret_cast<const i32x4*>(cp + 4 * g);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[4 * g + e] = bias[v[e]];
-          }
+          for (int e = 0; e < 4; ++e) s[4 * g + e] = at[c[e]];
         }
       } else {
 #pragma unroll
@@ -231,7 +247,6 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] = 0.f;
-      // do v^T first: it needs nothing from global memory and hides the latency of the bias
 #pragma unroll
       for (int k = 0; k < NM; ++k) dp = mma(TL::row_frag(vt, 32 * u + tile_row(li), k, half), go[k], dp);
 #pragma unroll
@@ -244,13 +259,14 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = (my >> r) & 1 ? s[r] : 0.f;
       }
-      if (want) {
-        if (D.linear) {
+      if constexpr (BIAS == 1) {
+        if (want) {
           base = key0 + 16 * half - qw;
           mine[half * P.ring + ((base - 1 - li) & rmask)] = diagonals(s, pend, li);
-        } else {
-          rectangles(s, skew, mine, rmask, key0, qw, D.width, lane);
         }
+      }
+      if constexpr (BIAS == 2) {
+        if (want) rectangles(s, skew, mine, rmask, key0, qw, D.width, lane);
       }
 #pragma unroll
       for (int c = 0; c < NCS; ++c) {
@@ -269,12 +285,12 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
   }
   if (want) {
     if (t0 < t1) {
-      if (D.linear) {
+      if constexpr (BIAS == 1) {
         if (li >= 16) mine[half * P.ring + ((base + 31 - li) & rmask)] = pend;
         __syncthreads();
       }
       const int kl = (t1 * BK < D.Lk ? t1 * BK : D.Lk) - 1;
-      flush(D.code[kl] - cqf + 1);
+      flush((BIAS == 1 ? kl : D.code[kl]) - cqf + 1, 0);
     }
     for (int v = flushed + tid; v < v0 + P.strip; v += 256) strip[v - v0] = 0.f;
   }
@@ -295,20 +311,22 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
     }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int BIAS>
 __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha_dkv_k(const BwdP P) {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::frag frag;
   constexpr int E = Elem<T>::E, KM = 2 * E, NM = DP / KM, NT = DP / 32, NCS = 32 / KM;
   constexpr int TILE = BK * TL::kRowBytes;
-  extern __shared__ __attribute__((aligned(16))) char sm[];          // [2][Q tile | dO tile | lse | delta]
-  constexpr int STAGE = 2 * TILE + 2 * BK * 4;
+  extern __shared__ __attribute__((aligned(16))) char sm[];          // [stages][Q tile | dO tile | lse | delta | bias | codes]
+  const int STAGE = 2 * TILE + 2 * BK * 4 + (BIAS ? 4 * (P.seg + (BIAS == 2 ? BK : 0)) : 0);
   const so_mha_desc& D = P.d;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
-  const int bh = (int)((blockIdx.x + blockIdx.y) % gridDim.x), b = bh / D.Hk, hk = bh - b * D.Hk, G = D.Hq / D.Hk;
-  const int key = blockIdx.y * 128 + 32 * wave + li;
+  const int G = D.Hq / D.Hk;
+  // samples and heads in turn: the blocks behind a short sample's last key have nothing to do and are spread over all XCDs
+  const int bh = (int)(blockIdx.x % (unsigned)(D.B * D.Hk)), kt = (int)(blockIdx.x / (unsigned)(D.B * D.Hk)), b = bh / D.Hk, hk = bh - b * D.Hk;
+  const int key = kt * 128 + 32 * wave + li;
   const unsigned long long* words = D.words ? (const unsigned long long*)D.words + (size_t)b * D.nwords : nullptr;
-  const int w0 = 2 * blockIdx.y;
+  const int w0 = 2 * kt;
   const unsigned long long wa = tail_word(w0, D.Lk) & (words ? words[w0] : ~0ULL);
   const unsigned long long wb = w0 + 1 < D.nwords ? tail_word(w0 + 1, D.Lk) & (words ? words[w0 + 1] : ~0ULL) : 0ULL;
   const bool keyv = key < D.Lk, vis = ((wave < 2 ? wa : wb) >> (key & 63)) & 1;
@@ -324,26 +342,30 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
       v[m] = as_frag<T>(load_chunk<T>(vr, ch, vis && ch * E < D.D));
     }
   }
-  const float* bias0 = D.bias ? D.bias + D.code_max + D.code[keyv ? key : D.Lk - 1] : nullptr;
+  // first key's and last key's codes; the first offset of a tile's piece of the bias is code(first key) - code(last row of the tile)
+  const int ckf = BIAS == 2 ? D.code[kt * 128] : kt * 128, ckl = BIAS == 2 ? D.code[kt * 128 + 127] : kt * 128 + 127;
+  const int mine_k = BIAS == 2 ? D.code[key] - ckf : 32 * wave + li;
 
   const int qt = (D.Lq + BK - 1) / BK, n = (wa | wb) ? G * qt : 0;    // a block without a visible key writes zeros
   const int wave_u = __builtin_amdgcn_readfirstlane(wave);
   const Filler<T, DP, BK, 4> fq(D.D, (unsigned)(D.sql * sizeof(T)), tid), fg(D.D, (unsigned)((size_t)D.Hq * D.D * sizeof(T)), tid);
-  float sreg = 0.f;
   auto fetch = [&](int t, int st) {
     const int head = hk * G + t / qt, q0 = (t % qt) * BK;
     const unsigned long long rows = tail_word(t % qt, D.Lq);
     char* qtile = sm + st * STAGE;
     fq.fill(qtile, (const T*)D.q + (size_t)b * D.sqb + (size_t)head * D.sqh + (size_t)q0 * D.sql, rows, 0, wave_u);
     fg.fill(qtile + TILE, (const T*)D.dout + (((size_t)b * D.Lq + q0) * D.Hq + head) * D.D, rows, 0, wave_u);
-    if (tid < 2 * BK) {
-      const int i = q0 + (tid & (BK - 1));
-      const float* src = (tid < BK ? D.lse : D.delta) + ((size_t)b * D.Hq + head) * D.Lq;
-      sreg = i < D.Lq ? src[i] : tid < BK ? INFINITY : 0.f;
+    char* stats = qtile + 2 * TILE;
+    const size_t at = ((size_t)b * D.Hq + head) * D.Lq + q0;
+    const unsigned left = D.Lq - q0 < BK ? 4 * (D.Lq - q0) : 4 * BK;
+    fill_dwords<4>(stats, D.lse + at, BK, left, wave_u, lane);
+    fill_dwords<4>(stats + 4 * BK, D.delta + at, BK, left, (wave_u + 1) & 3, lane);
+    if constexpr (BIAS != 0) {
+      const int* cp = D.code + D.q_start + q0;
+      const int cl = BIAS == 2 ? cp[BK - 1] : D.q_start + q0 + BK - 1, n = BIAS == 2 ? ckl - cp[0] - (ckf - cl) + 1 : 128 + BK - 1;
+      fill_dwords<4>(stats + 8 * BK, D.bias + (size_t)head * D.V + D.code_max + ckf - cl, n, 0x7FFFFFFFu, (wave_u + 2) & 3, lane);
+      if constexpr (BIAS == 2) fill_dwords<4>(stats + 8 * BK + 4 * P.seg, cp, BK, 0x7FFFFFFFu, (wave_u + 3) & 3, lane);
     }
-  };
-  auto store = [&](int st) {
-    if (tid < 2 * BK) reinterpret_cast<float*>(sm + st * STAGE + 2 * TILE)[tid] = sreg;
   };
 
   f32x16 dk[NT], dv[NT];
@@ -351,10 +373,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[t][r] = dv[t][r] = 0.f;
-  if (n) {
-    fetch(0, 0);
-    store(0);
-  }
+  if (n) fetch(0, 0);
   SO_DMA_DRAIN();
   __syncthreads();
   for (int t = 0; t < n; ++t) {
@@ -363,24 +382,23 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
     const char* gtile = qtile + TILE;
     const float* stats = reinterpret_cast<const float*>(qtile + 2 * TILE);
     if (P.stages == 2 && t + 1 < n) fetch(t + 1, st ^ 1);
-    const int head = hk * G + t / qt, q0 = (t % qt) * BK;
+    const int q0 = (t % qt) * BK;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       f32x16 s, dp;
-      if (bias0) {
-        const float* bias = bias0 + (size_t)head * D.V;
-        if (D.linear) {      // consecutive rows are floats downwards
-          const float* bp = bias - (D.q_start + q0 + 32 * u + 16 * half) - 3;
+      const int r0 = 32 * u + 16 * half;
+      if constexpr (BIAS == 1) {
+        const float* at = stats + 2 * BK + mine_k + BK - 1 - r0;
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const f32x4u x = *reinterpret_cast<const f32x4u*>(bp - 4 * g);
+        for (int r = 0; r < 16; ++r) s[r] = at[-r];
+      } else if constexpr (BIAS == 2) {
+        const int* codes = reinterpret_cast<const int*>(stats + 2 * BK + P.seg);
+        const float* at = stats + 2 * BK + mine_k + codes[BK - 1];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[4 * g + e] = x[3 - e];
-          }
-        } else {
-          const int* cp = D.code + D.q_start + q0 + 32 * u + 16 * half;
+        for (int g = 0; g < 4; ++g) {
+          const i32x4 c = *reinterpret_cast<const i32x4*>(codes + r0 + 4 * g);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = bias[-cp[r]];
+          for (int e = 0; e < 4; ++e) s[4 * g + e] = at[-c[e]];
         }
       } else {
 #pragma unroll
@@ -424,7 +442,6 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
       __syncthreads();
       if (t + 1 < n) fetch(t + 1, 0);
     }
-    if (t + 1 < n) store(P.stages == 2 ? st ^ 1 : 0);
     SO_DMA_DRAIN();
     __syncthreads();
   }
@@ -489,10 +506,16 @@ int make(const so_mha_desc* d, BwdP& p) {
   p.d = *d;
   p.c = d->scale * kLog2e;
   p.qtiles = (d->Lq + 127) / 128;
+  p.ktiles = (d->Lk + 127) / 128;
   p.stages = 2;
-  p.per_wave = d->linear ? 2 : 1;
+  if (d->bias) {
+    if (d->width < 1) return SO_ERR_SHAPE;
+    const int w = d->linear ? 1 : d->width;
+    p.seg = (code_span(128, w) + code_span(BK, w) + 1 + 63) / 64 * 64;
+    if (p.seg > 2048) return SO_ERR_SHAPE;
+  }
   if (d->strips) {
-    if (!d->bias || d->width < 1) return SO_ERR_SHAPE;
+    if (!d->bias) return SO_ERR_SHAPE;
     const int w = d->linear ? 1 : d->width;
     // the offsets that one tile of keys can reach from the block's rows, and those of the tile before still being written out (256
     // cover a sequence: 47 in front of the tile's first key, 128 rows behind it, 64 of the tile before)
@@ -512,33 +535,39 @@ int lds_limit(K k, size_t lds) {
   return (int)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int BIAS>
 int launch(BwdP p, hipStream_t st) {
   typedef Tile<T, DP> TL;
   constexpr size_t tile = (size_t)BK * TL::kRowBytes;
-  const size_t rings = p.d.strips ? ((size_t)4 * p.per_wave * p.ring + (p.d.linear ? 0 : 4 * kSkew)) * 4 : 0;
-  p.stages = 4 * tile + rings <= kLds ? 2 : 1;
-  size_t lds = p.stages * 2 * tile + rings;
+  const size_t piece = BIAS ? 4 * (size_t)(p.seg + (BIAS == 2 ? BK : 0)) : 0;
+  const size_t rings = p.d.strips ? ((size_t)(BIAS == 1 ? 8 : 4) * p.ring + (BIAS == 2 ? 4 * kSkew : 0)) * 4 : 0;
+  size_t stage = 2 * tile + piece;
+  p.stages = 2 * stage + rings <= kLds ? 2 : 1;
+  size_t lds = p.stages * stage + rings;
   if (lds > kLds) return SO_ERR_SHAPE;
-  int err = lds_limit(mha_dq_k<T, DP>, lds);
+  int err = lds_limit(mha_dq_k<T, DP, BIAS>, lds);
   if (err) return err;
-  hipLaunchKernelGGL((mha_dq_k<T, DP>), dim3(p.d.B * p.d.Hq, p.qtiles), dim3(256), lds, st, p);
+  hipLaunchKernelGGL((mha_dq_k<T, DP, BIAS>), dim3((unsigned)((long long)p.d.B * p.d.Hq * p.qtiles)), dim3(256), lds, st, p);
   err = SO_LAUNCH_CHECK();
   if (err) return err;
-  constexpr size_t stage = 2 * tile + 2 * BK * 4;
+  stage = 2 * tile + 2 * BK * 4 + piece;
   p.stages = 2 * stage <= kLds ? 2 : 1;
   lds = p.stages * stage;
-  err = lds_limit(mha_dkv_k<T, DP>, lds);
+  err = lds_limit(mha_dkv_k<T, DP, BIAS>, lds);
   if (err) return err;
-  hipLaunchKernelGGL((mha_dkv_k<T, DP>), dim3(p.d.B * p.d.Hk, (p.d.Lk + 127) / 128), dim3(256), lds, st, p);
+  hipLaunchKernelGGL((mha_dkv_k<T, DP, BIAS>), dim3((unsigned)((long long)p.d.B * p.d.Hk * p.ktiles)), dim3(256), lds, st, p);
   return SO_LAUNCH_CHECK();
+}
+template <typename T, int DP>
+int launch_b(const BwdP& p, hipStream_t st) {
+  return !p.d.bias ? launch<T, DP, 0>(p, st) : p.d.linear ? launch<T, DP, 1>(p, st) : launch<T, DP, 2>(p, st);
 }
 template <typename T>
 int launch_d(const BwdP& p, hipStream_t st) {
-  if (p.d.D <= 32) return launch<T, 32>(p, st);
-  if (p.d.D <= 64) return launch<T, 64>(p, st);
-  if (p.d.D <= 96) return launch<T, 96>(p, st);
-  return launch<T, 128>(p, st);
+  if (p.d.D <= 32) return launch_b<T, 32>(p, st);
+  if (p.d.D <= 64) return launch_b<T, 64>(p, st);
+  if (p.d.D <= 96) return launch_b<T, 96>(p, st);
+  return launch_b<T, 128>(p, st);
 }
 
 }  // namespace
@@ -561,7 +590,7 @@ int so_mha_bwd(const void* desc, void* stream) {
   if (err) return err;
   if (!d->q || !d->k || !d->v || !d->o || !d->dout || !d->dq || !d->dk || !d->dv || !d->lse || !d->delta) return SO_ERR_SHAPE;
   if ((((uintptr_t)d->dout) | ((uintptr_t)d->dq) | ((uintptr_t)d->dk) | ((uintptr_t)d->dv)) & 15) return SO_ERR_ALIGN;
-  if ((long long)d->B * d->Hq > 0x7fffffffLL || p.qtiles > 65535) return SO_ERR_SHAPE;
+  if ((long long)d->B * d->Hq * p.qtiles > 0x7fffffffLL || (long long)d->B * d->Hk * p.ktiles > 0x7fffffffLL) return SO_ERR_SHAPE;
   return d->dtype == SO_F32 ? launch_d<float>(p, (hipStream_t)stream) : launch_d<__bf16>(p, (hipStream_t)stream);
 }
 

@@ -23,7 +23,7 @@ namespace {
 
 struct FwdP {
   so_mha_desc d;
-  int parts, tiles_per_part, tile_keys;
+  int parts, row_tiles;
   float c;              // scale * log2 e
 };
 
@@ -37,9 +37,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
   extern __shared__ __attribute__((aligned(16))) char sm[];         // [STAGES][K tile | V tile]
   const so_mha_desc& D = P.d;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
-  const int bh = (int)((blockIdx.x + blockIdx.y) % gridDim.x), b = bh / D.Hk, hk = bh - b * D.Hk, G = D.Hq / D.Hk, part = blockIdx.z;
-  const int rows = G * D.Lq;
-  const int row = blockIdx.y * (SPLIT ? 32 : 128) + (SPLIT ? 0 : 32 * wave) + li;
+  const int G = D.Hq / D.Hk, rows = G * D.Lq;
+  const BlockOf blk = block_of(D.B, D.Hk, P.row_tiles * P.parts);
+  const int b = blk.b, hk = blk.hk, part = blk.idx / P.row_tiles, tile = blk.idx - part * P.row_tiles, bh = b * D.Hk + hk;
+  const int row = tile * (SPLIT ? 32 : 128) + (SPLIT ? 0 : 32 * wave) + li;
   const bool rowv = row < rows;
   const int head = hk * G + (rowv ? row / D.Lq : 0), qi = rowv ? row % D.Lq : 0;
 
@@ -366,13 +367,13 @@ int launch(const FwdP& p, hipStream_t st) {
   constexpr int TK = SPLIT ? 128 : 64, TILE = TK * TL::kRowBytes, STAGES = 4 * TILE <= 150 * 1024 ? 2 : 1;
   constexpr int merge = (256 + 32 * (DP + 1)) * 4;
   constexpr int lds = SPLIT && merge > STAGES * 2 * TILE ? merge : STAGES * 2 * TILE;
-  const int rows = p.d.Hq / p.d.Hk * p.d.Lq, per = SPLIT ? 32 : 128;
+  
   auto k = mha_fwd_k<T, DP, SPLIT, TWO>;
   if (lds > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return (int)e;
   }
-  hipLaunchKernelGGL(k, dim3(p.d.B * p.d.Hk, (rows + per - 1) / per, p.parts), dim3(256), lds, st, p);
+  hipLaunchKernelGGL(k, dim3((unsigned)((long long)p.d.B * p.d.Hk * p.row_tiles * p.parts)), dim3(256), lds, st, p);
   return SO_LAUNCH_CHECK();
 }
 template <typename T, int DP>
@@ -397,7 +398,6 @@ int so_mha_check(const so_mha_desc* d) {
   if (!d || (d->dtype != SO_F32 && d->dtype != SO_BF16)) return SO_ERR_SHAPE;
   if (d->B < 1 || d->Hq < 1 || d->Hk < 1 || d->Hq % d->Hk || d->Lq < 1 || d->Lk < 1 || d->D < 1 || d->D > 128) return SO_ERR_SHAPE;
   if ((long long)d->B * d->Hk > 0x7fffffffLL || (long long)(d->Hq / d->Hk) * d->Lq > 0x7fffff00LL || d->Lk > 0x7fffff00) return SO_ERR_SHAPE;
-  if (((long long)(d->Hq / d->Hk) * d->Lq + 127) / 128 > 65535 || ((long long)d->Lk + 127) / 128 > 65535) return SO_ERR_SHAPE;   // grid.y
   if (!(d->scale > 0.f) || d->nwords != (d->Lk + 63) / 64) return SO_ERR_SHAPE;
   const int E = d->dtype == SO_F32 ? 4 : 8;
   if (d->D % E) return SO_ERR_ALIGN;
@@ -460,6 +460,8 @@ int so_mha_fwd(const void* desc, void* stream) {
   p.c = d->scale * kLog2e;
   const int rows = d->Hq / d->Hk * d->Lq;
   const bool split = rows <= 32;
+  p.row_tiles = split ? 1 : (rows + 127) / 128;
+  if ((long long)d->B * d->Hk * p.row_tiles * parts > 0x7fffffffLL) return SO_ERR_SHAPE;
   hipStream_t st = (hipStream_t)stream;
   int err = d->dtype == SO_F32 ? launch_d<float>(p, split, st) : launch_d<__bf16>(p, split, st);
   if (err || parts == 1) return err;
