@@ -65,43 +65,48 @@ struct Tile {
     return NP == 4 ? hi : NP == 8 ? hi | ((row & 2) << 1) : (hi | ((row & 3) << 2)) ^ ((row >> 1) & 8);
   }
   __device__ static __forceinline__ int at(int row, int chunk) { return row * kRowBytes + ((chunk ^ swz(row)) << 4); }
-
-  // A fragment "row, step m of the channel axis"
-  __device__ static __forceinline__ typename Elem<T>::frag row_frag(const char* t, int row, int m, int half) {
-    return *reinterpret_cast<const typename Elem<T>::frag*>(t + at(row, 2 * m + half));
-  }
 };
 
-// A fragment "column 32 t + lane, step c of the ROW axis" of the 32 rows from row0
-template <int DP>
-__device__ __forceinline__ f32x4 col_frag_f32(const char* tile, int row0, int t, int c, int lane) {
-  typedef Tile<float, DP> TL;
-  const int half = lane >> 5, col = 32 * t + (lane & 31);
-  f32x4 f;
+// Fragment addresses.  The swizzle is an XOR of address bits, so every fragment of a tile is (lane's base ^ constant) + constant.  The base
+// is made opaque at every use: otherwise hipcc keeps the two dozen addresses of a tile in registers over the whole loop, and spills.
+__device__ __forceinline__ int opaque(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+template <typename T, int DP>
+struct Reader {
+  typedef Tile<T, DP> TL;
+  typedef typename Elem<T>::frag frag;
+  const char* sm;
+  int rows, cols;      // bases of the lane's row and column fragments in a tile at sm
+  __device__ __forceinline__ Reader(const char* sm, int lane) : sm(sm) {
+    const int half = lane >> 5, li = lane & 31;
+    rows = TL::at(tile_row(li), half);
+    if constexpr (sizeof(T) == 4) cols = TL::at(16 * half, li >> 2) + 4 * (li & 3);
+    else cols = TL::at(16 * half + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 8 * (lane & 1);
+  }
+  // A fragment: row tile_row(lane) of the 32 rows at byte `at` of a tile, step m of the channel axis
+  __device__ __forceinline__ frag row(int base, int m, int at) const {
+    return *reinterpret_cast<const frag*>(sm + ((base ^ (m << 5)) + at));
+  }
+  // A fragment: column 32 t + lane, step c of the row axis of the 32 rows at byte `at`
+  __device__ __forceinline__ frag col(int base, int t, int c, int at) const {
+    if constexpr (sizeof(T) == 4) {
+      frag f;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int row = row0 + 16 * half + 4 * c + e;
-    f[e] = *reinterpret_cast<const float*>(tile + TL::at(row, col >> 2) + 4 * (col & 3));
+      for (int e = 0; e < 4; ++e)
+        f[e] = *reinterpret_cast<const float*>(sm + ((base ^ (((8 * t) ^ TL::swz(4 * c + e)) << 4)) + at + (4 * c + e) * TL::kRowBytes));
+      return f;
+    } else {
+      typedef __attribute__((address_space(3))) s16x4* lds_p;
+      union { s16x4 s[2]; frag f; } u;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        u.s[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_p)(sm + ((base ^ (((4 * t) ^ TL::swz(8 * c + 4 * i)) << 4)) + at + (8 * c + 4 * i) * TL::kRowBytes)));
+      return u.f;
+    }
   }
-  return f;
-}
-template <int DP>
-__device__ __forceinline__ bf16x8 col_frag_bf16(const char* tile, int row0, int t, int c, int lane) {
-  typedef Tile<__bf16, DP> TL;
-  const int half = lane >> 5, row = row0 + 16 * half + 8 * c + ((lane & 15) >> 2);
-  const int chunk = 4 * t + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), in = 8 * (lane & 1);
-  typedef __attribute__((address_space(3))) s16x4* lds_p;
-  union { s16x4 s[2]; bf16x8 f; } u;
-  u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(tile + TL::at(row, chunk) + in));
-  u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(tile + TL::at(row + 4, chunk) + in));
-  return u.f;
-}
-template <typename T, int DP> struct ColFrag;
-template <int DP> struct ColFrag<float, DP> {
-  __device__ static __forceinline__ f32x4 get(const char* t, int r0, int tt, int c, int lane) { return col_frag_f32<DP>(t, r0, tt, c, lane); }
-};
-template <int DP> struct ColFrag<__bf16, DP> {
-  __device__ static __forceinline__ bf16x8 get(const char* t, int r0, int tt, int c, int lane) { return col_frag_bf16<DP>(t, r0, tt, c, lane); }
 };
 
 // accumulator registers of step c as a B fragment; bf16 rounds here (half a step, 2^-8 of the value: the products run at the rate of
@@ -113,6 +118,24 @@ __device__ __forceinline__ void to_frag(const f32x16& a, int c, f32x4& f) {
 __device__ __forceinline__ void to_frag(const f32x16& a, int c, bf16x8& f) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) f[e] = (__bf16)a[8 * c + e];
+}
+
+// One product phase of N steps: step m multiplies with the fragment that was requested N steps ago and requests the one for step m of
+// the next phase into its place.  The order is pinned (sched_barrier): left to itself hipcc reads each fragment right before its MFMA and
+// exposes the LDS latency at every step.
+template <int N, typename F, typename Use, typename Next>
+__device__ __forceinline__ void phase(F (&buf)[N], Use use, Next next) {
+#pragma unroll
+  for (int m = 0; m < N; ++m) {
+    use(m, buf[m]);
+    buf[m] = next(m);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+template <int N, typename F, typename Use>
+__device__ __forceinline__ void last_phase(F (&buf)[N], Use use) {
+#pragma unroll
+  for (int m = 0; m < N; ++m) use(m, buf[m]);
 }
 
 // 16-byte chunk of a row in global memory, zero when `on` is false (the address is then not formed)

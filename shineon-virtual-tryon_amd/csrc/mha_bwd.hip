@@ -21,7 +21,7 @@ struct BwdP {
   so_mha_desc d;
   float c;            // scale * log2 e
   int ring, strip;    // floats of one LDS ring (a power of two) and of one block's strip
-  int stages, qtiles, ktiles;
+  int stages, stage_bytes, qtiles, ktiles;
   int seg;            // floats of the bias that a tile of 64 and a block of 128 tokens can meet, in whole 64s
 };
 
@@ -146,7 +146,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
 
   // codes of the block's first and last row; the first offset of tile t's piece of the bias is code(first key) - code(last row).  In a
   // sequence rows behind the last count as well.
-  const int STAGE = 2 * TILE + (BIAS ? 4 * (P.seg + (BIAS == 2 ? BK : 0)) : 0);
+  const int STAGE = P.stage_bytes;
+  const Reader<T, DP> rd(sm, lane);
+  constexpr int HALF = 32 * TL::kRowBytes;      // the second 32 rows of a tile
   const int cqf = BIAS == 0 ? 0 : BIAS == 1 ? D.q_start + q0 : D.code[D.q_start + q0];
   const int cql = BIAS == 0 ? 0 : BIAS == 1 ? D.q_start + qlast : D.code[D.q_start + qlast];
   const int cqe = BIAS == 1 ? D.q_start + q0 + 127 : cql;
@@ -206,6 +208,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
     }
   };
 
+  frag f[NM];      // NM = NT * NCS: every phase of a piece has as many steps
   f32x16 dq[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
@@ -217,7 +220,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
   for (int t = t0; t < t1; ++t) {
     const int st = P.stages == 2 ? (t - t0) & 1 : 0;
     const char* kt = sm + st * STAGE;
-    const char* vt = kt + TILE;
+    const int rows = rd.rows + st * STAGE, cols = rd.cols + st * STAGE;
     const float* seg = reinterpret_cast<const float*>(kt + 2 * TILE);
     const int* codes = reinterpret_cast<const int*>(seg + P.seg);
     const unsigned long long w64 = next;
@@ -247,10 +250,20 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] = 0.f;
+      if (u == 0) {
+        const int rb = opaque(rows);
 #pragma unroll
-      for (int k = 0; k < NM; ++k) dp = mma(TL::row_frag(vt, 32 * u + tile_row(li), k, half), go[k], dp);
-#pragma unroll
-      for (int k = 0; k < NM; ++k) s = mma(TL::row_frag(kt, 32 * u + tile_row(li), k, half), q[k], s);
+        for (int m = 0; m < NM; ++m) f[m] = rd.row(rb, m, TILE);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      {
+        const int rb = opaque(rows);
+        phase(f, [&](int m, const frag& a) { dp = mma(a, go[m], dp); }, [&](int m) { return rd.row(rb, m, HALF * u); });
+      }
+      {
+        const int cb = opaque(cols);
+        phase(f, [&](int m, const frag& a) { s = mma(a, q[m], s); }, [&](int m) { return rd.col(cb, m % NT, m / NT, HALF * u); });
+      }
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = exp2_(__builtin_fmaf(s[r], P.c, -lse)) * (dp[r] - delta);      // dS
       const unsigned w = (unsigned)(w64 >> (32 * u));
@@ -268,12 +281,15 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
       if constexpr (BIAS == 2) {
         if (want) rectangles(s, skew, mine, rmask, key0, qw, D.width, lane);
       }
+      frag g[NCS];
 #pragma unroll
-      for (int c = 0; c < NCS; ++c) {
-        frag f;
-        to_frag(s, c, f);
-#pragma unroll
-        for (int v = 0; v < NT; ++v) dq[v] = mma(ColFrag<T, DP>::get(kt, 32 * u, v, c, lane), f, dq[v]);
+      for (int c = 0; c < NCS; ++c) to_frag(s, c, g[c]);
+      const auto use = [&](int m, const frag& a) { dq[m % NT] = mma(a, g[m / NT], dq[m % NT]); };
+      if (u == 0) {
+        const int rb = opaque(rows);
+        phase(f, use, [&](int m) { return rd.row(rb, m, TILE + HALF); });
+      } else {
+        last_phase(f, use);
       }
     }
     if (P.stages == 1) {
@@ -318,10 +334,12 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
   constexpr int E = Elem<T>::E, KM = 2 * E, NM = DP / KM, NT = DP / 32, NCS = 32 / KM;
   constexpr int TILE = BK * TL::kRowBytes;
   extern __shared__ __attribute__((aligned(16))) char sm[];          // [stages][Q tile | dO tile | lse | delta | bias | codes]
-  const int STAGE = 2 * TILE + 2 * BK * 4 + (BIAS ? 4 * (P.seg + (BIAS == 2 ? BK : 0)) : 0);
   const so_mha_desc& D = P.d;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
   const int G = D.Hq / D.Hk;
+  const int STAGE = P.stage_bytes;
+  const Reader<T, DP> rd(sm, lane);
+  constexpr int HALF = 32 * TL::kRowBytes;
   // samples and heads in turn: the blocks behind a short sample's last key have nothing to do and are spread over all XCDs
   const int bh = (int)(blockIdx.x % (unsigned)(D.B * D.Hk)), kt = (int)(blockIdx.x / (unsigned)(D.B * D.Hk)), b = bh / D.Hk, hk = bh - b * D.Hk;
   const int key = kt * 128 + 32 * wave + li;
@@ -368,6 +386,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
     }
   };
 
+  frag f[NM];
   f32x16 dk[NT], dv[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
@@ -379,7 +398,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
   for (int t = 0; t < n; ++t) {
     const int st = P.stages == 2 ? t & 1 : 0;
     const char* qtile = sm + st * STAGE;
-    const char* gtile = qtile + TILE;
+    const int rows = rd.rows + st * STAGE, cols = rd.cols + st * STAGE;
     const float* stats = reinterpret_cast<const float*>(qtile + 2 * TILE);
     if (P.stages == 2 && t + 1 < n) fetch(t + 1, st ^ 1);
     const int q0 = (t % qt) * BK;
@@ -406,10 +425,20 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] = 0.f;
+      if (u == 0) {
+        const int rb = opaque(rows);
 #pragma unroll
-      for (int m = 0; m < NM; ++m) dp = mma(TL::row_frag(gtile, 32 * u + tile_row(li), m, half), v[m], dp);
-#pragma unroll
-      for (int m = 0; m < NM; ++m) s = mma(TL::row_frag(qtile, 32 * u + tile_row(li), m, half), k[m], s);
+        for (int m = 0; m < NM; ++m) f[m] = rd.row(rb, m, TILE);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      {
+        const int rb = opaque(rows);
+        phase(f, [&](int m, const frag& a) { dp = mma(a, v[m], dp); }, [&](int m) { return rd.row(rb, m, HALF * u); });
+      }
+      {
+        const int cb = opaque(cols);
+        phase(f, [&](int m, const frag& a) { s = mma(a, k[m], s); }, [&](int m) { return rd.col(cb, m % NT, m / NT, TILE + HALF * u); });
+      }
       const int rows_left = D.Lq - q0 - 32 * u;
       if (rows_left < 32) {      // rows behind the last query: their bias was read from whatever lies in front of the expanded table
 #pragma unroll
@@ -426,16 +455,22 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
           dp[r] = s[r] * (dp[r] - de[e]);
         }
       }
+      frag g[NCS];
 #pragma unroll
-      for (int c = 0; c < NCS; ++c) {
-        frag f, g;
-        to_frag(s, c, f);
-        to_frag(dp, c, g);
+      for (int c = 0; c < NCS; ++c) to_frag(s, c, g[c]);
+      {
+        const int cb = opaque(cols);
+        phase(f, [&](int m, const frag& a) { dv[m % NT] = mma(a, g[m / NT], dv[m % NT]); },
+              [&](int m) { return rd.col(cb, m % NT, m / NT, HALF * u); });
+      }
 #pragma unroll
-        for (int x = 0; x < NT; ++x) {
-          dv[x] = mma(ColFrag<T, DP>::get(gtile, 32 * u, x, c, lane), f, dv[x]);
-          dk[x] = mma(ColFrag<T, DP>::get(qtile, 32 * u, x, c, lane), g, dk[x]);
-        }
+      for (int c = 0; c < NCS; ++c) to_frag(dp, c, g[c]);
+      const auto use = [&](int m, const frag& a) { dk[m % NT] = mma(a, g[m / NT], dk[m % NT]); };
+      if (u == 0) {
+        const int rb = opaque(rows);
+        phase(f, use, [&](int m) { return rd.row(rb, m, TILE + HALF); });
+      } else {
+        last_phase(f, use);
       }
     }
     if (P.stages == 1) {
@@ -541,18 +576,20 @@ int launch(BwdP p, hipStream_t st) {
   constexpr size_t tile = (size_t)BK * TL::kRowBytes;
   const size_t piece = BIAS ? 4 * (size_t)(p.seg + (BIAS == 2 ? BK : 0)) : 0;
   const size_t rings = p.d.strips ? ((size_t)(BIAS == 1 ? 8 : 4) * p.ring + (BIAS == 2 ? 4 * kSkew : 0)) * 4 : 0;
-  size_t stage = 2 * tile + piece;
+  size_t stage = (2 * tile + piece + 511) & ~(size_t)511;      // the readers' XOR needs whole 512s
   p.stages = 2 * stage + rings <= kLds ? 2 : 1;
   size_t lds = p.stages * stage + rings;
   if (lds > kLds) return SO_ERR_SHAPE;
+  p.stage_bytes = (int)stage;
   int err = lds_limit(mha_dq_k<T, DP, BIAS>, lds);
   if (err) return err;
   hipLaunchKernelGGL((mha_dq_k<T, DP, BIAS>), dim3((unsigned)((long long)p.d.B * p.d.Hq * p.qtiles)), dim3(256), lds, st, p);
   err = SO_LAUNCH_CHECK();
   if (err) return err;
-  stage = 2 * tile + 2 * BK * 4 + piece;
+  stage = (2 * tile + 2 * BK * 4 + piece + 511) & ~(size_t)511;
   p.stages = 2 * stage <= kLds ? 2 : 1;
   lds = p.stages * stage;
+  p.stage_bytes = (int)stage;
   err = lds_limit(mha_dkv_k<T, DP, BIAS>, lds);
   if (err) return err;
   hipLaunchKernelGGL((mha_dkv_k<T, DP, BIAS>), dim3((unsigned)((long long)p.d.B * p.d.Hk * p.ktiles)), dim3(256), lds, st, p);

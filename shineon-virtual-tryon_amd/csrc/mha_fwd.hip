@@ -79,6 +79,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
     fv.fill(kt + TILE, vb + (size_t)t * TK * D.svl, next[0], next[1], wave_u);
   };
 
+  const Reader<T, DP> rd(sm, lane);
+  constexpr int HALF = 32 * TL::kRowBytes;      // 32 rows of a tile
+  frag f[NM];      // NM = NT * NCS: every phase has as many steps
   f32x16 o[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
@@ -125,8 +128,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
   __syncthreads();
   for (int t = t0; t < t1; ++t) {
     const int st = STAGES == 2 ? (t - t0) & 1 : 0;
-    const char* kt = sm + st * 2 * TILE;
-    const char* vt = kt + TILE;
+    const int fr = rd.rows + st * 2 * TILE + (SPLIT ? wave * HALF : 0), fc = rd.cols + st * 2 * TILE + (SPLIT ? wave * HALF : 0);
     bits[0] = next[0];
     bits[1] = next[1];
     if (STAGES == 2 && t + 1 < t1) fetch(t + 1, st ^ 1);
@@ -135,8 +137,20 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
 #pragma unroll
     for (int u = 0; u < SUBS; ++u) {
       const int r0 = SPLIT ? 32 * wave : 32 * u;
+      if (u == 0) {
+        const int rb = opaque(fr);
 #pragma unroll
-      for (int k = 0; k < NM; ++k) s[u] = mma(TL::row_frag(kt, r0 + tile_row(li), k, half), q[k], s[u]);
+        for (int k = 0; k < NM; ++k) f[k] = rd.row(rb, k, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      const auto use = [&](int k, const frag& a) { s[u] = mma(a, q[k], s[u]); };
+      if (u + 1 < SUBS) {
+        const int rb = opaque(fr);
+        phase(f, use, [&](int k) { return rd.row(rb, k, HALF); });
+      } else {
+        const int cb = opaque(fc);
+        phase(f, use, [&](int k) { return rd.col(cb, k % NT, k / NT, TILE); });
+      }
       const unsigned w = (unsigned)(bits[r0 >> 6] >> (r0 & 32));
       if (w != ~0u) {
         const unsigned mine = w >> (16 * half);
@@ -167,23 +181,26 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
     }
 #pragma unroll
     for (int u = 0; u < SUBS; ++u) {
-      const int r0 = SPLIT ? 32 * wave : 32 * u;
+      frag p[NCS], lo[NCS];
 #pragma unroll
       for (int c = 0; c < NCS; ++c) {
-        frag p, lo;
-        to_frag(s[u], c, p);
+        to_frag(s[u], c, p[c]);
         if constexpr (TWO) {
           f32x16 rest;
 #pragma unroll
-          for (int e = 0; e < E; ++e) rest[E * c + e] = s[u][E * c + e] - (float)p[e];
-          to_frag(rest, c, lo);
+          for (int e = 0; e < E; ++e) rest[E * c + e] = s[u][E * c + e] - (float)p[c][e];
+          to_frag(rest, c, lo[c]);
         }
-#pragma unroll
-        for (int v = 0; v < NT; ++v) {
-          const frag a = ColFrag<T, DP>::get(vt, r0, v, c, lane);
-          o[v] = mma(a, p, o[v]);
-          if constexpr (TWO) o[v] = mma(a, lo, o[v]);
-        }
+      }
+      const auto use = [&](int k, const frag& a) {
+        o[k % NT] = mma(a, p[k / NT], o[k % NT]);
+        if constexpr (TWO) o[k % NT] = mma(a, lo[k / NT], o[k % NT]);
+      };
+      if (u + 1 < SUBS) {
+        const int cb = opaque(fc);
+        phase(f, use, [&](int k) { return rd.col(cb, k % NT, k / NT, TILE + HALF); });
+      } else {
+        last_phase(f, use);
       }
     }
     if (t + 1 < t1) init(t + 1);
