@@ -198,7 +198,15 @@ __device__ __forceinline__ void fill_dwords(void* dst, const void* src, int n, u
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)((char*)dst + 4 * i), 4, 4 * (i + lane), 0, 0, 0);
 }
 
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+// sum / maximum over the two halves of a wave, without LDS
+__device__ __forceinline__ float half_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float half_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 
 // visible keys [64 w, 64 w + 64) of a sample as bits; keys behind the last are invisible
 __device__ __forceinline__ unsigned long long tail_word(int w, int Lk) {
@@ -244,6 +252,11 @@ __device__ __forceinline__ void word_range(const unsigned long long* words, int 
 
 // 2^x for the softmax: v_exp_f32 (1 ulp); x <= 0 here up to rounding, results below 2^-126 vanish
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// most codes between the first and last of n consecutive tokens of a map with rows of `width` (a sequence: 1)
+__host__ __device__ inline int code_span(int n, int width) {
+  return n < 2 ? 0 : (n - 1) + ((n - 2) / width + 1) * (width - 1);
+}
 
 // Block -> (sample, key head, block of that group).  A one-dimensional grid; XCD x = id % 8 gets the x-th contiguous eighth of an order
 // in which the blocks of a (sample, key head), which read the same keys and values, follow each other: they stay in that XCD's L2

@@ -27,11 +27,6 @@ struct BwdP {
 
 constexpr int BK = 64;          // keys (mha_dq_k) or query rows (mha_dkv_k) of a tile
 
-// most codes between the first and last of n consecutive tokens
-__host__ __device__ inline int code_span(int n, int width) {
-  return n < 2 ? 0 : (n - 1) + ((n - 2) / width + 1) * (width - 1);
-}
-
 template <int CTRL, bool ZERO>
 __device__ __forceinline__ float dpp(float old, float v) {
   return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), CTRL, 0xF, 0xF, ZERO));
@@ -138,7 +133,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
         for (int e = 0; e < E; ++e) delta += (float)go[m][e] * (float)lv[e];
       }
     }
-    delta += other_half(delta);
+    delta = half_sum(delta);
   }
   const size_t stat = ((size_t)b * D.Hq + head) * D.Lq + qi;
   const float lse = rowv ? D.lse[stat] : INFINITY;

@@ -7,14 +7,9 @@
 // ENTERS AS THE INITIAL ACCUMULATOR of the q k^T product, so adding it costs no vector instruction beyond its load: the scores in
 // log2 units are acc * (scale log2 e) in one multiply-add with -m.
 //
-// A block is four waves.  Query heads that share a key head are consecutive rows of one problem (row = head in group * Lq + i), so a
-// single token's heads fill one tile.
-//   SPLIT = false: 128 rows per block, 32 per wave; all waves walk the same 64-key tiles.
-//   SPLIT = true (rows of a key head <= 32): 32 rows per block; each wave takes 32 of the 128 keys of a tile and the four running
-//   softmaxes are merged through LDS at the end - with few rows the kernel is bound by reading keys and values, and this puts the
-//   four waves on different ones.
-// When there are too few blocks to fill the chip the keys are cut into gridDim.z parts, each leaves (o, m, l) in fp32 and
-// so_mha_join merges them.
+// A block is four waves; mha_fwd_k takes 128 rows of a head, mha_few_k (at most 32 rows to a key head) all rows and cuts the keys over its
+// waves.  When there are too few blocks to fill the chip the keys are cut into parts as well, each leaves (o, m, l) in fp32 and mha_join_k
+// merges them.
 #include "mha.h"
 
 using namespace mha;
@@ -24,235 +19,19 @@ namespace {
 struct FwdP {
   so_mha_desc d;
   int parts, row_tiles;
+  int stages, stage_bytes, seg;      // seg: floats of the bias that a tile of 64 and a block of 128 tokens can meet, in whole 64s
   float c;              // scale * log2 e
 };
 
-template <typename T, int DP, bool SPLIT, bool TWO>   // TWO: the probabilities as hi + lo pair of bf16 products
-__global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 96 ? 2 : 1))) void mha_fwd_k(const FwdP P) {
-  typedef Tile<T, DP> TL;
-  typedef typename Elem<T>::frag frag;
-  constexpr int E = Elem<T>::E, KM = 2 * E, NM = DP / KM, NT = DP / 32, NCS = 32 / KM;
-  constexpr int TK = SPLIT ? 128 : 64, SUBS = SPLIT ? 1 : 2;       // keys of a tile; 32-key pieces of it that one wave takes
-  constexpr int TILE = TK * TL::kRowBytes, STAGES = 4 * TILE <= 150 * 1024 ? 2 : 1;
-  extern __shared__ __attribute__((aligned(16))) char sm[];         // [STAGES][K tile | V tile]
+constexpr int kLds = 160 * 1024;
+
+// one row's result: o / l (or o, m, l of a part), its rounding rest and log2 of its sum
+template <typename T, int NT>
+__device__ __forceinline__ void write_row(const FwdP& P, const f32x16 (&o)[NT], float m, float l, int b, int hk, int head, int qi, int part, int half) {
   const so_mha_desc& D = P.d;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
-  const int G = D.Hq / D.Hk, rows = G * D.Lq;
-  const BlockOf blk = block_of(D.B, D.Hk, P.row_tiles * P.parts);
-  const int b = blk.b, hk = blk.hk, part = blk.idx / P.row_tiles, tile = blk.idx - part * P.row_tiles, bh = b * D.Hk + hk;
-  const int row = tile * (SPLIT ? 32 : 128) + (SPLIT ? 0 : 32 * wave) + li;
-  const bool rowv = row < rows;
-  const int head = hk * G + (rowv ? row / D.Lq : 0), qi = rowv ? row % D.Lq : 0;
-
-  // keys of this part
-  const unsigned long long* words = D.words ? (const unsigned long long*)D.words + (size_t)b * D.nwords : nullptr;
-  int wlo, whi;
-  word_range(words, D.Lk, lane, wlo, whi);
-  constexpr int WPT = TK / 64;
-  int t0 = wlo / WPT, t1 = (whi + WPT - 1) / WPT;                   // visible tiles
-  if (P.parts > 1) {
-    const int n = t1 > t0 ? t1 - t0 : 0, per = (n + P.parts - 1) / P.parts;
-    t0 += part * per;
-    t1 = t0 + per < t1 ? t0 + per : t1;
-  }
-
-  frag q[NM];
-  {
-    const T* qr = (const T*)D.q + (size_t)b * D.sqb + (size_t)qi * D.sql + (size_t)head * D.sqh;
-#pragma unroll
-    for (int m = 0; m < NM; ++m) q[m] = as_frag<T>(load_chunk<T>(qr, 2 * m + half, rowv && (2 * m + half) * E < D.D));
-  }
-  const float* bias = nullptr;
-  if (D.bias) bias = D.bias + (size_t)head * D.V + D.code_max - D.code[D.q_start + qi];
-
-  const T* kb = (const T*)D.k + (size_t)b * D.skb + (size_t)hk * D.skh;
-  const T* vb = (const T*)D.v + (size_t)b * D.svb + (size_t)hk * D.svh;
-  const int wave_u = __builtin_amdgcn_readfirstlane(wave);
-  const Filler<T, DP, TK, 4> fk(D.D, (unsigned)(D.skl * sizeof(T)), tid), fv(D.D, (unsigned)(D.svl * sizeof(T)), tid);
-  KeyWords kw(words, D.nwords, D.Lk, lane);
-  unsigned long long bits[2] = {0, 0}, next[2] = {0, 0};
-  auto fetch = [&](int t, int st) {      // tile t -> stage st; its mask words -> next
-    next[0] = kw.get(WPT * t);
-    if (WPT == 2) next[1] = kw.get(WPT * t + 1);
-    char* kt = sm + st * 2 * TILE;
-    fk.fill(kt, kb + (size_t)t * TK * D.skl, next[0], next[1], wave_u);
-    fv.fill(kt + TILE, vb + (size_t)t * TK * D.svl, next[0], next[1], wave_u);
-  };
-
-  const Reader<T, DP> rd(sm, lane);
-  constexpr int HALF = 32 * TL::kRowBytes;      // 32 rows of a tile
-  frag f[NM];      // NM = NT * NCS: every phase has as many steps
-  f32x16 o[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
-  float m = -INFINITY, l = 0.f;
-
-  // initial accumulators of tile t: the bias.  Requested in front of the wait that ends the tile before.
-  f32x16 s[SUBS];
-  auto init = [&](int t) {
-#pragma unroll
-    for (int u = 0; u < SUBS; ++u) {
-      const int key0 = t * TK + (SPLIT ? 32 * wave : 32 * u);
-      if (bias) {
-        if (D.linear) {
-          const float* bp = bias + key0 + 16 * half;
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const f32x4u v = *reinterpret_cast<const f32x4u*>(bp + 4 * g);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[u][4 * g + e] = v[e];
-          }
-        } else {
-          const int* cp = D.code + key0 + 16 * half;
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const i32x4 v = *reinterpret_cast<const i32x4*>(cp + 4 * g);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[u][4 * g + e] = bias[v[e]];
-          }
-        }
-      } else {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
-      }
-    }
-  };
-
-  if (t0 < t1) {
-    fetch(t0, 0);
-    init(t0);
-  }
-  SO_DMA_DRAIN();
-  __syncthreads();
-  for (int t = t0; t < t1; ++t) {
-    const int st = STAGES == 2 ? (t - t0) & 1 : 0;
-    const int fr = rd.rows + st * 2 * TILE + (SPLIT ? wave * HALF : 0), fc = rd.cols + st * 2 * TILE + (SPLIT ? wave * HALF : 0);
-    bits[0] = next[0];
-    bits[1] = next[1];
-    if (STAGES == 2 && t + 1 < t1) fetch(t + 1, st ^ 1);
-    // scores of this wave's keys
-    float mx = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < SUBS; ++u) {
-      const int r0 = SPLIT ? 32 * wave : 32 * u;
-      if (u == 0) {
-        const int rb = opaque(fr);
-#pragma unroll
-        for (int k = 0; k < NM; ++k) f[k] = rd.row(rb, k, 0);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      const auto use = [&](int k, const frag& a) { s[u] = mma(a, q[k], s[u]); };
-      if (u + 1 < SUBS) {
-        const int rb = opaque(fr);
-        phase(f, use, [&](int k) { return rd.row(rb, k, HALF); });
-      } else {
-        const int cb = opaque(fc);
-        phase(f, use, [&](int k) { return rd.col(cb, k % NT, k / NT, TILE); });
-      }
-      const unsigned w = (unsigned)(bits[r0 >> 6] >> (r0 & 32));
-      if (w != ~0u) {
-        const unsigned mine = w >> (16 * half);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[u][r] = (mine >> r) & 1 ? s[u][r] : -INFINITY;
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[u][r]);
-    }
-    mx = fmaxf(mx, other_half(mx)) * P.c;
-    const float mn = fmaxf(m, mx), ms = mn == -INFINITY ? 0.f : mn;
-    const float alpha = exp2_(m - ms);
-    m = mn;
-    float sum = 0.f;
-#pragma unroll
-    for (int u = 0; u < SUBS; ++u)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[u][r] = exp2_(__builtin_fmaf(s[u][r], P.c, -ms));
-        sum += s[u][r];
-      }
-    l = l * alpha + sum;
-    if (__any(alpha != 1.f)) {
-#pragma unroll
-      for (int v = 0; v < NT; ++v)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[v][r] *= alpha;
-    }
-#pragma unroll
-    for (int u = 0; u < SUBS; ++u) {
-      frag p[NCS], lo[NCS];
-#pragma unroll
-      for (int c = 0; c < NCS; ++c) {
-        to_frag(s[u], c, p[c]);
-        if constexpr (TWO) {
-          f32x16 rest;
-#pragma unroll
-          for (int e = 0; e < E; ++e) rest[E * c + e] = s[u][E * c + e] - (float)p[c][e];
-          to_frag(rest, c, lo[c]);
-        }
-      }
-      const auto use = [&](int k, const frag& a) {
-        o[k % NT] = mma(a, p[k / NT], o[k % NT]);
-        if constexpr (TWO) o[k % NT] = mma(a, lo[k / NT], o[k % NT]);
-      };
-      if (u + 1 < SUBS) {
-        const int cb = opaque(fc);
-        phase(f, use, [&](int k) { return rd.col(cb, k % NT, k / NT, TILE + HALF); });
-      } else {
-        last_phase(f, use);
-      }
-    }
-    if (t + 1 < t1) init(t + 1);
-    if (STAGES == 1) {
-      __syncthreads();
-      if (t + 1 < t1) fetch(t + 1, 0);
-    }
-    SO_DMA_DRAIN();
-    __syncthreads();
-  }
-  l += other_half(l);
-
-  if constexpr (SPLIT) {
-    // merge the four waves' softmaxes: statistics first, then each wave adds its scaled rows in turn
-    float* st = reinterpret_cast<float*>(sm);                       // [4][32] m | [4][32] l | [32][DP + 1] o
-    if (half == 0) {
-      st[32 * wave + li] = m;
-      st[128 + 32 * wave + li] = l;
-    }
-    __syncthreads();
-    float mn = -INFINITY, ln = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) mn = fmaxf(mn, st[32 * w + li]);
-    const float ms = mn == -INFINITY ? 0.f : mn;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) ln += st[128 + 32 * w + li] * exp2_(st[32 * w + li] - ms);
-    const float f = exp2_(m - ms);
-    float* os = st + 256;
-    for (int w = 0; w < 4; ++w) {
-      if (wave == w) {
-#pragma unroll
-        for (int v = 0; v < NT; ++v)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            float* at = os + li * (DP + 1) + 32 * v + acc_row(r, half);
-            const float x = o[v][r] * f;
-            *at = w == 0 ? x : *at + x;
-          }
-      }
-      __syncthreads();
-    }
-    if (wave != 0) return;
-    m = mn;
-    l = ln;
-#pragma unroll
-    for (int v = 0; v < NT; ++v)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[v][r] = os[li * (DP + 1) + 32 * v + acc_row(r, half)];
-  }
-  if (!rowv) return;
-  if (P.parts > 1) {      // unnormalised rows and statistics for so_mha_join: [b][Hk][rows][parts]
-    const size_t at = ((size_t)bh * rows + row) * P.parts + part;
+  if (P.parts > 1) {      // unnormalised rows and statistics for mha_join_k: [b][Hk][rows][parts]
+    const int G = D.Hq / D.Hk;
+    const size_t at = (((size_t)b * D.Hk + hk) * G * D.Lq + (size_t)(head - hk * G) * D.Lq + qi) * P.parts + part;
     if (half == 0) {
       D.part_ml[2 * at] = m;
       D.part_ml[2 * at + 1] = l;
@@ -290,6 +69,359 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
       }
     }
   if (D.lse && half == 0) D.lse[((size_t)b * D.Hq + head) * D.Lq + qi] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
+// the running softmax of 32 keys per half: s -> probabilities against the new maximum; o and l are rescaled when it moves
+template <int N, int NT>
+__device__ __forceinline__ void softmax_step(f32x16 (&s)[N], f32x16 (&o)[NT], float& m, float& l, float c) {
+  float mx = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < N; ++u)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[u][r]);
+  const float mn = fmaxf(m, half_max(mx) * c), ms = mn == -INFINITY ? 0.f : mn;
+  const float alpha = exp2_(m - ms);
+  m = mn;
+  float sum = 0.f;
+#pragma unroll
+  for (int u = 0; u < N; ++u)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[u][r] = exp2_(__builtin_fmaf(s[u][r], c, -ms));
+      sum += s[u][r];
+    }
+  l = l * alpha + sum;
+  if (__any(alpha != 1.f)) {
+#pragma unroll
+    for (int v = 0; v < NT; ++v)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[v][r] *= alpha;
+  }
+}
+
+template <typename T, int NCS, bool TWO>
+__device__ __forceinline__ void prob_frags(const f32x16& s, typename Elem<T>::frag (&p)[NCS], typename Elem<T>::frag (&lo)[NCS]) {
+  constexpr int E = Elem<T>::E;
+#pragma unroll
+  for (int c = 0; c < NCS; ++c) {
+    to_frag(s, c, p[c]);
+    if constexpr (TWO) {
+      f32x16 rest;
+#pragma unroll
+      for (int e = 0; e < E; ++e) rest[E * c + e] = s[E * c + e] - (float)p[c][e];
+      to_frag(rest, c, lo[c]);
+    }
+  }
+}
+
+// Many rows: a block is 128 rows of one head, 32 per wave, and walks 64-key tiles.  BIAS: 0 none, 1 sequence, 2 map; the piece of the
+// expanded bias that a tile's offsets lie in travels to LDS with the tile.  (Read from global memory by every lane it took 120 of 495 us
+// at 8191 tokens, 16 heads of 64.)  TWO: the probabilities as a hi + lo pair of bf16 products.
+template <typename T, int DP, int BIAS, bool TWO>
+__global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 96 ? 2 : 1))) void mha_fwd_k(const FwdP P) {
+  typedef Tile<T, DP> TL;
+  typedef typename Elem<T>::frag frag;
+  constexpr int E = Elem<T>::E, KM = 2 * E, NM = DP / KM, NT = DP / 32, NCS = 32 / KM;
+  constexpr int TK = 64, TILE = TK * TL::kRowBytes, HALF = TILE / 2;
+  extern __shared__ __attribute__((aligned(16))) char sm[];         // [stages][K tile | V tile | bias | codes]
+  const so_mha_desc& D = P.d;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
+  const int wave_u = __builtin_amdgcn_readfirstlane(wave);
+  const int G = D.Hq / D.Hk;
+  const BlockOf blk = block_of(D.B, D.Hk, G * P.row_tiles * P.parts);
+  const int b = blk.b, hk = blk.hk, part = blk.idx / (G * P.row_tiles), gt = blk.idx - part * G * P.row_tiles;
+  const int head = hk * G + gt / P.row_tiles, q0 = gt % P.row_tiles * 128;
+  const int qlast = (q0 + 128 < D.Lq ? q0 + 128 : D.Lq) - 1, row = q0 + 32 * wave + li;
+  const bool rowv = row < D.Lq;
+  const int qi = rowv ? row : qlast;
+
+  const unsigned long long* words = D.words ? (const unsigned long long*)D.words + (size_t)b * D.nwords : nullptr;
+  int t0, t1;
+  word_range(words, D.Lk, lane, t0, t1);
+  if (P.parts > 1) {
+    const int n = t1 > t0 ? t1 - t0 : 0, per = (n + P.parts - 1) / P.parts;
+    t0 += part * per;
+    t1 = t0 + per < t1 ? t0 + per : t1;
+  }
+
+  frag q[NM];
+  {
+    const T* qr = (const T*)D.q + (size_t)b * D.sqb + (size_t)qi * D.sql + (size_t)head * D.sqh;
+#pragma unroll
+    for (int m = 0; m < NM; ++m) q[m] = as_frag<T>(load_chunk<T>(qr, 2 * m + half, rowv && (2 * m + half) * E < D.D));
+  }
+  // first offset of tile t's piece of the bias: code(first key) - code(last row); this lane's place in it
+  const int STAGE = P.stage_bytes;
+  const int cqf = BIAS == 2 ? D.code[D.q_start + q0] : 0;
+  const int cqe = BIAS == 0 ? 0 : BIAS == 1 ? D.q_start + q0 + 127 : D.code[D.q_start + qlast];
+  const int mine_q = BIAS == 0 ? 0 : BIAS == 1 ? 127 - 32 * wave - li : cqe - D.code[D.q_start + qi];
+  const float* bias = BIAS ? D.bias + (size_t)head * D.V + D.code_max - cqe : nullptr;
+
+  const T* kb = (const T*)D.k + (size_t)b * D.skb + (size_t)hk * D.skh;
+  const T* vb = (const T*)D.v + (size_t)b * D.svb + (size_t)hk * D.svh;
+  const Filler<T, DP, TK, 4> fk(D.D, (unsigned)(D.skl * sizeof(T)), tid), fv(D.D, (unsigned)(D.svl * sizeof(T)), tid);
+  const Reader<T, DP> rd(sm, lane);
+  KeyWords kw(words, D.nwords, D.Lk, lane);
+  unsigned long long next = 0;
+  auto fetch = [&](int t, int st) {
+    next = kw.get(t);
+    char* kt = sm + st * STAGE;
+    fk.fill(kt, kb + (size_t)t * TK * D.skl, next, 0, wave_u);
+    fv.fill(kt + TILE, vb + (size_t)t * TK * D.svl, next, 0, wave_u);
+    if constexpr (BIAS == 1) fill_dwords<4>(kt + 2 * TILE, bias + t * TK, TK + 127, 0x7FFFFFFFu, wave_u, lane);
+    if constexpr (BIAS == 2) {
+      const int c0 = D.code[t * TK];
+      fill_dwords<4>(kt + 2 * TILE, bias + c0, D.code[t * TK + TK - 1] - cqf - (c0 - cqe) + 1, 0x7FFFFFFFu, wave_u, lane);
+      fill_dwords<4>(kt + 2 * TILE + 4 * P.seg, D.code + t * TK, TK, 0x7FFFFFFFu, (wave_u + 1) & 3, lane);
+    }
+  };
+
+  frag f[NM];      // NM = NT * NCS: every phase has as many steps
+  f32x16 o[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  if (t0 < t1) fetch(t0, 0);
+  SO_DMA_DRAIN();
+  __syncthreads();
+  for (int t = t0; t < t1; ++t) {
+    const int st = P.stages == 2 ? (t - t0) & 1 : 0;
+    const int fr = rd.rows + st * STAGE, fc = rd.cols + st * STAGE;
+    const float* seg = reinterpret_cast<const float*>(sm + st * STAGE + 2 * TILE);
+    const unsigned long long w64 = next;
+    if (P.stages == 2 && t + 1 < t1) fetch(t + 1, st ^ 1);
+    f32x16 s[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if constexpr (BIAS == 1) {
+        const float* at = seg + 32 * u + 16 * half + mine_q;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[u][r] = at[r];
+      } else if constexpr (BIAS == 2) {
+        const int* codes = reinterpret_cast<const int*>(seg + P.seg);
+        const float* at = seg + mine_q - codes[0];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const i32x4 c = *reinterpret_cast<const i32x4*>(codes + 32 * u + 16 * half + 4 * g);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[u][4 * g + e] = at[c[e]];
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
+      }
+    }
+    {
+      const int rb = opaque(fr);
+#pragma unroll
+      for (int k = 0; k < NM; ++k) f[k] = rd.row(rb, k, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    {
+      const int rb = opaque(fr);
+      phase(f, [&](int k, const frag& a) { s[0] = mma(a, q[k], s[0]); }, [&](int k) { return rd.row(rb, k, HALF); });
+    }
+    {
+      const int cb = opaque(fc);
+      phase(f, [&](int k, const frag& a) { s[1] = mma(a, q[k], s[1]); }, [&](int k) { return rd.col(cb, k % NT, k / NT, TILE); });
+    }
+    if (w64 != ~0ULL) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const unsigned mine = (unsigned)(w64 >> (32 * u)) >> (16 * half);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[u][r] = (mine >> r) & 1 ? s[u][r] : -INFINITY;
+      }
+    }
+    softmax_step(s, o, m, l, P.c);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      frag p[NCS], lo[NCS];
+      prob_frags<T, NCS, TWO>(s[u], p, lo);
+      const auto use = [&](int k, const frag& a) {
+        o[k % NT] = mma(a, p[k / NT], o[k % NT]);
+        if constexpr (TWO) o[k % NT] = mma(a, lo[k / NT], o[k % NT]);
+      };
+      if (u == 0) {
+        const int cb = opaque(fc);
+        phase(f, use, [&](int k) { return rd.col(cb, k % NT, k / NT, TILE + HALF); });
+      } else {
+        last_phase(f, use);
+      }
+    }
+    if (P.stages == 1) {
+      __syncthreads();
+      if (t + 1 < t1) fetch(t + 1, 0);
+    }
+    SO_DMA_DRAIN();
+    __syncthreads();
+  }
+  l = half_sum(l);
+  if (rowv) write_row<T, NT>(P, o, m, l, b, hk, head, qi, part, half);
+}
+
+// Few rows: all (at most 32) rows of the query heads that share a key head, row = head in group * Lq + i, so that a single token's heads
+// fill one tile.  Bound by reading keys and values: each of the four waves takes 32 of the 128 keys of a tile, and the four running
+// softmaxes are merged through LDS at the end.
+template <typename T, int DP, bool TWO>
+__global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 96 ? 2 : 1))) void mha_few_k(const FwdP P) {
+  typedef Tile<T, DP> TL;
+  typedef typename Elem<T>::frag frag;
+  constexpr int E = Elem<T>::E, KM = 2 * E, NM = DP / KM, NT = DP / 32, NCS = 32 / KM;
+  constexpr int TK = 128, TILE = TK * TL::kRowBytes, HALF = 32 * TL::kRowBytes;
+  extern __shared__ __attribute__((aligned(16))) char sm[];         // [stages][K tile | V tile]; at the end [4][32] m | [4][32] l | [32][DP + 1] o
+  const so_mha_desc& D = P.d;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
+  const int wave_u = __builtin_amdgcn_readfirstlane(wave);
+  const int G = D.Hq / D.Hk, rows = G * D.Lq;
+  const BlockOf blk = block_of(D.B, D.Hk, P.parts);
+  const int b = blk.b, hk = blk.hk, part = blk.idx;
+  const bool rowv = li < rows;
+  const int head = hk * G + (rowv ? li / D.Lq : 0), qi = rowv ? li % D.Lq : 0;
+
+  const unsigned long long* words = D.words ? (const unsigned long long*)D.words + (size_t)b * D.nwords : nullptr;
+  int wlo, whi;
+  word_range(words, D.Lk, lane, wlo, whi);
+  int t0 = wlo / 2, t1 = (whi + 1) / 2;
+  if (P.parts > 1) {
+    const int n = t1 > t0 ? t1 - t0 : 0, per = (n + P.parts - 1) / P.parts;
+    t0 += part * per;
+    t1 = t0 + per < t1 ? t0 + per : t1;
+  }
+
+  frag q[NM];
+  {
+    const T* qr = (const T*)D.q + (size_t)b * D.sqb + (size_t)qi * D.sql + (size_t)head * D.sqh;
+#pragma unroll
+    for (int m = 0; m < NM; ++m) q[m] = as_frag<T>(load_chunk<T>(qr, 2 * m + half, rowv && (2 * m + half) * E < D.D));
+  }
+  const float* bias = nullptr;
+  if (D.bias) bias = D.bias + (size_t)head * D.V + D.code_max - D.code[D.q_start + qi];
+  const T* kb = (const T*)D.k + (size_t)b * D.skb + (size_t)hk * D.skh;
+  const T* vb = (const T*)D.v + (size_t)b * D.svb + (size_t)hk * D.svh;
+  const Filler<T, DP, TK, 4> fk(D.D, (unsigned)(D.skl * sizeof(T)), tid), fv(D.D, (unsigned)(D.svl * sizeof(T)), tid);
+  const Reader<T, DP> rd(sm, lane);
+  KeyWords kw(words, D.nwords, D.Lk, lane);
+  unsigned long long bits[2] = {0, 0}, next[2] = {0, 0};
+  auto fetch = [&](int t, int st) {
+    next[0] = kw.get(2 * t);
+    next[1] = kw.get(2 * t + 1);
+    char* kt = sm + st * 2 * TILE;
+    fk.fill(kt, kb + (size_t)t * TK * D.skl, next[0], next[1], wave_u);
+    fv.fill(kt + TILE, vb + (size_t)t * TK * D.svl, next[0], next[1], wave_u);
+  };
+  // initial accumulators of tile t: the bias, requested in front of the wait that ends the tile before
+  f32x16 s[1];
+  auto init = [&](int t) {
+    const int key0 = t * TK + 32 * wave + 16 * half;
+    if (!bias) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
+    } else if (D.linear) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4u v = *reinterpret_cast<const f32x4u*>(bias + key0 + 4 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[0][4 * g + e] = v[e];
+      }
+    } else {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const i32x4 v = *reinterpret_cast<const i32x4*>(D.code + key0 + 4 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[0][4 * g + e] = bias[v[e]];
+      }
+    }
+  };
+
+  frag f[NM];
+  f32x16 o[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  if (t0 < t1) {
+    fetch(t0, 0);
+    init(t0);
+  }
+  SO_DMA_DRAIN();
+  __syncthreads();
+  for (int t = t0; t < t1; ++t) {
+    const int st = P.stages == 2 ? (t - t0) & 1 : 0;
+    const int fr = rd.rows + st * 2 * TILE + wave * HALF, fc = rd.cols + st * 2 * TILE + wave * HALF;
+    bits[0] = next[0];
+    bits[1] = next[1];
+    if (P.stages == 2 && t + 1 < t1) fetch(t + 1, st ^ 1);
+    {
+      const int rb = opaque(fr);
+#pragma unroll
+      for (int k = 0; k < NM; ++k) f[k] = rd.row(rb, k, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    {
+      const int cb = opaque(fc);
+      phase(f, [&](int k, const frag& a) { s[0] = mma(a, q[k], s[0]); }, [&](int k) { return rd.col(cb, k % NT, k / NT, TILE); });
+    }
+    const unsigned w = (unsigned)(bits[wave >> 1] >> (32 * (wave & 1)));
+    if (w != ~0u) {
+      const unsigned mine = w >> (16 * half);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[0][r] = (mine >> r) & 1 ? s[0][r] : -INFINITY;
+    }
+    softmax_step(s, o, m, l, P.c);
+    frag p[NCS], lo[NCS];
+    prob_frags<T, NCS, TWO>(s[0], p, lo);
+    last_phase(f, [&](int k, const frag& a) {
+      o[k % NT] = mma(a, p[k / NT], o[k % NT]);
+      if constexpr (TWO) o[k % NT] = mma(a, lo[k / NT], o[k % NT]);
+    });
+    if (t + 1 < t1) init(t + 1);
+    if (P.stages == 1) {
+      __syncthreads();
+      if (t + 1 < t1) fetch(t + 1, 0);
+    }
+    SO_DMA_DRAIN();
+    __syncthreads();
+  }
+  l = half_sum(l);
+
+  // merge the four waves' softmaxes: statistics first, then each wave adds its scaled rows in turn
+  float* stats = reinterpret_cast<float*>(sm);
+  if (half == 0) {
+    stats[32 * wave + li] = m;
+    stats[128 + 32 * wave + li] = l;
+  }
+  __syncthreads();
+  float mn = -INFINITY, ln = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) mn = fmaxf(mn, stats[32 * w + li]);
+  const float ms = mn == -INFINITY ? 0.f : mn;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) ln += stats[128 + 32 * w + li] * exp2_(stats[32 * w + li] - ms);
+  const float scale = exp2_(m - ms);
+  float* os = stats + 256;
+  for (int w = 0; w < 4; ++w) {
+    if (wave == w) {
+#pragma unroll
+      for (int v = 0; v < NT; ++v)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float* at = os + li * (DP + 1) + 32 * v + acc_row(r, half);
+          const float x = o[v][r] * scale;
+          *at = w == 0 ? x : *at + x;
+        }
+    }
+    __syncthreads();
+  }
+  if (wave != 0 || !rowv) return;
+#pragma unroll
+  for (int v = 0; v < NT; ++v)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[v][r] = os[li * (DP + 1) + 32 * v + acc_row(r, half)];
+  write_row<T, NT>(P, o, mn, ln, b, hk, head, qi, part, half);
 }
 
 // joins the parts of a row: weights 2^(m_p - max m), fixed order.  One wave per row.
@@ -378,35 +510,52 @@ __global__ __launch_bounds__(256) void mha_prep_k(const PrepP p) {
   if (lane == 0) p.words[i] = bits;
 }
 
-template <typename T, int DP, bool SPLIT, bool TWO>
-int launch(const FwdP& p, hipStream_t st) {
-  typedef Tile<T, DP> TL;
-  constexpr int TK = SPLIT ? 128 : 64, TILE = TK * TL::kRowBytes, STAGES = 4 * TILE <= 150 * 1024 ? 2 : 1;
-  constexpr int merge = (256 + 32 * (DP + 1)) * 4;
-  constexpr int lds = SPLIT && merge > STAGES * 2 * TILE ? merge : STAGES * 2 * TILE;
-  
-  auto k = mha_fwd_k<T, DP, SPLIT, TWO>;
+template <typename K>
+int start(K k, const FwdP& p, size_t lds, long long blocks, hipStream_t st) {
   if (lds > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return (int)e;
   }
-  hipLaunchKernelGGL(k, dim3((unsigned)((long long)p.d.B * p.d.Hk * p.row_tiles * p.parts)), dim3(256), lds, st, p);
+  hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(256), lds, st, p);
   return SO_LAUNCH_CHECK();
 }
-template <typename T, int DP>
-int launch_mode(const FwdP& p, bool split, hipStream_t st) {
-  if constexpr (sizeof(T) == 2) {
-    if (p.d.two) return split ? launch<T, DP, true, true>(p, st) : launch<T, DP, false, true>(p, st);
+template <typename T, int DP, bool TWO>
+int launch(FwdP p, bool few, hipStream_t st) {
+  constexpr size_t row = Tile<T, DP>::kRowBytes;
+  const long long groups = (long long)p.d.B * p.d.Hk;
+  if (few) {
+    constexpr size_t stage = 2 * 128 * row, merge = (256 + 32 * (DP + 1)) * 4;
+    p.stages = 2 * stage <= kLds ? 2 : 1;
+    const size_t lds = p.stages * stage > merge ? p.stages * stage : merge;
+    return start(mha_few_k<T, DP, TWO>, p, lds, groups * p.parts, st);
   }
-  return split ? launch<T, DP, true, false>(p, st) : launch<T, DP, false, false>(p, st);
+  const int w = p.d.linear ? 1 : p.d.width;
+  p.seg = p.d.bias ? (code_span(128, w) + code_span(64, w) + 1 + 63) / 64 * 64 : 0;
+  const size_t stage = (2 * 64 * row + 4 * (size_t)p.seg + (p.d.bias && !p.d.linear ? 256 : 0) + 511) & ~(size_t)511;   // the readers' XOR needs whole 512s
+  p.stage_bytes = (int)stage;
+  p.stages = 2 * stage <= kLds ? 2 : 1;
+  const long long blocks = groups * (p.d.Hq / p.d.Hk) * p.row_tiles * p.parts;
+  const size_t lds = p.stages * stage;
+  if (!p.d.bias) return start(mha_fwd_k<T, DP, 0, TWO>, p, lds, blocks, st);
+  return p.d.linear ? start(mha_fwd_k<T, DP, 1, TWO>, p, lds, blocks, st) : start(mha_fwd_k<T, DP, 2, TWO>, p, lds, blocks, st);
+}
+template <typename T, int DP>
+int launch_two(const FwdP& p, bool few, hipStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (p.d.two) return launch<T, DP, true>(p, few, st);
+  }
+  return launch<T, DP, false>(p, few, st);
 }
 template <typename T>
-int launch_d(const FwdP& p, bool split, hipStream_t st) {
-  if (p.d.D <= 32) return launch_mode<T, 32>(p, split, st);
-  if (p.d.D <= 64) return launch_mode<T, 64>(p, split, st);
-  if (p.d.D <= 96) return launch_mode<T, 96>(p, split, st);
-  return launch_mode<T, 128>(p, split, st);
+int launch_d(const FwdP& p, bool few, hipStream_t st) {
+  if (p.d.D <= 32) return launch_two<T, 32>(p, few, st);
+  if (p.d.D <= 64) return launch_two<T, 64>(p, few, st);
+  if (p.d.D <= 96) return launch_two<T, 96>(p, few, st);
+  return launch_two<T, 128>(p, few, st);
 }
+
+// few rows: everything that shares a key head fits one 32-row tile
+bool is_few(const so_mha_desc* d) { return (long long)(d->Hq / d->Hk) * d->Lq <= 32; }
 
 }  // namespace
 
@@ -426,6 +575,7 @@ int so_mha_check(const so_mha_desc* d) {
     if (x % E) return SO_ERR_ALIGN;
   if ((((uintptr_t)d->q) | ((uintptr_t)d->k) | ((uintptr_t)d->v) | ((uintptr_t)d->o) | ((uintptr_t)d->o_lo)) & 15) return SO_ERR_ALIGN;
   if (d->bias && (!d->code || (((uintptr_t)d->code) & 15) || d->V != 2 * d->code_max + 1 || d->q_start < 0)) return SO_ERR_SHAPE;
+  if (d->bias && !d->linear && (d->width < 1 || d->width > 512)) return SO_ERR_SHAPE;
   if (d->bias && (d->q_start + (long long)d->Lq > d->tokens || d->Lk > d->tokens)) return SO_ERR_SHAPE;
   return 0;
 }
@@ -457,10 +607,9 @@ int so_mha_parts(const void* desc) {
   const so_mha_desc* d = (const so_mha_desc*)desc;
   const int err = so_mha_check(d);
   if (err) return err;
-  const int rows = d->Hq / d->Hk * d->Lq;
-  const bool split = rows <= 32;
-  const long long blocks = (long long)d->B * d->Hk * (split ? 1 : (rows + 127) / 128);
-  const int tiles = (d->Lk + (split ? 127 : 63)) / (split ? 128 : 64);
+  const bool few = is_few(d);
+  const long long blocks = (long long)d->B * (few ? d->Hk : (long long)d->Hq * ((d->Lq + 127) / 128));
+  const int tiles = (d->Lk + (few ? 127 : 63)) / (few ? 128 : 64);
   long long parts = (512 + blocks - 1) / blocks;
   if (parts > tiles / 2) parts = tiles / 2;
   return parts < 2 ? 1 : (int)(parts > 256 ? 256 : parts);
@@ -475,14 +624,13 @@ int so_mha_fwd(const void* desc, void* stream) {
   p.d = *d;
   p.parts = parts;
   p.c = d->scale * kLog2e;
-  const int rows = d->Hq / d->Hk * d->Lq;
-  const bool split = rows <= 32;
-  p.row_tiles = split ? 1 : (rows + 127) / 128;
-  if ((long long)d->B * d->Hk * p.row_tiles * parts > 0x7fffffffLL) return SO_ERR_SHAPE;
+  const bool few = is_few(d);
+  p.row_tiles = (d->Lq + 127) / 128;
+  if ((long long)d->B * d->Hq * p.row_tiles * parts > 0x7fffffffLL) return SO_ERR_SHAPE;
   hipStream_t st = (hipStream_t)stream;
-  int err = d->dtype == SO_F32 ? launch_d<float>(p, split, st) : launch_d<__bf16>(p, split, st);
+  const int err = d->dtype == SO_F32 ? launch_d<float>(p, few, st) : launch_d<__bf16>(p, few, st);
   if (err || parts == 1) return err;
-  const long long n = ((long long)d->B * d->Hk * rows + 3) / 4;
+  const long long n = ((long long)d->B * d->Hq * d->Lq + 3) / 4;
   if (n > 0x7fffffffLL) return SO_ERR_SHAPE;
   if (d->dtype == SO_F32) hipLaunchKernelGGL(mha_join_k<float>, dim3((unsigned)n), dim3(256), 0, st, p);
   else hipLaunchKernelGGL(mha_join_k<__bf16>, dim3((unsigned)n), dim3(256), 0, st, p);
