@@ -154,9 +154,27 @@ __device__ __forceinline__ typename Elem<T>::frag as_frag(f32x4 v) {
 
 // Fills a tile of ROWS rows in LDS from rows `stride` bytes apart, by LDS-DMA (no registers, no ds_write).  A fill writes lane after
 // lane, so the chunk swizzle is applied on the source side.  Rows whose bit is clear and channels behind D are requested at an offset
-// outside the descriptor and arrive as zeros; nothing outside the operand is read.  The caller drains (SO_DMA_DRAIN) before the barrier
-// that publishes the tile.
-typedef __attribute__((address_space(3))) void* lds_ptr;
+// outside the descriptor and arrive as zeros; nothing outside the operand is read.  The caller drains before the barrier that publishes
+// the tile.
+//
+// The fills are written in assembly so that hipcc does not know of them: it makes every ds_read_b64_tr wait for all fills in flight
+// (vmcnt 0), and the tile after the current one would arrive with its full latency exposed.  They have no register results; s_nop 4
+// covers a descriptor that a vector instruction (v_readfirstlane) has just written, which hipcc does not see to in assembly; drain()
+// is the wait that a barrier needs in front of it.  An own wait of hipcc's for its loads can only become longer by them.
+typedef __attribute__((address_space(3))) char* lds_ptr;
+__device__ __forceinline__ i32x4 rsrc_of(const void* base, unsigned bytes) {      // raw buffer over [base, base + bytes)
+  const unsigned long long a = (unsigned long long)base;
+  return i32x4{__builtin_amdgcn_readfirstlane((int)(unsigned)a), __builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32) & 0xFFFF),
+               __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000};
+}
+__device__ __forceinline__ int lds_at(const char* p) { return __builtin_amdgcn_readfirstlane((int)(unsigned)(unsigned long long)(lds_ptr)p); }
+__device__ __forceinline__ void dma16(i32x4 rsrc, int lds, unsigned off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc) : "memory", "m0");
+}
+__device__ __forceinline__ void dma4(i32x4 rsrc, int lds, unsigned off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc) : "memory", "m0");
+}
+__device__ __forceinline__ void drain() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 template <typename T, int DP, int ROWS, int WAVES>
 struct Filler {
   typedef Tile<T, DP> TL;
@@ -174,7 +192,8 @@ struct Filler {
   }
   // rows [base_row, base_row + ROWS) of the tile at `src`; bits: one per row (64 rows from base_row 0, further ones in `more`)
   __device__ __forceinline__ void fill(char* tile, const void* src, unsigned long long bits, unsigned long long more, int wave) const {
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(src), 0, 0x7FFFFFFF, 0x00020000);
+    const i32x4 r = rsrc_of(src, 0x7FFFFFFFu);
+    const int at = lds_at(tile) + wave * 1024;
     const bool all = bits == ~0ULL && (ROWS <= 64 || more == ~0ULL);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -184,7 +203,7 @@ struct Filler {
         const unsigned long long w = ROWS > 64 && row >= 64 ? more : bits;
         o = (w >> (row & 63)) & 1 ? o : 0x80000000u;
       }
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(tile + (j * WAVES + wave) * 1024), 16, (int)o, 0, 0, 0);
+      dma16(r, at + j * WAVES * 1024, o);
     }
   }
 };
@@ -193,9 +212,10 @@ struct Filler {
 // (what lies behind arrives as zeros).  LDS is written in whole pieces.
 template <int WAVES>
 __device__ __forceinline__ void fill_dwords(void* dst, const void* src, int n, unsigned bytes, int wave, int lane) {
-  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(src), 0, (int)bytes, 0x00020000);
+  const i32x4 r = rsrc_of(src, bytes);
+  const int at = lds_at((const char*)dst);
   for (int i = 64 * wave; i < n; i += 64 * WAVES)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)((char*)dst + 4 * i), 4, 4 * (i + lane), 0, 0, 0);
+    dma4(r, at + 4 * i, 4 * (i + lane));
 }
 
 // sum / maximum over the two halves of a wave, without LDS

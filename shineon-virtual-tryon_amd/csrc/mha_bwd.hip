@@ -210,7 +210,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
 #pragma unroll
     for (int r = 0; r < 16; ++r) dq[t][r] = 0.f;
   if (t0 < t1) fetch(t0, 0);
-  SO_DMA_DRAIN();
+  drain();
   __syncthreads();
   for (int t = t0; t < t1; ++t) {
     const int st = P.stages == 2 ? (t - t0) & 1 : 0;
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
       __syncthreads();
       if (t + 1 < t1) fetch(t + 1, 0);
     }
-    SO_DMA_DRAIN();
+    drain();
     __syncthreads();
   }
   if (want) {
@@ -388,7 +388,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[t][r] = dv[t][r] = 0.f;
   if (n) fetch(0, 0);
-  SO_DMA_DRAIN();
+  drain();
   __syncthreads();
   for (int t = 0; t < n; ++t) {
     const int st = P.stages == 2 ? t & 1 : 0;
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
       __syncthreads();
       if (t + 1 < n) fetch(t + 1, 0);
     }
-    SO_DMA_DRAIN();
+    drain();
     __syncthreads();
   }
   if (!keyv) return;

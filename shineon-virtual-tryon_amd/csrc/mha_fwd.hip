@@ -184,7 +184,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
     for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
   float m = -INFINITY, l = 0.f;
   if (t0 < t1) fetch(t0, 0);
-  SO_DMA_DRAIN();
+  drain();
   __syncthreads();
   for (int t = t0; t < t1; ++t) {
     const int st = P.stages == 2 ? (t - t0) & 1 : 0;
@@ -255,7 +255,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
       __syncthreads();
       if (t + 1 < t1) fetch(t + 1, 0);
     }
-    SO_DMA_DRAIN();
+    drain();
     __syncthreads();
   }
   l = half_sum(l);
@@ -347,7 +347,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
     fetch(t0, 0);
     init(t0);
   }
-  SO_DMA_DRAIN();
+  drain();
   __syncthreads();
   for (int t = t0; t < t1; ++t) {
     const int st = P.stages == 2 ? (t - t0) & 1 : 0;
@@ -383,7 +383,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
       __syncthreads();
       if (t + 1 < t1) fetch(t + 1, 0);
     }
-    SO_DMA_DRAIN();
+    drain();
     __syncthreads();
   }
   l = half_sum(l);
