@@ -67,8 +67,20 @@ struct Tile {
   __device__ static __forceinline__ int at(int row, int chunk) { return row * kRowBytes + ((chunk ^ swz(row)) << 4); }
 };
 
-// Fragment addresses.  The swizzle is an XOR of address bits, so every fragment of a tile is (lane's base ^ constant) + constant.  The base
-// is made opaque at every use: otherwise hipcc keeps the two dozen addresses of a tile in registers over the whole loop, and spills.
+// LDS by byte address, so that constants end up in the offset field of the instruction
+typedef __attribute__((address_space(3))) char* lds_ptr;
+__device__ __forceinline__ int lds_at(const char* p) { return __builtin_amdgcn_readfirstlane((int)(unsigned)(unsigned long long)(lds_ptr)p); }
+template <typename V>
+__device__ __forceinline__ V lds_read(int at) {
+  return *reinterpret_cast<const __attribute__((address_space(3))) V*>((unsigned)at);
+}
+
+// A branch whose condition is the same for the whole block and rarely true: keeps hipcc from computing both sides
+__device__ __forceinline__ void seldom() { asm volatile("; seldom"); }
+
+// Fragment addresses.  The swizzle is an XOR of address bits, so every fragment of a tile is (lane's base ^ constant) + constant; tiles
+// start at multiples of 512 bytes.  The base is made opaque at every use: otherwise hipcc keeps the two dozen addresses of a tile in
+// registers over the whole loop, and spills.
 __device__ __forceinline__ int opaque(int x) {
   asm volatile("" : "+v"(x));
   return x;
@@ -77,25 +89,21 @@ template <typename T, int DP>
 struct Reader {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::frag frag;
-  const char* sm;
-  int rows, cols;      // bases of the lane's row and column fragments in a tile at sm
-  __device__ __forceinline__ Reader(const char* sm, int lane) : sm(sm) {
+  int rows, cols;      // byte addresses of the lane's row and column fragments in a tile at sm
+  __device__ __forceinline__ Reader(const char* sm, int lane) {
     const int half = lane >> 5, li = lane & 31;
-    rows = TL::at(tile_row(li), half);
-    if constexpr (sizeof(T) == 4) cols = TL::at(16 * half, li >> 2) + 4 * (li & 3);
-    else cols = TL::at(16 * half + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 8 * (lane & 1);
+    rows = lds_at(sm) + TL::at(tile_row(li), half);
+    if constexpr (sizeof(T) == 4) cols = lds_at(sm) + TL::at(16 * half, li >> 2) + 4 * (li & 3);
+    else cols = lds_at(sm) + TL::at(16 * half + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 8 * (lane & 1);
   }
   // A fragment: row tile_row(lane) of the 32 rows at byte `at` of a tile, step m of the channel axis
-  __device__ __forceinline__ frag row(int base, int m, int at) const {
-    return *reinterpret_cast<const frag*>(sm + ((base ^ (m << 5)) + at));
-  }
+  __device__ __forceinline__ frag row(int base, int m, int at) const { return lds_read<frag>((base ^ (m << 5)) + at); }
   // A fragment: column 32 t + lane, step c of the row axis of the 32 rows at byte `at`
   __device__ __forceinline__ frag col(int base, int t, int c, int at) const {
     if constexpr (sizeof(T) == 4) {
       frag f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        f[e] = *reinterpret_cast<const float*>(sm + ((base ^ (((8 * t) ^ TL::swz(4 * c + e)) << 4)) + at + (4 * c + e) * TL::kRowBytes));
+      for (int e = 0; e < 4; ++e) f[e] = lds_read<float>((base ^ (((8 * t) ^ TL::swz(4 * c + e)) << 4)) + at + (4 * c + e) * TL::kRowBytes);
       return f;
     } else {
       typedef __attribute__((address_space(3))) s16x4* lds_p;
@@ -103,11 +111,17 @@ struct Reader {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         u.s[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_p)(sm + ((base ^ (((4 * t) ^ TL::swz(8 * c + 4 * i)) << 4)) + at + (8 * c + 4 * i) * TL::kRowBytes)));
+            (lds_p)(unsigned)((base ^ (((4 * t) ^ TL::swz(8 * c + 4 * i)) << 4)) + at + (8 * c + 4 * i) * TL::kRowBytes));
       return u.f;
     }
   }
 };
+
+// sixteen consecutive floats at a byte address that is a multiple of 4
+__device__ __forceinline__ void lds_read16(int at, f32x16& v) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) v[r] = lds_read<float>(at + 4 * r);
+}
 
 // accumulator registers of step c as a B fragment; bf16 rounds here (half a step, 2^-8 of the value: the products run at the rate of
 // 16-bit operands; sums, statistics and accumulators stay fp32)
@@ -161,13 +175,11 @@ __device__ __forceinline__ typename Elem<T>::frag as_frag(f32x4 v) {
 // (vmcnt 0), and the tile after the current one would arrive with its full latency exposed.  They have no register results; s_nop 4
 // covers a descriptor that a vector instruction (v_readfirstlane) has just written, which hipcc does not see to in assembly; drain()
 // is the wait that a barrier needs in front of it.  An own wait of hipcc's for its loads can only become longer by them.
-typedef __attribute__((address_space(3))) char* lds_ptr;
 __device__ __forceinline__ i32x4 rsrc_of(const void* base, unsigned bytes) {      // raw buffer over [base, base + bytes)
   const unsigned long long a = (unsigned long long)base;
   return i32x4{__builtin_amdgcn_readfirstlane((int)(unsigned)a), __builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32) & 0xFFFF),
                __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000};
 }
-__device__ __forceinline__ int lds_at(const char* p) { return __builtin_amdgcn_readfirstlane((int)(unsigned)(unsigned long long)(lds_ptr)p); }
 __device__ __forceinline__ void dma16(i32x4 rsrc, int lds, unsigned off) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc) : "memory", "m0");
 }

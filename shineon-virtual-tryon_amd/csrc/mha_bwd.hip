@@ -32,20 +32,27 @@ __device__ __forceinline__ float dpp(float old, float v) {
   return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), CTRL, 0xF, 0xF, ZERO));
 }
 
-// Diagonal sums of 16 keys x 32 queries of a sequence, in vector instructions.  Per row of 16 lanes, lane j holds query j, s[r] key r:
-// the running sums move one lane up per key (lane j then holds diagonal r - j); what leaves lane 15 is finished and enters lane 0 of a
-// second register, which moves along.  At the end run = diagonal 15 - j, fin = diagonal -1 - j (lane 15: zero), against the row's first
-// query.  The diagonals of the second row's run are those of the first row's fin, and the first row's run (pend, kept in the second
-// row's lanes) are those of the second row's fin 32 keys further on, where this half of the wave works next.  So every call finishes
-// the 32 diagonals in front of its keys: lane l returns diagonal -1 - l against the half's first key and the wave's first query.
-__device__ __forceinline__ float diagonals(const f32x16& s, float& pend, int li) {
+// Diagonal sums of a 16 x 16 piece per row of 16 lanes, in vector instructions: lane j holds query j, s[r] key r.  The running sums move
+// one lane up per key (lane j then holds diagonal r - j); what leaves lane 15 is finished and enters lane 0 of a second register, which
+// moves along.  At the end run = diagonal 15 - j, fin = diagonal -1 - j (lane 15: zero).
+__device__ __forceinline__ void diagonals16(const f32x16& s, float& run, float& fin) {
   constexpr int kShr1 = 0x111, kRor1 = 0x121;
-  float run = s[0], fin = 0.f;
+  run = s[0];
+  fin = 0.f;
 #pragma unroll
   for (int r = 1; r < 16; ++r) {
     fin = dpp<kShr1, false>(dpp<kRor1, true>(0.f, run), fin);
     run = s[r] + dpp<kShr1, true>(0.f, run);
   }
+}
+
+// The 16 keys x 32 queries of one half, tokens of a sequence: the diagonals of the second row's run are those of the first row's fin, and
+// the first row's run (pend, kept in the second row's lanes) are those of the second row's fin 32 keys further on, where this half of the
+// wave works next.  So every call finishes the 32 diagonals in front of its keys: lane l returns diagonal -1 - l against the half's first
+// key and the wave's first query.
+__device__ __forceinline__ float diagonals(const f32x16& s, float& pend, int li) {
+  float run, fin;
+  diagonals16(s, run, fin);
   // rows 0 1 2 3 -> first: 0 0 2 2, second: 1 1 3 3
   const auto rows = __builtin_amdgcn_permlane16_swap(__float_as_uint(run), __float_as_uint(run), false, false);
   const float x = fin + (li < 16 ? __uint_as_float(rows[1]) : pend);
@@ -53,61 +60,89 @@ __device__ __forceinline__ float diagonals(const f32x16& s, float& pend, int li)
   return x;
 }
 
-// The same for a piece of a map, where 32 consecutive keys or queries may lie in several map rows and equal token distances are equal
-// offsets only inside one (key row, query row) rectangle: the piece goes through LDS and for every rectangle lane l walks diagonal
-// l - (queries - 1).  Different lanes of a rectangle add to different words of the ring.
-constexpr int kSkewPitch = 33, kSkew = 32 * kSkewPitch;
-__device__ __forceinline__ void rectangles(const f32x16& s, float* skew, float* ring, int rmask, int key0, int q0, int width, int lane) {
-  const int li = lane & 31, half = lane >> 5;
+// The same for tokens of a map.  A row of 16 lanes holds queries of one map row (see map_query) whose codes count up from cq; the half's
+// 16 keys from column x of map row y may reach over map rows, and equal token distances are equal offsets only inside one: a pass per map
+// row, the other keys zero.  Sums that are zero are not added: their place may belong to offsets that are being written out.
+__device__ __forceinline__ void map_diagonals(const f32x16& s, float* ring, int rmask, int y, int x, int width, int cq, int lj) {
+  int from = 0;
+  while (__any(from < 16)) {
+    const int to = from + width - x < 16 ? from + width - x : 16;
+    float run, fin;
+    if (__all(from == 0 && to == 16)) {
+      diagonals16(s, run, fin);
+    } else {
+      const int mask = (1 << to) - (1 << from);
+      f32x16 z;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) skew[(16 * half + r) * kSkewPitch + li] = s[r];
-  __builtin_amdgcn_wave_barrier();      // one wave's LDS operations complete in order
-  int ky = key0 / width, kx = key0 - ky * width;
-  for (int ka = 0; ka < 32;) {
-    const int nk = width - kx < 32 - ka ? width - kx : 32 - ka;
-    int qy = q0 / width, qx = q0 - qy * width;
-    for (int qa = 0; qa < 32;) {
-      const int nq = width - qx < 32 - qa ? width - qx : 32 - qa;
-      const int d = lane - (nq - 1);
-      float x = 0.f;
-#pragma unroll 8
-      for (int k = 0; k < nk; ++k) {
-        const int q = k - d;
-        const bool on = q >= 0 && q < nq;
-        const float y = skew[(ka + k) * kSkewPitch + qa + (on ? q : 0)];
-        x += on ? y : 0.f;
-      }
-      if (d < nk) ring[((ky - qy) * (2 * width - 1) + kx - qx + d) & rmask] += x;
-      __builtin_amdgcn_wave_barrier();
-      qa += nq;
-      qx = 0;
-      ++qy;
+      for (int r = 0; r < 16; ++r) z[r] = __int_as_float(__float_as_int(s[r]) & __builtin_amdgcn_sbfe(mask, r, 1));
+      diagonals16(z, run, fin);
     }
-    ka += nk;
-    kx = 0;
-    ++ky;
+    const int v = y * (2 * width - 1) + x - from + 15 - cq - lj;
+    if (run != 0.f) ring[v & rmask] += run;
+    if (fin != 0.f) ring[(v - 16) & rmask] += fin;
+    from = to;
+    x = 0;
+    ++y;
   }
+}
+
+// Query rows of mha_dq_k in a map: map rows are padded to a multiple of 16 lanes.  The i-th of these places, counted from the map row of
+// the first query, is column x of map row y.
+struct MapQuery { int y, x; };
+__device__ __forceinline__ MapQuery map_query(const so_mha_desc& D, int i) {
+  const int pitch = (D.width + 15) & ~15, y = i / pitch;
+  return MapQuery{D.q_start / D.width + y, i - y * pitch};
+}
+// codes of the first and the last query that block t of mha_dq_k can hold
+__device__ __forceinline__ void block_codes(const so_mha_desc& D, int t, bool map, int& first, int& last) {
+  const int q0 = 128 * t, ql = (q0 + 128 < D.Lq ? q0 + 128 : D.Lq) - 1;
+  first = D.q_start + q0;
+  last = D.q_start + ql;
+  if (!map) return;
+  const int w = D.width, wc = 2 * w - 1, end = D.q_start + D.Lq - 1;
+  const MapQuery a = map_query(D, q0), b = map_query(D, q0 + 127);
+  const int lo = D.q_start / w * wc + D.q_start % w, hi = end / w * wc + end % w;
+  first = a.y * wc + (a.x < w ? a.x : w - 1);
+  last = b.y * wc + (b.x < w ? b.x : w - 1);
+  if (first < lo) first = lo;
+  if (last > hi) last = hi;
+  if (first > last) first = last;
 }
 
 // BIAS: 0 none, 1 tokens of a sequence (offset = key - query), 2 tokens of a map.  Everything a tile needs travels by LDS-DMA: K, V,
 // the piece of the expanded bias that its offsets lie in and (maps) the keys' codes; nothing in the loop waits for global memory
 // except the one drain per tile.
 template <typename T, int DP, int BIAS>
-__global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha_dq_k(const BwdP P) {
+__global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : DP <= 64 ? 2 : 1)) void mha_dq_k(const BwdP P) {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::frag frag;
   constexpr int E = Elem<T>::E, KM = 2 * E, NM = DP / KM, NT = DP / 32, NCS = 32 / KM;
   constexpr int TILE = BK * TL::kRowBytes;
-  extern __shared__ __attribute__((aligned(16))) char sm[];          // [stages][K tile | V tile | bias | codes] | rings | skew
+  // start the product do v^T at -delta (sixteen registers that hold it) where that does not spill; else subtract it
+  constexpr bool kInit = sizeof(T) == 2 ? DP <= 32 : DP > 64;
+  extern __shared__ __attribute__((aligned(512))) char sm[];          // [stages][K tile | V tile | bias | codes] | rings
   const so_mha_desc& D = P.d;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
   const int G = D.Hq / D.Hk;
   const BlockOf blk = block_of(D.B, D.Hk, G * P.qtiles);
   const int b = blk.b, hk = blk.hk, head = hk * G + blk.idx / P.qtiles, qtile = blk.idx % P.qtiles, bh = b * D.Hq + head;
-  const int q0 = qtile * 128, qlast = (q0 + 128 < D.Lq ? q0 + 128 : D.Lq) - 1;
-  const int row = q0 + 32 * wave + li;
-  const bool rowv = row < D.Lq;
-  const int qi = rowv ? row : qlast;
+  const int q0 = qtile * 128;
+  // this lane's query and its code; lanes without one compute with a place in the block's range and zero operands
+  int cqf, cql, row = q0 + 32 * wave + li, cq = 0, cq16 = 0;
+  block_codes(D, qtile, BIAS == 2, cqf, cql);
+  bool rowv = row < D.Lq;
+  if constexpr (BIAS == 2) {
+    const MapQuery m = map_query(D, row);
+    row = m.y * D.width + m.x - D.q_start;
+    rowv = m.x < D.width && row >= 0 && row < D.Lq;
+    cq = m.y * (2 * D.width - 1) + m.x;
+    cq16 = cq - (li & 15);
+    cq = cq < cqf ? cqf : cq > cql ? cql : cq;
+  } else {
+    cq = rowv ? D.q_start + row : cql;
+  }
+  const int qi = rowv ? row : 0;
+  const bool idle = !__any(rowv);      // this wave only helps to fill tiles
 
   const unsigned long long* words = D.words ? (const unsigned long long*)D.words + (size_t)b * D.nwords : nullptr;
   int t0, t1;
@@ -137,25 +172,20 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
   }
   const size_t stat = ((size_t)b * D.Hq + head) * D.Lq + qi;
   const float lse = rowv ? D.lse[stat] : INFINITY;
-  if (rowv && half == 0) D.delta[stat] = delta;
+  if (rowv && half == 0) D.delta[stat] = -delta;
 
-  // codes of the block's first and last row; the first offset of tile t's piece of the bias is code(first key) - code(last row).  In a
-  // sequence rows behind the last count as well.
+  // the first offset of tile t's piece of the bias is code(first key) - code(last query)
   const int STAGE = P.stage_bytes;
   const Reader<T, DP> rd(sm, lane);
   constexpr int HALF = 32 * TL::kRowBytes;      // the second 32 rows of a tile
-  const int cqf = BIAS == 0 ? 0 : BIAS == 1 ? D.q_start + q0 : D.code[D.q_start + q0];
-  const int cql = BIAS == 0 ? 0 : BIAS == 1 ? D.q_start + qlast : D.code[D.q_start + qlast];
-  const int cqe = BIAS == 1 ? D.q_start + q0 + 127 : cql;
-  const int mine_q = BIAS == 0 ? 0 : BIAS == 1 ? cqe - (D.q_start + row) : cqe - D.code[D.q_start + qi];   // this lane's place in a piece
-  const float* bias = BIAS ? D.bias + (size_t)head * D.V + D.code_max - cqe : nullptr;
+  const int mine_q = BIAS == 0 ? 0 : cql - cq + (BIAS == 1 ? 16 * half : 0);      // this lane's place in a tile's piece of the bias
+  const float* bias = BIAS ? D.bias + (size_t)head * D.V + D.code_max - cql : nullptr;
 
   // bias gradient: rings cleared, strip filled with zeros up to the first offset that the walk can reach
-  constexpr int RINGS = BIAS == 1 ? 8 : 4;
+  constexpr int RINGS = 8;
   const bool want = BIAS && D.strips != nullptr;
   float* rings = reinterpret_cast<float*>(sm + P.stages * STAGE);
-  float* mine = rings + wave * (RINGS / 4) * P.ring;
-  float* skew = rings + RINGS * P.ring + wave * kSkew;               // maps only
+  float* mine = rings + (2 * wave + half) * P.ring;
   const int qw = D.q_start + q0 + 32 * wave;                         // first token of the wave's rows
   const int rmask = P.ring - 1;
   const int v0 = -cql;                                                 // code[0] = 0
@@ -195,10 +225,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
     char* kt = sm + st * STAGE;
     fk.fill(kt, kb + (size_t)t * BK * D.skl, next, 0, wave_u);
     fv.fill(kt + TILE, vb + (size_t)t * BK * D.svl, next, 0, wave_u);
-    if constexpr (BIAS == 1) fill_dwords<4>(kt + 2 * TILE, bias + t * BK, BK + 127, 0x7FFFFFFFu, wave_u, lane);
+    if constexpr (BIAS == 1) fill_dwords<4>(kt + 2 * TILE, bias + t * BK, BK + cql - cqf, 0x7FFFFFFFu, wave_u, lane);
     if constexpr (BIAS == 2) {
       const int c0 = D.code[t * BK];
-      fill_dwords<4>(kt + 2 * TILE, bias + c0, D.code[t * BK + BK - 1] - cqf - (c0 - cqe) + 1, 0x7FFFFFFFu, wave_u, lane);
+      fill_dwords<4>(kt + 2 * TILE, bias + c0, D.code[t * BK + BK - 1] - cqf - (c0 - cql) + 1, 0x7FFFFFFFu, wave_u, lane);
       fill_dwords<4>(kt + 2 * TILE + 4 * P.seg, D.code + t * BK, BK, 0x7FFFFFFFu, (wave_u + 1) & 3, lane);
     }
   };
@@ -214,37 +244,34 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
   __syncthreads();
   for (int t = t0; t < t1; ++t) {
     const int st = P.stages == 2 ? (t - t0) & 1 : 0;
-    const char* kt = sm + st * STAGE;
     const int rows = rd.rows + st * STAGE, cols = rd.cols + st * STAGE;
-    const float* seg = reinterpret_cast<const float*>(kt + 2 * TILE);
-    const int* codes = reinterpret_cast<const int*>(seg + P.seg);
+    const int seg = opaque(lds_at(sm) + st * STAGE + 2 * TILE + 4 * mine_q), codes = lds_at(sm) + st * STAGE + 2 * TILE + 4 * P.seg;
     const unsigned long long w64 = next;
     if (P.stages == 2 && t + 1 < t1) fetch(t + 1, st ^ 1);
     // offsets below those of this tile are final, and nothing adds to them any more (a sequence's rings are written up to the last
     // row's first key exclusively)
-    if (want && t > t0) flush(BIAS == 1 ? t * BK - D.q_start - q0 - 128 : codes[0] - cql, t & 3);
+    if (want && t > t0) flush(BIAS == 1 ? t * BK - D.q_start - q0 - 128 : lds_read<int>(codes) - cql, t & 3);
+    if (!idle) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int key0 = t * BK + 32 * u;
       f32x16 s, dp;
       if constexpr (BIAS == 1) {
-        const float* at = seg + 32 * u + 16 * half + mine_q;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = at[r];
+        lds_read16(seg + 128 * u, s);
       } else if constexpr (BIAS == 2) {
-        const float* at = seg + mine_q - codes[0];
+        const int first = lds_read<int>(codes);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const i32x4 c = *reinterpret_cast<const i32x4*>(codes + 32 * u + 16 * half + 4 * g);
+          const i32x4 c = lds_read<i32x4>(codes + 64 * half + 128 * u + 16 * g);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[4 * g + e] = at[c[e]];
+          for (int e = 0; e < 4; ++e) s[4 * g + e] = lds_read<float>(seg + 4 * (c[e] - first));
         }
       } else {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = 0.f;
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) dp[r] = 0.f;
+      for (int r = 0; r < 16; ++r) dp[r] = kInit ? -delta : 0.f;
       if (u == 0) {
         const int rb = opaque(rows);
 #pragma unroll
@@ -260,9 +287,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
         phase(f, [&](int m, const frag& a) { s = mma(a, q[m], s); }, [&](int m) { return rd.col(cb, m % NT, m / NT, HALF * u); });
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = exp2_(__builtin_fmaf(s[r], P.c, -lse)) * (dp[r] - delta);      // dS
+      for (int r = 0; r < 16; ++r) s[r] = exp2_(__builtin_fmaf(s[r], P.c, -lse)) * (kInit ? dp[r] : dp[r] - delta);      // dS
       const unsigned w = (unsigned)(w64 >> (32 * u));
       if (w != ~0u) {
+        seldom();
         const unsigned my = w >> (16 * half);
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = (my >> r) & 1 ? s[r] : 0.f;
@@ -270,11 +298,14 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
       if constexpr (BIAS == 1) {
         if (want) {
           base = key0 + 16 * half - qw;
-          mine[half * P.ring + ((base - 1 - li) & rmask)] = diagonals(s, pend, li);
+          mine[(base - 1 - li) & rmask] = diagonals(s, pend, li);
         }
       }
       if constexpr (BIAS == 2) {
-        if (want) rectangles(s, skew, mine, rmask, key0, qw, D.width, lane);
+        if (want) {
+          const int ya = key0 / D.width, xa = key0 - ya * D.width, yb = (key0 + 16) / D.width, xb = key0 + 16 - yb * D.width;
+          map_diagonals(s, mine, rmask, half ? yb : ya, half ? xb : xa, D.width, cq16, li & 15);
+        }
       }
       frag g[NCS];
 #pragma unroll
@@ -287,6 +318,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
         last_phase(f, use);
       }
     }
+    }
     if (P.stages == 1) {
       __syncthreads();
       if (t + 1 < t1) fetch(t + 1, 0);
@@ -297,7 +329,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
   if (want) {
     if (t0 < t1) {
       if constexpr (BIAS == 1) {
-        if (li >= 16) mine[half * P.ring + ((base + 31 - li) & rmask)] = pend;
+        if (li >= 16 && !idle) mine[(base + 31 - li) & rmask] = pend;
         __syncthreads();
       }
       const int kl = (t1 * BK < D.Lk ? t1 * BK : D.Lk) - 1;
@@ -328,7 +360,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
   typedef typename Elem<T>::frag frag;
   constexpr int E = Elem<T>::E, KM = 2 * E, NM = DP / KM, NT = DP / 32, NCS = 32 / KM;
   constexpr int TILE = BK * TL::kRowBytes;
-  extern __shared__ __attribute__((aligned(16))) char sm[];          // [stages][Q tile | dO tile | lse | delta | bias | codes]
+  extern __shared__ __attribute__((aligned(512))) char sm[];          // [stages][Q tile | dO tile | lse | -delta | bias | codes]
   const so_mha_desc& D = P.d;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
   const int G = D.Hq / D.Hk;
@@ -344,6 +376,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
   const unsigned long long wb = w0 + 1 < D.nwords ? tail_word(w0 + 1, D.Lk) & (words ? words[w0 + 1] : ~0ULL) : 0ULL;
   const bool keyv = key < D.Lk, vis = ((wave < 2 ? wa : wb) >> (key & 63)) & 1;
 
+  const bool idle = !__any(vis);       // this wave only helps to fill tiles
+
   frag k[NM], v[NM];
   {
     const T* kr = (const T*)D.k + (size_t)b * D.skb + (size_t)(keyv ? key : 0) * D.skl + (size_t)hk * D.skh;
@@ -357,7 +391,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
   }
   // first key's and last key's codes; the first offset of a tile's piece of the bias is code(first key) - code(last row of the tile)
   const int ckf = BIAS == 2 ? D.code[kt * 128] : kt * 128, ckl = BIAS == 2 ? D.code[kt * 128 + 127] : kt * 128 + 127;
-  const int mine_k = BIAS == 2 ? D.code[key] - ckf : 32 * wave + li;
+  const int mine_k = BIAS == 2 ? D.code[key] - ckf : 32 * wave + li - 16 * half;
 
   const int qt = (D.Lq + BK - 1) / BK, n = (wa | wb) ? G * qt : 0;    // a block without a visible key writes zeros
   const int wave_u = __builtin_amdgcn_readfirstlane(wave);
@@ -368,7 +402,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
     char* qtile = sm + st * STAGE;
     fq.fill(qtile, (const T*)D.q + (size_t)b * D.sqb + (size_t)head * D.sqh + (size_t)q0 * D.sql, rows, 0, wave_u);
     fg.fill(qtile + TILE, (const T*)D.dout + (((size_t)b * D.Lq + q0) * D.Hq + head) * D.D, rows, 0, wave_u);
-    char* stats = qtile + 2 * TILE;
+    char* stats = qtile + 2 * TILE;      // lse | -delta | bias | codes
     const size_t at = ((size_t)b * D.Hq + head) * D.Lq + q0;
     const unsigned left = D.Lq - q0 < BK ? 4 * (D.Lq - q0) : 4 * BK;
     fill_dwords<4>(stats, D.lse + at, BK, left, wave_u, lane);
@@ -392,34 +426,35 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
   __syncthreads();
   for (int t = 0; t < n; ++t) {
     const int st = P.stages == 2 ? t & 1 : 0;
-    const char* qtile = sm + st * STAGE;
     const int rows = rd.rows + st * STAGE, cols = rd.cols + st * STAGE;
-    const float* stats = reinterpret_cast<const float*>(qtile + 2 * TILE);
+    const int stats = opaque(lds_at(sm) + st * STAGE + 2 * TILE + 64 * half), seg = opaque(lds_at(sm) + st * STAGE + 2 * TILE + 8 * BK + 4 * mine_k);
     if (P.stages == 2 && t + 1 < n) fetch(t + 1, st ^ 1);
     const int q0 = (t % qt) * BK;
+    if (!idle) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       f32x16 s, dp;
-      const int r0 = 32 * u + 16 * half;
-      if constexpr (BIAS == 1) {
-        const float* at = stats + 2 * BK + mine_k + BK - 1 - r0;
+      if constexpr (BIAS == 1) {      // rows upwards are offsets downwards
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = at[-r];
+        for (int r = 0; r < 16; ++r) s[r] = lds_read<float>(seg + 4 * (BK - 1 - 32 * u - r));
       } else if constexpr (BIAS == 2) {
-        const int* codes = reinterpret_cast<const int*>(stats + 2 * BK + P.seg);
-        const float* at = stats + 2 * BK + mine_k + codes[BK - 1];
+        const int codes = lds_at(sm) + st * STAGE + 2 * TILE + 8 * BK + 4 * P.seg, last = seg + 4 * lds_read<int>(codes + 4 * (BK - 1));
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const i32x4 c = *reinterpret_cast<const i32x4*>(codes + r0 + 4 * g);
+          const i32x4 c = lds_read<i32x4>(codes + 64 * half + 128 * u + 16 * g);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[4 * g + e] = at[-c[e]];
+          for (int e = 0; e < 4; ++e) s[4 * g + e] = lds_read<float>(last - 4 * c[e]);
         }
       } else {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = 0.f;
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) dp[r] = 0.f;
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 de = lds_read<f32x4>(stats + 4 * BK + 128 * u + 16 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dp[4 * g + e] = de[e];
+      }
       if (u == 0) {
         const int rb = opaque(rows);
 #pragma unroll
@@ -435,19 +470,20 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
         phase(f, [&](int m, const frag& a) { s = mma(a, k[m], s); }, [&](int m) { return rd.col(cb, m % NT, m / NT, TILE + HALF * u); });
       }
       const int rows_left = D.Lq - q0 - 32 * u;
-      if (rows_left < 32) {      // rows behind the last query: their bias was read from whatever lies in front of the expanded table
+      if (rows_left < 32) {      // rows behind the last query: their bias is whatever lies in front of the expanded table
+        seldom();
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = 16 * half + r < rows_left ? s[r] : -INFINITY;
       }
+      // a hidden key's lane computes like the others (its k and v are zero) and stores zeros at the end
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const f32x4 ls = *reinterpret_cast<const f32x4*>(stats + 32 * u + 16 * half + 4 * g);
-        const f32x4 de = *reinterpret_cast<const f32x4*>(stats + BK + 32 * u + 16 * half + 4 * g);
+        const f32x4 ls = lds_read<f32x4>(stats + 128 * u + 16 * g);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = 4 * g + e;
-          s[r] = vis ? exp2_(__builtin_fmaf(s[r], P.c, -ls[e])) : 0.f;
-          dp[r] = s[r] * (dp[r] - de[e]);
+          s[r] = exp2_(__builtin_fmaf(s[r], P.c, -ls[e]));
+          dp[r] *= s[r];
         }
       }
       frag g[NCS];
@@ -467,6 +503,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
       } else {
         last_phase(f, use);
       }
+    }
     }
     if (P.stages == 1) {
       __syncthreads();
@@ -503,7 +540,9 @@ __global__ __launch_bounds__(256) void mha_dvec_k(const BwdP P, float* dvec) {
   const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6, i = blockIdx.x * 64 + tx, h = blockIdx.y, v = i - D.code_max;
   float x = 0.f;
   for (int t = ty; t < P.qtiles; t += 4) {
-    const int ql = (128 * t + 128 < D.Lq ? 128 * t + 128 : D.Lq) - 1, at = v + D.code[D.q_start + ql];
+    int first, last;
+    block_codes(D, t, !D.linear, first, last);
+    const int at = v + last;
     if (i >= D.V || at < 0 || at >= P.strip) continue;
     const float* p = D.strips + ((size_t)h * P.qtiles + t) * P.strip + at;
 #pragma unroll 4
@@ -536,6 +575,11 @@ int make(const so_mha_desc* d, BwdP& p) {
   p.d = *d;
   p.c = d->scale * kLog2e;
   p.qtiles = (d->Lq + 127) / 128;
+  if (d->bias && !d->linear) {      // map rows padded to 16 lanes (map_query)
+    const int pitch = (d->width + 15) & ~15, rows = (d->q_start + d->Lq - 1) / d->width - d->q_start / d->width + 1;
+    if ((long long)rows * pitch > 0x7fffff00LL) return SO_ERR_SHAPE;
+    p.qtiles = (rows * pitch + 127) / 128;
+  }
   p.ktiles = (d->Lk + 127) / 128;
   p.stages = 2;
   if (d->bias) {
@@ -570,7 +614,7 @@ int launch(BwdP p, hipStream_t st) {
   typedef Tile<T, DP> TL;
   constexpr size_t tile = (size_t)BK * TL::kRowBytes;
   const size_t piece = BIAS ? 4 * (size_t)(p.seg + (BIAS == 2 ? BK : 0)) : 0;
-  const size_t rings = p.d.strips ? ((size_t)(BIAS == 1 ? 8 : 4) * p.ring + (BIAS == 2 ? 4 * kSkew : 0)) * 4 : 0;
+  const size_t rings = p.d.strips ? (size_t)8 * p.ring * 4 : 0;
   size_t stage = (2 * tile + piece + 511) & ~(size_t)511;      // the readers' XOR needs whole 512s
   p.stages = 2 * stage + rings <= kLds ? 2 : 1;
   size_t lds = p.stages * stage + rings;

@@ -123,7 +123,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
   typedef typename Elem<T>::frag frag;
   constexpr int E = Elem<T>::E, KM = 2 * E, NM = DP / KM, NT = DP / 32, NCS = 32 / KM;
   constexpr int TK = 64, TILE = TK * TL::kRowBytes, HALF = TILE / 2;
-  extern __shared__ __attribute__((aligned(16))) char sm[];         // [stages][K tile | V tile | bias | codes]
+  extern __shared__ __attribute__((aligned(512))) char sm[];         // [stages][K tile | V tile | bias | codes]
   const so_mha_desc& D = P.d;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
   const int wave_u = __builtin_amdgcn_readfirstlane(wave);
@@ -134,6 +134,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
   const int qlast = (q0 + 128 < D.Lq ? q0 + 128 : D.Lq) - 1, row = q0 + 32 * wave + li;
   const bool rowv = row < D.Lq;
   const int qi = rowv ? row : qlast;
+  const bool idle = !__any(rowv);      // this wave only helps to fill tiles
 
   const unsigned long long* words = D.words ? (const unsigned long long*)D.words + (size_t)b * D.nwords : nullptr;
   int t0, t1;
@@ -154,7 +155,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
   const int STAGE = P.stage_bytes;
   const int cqf = BIAS == 2 ? D.code[D.q_start + q0] : 0;
   const int cqe = BIAS == 0 ? 0 : BIAS == 1 ? D.q_start + q0 + 127 : D.code[D.q_start + qlast];
-  const int mine_q = BIAS == 0 ? 0 : BIAS == 1 ? 127 - 32 * wave - li : cqe - D.code[D.q_start + qi];
+  const int mine_q = BIAS == 0 ? 0 : BIAS == 1 ? 127 - 32 * wave - li + 16 * half : cqe - D.code[D.q_start + qi];
   const float* bias = BIAS ? D.bias + (size_t)head * D.V + D.code_max - cqe : nullptr;
 
   const T* kb = (const T*)D.k + (size_t)b * D.skb + (size_t)hk * D.skh;
@@ -189,24 +190,22 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
   for (int t = t0; t < t1; ++t) {
     const int st = P.stages == 2 ? (t - t0) & 1 : 0;
     const int fr = rd.rows + st * STAGE, fc = rd.cols + st * STAGE;
-    const float* seg = reinterpret_cast<const float*>(sm + st * STAGE + 2 * TILE);
+    const int seg = opaque(lds_at(sm) + st * STAGE + 2 * TILE + 4 * mine_q);      // this lane's place in the tile's piece of the bias
     const unsigned long long w64 = next;
     if (P.stages == 2 && t + 1 < t1) fetch(t + 1, st ^ 1);
+    if (!idle) {
     f32x16 s[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       if constexpr (BIAS == 1) {
-        const float* at = seg + 32 * u + 16 * half + mine_q;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[u][r] = at[r];
+        lds_read16(seg + 128 * u, s[u]);
       } else if constexpr (BIAS == 2) {
-        const int* codes = reinterpret_cast<const int*>(seg + P.seg);
-        const float* at = seg + mine_q - codes[0];
+        const int codes = lds_at(sm) + st * STAGE + 2 * TILE + 4 * P.seg, first = lds_read<int>(codes);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const i32x4 c = *reinterpret_cast<const i32x4*>(codes + 32 * u + 16 * half + 4 * g);
+          const i32x4 c = lds_read<i32x4>(codes + 64 * half + 128 * u + 16 * g);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[u][4 * g + e] = at[c[e]];
+          for (int e = 0; e < 4; ++e) s[u][4 * g + e] = lds_read<float>(seg + 4 * (c[e] - first));
         }
       } else {
 #pragma unroll
@@ -228,6 +227,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
       phase(f, [&](int k, const frag& a) { s[1] = mma(a, q[k], s[1]); }, [&](int k) { return rd.col(cb, k % NT, k / NT, TILE); });
     }
     if (w64 != ~0ULL) {
+      seldom();
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const unsigned mine = (unsigned)(w64 >> (32 * u)) >> (16 * half);
@@ -251,6 +251,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
         last_phase(f, use);
       }
     }
+    }
     if (P.stages == 1) {
       __syncthreads();
       if (t + 1 < t1) fetch(t + 1, 0);
@@ -271,7 +272,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
   typedef typename Elem<T>::frag frag;
   constexpr int E = Elem<T>::E, KM = 2 * E, NM = DP / KM, NT = DP / 32, NCS = 32 / KM;
   constexpr int TK = 128, TILE = TK * TL::kRowBytes, HALF = 32 * TL::kRowBytes;
-  extern __shared__ __attribute__((aligned(16))) char sm[];         // [stages][K tile | V tile]; at the end [4][32] m | [4][32] l | [32][DP + 1] o
+  extern __shared__ __attribute__((aligned(512))) char sm[];         // [stages][K tile | V tile]; at the end [4][32] m | [4][32] l | [32][DP + 1] o
   const so_mha_desc& D = P.d;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
   const int wave_u = __builtin_amdgcn_readfirstlane(wave);
@@ -367,6 +368,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
     }
     const unsigned w = (unsigned)(bits[wave >> 1] >> (32 * (wave & 1)));
     if (w != ~0u) {
+      seldom();
       const unsigned mine = w >> (16 * half);
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[0][r] = (mine >> r) & 1 ? s[0][r] : -INFINITY;

@@ -315,7 +315,7 @@ class RelativePositions:
             raise ValueError(f"map rows of at most 512 tokens (got {w})")
         self.shape, self.tokens, self.width = (h, w), h * w, w
         self.num_buckets, self.max_distance, self.bidirectional = num_buckets, max_distance, bidirectional
-        self.linear = int(h == 1)
+        self.linear = int(h == 1 or w == 1)      # code[t] = t
         self.code_max = (h - 1) * (2 * w - 1) + w - 1
         if 2 * self.code_max + 1 > 1 << 28:
             raise ValueError(f"shape {shape} has too many offsets")
