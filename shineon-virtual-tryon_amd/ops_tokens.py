@@ -20,30 +20,40 @@ from .ops import _require_cuda
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 
-def _dtype(*ts):
-    for t in ts:
-        _require_cuda(t)
-        if t.dtype not in _DTYPES:
-            raise TypeError(f"float32 or bfloat16 only (got {t.dtype})")
-        if t.dtype != ts[0].dtype:
-            raise TypeError(f"operands of one type only (got {ts[0].dtype} and {t.dtype})")
-        if t.device != ts[0].device:
-            raise ValueError(f"operands on one device only (got {ts[0].device} and {t.device})")
-    return _DTYPES[ts[0].dtype]
+def _dtype(t, *others):
+    """Type code of the operands; refuses CPU tensors, other types, mixed types and mixed devices."""
+    _require_cuda(t)
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"float32 or bfloat16 only (got {t.dtype})")
+    for o in others:
+        if o.dtype != t.dtype:
+            raise TypeError(f"operands of one type only (got {t.dtype} and {o.dtype})")
+        if o.device != t.device:
+            _require_cuda(o)
+            raise ValueError(f"operands on one device only (got {t.device} and {o.device})")
+    return code
 
 
 def _fp32_param(t, shape, device, what):
     if t.dtype != torch.float32:
         raise TypeError(f"{what}: float32 only (got {t.dtype})")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.device != device:
         raise ValueError(f"{what}: expected on {device}, got {t.device}")
-    return t.detach().contiguous()
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+def _launch(device, fn, what, *args):
+    """fn(*args, stream) on `device`'s current stream; launches go to the current device, so that is switched when it is another."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if device.index == torch.cuda.current_device():
+        err = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            err = fn(*args, stream)
+    if err:
+        check(err, what)
 
 
 # ------------------------------------------------------------------------------------------------
@@ -70,8 +80,7 @@ def rng_draw(state, numel):
     _require_cuda(state)
     _check_rng(state, state.device)
     out = torch.empty_like(state)
-    with torch.cuda.device(state.device):
-        check(lib().so_rng_draw(state.data_ptr(), out.data_ptr(), (int(numel) + 3) // 4, _stream(state.device)), "rng_draw")
+    _launch(state.device, lib().so_rng_draw, "rng_draw", state.data_ptr(), out.data_ptr(), (int(numel) + 3) // 4)
     return out
 
 
@@ -107,38 +116,43 @@ def _in_order(t):
     return t, rows
 
 
-def _dropout_launch(x, p, rng, residual):
-    dt = _dtype(x) if residual is None else _dtype(x, residual)
-    y = _like_rows(x)
-    if x.numel() == 0:
-        return y
-    x, (rows, c, ldx) = _in_order(x)
-    ldr = 0
-    if residual is not None:
-        residual, (rr, rc, ldr) = _in_order(residual)
-        if rr != rows:      # one of the two is dense, the other has a pitch: both as rows
-            c = c if rows > 1 else rc
-            rows = x.numel() // c
-            ldx, ldr = (ldx if ldx < x.numel() else c), (ldr if ldr < x.numel() else c)
-    with torch.cuda.device(x.device):
-        check(lib().so_dropout(dt, x.data_ptr(), ldx, None if residual is None else residual.data_ptr(), ldr, y.data_ptr(),
-                               c, rows, c, rng.data_ptr(), int(round(p * 2.0 ** 32)), 1.0 / (1.0 - p) if p < 1.0 else 0.0,
-                               _stream(x.device)), "dropout")
+def _dense_in_order(t):
+    return t.is_contiguous(memory_format=torch.channels_last) if t.dim() == 4 else t.is_contiguous()
+
+
+def _dropout_launch(dt, x, p, rng, residual):
+    n = x.numel()
+    rows, c, ldx, ldr = 1, n, n, n
+    if _dense_in_order(x) and (residual is None or _dense_in_order(residual)):
+        y = torch.empty_like(x)
+    else:
+        y = _like_rows(x)
+        x, (rows, c, ldx) = _in_order(x)
+        if residual is not None:
+            residual, (rr, rc, ldr) = _in_order(residual)
+            if rr != rows:      # one of the two is dense, the other has a pitch: both as rows
+                c = c if rows > 1 else rc
+                rows = n // c
+                ldx, ldr = (ldx if ldx < n else c), (ldr if ldr < n else c)
+    if n:
+        _launch(x.device, lib().so_dropout, "dropout", dt, x.data_ptr(), ldx, None if residual is None else residual.data_ptr(), ldr,
+                y.data_ptr(), c, rows, c, rng.data_ptr(), round(p * 4294967296.0), 1.0 / (1.0 - p) if p < 1.0 else 0.0)
     return y
 
 
 class _DropoutFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, p, rng):
-        ctx.p = p
+    def forward(ctx, x, residual, p, rng, dt):
+        ctx.cfg = (p, dt)
         ctx.save_for_backward(rng)
-        return _dropout_launch(x, p, rng, residual)
+        return _dropout_launch(dt, x, p, rng, residual)
 
     @staticmethod
     def backward(ctx, dy):
         (rng,) = ctx.saved_tensors
-        dx = _dropout_launch(dy, ctx.p, rng, None) if ctx.needs_input_grad[0] else None
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None
+        p, dt = ctx.cfg
+        need_x, need_r = ctx.needs_input_grad[:2]
+        return _dropout_launch(dt, dy, p, rng, None) if need_x else None, dy if need_r else None, None, None, None
 
 
 def dropout(x, p, rng, residual=None):
@@ -149,13 +163,11 @@ def dropout(x, p, rng, residual=None):
     p = float(p)
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout probability outside [0, 1]: {p}")
-    _dtype(x)
+    dt = _dtype(x) if residual is None else _dtype(x, residual)
     _check_rng(rng, x.device)
-    if residual is not None:
-        _dtype(x, residual)
-        if residual.shape != x.shape:
-            raise ValueError(f"residual of shape {tuple(residual.shape)} for x of shape {tuple(x.shape)}")
-    return _DropoutFn.apply(x, residual, p, rng)
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"residual of shape {tuple(residual.shape)} for x of shape {tuple(x.shape)}")
+    return _DropoutFn.apply(x, residual, p, rng, dt)
 
 
 # ------------------------------------------------------------------------------------------------
@@ -191,50 +203,41 @@ def _heads(t, what):
 
 class _QkNormRotaryFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, wq, wk, cos, sin, positions, start, eps):
-        dt = _dtype(q, k)
+    def forward(ctx, q, k, wq, wk, cos, sin, positions, start, eps, dt):
         q, k = _heads(q, "q"), _heads(k, "k")
         b, n, hq, d = q.shape
         yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
         ctx.save_for_backward(q, k, wq, wk, cos, sin, positions)
-        ctx.cfg = (dt, start, eps)
-        if q.numel():
-            with torch.cuda.device(q.device):
-                check(lib().so_qk_norm_rotary_fwd(*_QkNormRotaryFn._common(dt, q, k, wq, wk, cos, sin, positions, start),
-                                                  yq.data_ptr(), yk.data_ptr(), b, n, d, 2 * cos.shape[1], eps, _stream(q.device)),
-                      "qk_norm_rotary_fwd")
+        pp = p64 = psb = psl = 0
+        if positions is not None:
+            pp, p64, psl = positions.data_ptr(), int(positions.dtype == torch.int64), positions.stride(-1)
+            psb = positions.stride(0) if positions.dim() == 2 else 0
+        # what both passes read, in the order of the C entry points (the tensors are saved and stay where they are)
+        head = (dt, q.data_ptr(), *q.stride()[:3], hq, k.data_ptr(), *k.stride()[:3], k.shape[2], wq.data_ptr(), wk.data_ptr(),
+                cos.data_ptr(), sin.data_ptr(), cos.shape[0], pp, p64, psb, psl, start)
+        tail = (b, n, d, 2 * cos.shape[1], eps)
+        ctx.args = (head, tail)
+        if b and n:
+            _launch(q.device, lib().so_qk_norm_rotary_fwd, "qk_norm_rotary_fwd", *head, yq.data_ptr(), yk.data_ptr(), *tail)
         return yq, yk
 
     @staticmethod
-    def _common(dt, q, k, wq, wk, cos, sin, positions, start):
-        psb = psl = 0
-        if positions is not None:
-            psl = positions.stride(-1)
-            psb = positions.stride(0) if positions.dim() == 2 else 0
-        return (dt, q.data_ptr(), *q.stride()[:3], q.shape[2], k.data_ptr(), *k.stride()[:3], k.shape[2], wq.data_ptr(), wk.data_ptr(),
-                cos.data_ptr(), sin.data_ptr(), cos.shape[0], None if positions is None else positions.data_ptr(),
-                int(positions is not None and positions.dtype == torch.int64), psb, psl, start)
-
-    @staticmethod
     def backward(ctx, dyq, dyk):
-        q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
-        dt, start, eps = ctx.cfg
-        b, n, hq, d = q.shape
-        dev = q.device
+        q, k, wq, wk = ctx.saved_tensors[:4]
+        head, tail = ctx.args
         dyq, dyk = dyq.contiguous(), dyk.contiguous()
-        dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=dev)
-        if not q.numel():
-            return dq, dk, torch.zeros_like(wq), torch.zeros_like(wk), None, None, None, None, None
-        dwq, dwk = torch.empty_like(wq), torch.empty_like(wk)
+        dq, dk = torch.empty_like(dyq), torch.empty_like(dyk)
+        if not (tail[0] and tail[1]):
+            return dq, dk, torch.zeros_like(wq), torch.zeros_like(wk), None, None, None, None, None, None
+        d = tail[2]
         L = lib()
-        ws = torch.empty(L.so_qk_norm_rotary_ws_floats(d), dtype=torch.float32, device=dev)
-        with torch.cuda.device(dev):
-            check(L.so_qk_norm_rotary_bwd(*_QkNormRotaryFn._common(dt, q, k, wq, wk, cos, sin, positions, start), dyq.data_ptr(),
-                                          dyk.data_ptr(), dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(), dwk.data_ptr(), b, n, d,
-                                          2 * cos.shape[1], eps, ws.data_ptr(), ws.numel(), _stream(dev)), "qk_norm_rotary_bwd")
-        return dq, dk, dwq, dwk, None, None, None, None, None
+        n = L.so_qk_norm_rotary_ws_floats(d)
+        buf = torch.empty((2 + n // d, d), dtype=torch.float32, device=q.device)      # dwq | dwk | scratch
+        at = buf.data_ptr()
+        _launch(q.device, L.so_qk_norm_rotary_bwd, "qk_norm_rotary_bwd", *head, dyq.data_ptr(), dyk.data_ptr(), dq.data_ptr(),
+                dk.data_ptr(), at, at + 4 * d, *tail, at + 8 * d, n)
+        return dq, dk, buf[0], buf[1], None, None, None, None, None, None
 
 
 def qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions=None, start=0, eps=1e-6):
@@ -243,7 +246,7 @@ def qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions=None, start=0, 
     positions: int32 / int64, [L] or [B, L]; without it token l has position start + l.  q and k may be slices of one projection.  D
     even, at most 128.  A position outside the table makes that token's outputs NaN (its position is only known on the device).
     Returns dense (q', k')."""
-    _dtype(q, k)
+    dt = _dtype(q, k)
     if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
         raise ValueError(f"q [B, L, Hq, D] and k [B, L, Hk, D] expected, got {tuple(q.shape)} and {tuple(k.shape)}")
     b, n, _, d = q.shape
@@ -251,7 +254,8 @@ def qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions=None, start=0, 
         raise ValueError(f"head size must be even and at most 128, at least one head each (got {tuple(q.shape)}, {tuple(k.shape)})")
     if cos.dim() != 2 or 2 * cos.shape[1] > d:
         raise ValueError(f"cos / sin of shape [P, R/2] with R <= {d} expected, got {tuple(cos.shape)}")
-    cos, sin = _fp32_param(cos, cos.shape, q.device, "cos"), _fp32_param(sin, cos.shape, q.device, "sin")
+    _fp32_param(cos, cos.shape, q.device, "cos")
+    _fp32_param(sin, cos.shape, q.device, "sin")
     if positions is None:
         if start < 0 or start + n > cos.shape[0]:
             raise ValueError(f"positions {start} .. {start + n - 1} outside a table of {cos.shape[0]} rows")
@@ -262,9 +266,10 @@ def qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions=None, start=0, 
             raise TypeError(f"positions: int32 or int64 on {q.device}")
         if tuple(positions.shape) not in ((n,), (b, n)):
             raise ValueError(f"positions of shape ({n},) or ({b}, {n}) expected, got {tuple(positions.shape)}")
-    for t, what in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        _fp32_param(t, (d,), q.device, what)
-    return _QkNormRotaryFn.apply(q, k, q_weight.contiguous(), k_weight.contiguous(), cos, sin, positions, int(start), float(eps))
+    _fp32_param(q_weight, (d,), q.device, "q_weight")
+    _fp32_param(k_weight, (d,), q.device, "k_weight")
+    return _QkNormRotaryFn.apply(q, k, q_weight.contiguous(), k_weight.contiguous(), cos.contiguous(), sin.contiguous(), positions,
+                                 int(start), float(eps), dt)
 
 
 # ------------------------------------------------------------------------------------------------
@@ -348,112 +353,103 @@ def _rows16(t, what):
     d = t.shape[3]
     if d % e:
         t = torch.nn.functional.pad(t, (0, e - d % e))
-    if t.data_ptr() % 16 or any(s % e for s, n in zip(t.stride()[:3], t.shape[:3]) if n > 1):
+    sb, sl, sh, _ = t.stride()
+    if t.data_ptr() % 16 or (sb % e or sl % e or sh % e) and any(s % e for s, n in zip((sb, sl, sh), t.shape) if n > 1):
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
 def _strides(t):
     """Strides of the first three axes; an axis of one entry counts as stride 0."""
-    return [s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3])]
+    (b, n, h, _), (sb, sl, sh, _) = t.shape, t.stride()
+    return sb if b > 1 else 0, sl if n > 1 else 0, sh if h > 1 else 0
 
 
 class _AttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, table, mask, rel, q_start, scale, train):
+    def forward(ctx, q, k, v, table, mask, rel, q_start, scale, train, dt):
         d_true = q.shape[3]
         q, k, v = _rows16(q, "q"), _rows16(k, "k"), _rows16(v, "v")
         b, lq, hq, d = q.shape
         lk, hk = k.shape[1], k.shape[2]
         dev, L = q.device, lib()
         o = torch.empty((b, lq, hq, d), dtype=q.dtype, device=dev)
-        ctx.dims = (d_true, q_start, scale)
-        ctx.rel = rel
-        if not q.numel() or not lk:
-            ctx.save_for_backward(q, k, v, table)
-            ctx.empty = True
-            return o.zero_()[..., :d_true]
-        ctx.empty = False
-        f = lambda *s: torch.empty(s, dtype=torch.float32, device=dev)  # noqa: E731
-        x = _Desc(dtype=_DTYPES[q.dtype], B=b, Hq=hq, Hk=hk, Lq=lq, Lk=lk, D=d, nwords=(lk + 63) // 64, scale=scale, q=q.data_ptr(),
-                  k=k.data_ptr(), v=v.data_ptr(), o=o.data_ptr())
-        (x.sqb, x.sql, x.sqh), (x.skb, x.skl, x.skh), (x.svb, x.svl, x.svh) = _strides(q), _strides(k), _strides(v)
-        words = bias = lse = o_lo = None
-        with torch.cuda.device(dev):
-            st = _stream(dev)
-            if mask is not None:
-                words = torch.empty((b, x.nwords), dtype=torch.int64, device=dev)
-                x.words = words.data_ptr()
-            if table is not None:
-                x.V, x.code_max, x.tokens, x.q_start, x.linear, x.width = (2 * rel.code_max + 1, rel.code_max, rel.tokens, q_start,
-                                                                           rel.linear, rel.width)
-                bias = f(hq * x.V + 256)      # readable on both sides: 128 floats
-                x.bias, x.code = bias.data_ptr() + 512, rel.code.data_ptr()
-            if table is not None or mask is not None:
-                check(L.so_mha_prep(None if table is None else table.data_ptr(), None if table is None else rel.lut.data_ptr(), x.V, hq,
-                                    scale, x.bias, None if mask is None else mask.data_ptr(), 0 if mask is None else mask.stride(0), b,
-                                    lk, x.words, st), "mha_prep")
+        ctx.d_true, ctx.rel, ctx.desc = d_true, rel, None
+        if not (b and lq and lk):
             if train:
-                lse = f(b, hq, lq)
-                x.lse = lse.data_ptr()
-                if q.dtype == torch.bfloat16:
-                    o_lo = torch.empty_like(o)
-                    x.o_lo = o_lo.data_ptr()
-                    x.two = int(table is not None and ctx.needs_input_grad[3])
-            parts = L.so_mha_parts(ctypes.addressof(x))
-            if parts < 0:
-                check(parts, "mha_parts")
-            if parts > 1:
-                po, pml = f(b * hq * lq * parts * d), f(b * hq * lq * parts * 2)
-                x.part_o, x.part_ml = po.data_ptr(), pml.data_ptr()
-            check(L.so_mha_fwd(ctypes.addressof(x), st), "mha_fwd")
+                ctx.save_for_backward(q, k, v, table)
+            return o.zero_()[..., :d_true]
+        x = _Desc(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr())
+        (x.sqb, x.sql, x.sqh), (x.skb, x.skl, x.skh), (x.svb, x.svl, x.svh) = _strides(q), _strides(k), _strides(v)
+        x.dtype, x.B, x.Hq, x.Hk, x.Lq, x.Lk, x.D, x.nwords, x.scale = dt, b, hq, hk, lq, lk, d, (lk + 63) // 64, scale
+        words = bias = lse = o_lo = None
+        mp = msb = tp = lp = None
+        if mask is not None:
+            words = torch.empty((b, x.nwords), dtype=torch.int64, device=dev)
+            x.words, mp, msb = words.data_ptr(), mask.data_ptr(), mask.stride(0)
+        if table is not None:
+            x.V, x.code_max, x.tokens, x.q_start, x.linear, x.width = (2 * rel.code_max + 1, rel.code_max, rel.tokens, q_start,
+                                                                       rel.linear, rel.width)
+            bias = torch.empty(hq * x.V + 256, dtype=torch.float32, device=dev)      # readable on both sides: 128 floats
+            x.bias, x.code, tp, lp = bias.data_ptr() + 512, rel.code.data_ptr(), table.data_ptr(), rel.lut.data_ptr()
+        if mp is not None or tp is not None:
+            _launch(dev, L.so_mha_prep, "mha_prep", tp, lp, x.V, hq, scale, x.bias, mp, msb or 0, b, lk, x.words)
         if train:
+            lse = torch.empty((b, hq, lq), dtype=torch.float32, device=dev)
+            x.lse = lse.data_ptr()
+            if dt == 1:
+                o_lo = torch.empty_like(o)
+                x.o_lo = o_lo.data_ptr()
+                x.two = int(table is not None and ctx.needs_input_grad[3])
+        at = ctypes.addressof(x)
+        parts = L.so_mha_parts(at)
+        if parts < 0:
+            check(parts, "mha_parts")
+        if parts > 1:
+            part = torch.empty(b * hq * lq * parts * (d + 2), dtype=torch.float32, device=dev)
+            x.part_o = part.data_ptr()
+            x.part_ml = x.part_o + 4 * b * hq * lq * parts * d
+        _launch(dev, L.so_mha_fwd, "mha_fwd", at)
+        if train:
+            ctx.desc = x      # the backward pass reads the same operands (saved: they stay where they are)
             ctx.save_for_backward(q, k, v, table, o, o_lo, lse, bias, words)
         return o if d == d_true else o[..., :d_true].contiguous()
 
     @staticmethod
     def backward(ctx, dout):
-        d_true, q_start, scale = ctx.dims
-        if ctx.empty:
+        d_true, rel = ctx.d_true, ctx.rel
+        if ctx.desc is None:
             q, k, v, table = ctx.saved_tensors
-            return (*(torch.zeros_like(t[..., :d_true]) for t in (q, k, v)), None if table is None else torch.zeros_like(table), None,
-                    None, None, None, None)
-        q, k, v, table, o, o_lo, lse, bias, words = ctx.saved_tensors
-        rel = ctx.rel
+            return (*(torch.zeros_like(t[..., :d_true]) for t in (q, k, v)), None if table is None else torch.zeros_like(table),
+                    None, None, None, None, None, None)
+        q, k, v, table, o = ctx.saved_tensors[:5]
+        x = _Desc.from_buffer_copy(ctx.desc)      # a second backward pass of the same graph must not see this one's pointers
         b, lq, hq, d = q.shape
-        lk, hk = k.shape[1], k.shape[2]
         dev, L = q.device, lib()
-        dout = dout if d == d_true else torch.nn.functional.pad(dout, (0, d - d_true))
+        if d != d_true:
+            dout = torch.nn.functional.pad(dout, (0, d - d_true))
         dout = dout.contiguous()
         if dout.data_ptr() % 16:
             dout = dout.clone()
-        dq, dk, dv = torch.empty_like(o), torch.empty((b, lk, hk, d), dtype=k.dtype, device=dev), torch.empty((b, lk, hk, d), dtype=k.dtype, device=dev)
-        f = lambda *s: torch.empty(s, dtype=torch.float32, device=dev)  # noqa: E731
-        delta, dtable = f(b, hq, lq), None
-        x = _Desc(dtype=_DTYPES[q.dtype], B=b, Hq=hq, Hk=hk, Lq=lq, Lk=lk, D=d, nwords=(lk + 63) // 64, scale=scale, q=q.data_ptr(),
-                  k=k.data_ptr(), v=v.data_ptr(), o=o.data_ptr(), o_lo=None if o_lo is None else o_lo.data_ptr(), lse=lse.data_ptr(),
-                  words=None if words is None else words.data_ptr(), dout=dout.data_ptr(), dq=dq.data_ptr(), dk=dk.data_ptr(),
-                  dv=dv.data_ptr(), delta=delta.data_ptr())
-        (x.sqb, x.sql, x.sqh), (x.skb, x.skl, x.skh), (x.svb, x.svl, x.svh) = _strides(q), _strides(k), _strides(v)
-        if bias is not None:
-            x.V, x.code_max, x.tokens, x.q_start, x.linear, x.width = (2 * rel.code_max + 1, rel.code_max, rel.tokens, q_start, rel.linear,
-                                                                       rel.width)
-            x.bias, x.code = bias.data_ptr() + 512, rel.code.data_ptr()
-        with torch.cuda.device(dev):
-            st = _stream(dev)
-            if bias is not None and ctx.needs_input_grad[3]:
-                n = L.so_mha_strip_floats(ctypes.addressof(x))
-                if n < 0:
-                    check(int(n), "mha_strip_floats")
-                strips, dvec, dtable = f(n), f(hq * x.V), f(rel.rows, hq)
-                x.strips = strips.data_ptr()
-            check(L.so_mha_bwd(ctypes.addressof(x), st), "mha_bwd")
-            if dtable is not None:
-                check(L.so_mha_dtable(ctypes.addressof(x), rel.order.data_ptr(), rel.start.data_ptr(), rel.rows, dvec.data_ptr(),
-                                      dtable.data_ptr(), st), "mha_dtable")
+        dq = torch.empty((b, lq, hq, d), dtype=q.dtype, device=dev)
+        dk, dv = (torch.empty((b, x.Lk, x.Hk, d), dtype=q.dtype, device=dev) for _ in range(2))
+        delta, dtable = torch.empty((b, hq, lq), dtype=torch.float32, device=dev), None
+        x.dout, x.dq, x.dk, x.dv, x.delta = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr()
+        at = ctypes.addressof(x)
+        if table is not None and ctx.needs_input_grad[3]:
+            n = L.so_mha_strip_floats(at)
+            if n < 0:
+                check(int(n), "mha_strip_floats")
+            strips = torch.empty(n + hq * x.V, dtype=torch.float32, device=dev)      # strips | sums over offsets
+            x.strips = strips.data_ptr()
+            dtable = torch.empty((rel.rows, hq), dtype=torch.float32, device=dev)
+        _launch(dev, L.so_mha_bwd, "mha_bwd", at)
+        if dtable is not None:
+            _launch(dev, L.so_mha_dtable, "mha_dtable", at, rel.order.data_ptr(), rel.start.data_ptr(), rel.rows, x.strips + 4 * n,
+                    dtable.data_ptr())
         if d != d_true:
             dq, dk, dv = (t[..., :d_true] for t in (dq, dk, dv))
-        return dq, dk, dv, dtable, None, None, None, None, None
+        return dq, dk, dv, dtable, None, None, None, None, None, None
 
 
 def attention(q, k, v, scale=None, key_mask=None, relative=None, bias_table=None, q_start=0):
@@ -471,7 +467,7 @@ def attention(q, k, v, scale=None, key_mask=None, relative=None, bias_table=None
 
     One or a few queries over long keys (a new token against what came before) are split over the keys.  Returns [B, Lq, Hq, D];
     differentiable in q, k, v and bias_table.  The order of all sums is fixed: the same inputs give the same bits."""
-    _dtype(q, k, v)
+    dt = _dtype(q, k, v)
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
         raise ValueError(f"q [B, Lq, Hq, D], k and v [B, Lk, Hk, D] expected, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     b, lq, hq, d = q.shape
@@ -499,4 +495,4 @@ def attention(q, k, v, scale=None, key_mask=None, relative=None, bias_table=None
     elif q_start:
         raise ValueError("q_start without relative positions")
     train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias_table))
-    return _AttentionFn.apply(q, k, v, bias_table, key_mask, relative, int(q_start), scale, train)
+    return _AttentionFn.apply(q, k, v, bias_table, key_mask, relative, int(q_start), scale, train, dt)
