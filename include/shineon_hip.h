@@ -527,18 +527,21 @@ int so_dropout(int dtype, const void* x, long long ldx, const void* residual, lo
 
 /* Per-head RMS norm of q [B][L][Hq][D] and k [B][L][Hk][D] (strides in elements, channels contiguous, D even and <= 128; weights
  * [D] fp32) followed by the rotation of the first R channels (pairs i, i + R/2) by row pos of the [P][R/2] tables; pos: int32 /
- * int64 with strides, or NULL = start + token index.  A position outside the table gives NaN.  yq, yk: dense.
+ * int64 (pos64) with strides, or NULL = start + token index.  A position outside the table gives NaN.  yq, yk: dense.
  * _bwd: dy, dq, dk dense; dwq, dwk [D]; ws: so_qk_norm_rotary_ws_floats(D) floats. */
-int so_qk_norm_rotary_fwd(int dtype, const void* q, long long sqb, long long sql, long long sqh, int Hq, const void* k, long long skb,
-                          long long skl, long long skh, int Hk, const float* wq, const float* wk, const float* cosv,
-                          const float* sinv, long long P, const void* pos, int pos64, long long pos_sb, long long pos_sl,
-                          long long start, void* yq, void* yk, int B, int L, int D, int R, float eps, void* stream);
+typedef struct so_qk_desc {
+  const void *q, *k;
+  const float *wq, *wk, *cosv, *sinv;
+  const void* pos;
+  long long sqb, sql, sqh, skb, skl, skh, P, pos_sb, pos_sl, start;
+  int dtype, Hq, Hk, pos64, B, L, D, R;
+  float eps;
+} so_qk_desc;
+int so_qk_desc_bytes(void);
+int so_qk_norm_rotary_fwd(const void* desc, void* yq, void* yk, void* stream);
 long long so_qk_norm_rotary_ws_floats(int D);
-int so_qk_norm_rotary_bwd(int dtype, const void* q, long long sqb, long long sql, long long sqh, int Hq, const void* k, long long skb,
-                          long long skl, long long skh, int Hk, const float* wq, const float* wk, const float* cosv,
-                          const float* sinv, long long P, const void* pos, int pos64, long long pos_sb, long long pos_sl,
-                          long long start, const void* dyq, const void* dyk, void* dq, void* dk, float* dwq, float* dwk, int B, int L,
-                          int D, int R, float eps, float* ws, long long ws_floats, void* stream);
+int so_qk_norm_rotary_bwd(const void* desc, const void* dyq, const void* dyk, void* dq, void* dk, float* dwq, float* dwk, float* ws,
+                          long long ws_floats, void* stream);
 
 /* ---- multi-head attention with a learned relative position bias (csrc/mha_fwd.hip, csrc/mha_bwd.hip) -----------------
  * The form of models/networks/attention/sagan.py:29-54 with heads, a scale, a key mask and positions:

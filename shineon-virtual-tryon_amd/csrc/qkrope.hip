@@ -33,6 +33,10 @@ struct QkP {
   float eps;
 };
 
+// heads of an item and blocks of a side in the backward pass.  2 x 8191 tokens, 20 heads of 128, bf16: forward 38 us with 4 heads, 56 with
+// one (4.5 TB/s); backward 61 us with 2 heads and 512 blocks (4.2 TB/s), 66 with 1024, 70 with one head, 91 with 4 (registers)
+constexpr int kHeadsFwd = 4, kHeadsBwd = 2, kBlocksBwd = 512;
+
 template <typename T, int V> struct VecOf { typedef T t __attribute__((ext_vector_type(V))); };
 template <typename T> struct VecOf<T, 1> { struct t { T v; __device__ T& operator[](int) { return v; } __device__ T operator[](int) const { return v; } }; };
 
@@ -51,7 +55,10 @@ __device__ __forceinline__ long long angle_row(const QkP& p, int b, int l) {
   return at >= 0 && at < p.P ? at : -1;
 }
 
-template <typename T, int V, bool BWD>
+// A group of lanes takes U heads of one token at a time: the angles (twice the bytes of a bf16 head) are read once for them, and their
+// loads are in flight together.  Items =
+// (token, U heads) are stepped by carries; a division per item costs as much as a head.
+template <typename T, int V, bool BWD, int U>
 __global__ __launch_bounds__(256) void qk_norm_rotary_k(const QkP p) {
   typedef typename VecOf<T, V>::t vec;
   const Side& s = p.s[blockIdx.y];
@@ -68,51 +75,62 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_k(const QkP p) {
     wb[i] = live ? s.w[cb + i] : 0.f;
     da[i] = db[i] = 0.f;
   }
-  const long long rows = (long long)p.B * p.L * s.H;
-  for (long long row = (long long)blockIdx.x * per + g; row < rows; row += (long long)s.blocks * per) {
-    const long long tok = row / s.H;
-    const int h = (int)(row - tok * s.H), b = (int)(tok / p.L), l = (int)(tok - (long long)b * p.L);
-    const T* x = (const T*)s.x + b * s.sb + l * s.sl + h * s.sh;
-    float xa[V], xb[V], cs[V], sn[V], sq = 0.f;
-    if (live) {
-      const vec a = *(const vec*)(x + ca), bb = *(const vec*)(x + cb);
-      long long at = turns ? angle_row(p, b, l) : 0;
+  const int chunks = (s.H + U - 1) / U;
+  const long long items = (long long)p.B * p.L * chunks;
+  // this group's items: first, first + step, ...; step = ((sb * L) + sl) * chunks + sc
+  const long long first = (long long)blockIdx.x * per + g, step = (long long)s.blocks * per;
+  const int sc = (int)(step % chunks), sl = (int)(step / chunks % p.L), sb = (int)(step / chunks / p.L);
+  int c = (int)(first % chunks), l = (int)(first / chunks % p.L), b = (int)(first / chunks / p.L);
+  for (long long item = first; item < items; item += step) {
+    vec xa0[U], xb0[U], ya0[U], yb0[U];
+    float cs[V], sn[V];
+    const long long row = ((long long)b * p.L + l) * s.H + c * U;
+    const int heads = live ? (s.H - c * U < U ? s.H - c * U : U) : 0;
+    const T* x = (const T*)s.x + b * s.sb + l * s.sl + (long long)(c * U) * s.sh;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        cs[i] = turns ? (at < 0 ? __builtin_nanf("") : p.cosv[at * half + ca + i]) : 1.f;
-        sn[i] = turns ? (at < 0 ? __builtin_nanf("") : p.sinv[at * half + ca + i]) : 0.f;
+    for (int u = 0; u < U; ++u)
+      if (u < heads) {
+        xa0[u] = *(const vec*)(x + u * s.sh + ca);
+        xb0[u] = *(const vec*)(x + u * s.sh + cb);
+        if (BWD) {
+          const T* dy = (const T*)s.dy + (row + u) * p.D;
+          ya0[u] = *(const vec*)(dy + ca);
+          yb0[u] = *(const vec*)(dy + cb);
+        }
       }
+    const long long at = turns ? angle_row(p, b, l) : -1;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      cs[i] = at >= 0 ? p.cosv[at * half + ca + i] : turns ? __builtin_nanf("") : 1.f;
+      sn[i] = at >= 0 ? p.sinv[at * half + ca + i] : turns ? __builtin_nanf("") : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool on = u < heads;
+      float xa[V], xb[V], sq = 0.f;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        xa[i] = (float)a[i];
-        xb[i] = (float)bb[i];
+        xa[i] = on ? (float)xa0[u][i] : 0.f;
+        xb[i] = on ? (float)xb0[u][i] : 0.f;
         sq += xa[i] * xa[i] + xb[i] * xb[i];
       }
-    }
-    sq = group_sum(sq, p.lanes);
-    const float r = 1.0f / sqrtf(sq * inv_d + p.eps);
-    T* y = (T*)s.y + row * p.D;
-    if (!BWD) {
-      if (live) {
-        vec a, bb;
+      sq = group_sum(sq, p.lanes);
+      const float r = 1.0f / sqrtf(sq * inv_d + p.eps);
+      T* y = (T*)s.y + (row + u) * p.D;
+      vec oa, ob;
+      if (!BWD) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const float na = xa[i] * r * wa[i], nb = xb[i] * r * wb[i];
-          a[i] = (T)(turns ? na * cs[i] - nb * sn[i] : na);
-          bb[i] = (T)(turns ? nb * cs[i] + na * sn[i] : nb);
+          oa[i] = (T)(turns ? na * cs[i] - nb * sn[i] : na);
+          ob[i] = (T)(turns ? nb * cs[i] + na * sn[i] : nb);
         }
-        *(vec*)(y + ca) = a;
-        *(vec*)(y + cb) = bb;
-      }
-    } else {
-      const T* dy = (const T*)s.dy + row * p.D;
-      float ga[V], gb[V], dot = 0.f;
-      if (live) {
-        const vec a = *(const vec*)(dy + ca), bb = *(const vec*)(dy + cb);
+      } else {
+        float ga[V], gb[V], dot = 0.f;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float ya = (float)a[i], yb = (float)bb[i];
-          const float na = turns ? ya * cs[i] + yb * sn[i] : ya, nb = turns ? yb * cs[i] - ya * sn[i] : yb;
+          const float ya = on ? (float)ya0[u][i] : 0.f, yb = on ? (float)yb0[u][i] : 0.f;
+          const float na = turns && on ? ya * cs[i] + yb * sn[i] : ya, nb = turns && on ? yb * cs[i] - ya * sn[i] : yb;
           xa[i] *= r;
           xb[i] *= r;
           da[i] += na * xa[i];
@@ -121,19 +139,23 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_k(const QkP p) {
           gb[i] = nb * wb[i];
           dot += ga[i] * xa[i] + gb[i] * xb[i];
         }
-      }
-      dot = group_sum(dot, p.lanes) * inv_d;
-      if (live) {
-        vec a, bb;
+        dot = group_sum(dot, p.lanes) * inv_d;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          a[i] = (T)(r * (ga[i] - xa[i] * dot));
-          bb[i] = (T)(r * (gb[i] - xb[i] * dot));
+          oa[i] = (T)(r * (ga[i] - xa[i] * dot));
+          ob[i] = (T)(r * (gb[i] - xb[i] * dot));
         }
-        *(vec*)(y + ca) = a;
-        *(vec*)(y + cb) = bb;
+      }
+      if (on) {
+        *(vec*)(y + ca) = oa;
+        *(vec*)(y + cb) = ob;
       }
     }
+    c += sc;
+    l += sl;
+    b += sb;
+    if (c >= chunks) { c -= chunks; ++l; }
+    if (l >= p.L) { l -= p.L; ++b; }
   }
   if (BWD) {
     // the block's sum of dw: each lane writes its own slots, then one thread per channel adds the row groups in order
@@ -186,18 +208,18 @@ bool fits(const QkP& p, int V, int esize, bool bwd) {
 template <typename T, int V>
 void launch(QkP& p, bool bwd, int nq, int nk, hipStream_t st) {
   const dim3 grid(nq > nk ? nq : nk, 2);
-  if (bwd) hipLaunchKernelGGL((qk_norm_rotary_k<T, V, true>), grid, dim3(256), (size_t)(256 / p.lanes) * p.D * 4, st, p);
-  else hipLaunchKernelGGL((qk_norm_rotary_k<T, V, false>), grid, dim3(256), 0, st, p);
+  if (bwd) hipLaunchKernelGGL((qk_norm_rotary_k<T, V, true, kHeadsBwd>), grid, dim3(256), (size_t)(256 / p.lanes) * p.D * 4, st, p);
+  else hipLaunchKernelGGL((qk_norm_rotary_k<T, V, false, kHeadsFwd>), grid, dim3(256), 0, st, p);
 }
 
-// blocks of one side: enough to fill the chip eight blocks deep, never more than there are groups of rows
-int side_blocks(long long rows, int per) {
+// blocks of one side: a group of rows each, at most `most` (backward: each leaves a partial sum of dw)
+int side_blocks(long long rows, int per, int most) {
   const long long n = (rows + per - 1) / per;
-  return (int)(n < 1 ? 1 : n > 1024 ? 1024 : n);
+  return (int)(n < 1 ? 1 : n > most ? most : n);
 }
 
 int run(QkP& p, int dtype, bool bwd, float* dwq, float* dwk, float* ws, long long ws_floats, hipStream_t st) {
-  if (p.B < 0 || p.L < 0 || p.s[0].H < 1 || p.s[1].H < 1 || p.D < 2 || (p.D & 1) || p.D > 128 || p.R < 0 || (p.R & 1) || p.R > p.D)
+  if (p.B < 1 || p.L < 1 || p.s[0].H < 1 || p.s[1].H < 1 || p.D < 2 || (p.D & 1) || p.D > 128 || p.R < 0 || (p.R & 1) || p.R > p.D)
     return SO_ERR_SHAPE;
   if ((dtype != SO_F32 && dtype != SO_BF16) || (!p.pos && (p.start < 0 || p.start + p.L > p.P))) return SO_ERR_SHAPE;
   const int esize = dtype == SO_F32 ? 4 : 2;
@@ -206,8 +228,8 @@ int run(QkP& p, int dtype, bool bwd, float* dwq, float* dwk, float* ws, long lon
   if (V == 1 && !fits(p, 1, esize, bwd)) return SO_ERR_ALIGN;
   p.lanes = 1;
   while (p.lanes < p.D / (2 * V)) p.lanes <<= 1;
-  const int per = 256 / p.lanes;
-  for (int i = 0; i < 2; ++i) p.s[i].blocks = side_blocks((long long)p.B * p.L * p.s[i].H, per);
+  const int per = 256 / p.lanes, u = bwd ? kHeadsBwd : kHeadsFwd;
+  for (int i = 0; i < 2; ++i) p.s[i].blocks = side_blocks((long long)p.B * p.L * ((p.s[i].H + u - 1) / u), per, bwd ? kBlocksBwd : 1 << 20);
   if (bwd) {
     if (ws_floats < (long long)(p.s[0].blocks + p.s[1].blocks) * p.D) return SO_ERR_SHAPE;
     p.s[0].part = ws;
@@ -230,14 +252,12 @@ int run(QkP& p, int dtype, bool bwd, float* dwq, float* dwk, float* ws, long lon
   return SO_LAUNCH_CHECK();
 }
 
-QkP make(const void* q, long long sqb, long long sql, long long sqh, int Hq, const void* k, long long skb, long long skl,
-         long long skh, int Hk, const float* wq, const float* wk, const float* cosv, const float* sinv, long long P, const void* pos,
-         int pos64, long long pos_sb, long long pos_sl, long long start, int B, int L, int D, int R, float eps) {
+QkP make(const so_qk_desc& d) {
   QkP p = {};
-  p.s[0].x = q; p.s[0].sb = sqb; p.s[0].sl = sql; p.s[0].sh = sqh; p.s[0].H = Hq; p.s[0].w = wq;
-  p.s[1].x = k; p.s[1].sb = skb; p.s[1].sl = skl; p.s[1].sh = skh; p.s[1].H = Hk; p.s[1].w = wk;
-  p.cosv = cosv; p.sinv = sinv; p.P = P; p.pos = pos; p.pos64 = pos64; p.pos_sb = pos_sb; p.pos_sl = pos_sl; p.start = start;
-  p.B = B; p.L = L; p.D = D; p.R = R; p.eps = eps;
+  p.s[0].x = d.q; p.s[0].sb = d.sqb; p.s[0].sl = d.sql; p.s[0].sh = d.sqh; p.s[0].H = d.Hq; p.s[0].w = d.wq;
+  p.s[1].x = d.k; p.s[1].sb = d.skb; p.s[1].sl = d.skl; p.s[1].sh = d.skh; p.s[1].H = d.Hk; p.s[1].w = d.wk;
+  p.cosv = d.cosv; p.sinv = d.sinv; p.P = d.P; p.pos = d.pos; p.pos64 = d.pos64; p.pos_sb = d.pos_sb; p.pos_sl = d.pos_sl; p.start = d.start;
+  p.B = d.B; p.L = d.L; p.D = d.D; p.R = d.R; p.eps = d.eps;
   return p;
 }
 
@@ -245,27 +265,25 @@ QkP make(const void* q, long long sqb, long long sql, long long sqh, int Hq, con
 
 extern "C" {
 
-int so_qk_norm_rotary_fwd(int dtype, const void* q, long long sqb, long long sql, long long sqh, int Hq, const void* k, long long skb,
-                          long long skl, long long skh, int Hk, const float* wq, const float* wk, const float* cosv,
-                          const float* sinv, long long P, const void* pos, int pos64, long long pos_sb, long long pos_sl,
-                          long long start, void* yq, void* yk, int B, int L, int D, int R, float eps, void* stream) {
-  QkP p = make(q, sqb, sql, sqh, Hq, k, skb, skl, skh, Hk, wq, wk, cosv, sinv, P, pos, pos64, pos_sb, pos_sl, start, B, L, D, R, eps);
+int so_qk_desc_bytes(void) { return (int)sizeof(so_qk_desc); }
+
+int so_qk_norm_rotary_fwd(const void* desc, void* yq, void* yk, void* stream) {
+  const so_qk_desc& d = *(const so_qk_desc*)desc;
+  QkP p = make(d);
   p.s[0].y = yq;
   p.s[1].y = yk;
-  return run(p, dtype, false, nullptr, nullptr, nullptr, 0, (hipStream_t)stream);
+  return run(p, d.dtype, false, nullptr, nullptr, nullptr, 0, (hipStream_t)stream);
 }
 
-long long so_qk_norm_rotary_ws_floats(int D) { return 2LL * 1024 * D; }
+long long so_qk_norm_rotary_ws_floats(int D) { return 2LL * kBlocksBwd * D; }
 
-int so_qk_norm_rotary_bwd(int dtype, const void* q, long long sqb, long long sql, long long sqh, int Hq, const void* k, long long skb,
-                          long long skl, long long skh, int Hk, const float* wq, const float* wk, const float* cosv,
-                          const float* sinv, long long P, const void* pos, int pos64, long long pos_sb, long long pos_sl,
-                          long long start, const void* dyq, const void* dyk, void* dq, void* dk, float* dwq, float* dwk, int B, int L,
-                          int D, int R, float eps, float* ws, long long ws_floats, void* stream) {
-  QkP p = make(q, sqb, sql, sqh, Hq, k, skb, skl, skh, Hk, wq, wk, cosv, sinv, P, pos, pos64, pos_sb, pos_sl, start, B, L, D, R, eps);
+int so_qk_norm_rotary_bwd(const void* desc, const void* dyq, const void* dyk, void* dq, void* dk, float* dwq, float* dwk, float* ws,
+                          long long ws_floats, void* stream) {
+  const so_qk_desc& d = *(const so_qk_desc*)desc;
+  QkP p = make(d);
   p.s[0].y = dq; p.s[0].dy = dyq;
   p.s[1].y = dk; p.s[1].dy = dyk;
-  return run(p, dtype, true, dwq, dwk, ws, ws_floats, (hipStream_t)stream);
+  return run(p, d.dtype, true, dwq, dwk, ws, ws_floats, (hipStream_t)stream);
 }
 
 }  // extern "C"

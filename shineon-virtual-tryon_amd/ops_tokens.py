@@ -201,6 +201,13 @@ def _heads(t, what):
     return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
 
 
+class _QkDesc(ctypes.Structure):
+    """so_qk_desc of include/shineon_hip.h."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "wq", "wk", "cosv", "sinv", "pos")]
+                + [(n, ctypes.c_longlong) for n in ("sqb", "sql", "sqh", "skb", "skl", "skh", "P", "pos_sb", "pos_sl", "start")]
+                + [(n, ctypes.c_int) for n in ("dtype", "Hq", "Hk", "pos64", "B", "L", "D", "R")] + [("eps", ctypes.c_float)])
+
+
 class _QkNormRotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, wq, wk, cos, sin, positions, start, eps, dt):
@@ -209,34 +216,31 @@ class _QkNormRotaryFn(torch.autograd.Function):
         yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
         ctx.save_for_backward(q, k, wq, wk, cos, sin, positions)
-        pp = p64 = psb = psl = 0
+        pp, p64, psb, psl = None, 0, 0, 0
         if positions is not None:
             pp, p64, psl = positions.data_ptr(), int(positions.dtype == torch.int64), positions.stride(-1)
             psb = positions.stride(0) if positions.dim() == 2 else 0
-        # what both passes read, in the order of the C entry points (the tensors are saved and stay where they are)
-        head = (dt, q.data_ptr(), *q.stride()[:3], hq, k.data_ptr(), *k.stride()[:3], k.shape[2], wq.data_ptr(), wk.data_ptr(),
-                cos.data_ptr(), sin.data_ptr(), cos.shape[0], pp, p64, psb, psl, start)
-        tail = (b, n, d, 2 * cos.shape[1], eps)
-        ctx.args = (head, tail)
+        # what both passes read (the tensors are saved and stay where they are)
+        ctx.desc = _QkDesc(q.data_ptr(), k.data_ptr(), wq.data_ptr(), wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), pp, *q.stride()[:3],
+                           *k.stride()[:3], cos.shape[0], psb, psl, start, dt, hq, k.shape[2], p64, b, n, d, 2 * cos.shape[1], eps)
         if b and n:
-            _launch(q.device, lib().so_qk_norm_rotary_fwd, "qk_norm_rotary_fwd", *head, yq.data_ptr(), yk.data_ptr(), *tail)
+            _launch(q.device, lib().so_qk_norm_rotary_fwd, "qk_norm_rotary_fwd", ctypes.addressof(ctx.desc), yq.data_ptr(), yk.data_ptr())
         return yq, yk
 
     @staticmethod
     def backward(ctx, dyq, dyk):
         q, k, wq, wk = ctx.saved_tensors[:4]
-        head, tail = ctx.args
+        x = ctx.desc
         dyq, dyk = dyq.contiguous(), dyk.contiguous()
         dq, dk = torch.empty_like(dyq), torch.empty_like(dyk)
-        if not (tail[0] and tail[1]):
+        if not (x.B and x.L):
             return dq, dk, torch.zeros_like(wq), torch.zeros_like(wk), None, None, None, None, None, None
-        d = tail[2]
-        L = lib()
+        d, L = x.D, lib()
         n = L.so_qk_norm_rotary_ws_floats(d)
         buf = torch.empty((2 + n // d, d), dtype=torch.float32, device=q.device)      # dwq | dwk | scratch
         at = buf.data_ptr()
-        _launch(q.device, L.so_qk_norm_rotary_bwd, "qk_norm_rotary_bwd", *head, dyq.data_ptr(), dyk.data_ptr(), dq.data_ptr(),
-                dk.data_ptr(), at, at + 4 * d, *tail, at + 8 * d, n)
+        _launch(q.device, L.so_qk_norm_rotary_bwd, "qk_norm_rotary_bwd", ctypes.addressof(x), dyq.data_ptr(), dyk.data_ptr(),
+                dq.data_ptr(), dk.data_ptr(), at, at + 4 * d, at + 8 * d, n)
         return dq, dk, buf[0], buf[1], None, None, None, None, None, None
 
 

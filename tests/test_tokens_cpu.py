@@ -90,7 +90,15 @@ def test_c_entry_points_refuse_before_launching():
     assert L.so_dropout(0, None, 4, None, 0, None, 4, 1, 4, None, 2 ** 32 + 1, 1.0, None) == shape
     assert L.so_dropout(0, None, 4, None, 0, None, 4, 0, 4, None, 0, 1.0, None) == 0
     assert L.so_rng_draw(None, None, 1, None) == shape
-    qk = (0, 256, 64, 64, 64, 1, 256, 64, 64, 64, 1, 256, 256, 256, 256)
-    assert L.so_qk_norm_rotary_fwd(*qk, 4, None, 0, 0, 0, 0, 256, 256, 1, 5, 64, 64, 1e-6, None) == shape      # five tokens, four rows of angles
-    assert L.so_qk_norm_rotary_fwd(*qk, 8, None, 0, 0, 0, 0, 256, 256, 1, 5, 63, 62, 1e-6, None) == shape
-    assert L.so_qk_norm_rotary_bwd(*qk, 8, None, 0, 0, 0, 0, 256, 256, 256, 256, 256, 256, 1, 5, 64, 64, 1e-6, 256, 10, None) == shape
+    assert L.so_qk_desc_bytes() == ctypes.sizeof(tok._QkDesc)
+
+    def qk(**kw):
+        base = dict(q=256, k=256, wq=256, wk=256, cosv=256, sinv=256, sqb=320, sql=64, sqh=64, skb=320, skl=64, skh=64, P=8, dtype=0, Hq=1, Hk=1, B=1,
+                    L=5, D=64, R=64, eps=1e-6)
+        return ctypes.addressof(keep.setdefault(str(kw), tok._QkDesc(**{**base, **kw})))
+
+    keep = {}
+    for kw, want in ((dict(P=4), shape), (dict(start=4), shape), (dict(start=-1), shape), (dict(D=63), shape), (dict(R=63), shape), (dict(R=66), shape),
+                     (dict(D=130), shape), (dict(dtype=3), shape), (dict(Hk=0), shape), (dict(q=258), align)):
+        assert L.so_qk_norm_rotary_fwd(qk(**kw), 256, 256, None) == want, kw
+    assert L.so_qk_norm_rotary_bwd(qk(), 256, 256, 256, 256, 256, 256, 256, 10, None) == shape      # too little scratch
