@@ -10,6 +10,7 @@
 // A block is four waves; mha_fwd_k takes 128 rows of a head, mha_few_k (at most 32 rows to a key head) all rows and cuts the keys over its
 // waves.  When there are too few blocks to fill the chip the keys are cut into parts as well, each leaves (o, m, l) in fp32 and mha_join_k
 // merges them.
+#include <math.h>
 #include "mha.h"
 
 using namespace mha;
@@ -604,17 +605,36 @@ int so_mha_prep(const float* table, const void* lut, int V, int H, float scale, 
   return SO_LAUNCH_CHECK();
 }
 
-// parts of the key axis: enough blocks to give every CU two, at least two tiles of keys to a part
+// Parts of the key axis.  Few rows (bound by reading keys): enough blocks to give every CU two, at least two tiles to a part.  Many rows:
+// blocks that share a CU share its matrix pipes, so the pass takes as long as the CU with most blocks - ceil(blocks parts / 256) / parts
+// of a block's time - and joining costs a launch and 8 bytes per element and part; the cheapest of up to eight parts is taken.  (bf16, 64 x
+// 36 map, 2 x 8 heads of 64, 288 blocks: PARTS_A; fp32, 2 x 2049 tokens, 8 heads of 64, 272 blocks: PARTS_B.)
 int so_mha_parts(const void* desc) {
   const so_mha_desc* d = (const so_mha_desc*)desc;
   const int err = so_mha_check(d);
   if (err) return err;
-  const bool few = is_few(d);
-  const long long blocks = (long long)d->B * (few ? d->Hk : (long long)d->Hq * ((d->Lq + 127) / 128));
-  const int tiles = (d->Lk + (few ? 127 : 63)) / (few ? 128 : 64);
-  long long parts = (512 + blocks - 1) / blocks;
-  if (parts > tiles / 2) parts = tiles / 2;
-  return parts < 2 ? 1 : (int)(parts > 256 ? 256 : parts);
+  if (is_few(d)) {
+    const long long blocks = (long long)d->B * d->Hk;
+    const int tiles = (d->Lk + 127) / 128;
+    long long parts = (512 + blocks - 1) / blocks;
+    if (parts > tiles / 2) parts = tiles / 2;
+    return parts < 2 ? 1 : (int)(parts > 256 ? 256 : parts);
+  }
+  const double full = d->Lq / 128, left = d->Lq % 128 ? (d->Lq % 128 + 31) / 32 * 0.25 : 0.0;      // a last tile pays for its waves with rows
+  const double blocks = (double)d->B * d->Hq * (full + left);
+  const double rate = d->dtype == SO_F32 ? 0.45e6 : 3.0e6;                                         // FLOP per us that a CU reaches in this kernel
+  const double block_us = 4.0 * 128 * d->D * d->Lk / rate, rows = (double)d->B * d->Hq * d->Lq;
+  const int tiles = (d->Lk + 63) / 64;
+  int best = 1;
+  double least = 0;
+  for (int p = 1; p <= 8 && p <= tiles / 2 + (p == 1); ++p) {
+    const double t = ceil(blocks * p / 256) / p * block_us + (p > 1 ? 6.0 + rows * d->D * 8 * p / 4.0e6 : 0.0);
+    if (p == 1 || t < 0.95 * least) {
+      best = p;
+      least = t;
+    }
+  }
+  return best;
 }
 
 int so_mha_fwd(const void* desc, void* stream) {

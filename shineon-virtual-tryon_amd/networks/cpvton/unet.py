@@ -8,8 +8,8 @@ of every attended block.
 from torch import nn
 
 from ... import ops
-from ..attention.sagan import SelfAttention
-from ..layers import (HipActivation, HipConv2d, HipGELU, HipInstanceNorm2d, HipBatchNorm2d, HipLeakyReLU, HipReLU,
+from ..attention import ATTENTION_TYPES
+from ..layers import (HipActivation, HipConv2d, HipDropout, HipGELU, HipInstanceNorm2d, HipBatchNorm2d, HipLeakyReLU, HipReLU,
                       HipUpsample2x, Sine, Swish)
 
 _NORMS = {"instance": HipInstanceNorm2d, "batch": HipBatchNorm2d}
@@ -30,20 +30,22 @@ def _resolve_norm(norm_layer):
 
 class UnetGenerator(nn.Module):
     def __init__(self, input_nc, output_nc, num_downs, num_attention, ngf=64, norm_layer=HipBatchNorm2d,
-                 use_dropout=False, use_self_attn=False, activation=None):
+                 use_dropout=False, use_self_attn=False, activation=None, attn_type="sagan"):
+        """attn_type: which entry of ATTENTION_TYPES the attended blocks use.  use_dropout: Dropout(0.5) behind the blocks between the
+        innermost one and the first that changes its channel count."""
         super().__init__()
-        if use_dropout:
-            raise NotImplementedError("use_dropout is never enabled on the reference's hot path")
+        if attn_type not in ATTENTION_TYPES:
+            raise ValueError(f"attn_type {attn_type!r}: one of {sorted(ATTENTION_TYPES)} expected")
 
         def attn():
-            return use_self_attn if use_self_attn and num_attention > 0 else None
+            return attn_type if use_self_attn and num_attention > 0 else None
 
         block = UnetSkipConnectionBlock(ngf * 8, ngf * 8, submodule=None, norm_layer=norm_layer, innermost=True,
                                         self_attn=attn(), activation=activation)
         num_attention -= 1
-        for _ in range(num_downs - 5):
+        for i in range(num_downs - 5):
             block = UnetSkipConnectionBlock(ngf * 8, ngf * 8, submodule=block, norm_layer=norm_layer,
-                                            self_attn=attn(), activation=activation)
+                                            self_attn=attn(), use_dropout=use_dropout, activation=activation, dropout_stream=i)
             num_attention -= 1
         for outer, inner in ((ngf * 4, ngf * 8), (ngf * 2, ngf * 4), (ngf, ngf * 2)):
             block = UnetSkipConnectionBlock(outer, inner, submodule=block, norm_layer=norm_layer,
@@ -62,7 +64,7 @@ class UnetSkipConnectionBlock(nn.Module):
          |-- downsampling -- |submodule| -- upsampling --|"""
 
     def __init__(self, outer_nc, inner_nc, input_nc=None, submodule=None, outermost=False, innermost=False,
-                 norm_layer=HipBatchNorm2d, self_attn=False, use_dropout=False, activation=None):
+                 norm_layer=HipBatchNorm2d, self_attn=False, use_dropout=False, activation=None, dropout_stream=0):
         super().__init__()
         norm_layer = _resolve_norm(norm_layer)
         self.outermost = outermost
@@ -91,8 +93,11 @@ class UnetSkipConnectionBlock(nn.Module):
         if not outermost and not innermost:
             downconv.zero_bias_grad = norm_kind                # downconv -> downnorm
         if self_attn:
-            down.append(SelfAttention(inner_nc, "relu"))
-            up.append(SelfAttention(outer_nc, "relu"))
+            attention = ATTENTION_TYPES["sagan" if self_attn is True else self_attn]
+            down.append(attention(inner_nc, "relu"))
+            up.append(attention(outer_nc, "relu"))
+        if use_dropout:
+            up.append(HipDropout(0.5, dropout_stream))
         model = down + ([] if innermost else [submodule]) + up
         self.model = nn.Sequential(*model)
 

@@ -12,7 +12,7 @@ import torch
 from torch import nn
 from torch.nn import init
 
-from .. import ops
+from .. import ops, ops_tokens
 
 
 def _ohwi_param(o, i, r, s):
@@ -163,6 +163,33 @@ class FusedReLU(nn.Module):
 
     def forward(self, x):
         return x
+
+
+class HipDropout(nn.Module):
+    """nn.Dropout(p), with the residual it is added to as an option.  The mask comes from a counter-based generator and is never stored;
+    the generator's state lives on the device and moves on with every draw, also in the replays of a captured graph.  The numbers follow
+    from torch's seed, the data-parallel rank and `stream`: modules of one network are given different streams.  The state is not part of
+    the state_dict."""
+
+    def __init__(self, p=0.5, stream=0):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"dropout probability outside [0, 1]: {p}")
+        self.p, self.stream = p, stream
+        rank = torch.distributed.get_rank() if torch.distributed.is_available() and torch.distributed.is_initialized() else 0
+        seed = torch.initial_seed() + 0x9E3779B97F4A7C15 * (65536 * stream + rank + 1)
+        self.register_buffer("rng_state", ops_tokens.rng_state(seed, "cpu"), persistent=False)
+
+    def active(self):
+        return self.training and self.p > 0.0
+
+    def forward(self, x, residual=None):
+        if not self.active():
+            return x if residual is None else ops.add(residual, x)
+        return ops_tokens.dropout(x, self.p, ops_tokens.rng_draw(self.rng_state, x.numel()), residual=residual)
+
+    def extra_repr(self):
+        return f"p={self.p}, stream={self.stream}"
 
 
 class HipUpsample2x(nn.Module):

@@ -14,6 +14,7 @@ from . import ops
 from .base_model import BaseModel
 from .io_png import StageWriter
 from .networks import init_weights
+from .networks.attention import ATTENTION_TYPES
 from .networks.cpvton.unet import UnetGenerator
 from .networks.layers import HipInstanceNorm2d
 from .networks.loss import VGGLoss
@@ -40,6 +41,9 @@ class UnetMaskModel(BaseModel):
         parser = super(UnetMaskModel, cls).modify_commandline_options(parser, is_train)
         parser.set_defaults(person_inputs=("agnostic", "densepose"))
         parser.add_argument("--pen_flow_mask", type=float, default=1.0, help="Penalty applied to flow mask loss")
+        parser.add_argument("--attn_type", default="sagan", choices=sorted(ATTENTION_TYPES),
+                            help="attention of --self_attn: sagan, or relative (heads, positions: networks/attention/relative.py)")
+        parser.add_argument("--use_dropout", action="store_true", help="Dropout(0.5) behind the middle blocks of the UNet")
         parser.add_argument("--vgg_weights", default=None, help="file with ImageNet VGG19 weights for the perceptual loss: "
                             "torchvision's vgg19 state_dict (features.N.weight/bias) or a checkpoint holding criterionVGG.*")
         parser.add_argument("--allow_random_vgg", action="store_true", help="train even though no pretrained VGG19 weights "
@@ -61,6 +65,8 @@ class UnetMaskModel(BaseModel):
             norm_layer=HipInstanceNorm2d,
             use_self_attn=hparams.self_attn,
             activation=hparams.activation,
+            use_dropout=getattr(hparams, "use_dropout", False),
+            attn_type=getattr(hparams, "attn_type", "sagan"),
         )
         self.resample = Resample2d()
         self.criterionVGG = VGGLoss(weights_file=getattr(hparams, "vgg_weights", None))

@@ -102,3 +102,50 @@ def test_c_entry_points_refuse_before_launching():
                      (dict(D=130), shape), (dict(dtype=3), shape), (dict(Hk=0), shape), (dict(q=258), align)):
         assert L.so_qk_norm_rotary_fwd(qk(**kw), 256, 256, None) == want, kw
     assert L.so_qk_norm_rotary_bwd(qk(), 256, 256, 256, 256, 256, 256, 256, 10, None) == shape      # too little scratch
+
+
+# ------------------------------------------------------------------------------------------------------------------- modules
+def test_attention_registry_and_options():
+    from shineon_virtual_tryon_amd.networks.attention import ATTENTION_TYPES
+    from shineon_virtual_tryon_amd.networks.attention.relative import RelativeAttention
+    from shineon_virtual_tryon_amd.networks.attention.sagan import SelfAttention
+    from shineon_virtual_tryon_amd.options import TrainOptions
+
+    assert ATTENTION_TYPES["sagan"] is SelfAttention and ATTENTION_TYPES["relative"] is RelativeAttention
+    base = ["--model", "tom", "--dataset", "synthetic", "--name", "t"]
+    opt = TrainOptions().parse(base, interactive=False)
+    assert opt.attn_type == "sagan" and not opt.use_dropout
+    opt = TrainOptions().parse(base + ["--self_attn", "--attn_type", "relative", "--use_dropout"], interactive=False)
+    assert opt.attn_type == "relative" and opt.use_dropout
+    for channels, head in ((512, 64), (96, 48), (1336, 8), (10, 10), (2, 2)):
+        m = RelativeAttention(channels)
+        assert (m.head_dim, m.heads) == (head, channels // head)
+    with pytest.raises(ValueError):
+        RelativeAttention(7)
+
+
+def test_unet_with_relative_attention_and_dropout():
+    """The options add modules behind the existing ones: what is there without them keeps its names, and its values for a seed."""
+    from shineon_virtual_tryon_amd.networks.attention.relative import RelativeAttention
+    from shineon_virtual_tryon_amd.networks.cpvton.unet import UnetGenerator
+    from shineon_virtual_tryon_amd.networks.layers import HipDropout
+
+    def build(**kw):
+        torch.manual_seed(3)
+        return UnetGenerator(10, 4, 7, 2, ngf=8, norm_layer="instance", activation="gelu", **kw)
+
+    plain, dropped = build(), build(use_dropout=True)
+    drops = [m for m in dropped.modules() if isinstance(m, HipDropout)]
+    assert len(drops) == 2 and all(m.p == 0.5 for m in drops) and not torch.equal(drops[0].rng_state, drops[1].rng_state)
+    assert list(plain.state_dict()) == list(dropped.state_dict())
+    assert all(torch.equal(a, b) for a, b in zip(plain.state_dict().values(), dropped.state_dict().values()))
+    again = [m for m in build(use_dropout=True).modules() if isinstance(m, HipDropout)]
+    assert all(torch.equal(a.rng_state, b.rng_state) for a, b in zip(drops, again))
+    net = build(use_self_attn=True, attn_type="relative")
+    found = [n for n, m in net.named_modules() if isinstance(m, RelativeAttention)]
+    sagan = build(use_self_attn=True)
+    assert len(found) == 4 and set(found) < {n for n, _ in sagan.named_modules()}
+    with pytest.raises(ValueError, match="attn_type"):
+        build(use_self_attn=True, attn_type="none")
+    with pytest.raises(ValueError):
+        HipDropout(1.5)

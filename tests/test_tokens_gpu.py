@@ -540,3 +540,85 @@ def test_refusals(tok):
         tok.attention(x, x, x, q_start=1)
     with pytest.raises(ValueError, match="plan is on"):
         tok.attention(x, x, x, relative=tok.RelativePositions(5, 8, 20, device="cpu"), bias_table=table)
+
+
+# ------------------------------------------------------------------------------------------------------------------- modules
+def test_relative_attention_module(tok):
+    """RelativeAttention on a map against its formula in 64 bits, outputs and the gradients of input and all parameters."""
+    from shineon_virtual_tryon_amd.networks.attention.relative import RelativeAttention
+
+    torch.manual_seed(0)
+    b, c, h, w = 2, 96, 6, 5
+    m = RelativeAttention(c, num_buckets=8, max_distance=9).cuda().train()
+    with torch.no_grad():
+        for p in (m.query_norm, m.key_norm, m.bias_table):
+            p.add_(0.3 * torch.randn_like(p))
+    x = normal(1, b, c, h, w).contiguous(memory_format=torch.channels_last).requires_grad_()
+    y = m(x)
+    dy = normal(2, b, c, h, w)
+    names = [n for n, _ in m.named_parameters()]
+    grads = torch.autograd.grad(y, [x, *m.parameters()], dy)
+    z = {n: d64(p).requires_grad_() for n, p in m.named_parameters()}
+    xd = d64(x).requires_grad_()
+    n, hd = h * w, m.head_dim
+    qkv = torch.einsum("bchw,oc->bhwo", xd, z["qkv_conv.weight"][:, :, 0, 0]) + z["qkv_conv.bias"]
+    q, k, v = qkv.reshape(b, n, 3, m.heads, hd).unbind(2)
+    cos, sin = (d64(t)[None] for t in tok.rotary_table((h, w), hd))
+    q, k = ref.norm_rotary(q, z["query_norm"], cos, sin, 1e-6), ref.norm_rotary(k, z["key_norm"], cos, sin, 1e-6)
+    s = torch.einsum("bihd,bjhd->bhij", q, k) * hd ** -0.5 + z["bias_table"].T[:, ref.pair_buckets((h, w), n, n, 0, 8, 9)]
+    o = torch.einsum("bhij,bjhd->bihd", s.softmax(-1), v).reshape(b, h, w, c)
+    want = xd + (o @ z["out_conv.weight"][:, :, 0, 0].T + z["out_conv.bias"]).permute(0, 3, 1, 2)
+    wgrads = torch.autograd.grad(want, [xd, *z.values()], d64(dy))
+    # fp32 throughout, sums over at most 3 c channels, n keys and b n rows: as many half steps of the largest entry
+    for name, a, e in zip(["y", "dx", *names], (y, *grads), (want, *wgrads)):
+        ref.check(a, e.detach(), torch.full_like(e, (3 * c + n + b * n) * ref.U32 * e.abs().max().item() + 1e-6).detach(), name)
+    assert torch.equal(m(x), m(x))
+    m.eval()
+    assert torch.equal(m(x), y)
+
+
+def test_relative_attention_dropout_and_graph(tok):
+    """With dropout: new masks every step, the same after reseeding, none in eval; first use of a shape inside a capture is refused."""
+    from shineon_virtual_tryon_amd.networks.attention.relative import RelativeAttention
+
+    torch.manual_seed(0)
+    m = RelativeAttention(32, dropout=0.4).cuda().train()
+    x = normal(1, 1, 32, 4, 4).contiguous(memory_format=torch.channels_last)
+    start = m.dropout.rng_state.clone()
+    a, b = m(x), m(x)
+    assert not torch.equal(a, b)
+    m.dropout.rng_state.copy_(start)
+    assert torch.equal(m(x), a)
+    m.eval()
+    e = m(x)
+    kept = a != x
+    assert torch.allclose((a - x)[kept], (e - x)[kept] / 0.6, rtol=1e-4, atol=1e-5) and 0.3 < kept.float().mean() < 0.9
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="first time"):
+        with torch.cuda.graph(g):
+            m(x[:, :, :3])
+
+
+def test_unet_trains_with_relative_attention_and_dropout(tok):
+    """UnetMaskModel with both options through the captured training step: gradients of every new parameter, replays draw new masks."""
+    import helpers
+    from shineon_virtual_tryon_amd.data import synthetic_batch
+    from shineon_virtual_tryon_amd.graphs import GraphedTrainStep
+    from shineon_virtual_tryon_amd.unet_mask_model import UnetMaskModel
+
+    torch.manual_seed(1)
+    model = UnetMaskModel(helpers.make_namespace(self_attn=True, attn_type="relative", use_dropout=True, activation="gelu", allow_random_vgg=True,
+                                                 ngf=8, fine_height=64, fine_width=64)).cuda().train()
+    batch = {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in synthetic_batch(1, "cpu", smooth=True).items()}
+    (opt,), _ = model.configure_optimizers()
+    step = GraphedTrainStep(model, opt, batch)
+    losses, grads = [], []
+    for _ in range(3):
+        losses.append(float(step().minimize))
+        grads.append(opt.flat_grads.clone())
+        torch.cuda.synchronize()
+    assert all(math.isfinite(v) for v in losses) and len(set(losses)) == 3          # weights stand still: only the masks differ
+    assert not torch.equal(grads[0], grads[1])
+    for name, p in model.unet.named_parameters():
+        if any(n in name for n in ("bias_table", "query_norm", "key_norm", "qkv_conv.weight", "out_conv.weight")):
+            assert p.grad.isfinite().all() and p.grad.abs().sum() > 0, name
