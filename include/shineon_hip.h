@@ -559,7 +559,7 @@ typedef struct so_mha_desc {
   const float* bias;
   const int* code;
   const void* words;
-  float *part_o, *part_ml;     /* so_mha_parts > 1: B * Hq * Lq * parts * D and * 2 floats */
+  float *part_o, *part_ml;     /* forward with so_mha_parts > 1: B * Hq * Lq * parts * D and * 2 floats; backward: so_mha_bwd_floats */
   const void* dout;            /* backward */
   void *dq, *dk, *dv;
   float* delta;                /* backward: [B][Hq][Lq] scratch */
@@ -582,6 +582,7 @@ int so_mha_fwd(const void* desc, void* stream);
 /* dq, dk, dv from dout; with strips also the per-block sums of the bias gradient over equal offsets, which so_mha_dtable adds up:
  * dtable[r][h] = sum over offsets v of row r (order[start[r]] .. order[start[r + 1] - 1]).  dvec: Hq * V floats of scratch. */
 long long so_mha_strip_floats(const void* desc);
+long long so_mha_bwd_floats(const void* desc);      /* part_o of the backward pass; 0: none needed */
 int so_mha_bwd(const void* desc, void* stream);
 int so_mha_dtable(const void* desc, const void* order, const void* start, int rows, float* dvec, float* dtable, void* stream);
 

@@ -315,3 +315,9 @@ __device__ __forceinline__ BlockOf block_of(int B, int Hk, int per) {
 }  // namespace mha
 
 int so_mha_check(const so_mha_desc* d);   // shape, type and alignment rules that all entry points share
+
+// 128-row tiles in n rows; the last pays for its 32-row waves only
+double mha_tiles(int n);
+// Parts that the sum axis of a kernel is cut into (at most `most`): blocks on one CU share its matrix pipes, so a pass takes as long as the
+// CU with most blocks, ceil(blocks parts / 256) / parts of a block's time; joining costs a launch and join_bytes per part.  More parts are taken when they bring the estimate below `gain` of the last choice.
+int mha_split_parts(double blocks, double block_flop, int dtype, double join_bytes, int most, double gain);

@@ -22,6 +22,8 @@ struct BwdP {
   float c;            // scale * log2 e
   int ring, strip;    // floats of one LDS ring (a power of two) and of one block's strip
   int stages, stage_bytes, qtiles, ktiles;
+  int dq_parts, dkv_parts;        // parts of the keys (mha_dq_k) and of the query rows (mha_dkv_k); their sums: d.part_o, joined by mha_sum_k
+  long long dkv_at;               // where those of dk, dv begin
   int seg;            // floats of the bias that a tile of 64 and a block of 128 tokens can meet, in whole 64s
 };
 
@@ -109,6 +111,36 @@ __device__ __forceinline__ void block_codes(const so_mha_desc& D, int t, bool ma
   if (first > last) first = last;
 }
 
+// one row of a part's sums
+template <int NT>
+__device__ __forceinline__ void write_part(float* out, const f32x16 (&x)[NT], int D, float scale, int half) {
+#pragma unroll
+  for (int v = 0; v < NT; ++v)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = 32 * v + 8 * g + 4 * half;
+      if (c < D) *reinterpret_cast<f32x4*>(out + c) = f32x4{x[v][4 * g] * scale, x[v][4 * g + 1] * scale, x[v][4 * g + 2] * scale, x[v][4 * g + 3] * scale};
+    }
+}
+
+// out[i] = sum over parts, in their order; four elements per thread (rows are whole 16-byte chunks)
+template <typename T>
+__global__ __launch_bounds__(256) void mha_sum_k(const float* part, T* out, long long n, int parts) {
+  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  f32x4 x = *reinterpret_cast<const f32x4*>(part + i);
+  for (int p = 1; p < parts; ++p) {
+    const f32x4 y = *reinterpret_cast<const f32x4*>(part + p * n + i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] += y[e];
+  }
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  t4 o;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = (T)x[e];
+  *reinterpret_cast<t4*>(out + i) = o;
+}
+
 // BIAS: 0 none, 1 tokens of a sequence (offset = key - query), 2 tokens of a map.  Everything a tile needs travels by LDS-DMA: K, V,
 // the piece of the expanded bias that its offsets lie in and (maps) the keys' codes; nothing in the loop waits for global memory
 // except the one drain per tile.
@@ -124,8 +156,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : DP <= 6
   const so_mha_desc& D = P.d;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
   const int G = D.Hq / D.Hk;
-  const BlockOf blk = block_of(D.B, D.Hk, G * P.qtiles);
-  const int b = blk.b, hk = blk.hk, head = hk * G + blk.idx / P.qtiles, qtile = blk.idx % P.qtiles, bh = b * D.Hq + head;
+  const BlockOf blk = block_of(D.B, D.Hk, G * P.qtiles * P.dq_parts);
+  const int b = blk.b, hk = blk.hk, part = blk.idx / (G * P.qtiles), gt = blk.idx - part * G * P.qtiles;
+  const int head = hk * G + gt / P.qtiles, qtile = gt % P.qtiles, bh = b * D.Hq + head;
   const int q0 = qtile * 128;
   // this lane's query and its code; lanes without one compute with a place in the block's range and zero operands
   int cqf, cql, row = q0 + 32 * wave + li, cq = 0, cq16 = 0;
@@ -147,6 +180,11 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : DP <= 6
   const unsigned long long* words = D.words ? (const unsigned long long*)D.words + (size_t)b * D.nwords : nullptr;
   int t0, t1;
   word_range(words, D.Lk, lane, t0, t1);
+  if (P.dq_parts > 1) {
+    const int n = t1 > t0 ? t1 - t0 : 0, per = (n + P.dq_parts - 1) / P.dq_parts;
+    t0 += part * per;
+    t1 = t0 + per < t1 ? t0 + per : t1;
+  }
 
   frag q[NM], go[NM];
   float delta = 0.f;
@@ -172,7 +210,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : DP <= 6
   }
   const size_t stat = ((size_t)b * D.Hq + head) * D.Lq + qi;
   const float lse = rowv ? D.lse[stat] : INFINITY;
-  if (rowv && half == 0) D.delta[stat] = -delta;
+  if (rowv && half == 0 && part == 0) D.delta[stat] = -delta;
 
   // the first offset of tile t's piece of the bias is code(first key) - code(last query)
   const int STAGE = P.stage_bytes;
@@ -189,7 +227,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : DP <= 6
   const int qw = D.q_start + q0 + 32 * wave;                         // first token of the wave's rows
   const int rmask = P.ring - 1;
   const int v0 = -cql;                                                 // code[0] = 0
-  float* strip = want ? D.strips + ((size_t)bh * P.qtiles + qtile) * P.strip : nullptr;
+  float* strip = want ? D.strips + (((size_t)bh * P.qtiles + qtile) * P.dq_parts + part) * P.strip : nullptr;
   int flushed = v0;
   if (want) {
     for (int i = tid; i < RINGS * P.ring; i += 256) rings[i] = 0.f;
@@ -338,7 +376,13 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : DP <= 6
     for (int v = flushed + tid; v < v0 + P.strip; v += 256) strip[v - v0] = 0.f;
   }
   if (!rowv) return;
-  T* out = (T*)D.dq + (((size_t)b * D.Lq + qi) * D.Hq + head) * D.D;
+  const size_t orow = ((size_t)b * D.Lq + qi) * D.Hq + head;
+  if (P.dq_parts > 1) {
+    float* out = D.part_o + ((size_t)part * D.B * D.Lq * D.Hq + orow) * D.D;
+    write_part<NT>(out, dq, D.D, D.scale, half);
+    return;
+  }
+  T* out = (T*)D.dq + orow * D.D;
 #pragma unroll
   for (int v = 0; v < NT; ++v)
 #pragma unroll
@@ -368,7 +412,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
   const Reader<T, DP> rd(sm, lane);
   constexpr int HALF = 32 * TL::kRowBytes;
   // samples and heads in turn: the blocks behind a short sample's last key have nothing to do and are spread over all XCDs
-  const int bh = (int)(blockIdx.x % (unsigned)(D.B * D.Hk)), kt = (int)(blockIdx.x / (unsigned)(D.B * D.Hk)), b = bh / D.Hk, hk = bh - b * D.Hk;
+  const int bh = (int)(blockIdx.x % (unsigned)(D.B * D.Hk)), kp = (int)(blockIdx.x / (unsigned)(D.B * D.Hk)), part = kp / P.ktiles, kt = kp - part * P.ktiles, b = bh / D.Hk, hk = bh - b * D.Hk;
   const int key = kt * 128 + 32 * wave + li;
   const unsigned long long* words = D.words ? (const unsigned long long*)D.words + (size_t)b * D.nwords : nullptr;
   const int w0 = 2 * kt;
@@ -393,7 +437,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
   const int ckf = BIAS == 2 ? D.code[kt * 128] : kt * 128, ckl = BIAS == 2 ? D.code[kt * 128 + 127] : kt * 128 + 127;
   const int mine_k = BIAS == 2 ? D.code[key] - ckf : 32 * wave + li - 16 * half;
 
-  const int qt = (D.Lq + BK - 1) / BK, n = (wa | wb) ? G * qt : 0;    // a block without a visible key writes zeros
+  const int qt = (D.Lq + BK - 1) / BK, all = (wa | wb) ? G * qt : 0;    // a block without a visible key writes zeros
+  const int each = (all + P.dkv_parts - 1) / P.dkv_parts, from = part * each < all ? part * each : all, n = from + each < all ? from + each : all;
   const int wave_u = __builtin_amdgcn_readfirstlane(wave);
   const Filler<T, DP, BK, 4> fq(D.D, (unsigned)(D.sql * sizeof(T)), tid), fg(D.D, (unsigned)((size_t)D.Hq * D.D * sizeof(T)), tid);
   auto fetch = [&](int t, int st) {
@@ -421,11 +466,11 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[t][r] = dv[t][r] = 0.f;
-  if (n) fetch(0, 0);
+  if (from < n) fetch(from, 0);
   drain();
   __syncthreads();
-  for (int t = 0; t < n; ++t) {
-    const int st = P.stages == 2 ? t & 1 : 0;
+  for (int t = from; t < n; ++t) {
+    const int st = P.stages == 2 ? (t - from) & 1 : 0;
     const int rows = rd.rows + st * STAGE, cols = rd.cols + st * STAGE;
     const int stats = opaque(lds_at(sm) + st * STAGE + 2 * TILE + 64 * half), seg = opaque(lds_at(sm) + st * STAGE + 2 * TILE + 8 * BK + 4 * mine_k);
     if (P.stages == 2 && t + 1 < n) fetch(t + 1, st ^ 1);
@@ -514,6 +559,19 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
   }
   if (!keyv) return;
   const size_t at = (((size_t)b * D.Lk + key) * D.Hk + hk) * D.D;
+  if (P.dkv_parts > 1) {
+    const size_t all_rows = (size_t)D.B * D.Lk * D.Hk * D.D;
+    float* pk = D.part_o + P.dkv_at + (size_t)part * all_rows + at;
+    if (!vis) {
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dk[x][r] = dv[x][r] = 0.f;
+    }
+    write_part<NT>(pk, dk, D.D, D.scale, half);
+    write_part<NT>(pk + P.dkv_parts * all_rows, dv, D.D, 1.f, half);
+    return;
+  }
 #pragma unroll
   for (int x = 0; x < NT; ++x)
 #pragma unroll
@@ -544,9 +602,10 @@ __global__ __launch_bounds__(256) void mha_dvec_k(const BwdP P, float* dvec) {
     block_codes(D, t, !D.linear, first, last);
     const int at = v + last;
     if (i >= D.V || at < 0 || at >= P.strip) continue;
-    const float* p = D.strips + ((size_t)h * P.qtiles + t) * P.strip + at;
+    const float* p = D.strips + ((size_t)h * P.qtiles + t) * P.dq_parts * P.strip + at;
+    for (int b = 0; b < D.B; ++b)
 #pragma unroll 4
-    for (int b = 0; b < D.B; ++b) x += p[(size_t)b * D.Hq * P.qtiles * P.strip];
+      for (int i = 0; i < P.dq_parts; ++i) x += p[((size_t)b * D.Hq * P.qtiles * P.dq_parts + i) * P.strip];
   }
   red[ty][tx] = x;
   __syncthreads();
@@ -581,6 +640,13 @@ int make(const so_mha_desc* d, BwdP& p) {
     p.qtiles = (rows * pitch + 127) / 128;
   }
   p.ktiles = (d->Lk + 127) / 128;
+  const double tiles = d->bias && !d->linear ? p.qtiles : mha_tiles(d->Lq), rows = (double)d->B * d->Lq * d->Hq * d->D, keys = (double)d->B * d->Lk * d->Hk * d->D;
+  // fp32, 2 x 2049 tokens, 8 heads of 64, 272 blocks: mha_dq_k 350 us whole, 221 + 8 us in three parts
+  p.dq_parts = mha_split_parts(d->B * d->Hq * tiles, 6.0 * 128 * d->D * d->Lk, d->dtype, rows * 8, d->Lk / 128, 0.95);
+  // (blocks of keys that a mask hides end at once, which the estimate does not know: the rows are only cut for a clear gain.  2 x 4097
+  // tokens, a fifth hidden, 4 x 128: 686 us whole, 749 + 28 us in two parts)
+  p.dkv_parts = mha_split_parts(d->B * d->Hk * mha_tiles(d->Lk), 8.0 * 128 * d->D * d->Lq * (d->Hq / d->Hk), d->dtype, keys * 16, (int)((long long)d->Lq * (d->Hq / d->Hk) / 128 < 8 ? (long long)d->Lq * (d->Hq / d->Hk) / 128 : 8), 0.7);
+  p.dkv_at = p.dq_parts > 1 ? (long long)rows * p.dq_parts : 0;
   p.stages = 2;
   if (d->bias) {
     if (d->width < 1) return SO_ERR_SHAPE;
@@ -609,6 +675,12 @@ int lds_limit(K k, size_t lds) {
   return (int)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
 }
 
+template <typename T>
+int sum_parts(const float* part, void* out, long long n, int parts, hipStream_t st) {
+  hipLaunchKernelGGL(mha_sum_k<T>, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, st, part, (T*)out, n, parts);
+  return SO_LAUNCH_CHECK();
+}
+
 template <typename T, int DP, int BIAS>
 int launch(BwdP p, hipStream_t st) {
   typedef Tile<T, DP> TL;
@@ -622,7 +694,7 @@ int launch(BwdP p, hipStream_t st) {
   p.stage_bytes = (int)stage;
   int err = lds_limit(mha_dq_k<T, DP, BIAS>, lds);
   if (err) return err;
-  hipLaunchKernelGGL((mha_dq_k<T, DP, BIAS>), dim3((unsigned)((long long)p.d.B * p.d.Hq * p.qtiles)), dim3(256), lds, st, p);
+  hipLaunchKernelGGL((mha_dq_k<T, DP, BIAS>), dim3((unsigned)((long long)p.d.B * p.d.Hq * p.qtiles * p.dq_parts)), dim3(256), lds, st, p);
   err = SO_LAUNCH_CHECK();
   if (err) return err;
   stage = (2 * tile + 2 * BK * 4 + piece + 511) & ~(size_t)511;
@@ -631,8 +703,13 @@ int launch(BwdP p, hipStream_t st) {
   p.stage_bytes = (int)stage;
   err = lds_limit(mha_dkv_k<T, DP, BIAS>, lds);
   if (err) return err;
-  hipLaunchKernelGGL((mha_dkv_k<T, DP, BIAS>), dim3((unsigned)((long long)p.d.B * p.d.Hk * p.ktiles)), dim3(256), lds, st, p);
-  return SO_LAUNCH_CHECK();
+  hipLaunchKernelGGL((mha_dkv_k<T, DP, BIAS>), dim3((unsigned)((long long)p.d.B * p.d.Hk * p.ktiles * p.dkv_parts)), dim3(256), lds, st, p);
+  err = SO_LAUNCH_CHECK();
+  const long long rows = (long long)p.d.B * p.d.Lq * p.d.Hq * p.d.D, keys = (long long)p.d.B * p.d.Lk * p.d.Hk * p.d.D;
+  if (!err && p.dq_parts > 1) err = sum_parts<T>(p.d.part_o, p.d.dq, rows, p.dq_parts, st);
+  if (!err && p.dkv_parts > 1) err = sum_parts<T>(p.d.part_o + p.dkv_at, p.d.dk, keys, p.dkv_parts, st);
+  if (!err && p.dkv_parts > 1) err = sum_parts<T>(p.d.part_o + p.dkv_at + p.dkv_parts * keys, p.d.dv, keys, p.dkv_parts, st);
+  return err;
 }
 template <typename T, int DP>
 int launch_b(const BwdP& p, hipStream_t st) {
@@ -656,7 +733,14 @@ long long so_mha_strip_floats(const void* desc) {
   d.strips = &one;       // only asked whether it is wanted
   BwdP p;
   const int err = make(&d, p);
-  return err ? err : (long long)d.B * d.Hq * p.qtiles * p.strip;
+  return err ? err : (long long)d.B * d.Hq * p.qtiles * p.dq_parts * p.strip;
+}
+
+long long so_mha_bwd_floats(const void* desc) {
+  const so_mha_desc& d = *(const so_mha_desc*)desc;
+  BwdP p;
+  const int err = make(&d, p);
+  return err ? err : p.dkv_at + (p.dkv_parts > 1 ? 2LL * p.dkv_parts * d.B * d.Lk * d.Hk * d.D : 0);
 }
 
 int so_mha_bwd(const void* desc, void* stream) {
@@ -666,7 +750,8 @@ int so_mha_bwd(const void* desc, void* stream) {
   if (err) return err;
   if (!d->q || !d->k || !d->v || !d->o || !d->dout || !d->dq || !d->dk || !d->dv || !d->lse || !d->delta) return SO_ERR_SHAPE;
   if ((((uintptr_t)d->dout) | ((uintptr_t)d->dq) | ((uintptr_t)d->dk) | ((uintptr_t)d->dv)) & 15) return SO_ERR_ALIGN;
-  if ((long long)d->B * d->Hq * p.qtiles > 0x7fffffffLL || (long long)d->B * d->Hk * p.ktiles > 0x7fffffffLL) return SO_ERR_SHAPE;
+  if ((p.dq_parts > 1 || p.dkv_parts > 1) && (!d->part_o || (((uintptr_t)d->part_o) & 15))) return SO_ERR_SHAPE;
+  if ((long long)d->B * d->Hq * p.qtiles * p.dq_parts > 0x7fffffffLL || (long long)d->B * d->Hk * p.ktiles * p.dkv_parts > 0x7fffffffLL) return SO_ERR_SHAPE;
   return d->dtype == SO_F32 ? launch_d<float>(p, (hipStream_t)stream) : launch_d<__bf16>(p, (hipStream_t)stream);
 }
 

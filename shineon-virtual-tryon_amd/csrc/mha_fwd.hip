@@ -583,6 +583,22 @@ int so_mha_check(const so_mha_desc* d) {
   return 0;
 }
 
+double mha_tiles(int n) { return n / 128 + (n % 128 + 31) / 32 * 0.25; }
+
+int mha_split_parts(double blocks, double block_flop, int dtype, double join_bytes, int most, double gain) {
+  const double us = block_flop / (dtype == SO_F32 ? 0.45e6 : 3.0e6);      // what a CU reaches in these kernels, FLOP per us
+  int best = 1;
+  double least = 0;
+  for (int p = 1; p <= 8 && (p == 1 || p <= most); ++p) {
+    const double t = ceil(blocks * p / 256) / p * us + (p > 1 ? 6.0 + join_bytes * p / 4.0e6 : 0.0);
+    if (p == 1 || t < gain * least) {
+      best = p;
+      least = t;
+    }
+  }
+  return best;
+}
+
 extern "C" {
 
 int so_mha_desc_bytes(void) { return (int)sizeof(so_mha_desc); }
@@ -607,8 +623,9 @@ int so_mha_prep(const float* table, const void* lut, int V, int H, float scale, 
 
 // Parts of the key axis.  Few rows (bound by reading keys): enough blocks to give every CU two, at least two tiles to a part.  Many rows:
 // blocks that share a CU share its matrix pipes, so the pass takes as long as the CU with most blocks - ceil(blocks parts / 256) / parts
-// of a block's time - and joining costs a launch and 8 bytes per element and part; the cheapest of up to eight parts is taken.  (bf16, 64 x
-// 36 map, 2 x 8 heads of 64, 288 blocks: PARTS_A; fp32, 2 x 2049 tokens, 8 heads of 64, 272 blocks: PARTS_B.)
+// of a block's time - and joining costs a launch and 8 bytes per element and part; the cheapest of up to eight parts is taken.  (fp32, 2 x
+// 2049 tokens, 8 heads of 64, 272 blocks: 287, 244, 213, 221 us with 1, 2, 3, 4 parts; bf16, 4 x 600 tokens, 16 heads of 128, 320 blocks: 35,
+// 57, 60, 66 us; one head of 1024: 25, 19, 17, 15 us.)
 int so_mha_parts(const void* desc) {
   const so_mha_desc* d = (const so_mha_desc*)desc;
   const int err = so_mha_check(d);
@@ -620,21 +637,8 @@ int so_mha_parts(const void* desc) {
     if (parts > tiles / 2) parts = tiles / 2;
     return parts < 2 ? 1 : (int)(parts > 256 ? 256 : parts);
   }
-  const double full = d->Lq / 128, left = d->Lq % 128 ? (d->Lq % 128 + 31) / 32 * 0.25 : 0.0;      // a last tile pays for its waves with rows
-  const double blocks = (double)d->B * d->Hq * (full + left);
-  const double rate = d->dtype == SO_F32 ? 0.45e6 : 3.0e6;                                         // FLOP per us that a CU reaches in this kernel
-  const double block_us = 4.0 * 128 * d->D * d->Lk / rate, rows = (double)d->B * d->Hq * d->Lq;
-  const int tiles = (d->Lk + 63) / 64;
-  int best = 1;
-  double least = 0;
-  for (int p = 1; p <= 8 && p <= tiles / 2 + (p == 1); ++p) {
-    const double t = ceil(blocks * p / 256) / p * block_us + (p > 1 ? 6.0 + rows * d->D * 8 * p / 4.0e6 : 0.0);
-    if (p == 1 || t < 0.95 * least) {
-      best = p;
-      least = t;
-    }
-  }
-  return best;
+  const double rows = (double)d->B * d->Hq * d->Lq;
+  return mha_split_parts((double)d->B * d->Hq * mha_tiles(d->Lq), 4.0 * 128 * d->D * d->Lk, d->dtype, rows * d->D * 8, d->Lk / 128, 0.95);
 }
 
 int so_mha_fwd(const void* desc, void* stream) {

@@ -447,6 +447,12 @@ class _AttentionFn(torch.autograd.Function):
             strips = torch.empty(n + hq * x.V, dtype=torch.float32, device=dev)      # strips | sums over offsets
             x.strips = strips.data_ptr()
             dtable = torch.empty((rel.rows, hq), dtype=torch.float32, device=dev)
+        m = L.so_mha_bwd_floats(at)
+        if m:
+            if m < 0:
+                check(int(m), "mha_bwd_floats")
+            part = torch.empty(m, dtype=torch.float32, device=dev)
+            x.part_o = part.data_ptr()
         _launch(dev, L.so_mha_bwd, "mha_bwd", at)
         if dtable is not None:
             _launch(dev, L.so_mha_dtable, "mha_dtable", at, rel.order.data_ptr(), rel.start.data_ptr(), rel.rows, x.strips + 4 * n,
