@@ -85,6 +85,12 @@ __device__ __forceinline__ int opaque(int x) {
   asm volatile("" : "+v"(x));
   return x;
 }
+// Values that must have arrived here: hipcc puts its wait for a load in front of the first use, and where that is inside a loop the wait
+// (vmcnt 0) comes in every iteration and covers the fills in flight
+template <typename V>
+__device__ __forceinline__ void settle(V& x) {
+  asm volatile("" : "+v"(x));
+}
 template <typename T, int DP>
 struct Reader {
   typedef Tile<T, DP> TL;
@@ -186,6 +192,18 @@ __device__ __forceinline__ void dma16(i32x4 rsrc, int lds, unsigned off) {
 __device__ __forceinline__ void dma4(i32x4 rsrc, int lds, unsigned off) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc) : "memory", "m0");
 }
+// all but the N youngest requests of the wave have arrived
+template <int N>
+__device__ __forceinline__ void arrived() {
+  static_assert(N < 64, "six bits");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+// the wave's LDS reads so far are in registers: what they read may be overwritten
+__device__ __forceinline__ void lds_done() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
 __device__ __forceinline__ void drain() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 template <typename T, int DP, int ROWS, int WAVES>
 struct Filler {
@@ -258,6 +276,7 @@ struct KeyWords {
     if (w < first || w >= first + 64) {
       first = w;
       mine = w + lane < n ? words[w + lane] : 0ULL;
+      settle(mine);
     }
     const unsigned lo = __builtin_amdgcn_readlane((int)(unsigned)mine, w - first), hi = __builtin_amdgcn_readlane((int)(unsigned)(mine >> 32), w - first);
     return tail & (((unsigned long long)hi << 32) | lo);
@@ -272,12 +291,21 @@ __device__ __forceinline__ void word_range(const unsigned long long* words, int 
   if (!words) return;
   lo = n;
   hi = 0;
-  for (int w0 = 0; w0 < n; w0 += 64) {
-    const int w = w0 + lane;
-    const unsigned long long any = __ballot(w < n && words[w < n ? w : 0] != 0);
-    if (any) {
-      if (lo == n) lo = w0 + __builtin_ctzll(any);
-      hi = w0 + 64 - __builtin_clzll(any);
+  // eight words per lane at a time, so that a long row costs one latency per 32768 keys
+  for (int w0 = 0; w0 < n; w0 += 512) {
+    unsigned long long x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int w = w0 + 64 * j + lane;
+      x[j] = words[w < n ? w : n - 1];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const unsigned long long any = __ballot(w0 + 64 * j + lane < n && x[j] != 0);
+      if (any) {
+        if (lo == n) lo = w0 + 64 * j + __builtin_ctzll(any);
+        hi = w0 + 64 * j + 64 - __builtin_clzll(any);
+      }
     }
   }
 }

@@ -150,8 +150,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : DP <= 6
   typedef typename Elem<T>::frag frag;
   constexpr int E = Elem<T>::E, KM = 2 * E, NM = DP / KM, NT = DP / 32, NCS = 32 / KM;
   constexpr int TILE = BK * TL::kRowBytes;
-  // start the product do v^T at -delta (sixteen registers that hold it) where that does not spill; else subtract it
-  constexpr bool kInit = sizeof(T) == 2 ? DP <= 32 : DP > 64;
+  // start the product do v^T at -delta (sixteen registers that hold it) where that does not spill; else subtract it.  Never in fp32: with
+  // a C operand that outlives the MFMA, hipcc reuses its registers right behind the fp32 form, and dq came out wrong at 128 channels.
+  constexpr bool kInit = sizeof(T) == 2 && DP <= 32;
   extern __shared__ __attribute__((aligned(512))) char sm[];          // [stages][K tile | V tile | bias | codes] | rings
   const so_mha_desc& D = P.d;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
@@ -278,6 +279,11 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : DP <= 6
 #pragma unroll
     for (int r = 0; r < 16; ++r) dq[t][r] = 0.f;
   if (t0 < t1) fetch(t0, 0);
+#pragma unroll
+  for (int m = 0; m < NM; ++m) {
+    settle(q[m]);
+    settle(go[m]);
+  }
   drain();
   __syncthreads();
   for (int t = t0; t < t1; ++t) {
@@ -467,6 +473,11 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[t][r] = dv[t][r] = 0.f;
   if (from < n) fetch(from, 0);
+#pragma unroll
+  for (int m = 0; m < NM; ++m) {
+    settle(k[m]);
+    settle(v[m]);
+  }
   drain();
   __syncthreads();
   for (int t = from; t < n; ++t) {
@@ -643,9 +654,12 @@ int make(const so_mha_desc* d, BwdP& p) {
   const double tiles = d->bias && !d->linear ? p.qtiles : mha_tiles(d->Lq), rows = (double)d->B * d->Lq * d->Hq * d->D, keys = (double)d->B * d->Lk * d->Hk * d->D;
   // fp32, 2 x 2049 tokens, 8 heads of 64, 272 blocks: mha_dq_k 350 us whole, 221 + 8 us in three parts
   p.dq_parts = mha_split_parts(d->B * d->Hq * tiles, 6.0 * 128 * d->D * d->Lk, d->dtype, rows * 8, d->Lk / 128, 0.95);
-  // (blocks of keys that a mask hides end at once, which the estimate does not know: the rows are only cut for a clear gain.  2 x 4097
-  // tokens, a fifth hidden, 4 x 128: 686 us whole, 749 + 28 us in two parts)
-  p.dkv_parts = mha_split_parts(d->B * d->Hk * mha_tiles(d->Lk), 8.0 * 128 * d->D * d->Lq * (d->Hq / d->Hk), d->dtype, keys * 16, (int)((long long)d->Lq * (d->Hq / d->Hk) / 128 < 8 ? (long long)d->Lq * (d->Hq / d->Hk) / 128 : 8), 0.7);
+  // (blocks of keys that a mask hides end at once, which the estimate does not know: the rows are only cut for a clear gain.  A training
+  // pass whole / cut: bf16, 2 x 4097 tokens, 16 heads on 4, 128 channels 2125 / 1725 us, with a fifth of the keys hidden 1935 / 1530;
+  // 9000 tokens, 8 on 4, 64 channels 1127 / 999; fp32, 2 x 2049, 8 of 64 1066 / 870; 1000 tokens, 8 on 1, 128 channels 371 / 164)
+  const double q_tiles = (double)d->Lq * (d->Hq / d->Hk) / 128;
+  p.dkv_parts = mha_split_parts(d->B * d->Hk * mha_tiles(d->Lk), 8.0 * 128 * 128 * d->D * q_tiles, d->dtype, keys * 16,
+                                q_tiles < 8 ? (int)q_tiles : 8, 0.7);
   p.dkv_at = p.dq_parts > 1 ? (long long)rows * p.dq_parts : 0;
   p.stages = 2;
   if (d->bias) {

@@ -186,6 +186,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
     for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
   float m = -INFINITY, l = 0.f;
   if (t0 < t1) fetch(t0, 0);
+#pragma unroll
+  for (int m = 0; m < NM; ++m) settle(q[m]);
   drain();
   __syncthreads();
   for (int t = t0; t < t1; ++t) {
@@ -265,18 +267,32 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
 }
 
 // Few rows: all (at most 32) rows of the query heads that share a key head, row = head in group * Lq + i, so that a single token's heads
-// fill one tile.  Bound by reading keys and values: each of the four waves takes 32 of the 128 keys of a tile, and the four running
-// softmaxes are merged through LDS at the end.
-template <typename T, int DP, bool TWO>
-__global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 96 ? 2 : 1))) void mha_few_k(const FwdP P) {
+// fill one tile.  Bound by reading keys and values.  Each of the four waves walks 32 of the 128 keys of a tile by itself, with its own
+// ring of `DEPTH` pieces of keys and of values in LDS: a piece is asked for again as soon as its fragments are in registers, no wave
+// waits for another, and 64 KB per block stay in flight or in use (two blocks a CU).  The four running softmaxes are merged through LDS
+// at the end.  8 rows of 32765 keys (a tenth hidden), 16 heads on 4, 128 channels, bf16, 483 MB: 97 us, 4.95 TB/s, the rate of a large
+// copy (118 us with block-wide tiles of 64 KB, two stages and barriers).
+//
+// BIAS: 0 none, 1 a sequence's, at most kFewBias rows: 32 floats per row come with the keys, 2 any other: read into registers, where
+// hipcc's wait for them covers the fills in flight too.
+constexpr int kFewBias = 8;
+template <typename T, int DP>
+struct Few {
+  static constexpr int kPiece = 32 * Tile<T, DP>::kRowBytes;
+  static constexpr int kDepth = kPiece >= 8192 ? 1 : 8192 / kPiece;
+  static constexpr int slot(int bias) { return 2 * kPiece + (bias == 1 ? kFewBias * 128 : 0); }
+};
+template <typename T, int DP, int BIAS, bool TWO>
+__global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha_few_k(const FwdP P) {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::frag frag;
+  typedef Filler<T, DP, 32, 1> Fill;
   constexpr int E = Elem<T>::E, KM = 2 * E, NM = DP / KM, NT = DP / 32, NCS = 32 / KM;
-  constexpr int TK = 128, TILE = TK * TL::kRowBytes, HALF = 32 * TL::kRowBytes;
-  extern __shared__ __attribute__((aligned(512))) char sm[];         // [stages][K tile | V tile]; at the end [4][32] m | [4][32] l | [32][DP + 1] o
+  constexpr int PIECE = Few<T, DP>::kPiece, DEPTH = Few<T, DP>::kDepth, SLOT = Few<T, DP>::slot(BIAS), TK = 128;
+  constexpr int NV = Fill::N, NK = NV + (BIAS == 1 ? kFewBias / 2 : 0);               // requests of a piece of values, of keys and bias
+  extern __shared__ __attribute__((aligned(512))) char sm[];         // [wave][DEPTH][K | V | bias]; at the end [4][32] m | [4][32] l | [32][DP + 1] o
   const so_mha_desc& D = P.d;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
-  const int wave_u = __builtin_amdgcn_readfirstlane(wave);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, half = lane >> 5;
   const int G = D.Hq / D.Hk, rows = G * D.Lq;
   const BlockOf blk = block_of(D.B, D.Hk, P.parts);
   const int b = blk.b, hk = blk.hk, part = blk.idx;
@@ -288,9 +304,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
   word_range(words, D.Lk, lane, wlo, whi);
   int t0 = wlo / 2, t1 = (whi + 1) / 2;
   if (P.parts > 1) {
-    const int n = t1 > t0 ? t1 - t0 : 0, per = (n + P.parts - 1) / P.parts;
-    t0 += part * per;
-    t1 = t0 + per < t1 ? t0 + per : t1;
+    const int lo = t0, n = t1 > t0 ? t1 - t0 : 0;
+    t0 = lo + (int)((long long)n * part / P.parts);
+    t1 = lo + (int)((long long)n * (part + 1) / P.parts);
   }
 
   frag q[NM];
@@ -299,97 +315,135 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
 #pragma unroll
     for (int m = 0; m < NM; ++m) q[m] = as_frag<T>(load_chunk<T>(qr, 2 * m + half, rowv && (2 * m + half) * E < D.D));
   }
-  const float* bias = nullptr;
-  if (D.bias) bias = D.bias + (size_t)head * D.V + D.code_max - D.code[D.q_start + qi];
   const T* kb = (const T*)D.k + (size_t)b * D.skb + (size_t)hk * D.skh;
   const T* vb = (const T*)D.v + (size_t)b * D.svb + (size_t)hk * D.svh;
-  const Filler<T, DP, TK, 4> fk(D.D, (unsigned)(D.skl * sizeof(T)), tid), fv(D.D, (unsigned)(D.svl * sizeof(T)), tid);
-  const Reader<T, DP> rd(sm, lane);
+  const Fill fk(D.D, (unsigned)(D.skl * sizeof(T)), lane), fv(D.D, (unsigned)(D.svl * sizeof(T)), lane);
+  const int mine = wave * DEPTH * SLOT;
+  const Reader<T, DP> rd(sm + mine, lane);
   KeyWords kw(words, D.nwords, D.Lk, lane);
-  unsigned long long bits[2] = {0, 0}, next[2] = {0, 0};
-  auto fetch = [&](int t, int st) {
-    next[0] = kw.get(2 * t);
-    next[1] = kw.get(2 * t + 1);
-    char* kt = sm + st * 2 * TILE;
-    fk.fill(kt, kb + (size_t)t * TK * D.skl, next[0], next[1], wave_u);
-    fv.fill(kt + TILE, vb + (size_t)t * TK * D.svl, next[0], next[1], wave_u);
-  };
-  // initial accumulators of tile t: the bias, requested in front of the wait that ends the tile before
-  f32x16 s[1];
-  auto init = [&](int t) {
-    const int key0 = t * TK + 32 * wave + 16 * half;
-    if (!bias) {
+  const auto bits_of = [&](int t) { return (unsigned)(kw.get(2 * t + (wave >> 1)) >> (32 * (wave & 1))); };
+  const float* bias = nullptr;      // of the lane's row
+  if constexpr (BIAS == 2) bias = D.bias + (size_t)head * D.V + D.code_max - D.code[D.q_start + qi];
+  i32x4 brs = {};
+  unsigned boff[kFewBias / 2];      // rows 2 j and 2 j + 1 of the block, one key per lane
+  if constexpr (BIAS == 1) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
-    } else if (D.linear) {
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4u v = *reinterpret_cast<const f32x4u*>(bias + key0 + 4 * g);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[0][4 * g + e] = v[e];
-      }
-    } else {
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const i32x4 v = *reinterpret_cast<const i32x4*>(D.code + key0 + 4 * g);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[0][4 * g + e] = bias[v[e]];
-      }
+    for (int j = 0; j < kFewBias / 2; ++j) {
+      const int r = 2 * j + half;
+      boff[j] = r < rows ? 4u * (unsigned)((hk * G + r / D.Lq) * (long long)D.V + D.code_max - (D.q_start + r % D.Lq) + li) : 0x80000000u;
     }
+    brs = rsrc_of(D.bias, (unsigned)(4LL * D.Hq * D.V));
+  }
+  const auto fetch_k = [&](int t, int at, unsigned bits) {
+    const size_t key0 = (size_t)t * TK + 32 * wave;
+    if constexpr (BIAS == 1) {
+#pragma unroll
+      for (int j = 0; j < kFewBias / 2; ++j) dma4(brs, lds_at(sm) + at + 2 * PIECE + 256 * j, boff[j] + 4u * (unsigned)key0);
+    }
+    fk.fill(sm + at, kb + key0 * D.skl, bits | 0xFFFFFFFF00000000ULL, 0, 0);
+  };
+  const auto fetch_v = [&](int t, int at, unsigned bits) {
+    fv.fill(sm + at + PIECE, vb + ((size_t)t * TK + 32 * wave) * D.svl, bits | 0xFFFFFFFF00000000ULL, 0, 0);
   };
 
   frag f[NM];
-  f32x16 o[NT];
+  f32x16 o[NT], s[1];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
   float m = -INFINITY, l = 0.f;
-  if (t0 < t1) {
-    fetch(t0, 0);
-    init(t0);
+#pragma unroll
+  for (int k = 0; k < NM; ++k) settle(q[k]);
+  unsigned ring[DEPTH];             // visible keys of the pieces in the ring
+#pragma unroll
+  for (int i = 0; i < DEPTH; ++i) {
+    ring[i] = 0;
+    if (t0 + i < t1) {
+      ring[i] = bits_of(t0 + i);
+      fetch_k(t0 + i, mine + i * SLOT, ring[i]);
+      fetch_v(t0 + i, mine + i * SLOT, ring[i]);
+    }
   }
-  drain();
-  __syncthreads();
+  int slot = 0;
   for (int t = t0; t < t1; ++t) {
-    const int st = P.stages == 2 ? (t - t0) & 1 : 0;
-    const int fr = rd.rows + st * 2 * TILE + wave * HALF, fc = rd.cols + st * 2 * TILE + wave * HALF;
-    bits[0] = next[0];
-    bits[1] = next[1];
-    if (P.stages == 2 && t + 1 < t1) fetch(t + 1, st ^ 1);
+    const bool more = t + DEPTH < t1;
+    const unsigned w = ring[0];
+#pragma unroll
+    for (int i = 0; i + 1 < DEPTH; ++i) ring[i] = ring[i + 1];
+    if constexpr (BIAS == 2) {
+      const int key0 = t * TK + 32 * wave + 16 * half;
+      if (D.linear) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4u v = *reinterpret_cast<const f32x4u*>(bias + key0 + 4 * g);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[0][4 * g + e] = v[e];
+        }
+      } else {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const i32x4 v = *reinterpret_cast<const i32x4*>(D.code + key0 + 4 * g);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[0][4 * g + e] = bias[v[e]];
+        }
+      }
+    }
+    // requests younger than this piece's keys: its values and the pieces behind it (near the end the ring is not full: wait for all)
+    if (more) arrived<NV + (DEPTH - 1) * (NK + NV)>();
+    else arrived<0>();
     {
-      const int rb = opaque(fr);
+      const int rb = opaque(rd.rows + slot * SLOT);
 #pragma unroll
       for (int k = 0; k < NM; ++k) f[k] = rd.row(rb, k, 0);
-      __builtin_amdgcn_sched_barrier(0);
     }
-    {
-      const int cb = opaque(fc);
-      phase(f, [&](int k, const frag& a) { s[0] = mma(a, q[k], s[0]); }, [&](int k) { return rd.col(cb, k % NT, k / NT, TILE); });
+    if constexpr (BIAS == 1) {      // lanes behind the last row read a row of the ring that nobody uses
+      const int at = lds_at(sm) + mine + slot * SLOT + 2 * PIECE + 128 * (li & (kFewBias - 1)) + 64 * half;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 v = lds_read<f32x4>(at + 16 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[0][4 * g + e] = v[e];
+      }
+    } else if constexpr (BIAS == 0) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
     }
-    const unsigned w = (unsigned)(bits[wave >> 1] >> (32 * (wave & 1)));
+    if (more) {
+      ring[DEPTH - 1] = bits_of(t + DEPTH);
+      lds_done();
+      fetch_k(t + DEPTH, mine + slot * SLOT, ring[DEPTH - 1]);
+    }
+#pragma unroll
+    for (int k = 0; k < NM; ++k) s[0] = mma(f[k], q[k], s[0]);
     if (w != ~0u) {
       seldom();
-      const unsigned mine = w >> (16 * half);
+      const unsigned seen = w >> (16 * half);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[0][r] = (mine >> r) & 1 ? s[0][r] : -INFINITY;
+      for (int r = 0; r < 16; ++r) s[0][r] = (seen >> r) & 1 ? s[0][r] : -INFINITY;
     }
     softmax_step(s, o, m, l, P.c);
     frag p[NCS], lo[NCS];
     prob_frags<T, NCS, TWO>(s[0], p, lo);
+    if (more) arrived<DEPTH * NK + (DEPTH - 1) * NV>();
+    else arrived<0>();
+    {
+      const int cb = opaque(rd.cols + slot * SLOT);
+#pragma unroll
+      for (int k = 0; k < NM; ++k) f[k] = rd.col(cb, k % NT, k / NT, PIECE);
+    }
+    if (more) {
+      lds_done();
+      fetch_v(t + DEPTH, mine + slot * SLOT, ring[DEPTH - 1]);
+    }
     last_phase(f, [&](int k, const frag& a) {
       o[k % NT] = mma(a, p[k / NT], o[k % NT]);
       if constexpr (TWO) o[k % NT] = mma(a, lo[k / NT], o[k % NT]);
     });
-    if (t + 1 < t1) init(t + 1);
-    if (P.stages == 1) {
-      __syncthreads();
-      if (t + 1 < t1) fetch(t + 1, 0);
-    }
-    drain();
-    __syncthreads();
+    slot = slot + 1 < DEPTH ? slot + 1 : 0;
   }
   l = half_sum(l);
+  __syncthreads();
 
   // merge the four waves' softmaxes: statistics first, then each wave adds its scaled rows in turn
   float* stats = reinterpret_cast<float*>(sm);
@@ -427,58 +481,119 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
   write_row<T, NT>(P, o, mn, ln, b, hk, head, qi, part, half);
 }
 
-// joins the parts of a row: weights 2^(m_p - max m), fixed order.  One wave per row.
+// Joining the parts of a row: o = sum_p w_p o_p / sum_p w_p l_p with w_p = 2^(m_p - max m), in a fixed order.  Bound by the latency of
+// one round of reads, so everything is requested before the first use.
+// 128 rows of 16 parts 4.9 us (13 as a wave per row that reads its weights first), 32784 rows of 64 channels in 3 parts 10 us (19).
+// four channels of a joined row
+template <typename T>
+__device__ __forceinline__ void write_joined(const so_mha_desc& D, long long at, int c, f32x4 x, float mn, float l) {
+  const int rows = D.Hq / D.Hk * D.Lq, bh = (int)(at / rows), row = (int)(at - (long long)bh * rows), b = bh / D.Hk, hk = bh - b * D.Hk;
+  const int head = hk * (D.Hq / D.Hk) + row / D.Lq, qi = row % D.Lq;
+  const size_t orow = (((size_t)b * D.Lq + qi) * D.Hq + head) * D.D;
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  t4 hi, lo;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float v = x[e] * inv;
+    hi[e] = (T)v;
+    lo[e] = (T)(v - (float)hi[e]);
+  }
+  *reinterpret_cast<t4*>((T*)D.o + orow + c) = hi;
+  if (D.o_lo) *reinterpret_cast<t4*>((T*)D.o_lo + orow + c) = lo;
+  if (D.lse && c == 0) D.lse[((size_t)b * D.Hq + head) * D.Lq + qi] = l == 0.f ? INFINITY : mn + __builtin_amdgcn_logf(l);
+}
+
+// up to kJoin parts: half a wave per row, four channels per lane
+constexpr int kJoin = 8;
 template <typename T>
 __global__ __launch_bounds__(256) void mha_join_k(const FwdP P) {
   const so_mha_desc& D = P.d;
-  const int G = D.Hq / D.Hk, rows = G * D.Lq, lane = threadIdx.x & 63;
-  const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (at >= (long long)D.B * D.Hk * rows) return;
-  const int bh = (int)(at / rows), row = (int)(at - (long long)bh * rows), b = bh / D.Hk, hk = bh - b * D.Hk;
-  // lane p holds the statistics of part p (and of p + 64, ...: at most 256)
+  const long long at = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), n = (long long)D.B * D.Hq * D.Lq;
+  const int c = 4 * (threadIdx.x & 31);
+  if (at >= n || c >= D.D) return;
   const float* ml = D.part_ml + 2 * at * P.parts;
-  float mp[4], w[4], mn = -INFINITY, l = 0.f;
+  const float* po = D.part_o + at * P.parts * D.D + c;
+  float m[kJoin], l[kJoin], mn = -INFINITY, ln = 0.f;
+  f32x4 o[kJoin], x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int p = lane + 64 * i;
-    mp[i] = p < P.parts ? ml[2 * p] : -INFINITY;
-    w[i] = p < P.parts ? ml[2 * p + 1] : 0.f;
-    mn = fmaxf(mn, mp[i]);
+  for (int p = 0; p < kJoin; ++p) {
+    const int i = p < P.parts ? p : 0;
+    m[p] = p < P.parts ? ml[2 * i] : -INFINITY;
+    l[p] = p < P.parts ? ml[2 * i + 1] : 0.f;
+    o[p] = p < P.parts ? *reinterpret_cast<const f32x4*>(po + (size_t)i * D.D) : f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  mn = so_wave_max(mn);
+#pragma unroll
+  for (int p = 0; p < kJoin; ++p) mn = fmaxf(mn, m[p]);
   const float ms = mn == -INFINITY ? 0.f : mn;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    mp[i] = exp2_(mp[i] - ms);
-    l += w[i] * mp[i];
-  }
-  l = so_wave_sum(l);
-  float x[2] = {0.f, 0.f};
-  const float* po = D.part_o + at * P.parts * D.D;
-  const bool c0 = lane < D.D, c1 = lane + 64 < D.D;
+  for (int p = 0; p < kJoin; ++p) {
+    const float w = exp2_(m[p] - ms);
+    ln += l[p] * w;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int n = P.parts - 64 * i < 64 ? P.parts - 64 * i : 64;
-#pragma unroll 8
-    for (int p = 0; p < n; ++p) {
-      const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mp[i]), p));
-      const float* row = po + (size_t)(64 * i + p) * D.D;
-      x[0] += c0 ? row[lane] * f : 0.f;
-      x[1] += c1 ? row[lane + 64] * f : 0.f;
+    for (int e = 0; e < 4; ++e) x[e] += o[p][e] * w;
+  }
+  write_joined<T>(D, at, c, x, mn, ln);
+}
+
+// more parts (at most 256; few rows): a block per row, eight parts at a time
+template <typename T>
+__global__ __launch_bounds__(256) void mha_join_many_k(const FwdP P) {
+  __shared__ float weight[256], sums[2];
+  __shared__ f32x4 piece[8][32];
+  const so_mha_desc& D = P.d;
+  const long long at = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, g = tid >> 5, c = 4 * (tid & 31);
+  const float* ml = D.part_ml + 2 * at * P.parts;
+  const float* po = D.part_o + at * P.parts * D.D + c;
+  f32x4 o[4], x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int p = g + 8 * j;
+    o[j] = p < P.parts && c < D.D ? *reinterpret_cast<const f32x4*>(po + (size_t)p * D.D) : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  if (tid < 64) {      // lane p holds the statistics of parts p, p + 64, ...
+    float m[4], l[4], mn = -INFINITY, ln = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = lane + 64 * i;
+      m[i] = p < P.parts ? ml[2 * p] : -INFINITY;
+      l[i] = p < P.parts ? ml[2 * p + 1] : 0.f;
+      mn = fmaxf(mn, m[i]);
+    }
+    mn = so_wave_max(mn);
+    const float ms = mn == -INFINITY ? 0.f : mn;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float w = exp2_(m[i] - ms);
+      weight[lane + 64 * i] = w;
+      ln += l[i] * w;
+    }
+    ln = so_wave_sum(ln);
+    if (lane == 0) {
+      sums[0] = mn;
+      sums[1] = ln;
     }
   }
-  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-  const int head = hk * G + row / D.Lq, qi = row % D.Lq;
-  const size_t orow = ((size_t)b * D.Lq + qi) * D.Hq + head;
+  __syncthreads();
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
-    if (lane + 64 * u < D.D) {
-      const float v = x[u] * inv;
-      const T hi = (T)v;
-      ((T*)D.o)[orow * D.D + lane + 64 * u] = hi;
-      if (D.o_lo) ((T*)D.o_lo)[orow * D.D + lane + 64 * u] = (T)(v - (float)hi);
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] += o[j][e] * weight[g + 8 * j];
+  if (c < D.D)
+    for (int p = g + 32; p < P.parts; p += 8) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(po + (size_t)p * D.D);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] += v[e] * weight[p];
     }
-  if (D.lse && lane == 0) D.lse[((size_t)b * D.Hq + head) * D.Lq + qi] = l == 0.f ? INFINITY : mn + __builtin_amdgcn_logf(l);
+  piece[g][tid & 31] = x;
+  __syncthreads();
+  if (tid >= 32 || c >= D.D) return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] += piece[i][tid][e];
+  write_joined<T>(D, at, c, x, sums[0], sums[1]);
 }
 
 // bias[h][v] = table[lut[v]][h] / scale, finite values kept finite; words[b][w] = bits of the mask bytes
@@ -527,10 +642,14 @@ int launch(FwdP p, bool few, hipStream_t st) {
   constexpr size_t row = Tile<T, DP>::kRowBytes;
   const long long groups = (long long)p.d.B * p.d.Hk;
   if (few) {
-    constexpr size_t stage = 2 * 128 * row, merge = (256 + 32 * (DP + 1)) * 4;
-    p.stages = 2 * stage <= kLds ? 2 : 1;
-    const size_t lds = p.stages * stage > merge ? p.stages * stage : merge;
-    return start(mha_few_k<T, DP, TWO>, p, lds, groups * p.parts, st);
+    constexpr size_t merge = (256 + 32 * (DP + 1)) * 4;
+    typedef Few<T, DP> F;
+    const auto lds = [&](int bias) { const size_t n = 4 * F::kDepth * F::slot(bias); return n > merge ? n : merge; };
+    if (!p.d.bias) return start(mha_few_k<T, DP, 0, TWO>, p, lds(0), groups * p.parts, st);
+    // the expanded bias is addressed with 31 bits
+    if (p.d.linear && p.d.Hq / p.d.Hk * p.d.Lq <= kFewBias && 4LL * p.d.Hq * p.d.V < 0x7fffffffLL)
+      return start(mha_few_k<T, DP, 1, TWO>, p, lds(1), groups * p.parts, st);
+    return start(mha_few_k<T, DP, 2, TWO>, p, lds(2), groups * p.parts, st);
   }
   const int w = p.d.linear ? 1 : p.d.width;
   p.seg = p.d.bias ? (code_span(128, w) + code_span(64, w) + 1 + 63) / 64 * 64 : 0;
@@ -656,10 +775,11 @@ int so_mha_fwd(const void* desc, void* stream) {
   hipStream_t st = (hipStream_t)stream;
   const int err = d->dtype == SO_F32 ? launch_d<float>(p, few, st) : launch_d<__bf16>(p, few, st);
   if (err || parts == 1) return err;
-  const long long n = ((long long)d->B * d->Hq * d->Lq + 3) / 4;
+  const long long rows = (long long)d->B * d->Hq * d->Lq, n = parts > kJoin ? rows : (rows + 7) / 8;
   if (n > 0x7fffffffLL) return SO_ERR_SHAPE;
-  if (d->dtype == SO_F32) hipLaunchKernelGGL(mha_join_k<float>, dim3((unsigned)n), dim3(256), 0, st, p);
-  else hipLaunchKernelGGL(mha_join_k<__bf16>, dim3((unsigned)n), dim3(256), 0, st, p);
+  void (*const join)(FwdP) = parts > kJoin ? (d->dtype == SO_F32 ? mha_join_many_k<float> : mha_join_many_k<__bf16>)
+                                           : (d->dtype == SO_F32 ? mha_join_k<float> : mha_join_k<__bf16>);
+  hipLaunchKernelGGL(join, dim3((unsigned)n), dim3(256), 0, st, p);
   return SO_LAUNCH_CHECK();
 }
 
