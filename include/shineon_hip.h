@@ -554,7 +554,7 @@ int so_qk_norm_rotary_bwd(const void* desc, const void* dyq, const void* dyk, vo
 typedef struct so_mha_desc {
   const void *q, *k, *v;
   void* o;
-  void* o_lo;                  /* bf16, training: what o's rounding left of the result; NULL otherwise */
+  float* o_f32;                /* bf16, training: the result before its rounding, laid out like o; NULL otherwise */
   float* lse;                  /* training: [B][Hq][Lq], log2 of the softmax denominators (+inf: empty row); or NULL */
   const float* bias;
   const int* code;
@@ -566,7 +566,7 @@ typedef struct so_mha_desc {
   float* strips;               /* backward, gradient of the bias: so_mha_strip_floats */
   long long sqb, sql, sqh, skb, skl, skh, svb, svl, svh;
   int dtype, B, Hq, Hk, Lq, Lk, D, V, code_max, tokens, q_start, linear, nwords;
-  int two;                     /* bf16 forward: probabilities as a pair of bf16 products (the bias gradient needs o to fp32 accuracy) */
+  int exact;                   /* bf16 forward: probabilities as three bf16 products (the bias gradient needs o to fp32 accuracy) */
   int width;                   /* tokens of a map row (a sequence: its length) */
   float scale;
 } so_mha_desc;

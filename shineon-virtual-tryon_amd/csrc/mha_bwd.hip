@@ -198,13 +198,17 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : DP <= 6
       const bool on = rowv && ch * E < D.D;
       q[m] = as_frag<T>(load_chunk<T>(qr, ch, on));
       go[m] = as_frag<T>(load_chunk<T>((const T*)D.dout + orow, ch, on));
-      const frag ov = as_frag<T>(load_chunk<T>((const T*)D.o + orow, ch, on));
+      if (D.o_f32) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) delta += (float)go[m][e] * (float)ov[e];
-      if (D.o_lo) {
-        const frag lv = as_frag<T>(load_chunk<T>((const T*)D.o_lo + orow, ch, on));
+        for (int h = 0; h < E / 4; ++h) {
+          const f32x4 ov = load_chunk<float>(D.o_f32 + orow, ch * (E / 4) + h, on);
 #pragma unroll
-        for (int e = 0; e < E; ++e) delta += (float)go[m][e] * (float)lv[e];
+          for (int e = 0; e < 4; ++e) delta += (float)go[m][4 * h + e] * ov[e];
+        }
+      } else {
+        const frag ov = as_frag<T>(load_chunk<T>((const T*)D.o + orow, ch, on));
+#pragma unroll
+        for (int e = 0; e < E; ++e) delta += (float)go[m][e] * (float)ov[e];
       }
     }
     delta = half_sum(delta);

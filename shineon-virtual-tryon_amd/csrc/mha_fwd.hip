@@ -50,7 +50,7 @@ __device__ __forceinline__ void write_row(const FwdP& P, const f32x16 (&o)[NT], 
   const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;        // an empty row gives zeros, NaN stays NaN
   const size_t orow = ((size_t)b * D.Lq + qi) * D.Hq + head;
   T* op = (T*)D.o + orow * D.D;
-  T* lp = D.o_lo ? (T*)D.o_lo + orow * D.D : nullptr;
+  float* fp = D.o_f32 ? D.o_f32 + orow * D.D : nullptr;
 #pragma unroll
   for (int v = 0; v < NT; ++v)
 #pragma unroll
@@ -58,15 +58,15 @@ __device__ __forceinline__ void write_row(const FwdP& P, const f32x16 (&o)[NT], 
       const int c = 32 * v + 8 * g + 4 * half;
       if (c < D.D) {
         typedef T t4 __attribute__((ext_vector_type(4)));
-        t4 hi, lo;
+        f32x4 x;
+        t4 y;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float x = o[v][4 * g + e] * inv;
-          hi[e] = (T)x;
-          lo[e] = (T)(x - (float)hi[e]);
+          x[e] = o[v][4 * g + e] * inv;
+          y[e] = (T)x[e];
         }
-        *reinterpret_cast<t4*>(op + c) = hi;
-        if (lp) *reinterpret_cast<t4*>(lp + c) = lo;
+        *reinterpret_cast<t4*>(op + c) = y;
+        if (fp) *reinterpret_cast<f32x4*>(fp + c) = x;
       }
     }
   if (D.lse && half == 0) D.lse[((size_t)b * D.Hq + head) * D.Lq + qi] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
@@ -100,25 +100,28 @@ __device__ __forceinline__ void softmax_step(f32x16 (&s)[N], f32x16 (&o)[NT], fl
   }
 }
 
-template <typename T, int NCS, bool TWO>
-__device__ __forceinline__ void prob_frags(const f32x16& s, typename Elem<T>::frag (&p)[NCS], typename Elem<T>::frag (&lo)[NCS]) {
+template <typename T, int NCS, bool EXACT>
+__device__ __forceinline__ void prob_frags(const f32x16& s, typename Elem<T>::frag (&p)[EXACT ? 3 : 1][NCS]) {
   constexpr int E = Elem<T>::E;
 #pragma unroll
   for (int c = 0; c < NCS; ++c) {
-    to_frag(s, c, p[c]);
-    if constexpr (TWO) {
+    to_frag(s, c, p[0][c]);
+    if constexpr (EXACT) {
       f32x16 rest;
 #pragma unroll
-      for (int e = 0; e < E; ++e) rest[E * c + e] = s[E * c + e] - (float)p[c][e];
-      to_frag(rest, c, lo[c]);
+      for (int i = 1; i < 3; ++i) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) rest[E * c + e] = (i == 1 ? s : rest)[E * c + e] - (float)p[i - 1][c][e];
+        to_frag(rest, c, p[i][c]);
+      }
     }
   }
 }
 
 // Many rows: a block is 128 rows of one head, 32 per wave, and walks 64-key tiles.  BIAS: 0 none, 1 sequence, 2 map; the piece of the
 // expanded bias that a tile's offsets lie in travels to LDS with the tile.  (Read from global memory by every lane it took 120 of 495 us
-// at 8191 tokens, 16 heads of 64.)  TWO: the probabilities as a hi + lo pair of bf16 products.
-template <typename T, int DP, int BIAS, bool TWO>
+// at 8191 tokens, 16 heads of 64.)  EXACT: the 24 bits of a probability as three bf16 products (rounded to 8 or 16 bits, delta = do . o no longer matches what the backward pass recomputes, and the sums over rows that cancel in the bias gradient show it).
+template <typename T, int DP, int BIAS, bool EXACT>
 __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 96 ? 2 : 1))) void mha_fwd_k(const FwdP P) {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::frag frag;
@@ -241,11 +244,11 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
     softmax_step(s, o, m, l, P.c);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      frag p[NCS], lo[NCS];
-      prob_frags<T, NCS, TWO>(s[u], p, lo);
+      frag p[EXACT ? 3 : 1][NCS];
+      prob_frags<T, NCS, EXACT>(s[u], p);
       const auto use = [&](int k, const frag& a) {
-        o[k % NT] = mma(a, p[k / NT], o[k % NT]);
-        if constexpr (TWO) o[k % NT] = mma(a, lo[k / NT], o[k % NT]);
+#pragma unroll
+        for (int i = 0; i < (EXACT ? 3 : 1); ++i) o[k % NT] = mma(a, p[i][k / NT], o[k % NT]);
       };
       if (u == 0) {
         const int cb = opaque(fc);
@@ -282,7 +285,7 @@ struct Few {
   static constexpr int kDepth = kPiece >= 8192 ? 1 : 8192 / kPiece;
   static constexpr int slot(int bias) { return 2 * kPiece + (bias == 1 ? kFewBias * 128 : 0); }
 };
-template <typename T, int DP, int BIAS, bool TWO>
+template <typename T, int DP, int BIAS, bool EXACT>
 __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha_few_k(const FwdP P) {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::frag frag;
@@ -423,8 +426,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
       for (int r = 0; r < 16; ++r) s[0][r] = (seen >> r) & 1 ? s[0][r] : -INFINITY;
     }
     softmax_step(s, o, m, l, P.c);
-    frag p[NCS], lo[NCS];
-    prob_frags<T, NCS, TWO>(s[0], p, lo);
+    frag p[EXACT ? 3 : 1][NCS];
+    prob_frags<T, NCS, EXACT>(s[0], p);
     if (more) arrived<DEPTH * NK + (DEPTH - 1) * NV>();
     else arrived<0>();
     {
@@ -437,8 +440,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
       fetch_v(t + DEPTH, mine + slot * SLOT, ring[DEPTH - 1]);
     }
     last_phase(f, [&](int k, const frag& a) {
-      o[k % NT] = mma(a, p[k / NT], o[k % NT]);
-      if constexpr (TWO) o[k % NT] = mma(a, lo[k / NT], o[k % NT]);
+#pragma unroll
+      for (int i = 0; i < (EXACT ? 3 : 1); ++i) o[k % NT] = mma(a, p[i][k / NT], o[k % NT]);
     });
     slot = slot + 1 < DEPTH ? slot + 1 : 0;
   }
@@ -492,15 +495,14 @@ __device__ __forceinline__ void write_joined(const so_mha_desc& D, long long at,
   const size_t orow = (((size_t)b * D.Lq + qi) * D.Hq + head) * D.D;
   const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
   typedef T t4 __attribute__((ext_vector_type(4)));
-  t4 hi, lo;
+  t4 y;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const float v = x[e] * inv;
-    hi[e] = (T)v;
-    lo[e] = (T)(v - (float)hi[e]);
+    x[e] *= inv;
+    y[e] = (T)x[e];
   }
-  *reinterpret_cast<t4*>((T*)D.o + orow + c) = hi;
-  if (D.o_lo) *reinterpret_cast<t4*>((T*)D.o_lo + orow + c) = lo;
+  *reinterpret_cast<t4*>((T*)D.o + orow + c) = y;
+  if (D.o_f32) *reinterpret_cast<f32x4*>(D.o_f32 + orow + c) = x;
   if (D.lse && c == 0) D.lse[((size_t)b * D.Hq + head) * D.Lq + qi] = l == 0.f ? INFINITY : mn + __builtin_amdgcn_logf(l);
 }
 
@@ -637,7 +639,7 @@ int start(K k, const FwdP& p, size_t lds, long long blocks, hipStream_t st) {
   hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(256), lds, st, p);
   return SO_LAUNCH_CHECK();
 }
-template <typename T, int DP, bool TWO>
+template <typename T, int DP, bool EXACT>
 int launch(FwdP p, bool few, hipStream_t st) {
   constexpr size_t row = Tile<T, DP>::kRowBytes;
   const long long groups = (long long)p.d.B * p.d.Hk;
@@ -645,11 +647,11 @@ int launch(FwdP p, bool few, hipStream_t st) {
     constexpr size_t merge = (256 + 32 * (DP + 1)) * 4;
     typedef Few<T, DP> F;
     const auto lds = [&](int bias) { const size_t n = 4 * F::kDepth * F::slot(bias); return n > merge ? n : merge; };
-    if (!p.d.bias) return start(mha_few_k<T, DP, 0, TWO>, p, lds(0), groups * p.parts, st);
+    if (!p.d.bias) return start(mha_few_k<T, DP, 0, EXACT>, p, lds(0), groups * p.parts, st);
     // the expanded bias is addressed with 31 bits
     if (p.d.linear && p.d.Hq / p.d.Hk * p.d.Lq <= kFewBias && 4LL * p.d.Hq * p.d.V < 0x7fffffffLL)
-      return start(mha_few_k<T, DP, 1, TWO>, p, lds(1), groups * p.parts, st);
-    return start(mha_few_k<T, DP, 2, TWO>, p, lds(2), groups * p.parts, st);
+      return start(mha_few_k<T, DP, 1, EXACT>, p, lds(1), groups * p.parts, st);
+    return start(mha_few_k<T, DP, 2, EXACT>, p, lds(2), groups * p.parts, st);
   }
   const int w = p.d.linear ? 1 : p.d.width;
   p.seg = p.d.bias ? (code_span(128, w) + code_span(64, w) + 1 + 63) / 64 * 64 : 0;
@@ -658,22 +660,22 @@ int launch(FwdP p, bool few, hipStream_t st) {
   p.stages = 2 * stage <= kLds ? 2 : 1;
   const long long blocks = groups * (p.d.Hq / p.d.Hk) * p.row_tiles * p.parts;
   const size_t lds = p.stages * stage;
-  if (!p.d.bias) return start(mha_fwd_k<T, DP, 0, TWO>, p, lds, blocks, st);
-  return p.d.linear ? start(mha_fwd_k<T, DP, 1, TWO>, p, lds, blocks, st) : start(mha_fwd_k<T, DP, 2, TWO>, p, lds, blocks, st);
+  if (!p.d.bias) return start(mha_fwd_k<T, DP, 0, EXACT>, p, lds, blocks, st);
+  return p.d.linear ? start(mha_fwd_k<T, DP, 1, EXACT>, p, lds, blocks, st) : start(mha_fwd_k<T, DP, 2, EXACT>, p, lds, blocks, st);
 }
 template <typename T, int DP>
-int launch_two(const FwdP& p, bool few, hipStream_t st) {
+int launch_exact(const FwdP& p, bool few, hipStream_t st) {
   if constexpr (sizeof(T) == 2) {
-    if (p.d.two) return launch<T, DP, true>(p, few, st);
+    if (p.d.exact) return launch<T, DP, true>(p, few, st);
   }
   return launch<T, DP, false>(p, few, st);
 }
 template <typename T>
 int launch_d(const FwdP& p, bool few, hipStream_t st) {
-  if (p.d.D <= 32) return launch_two<T, 32>(p, few, st);
-  if (p.d.D <= 64) return launch_two<T, 64>(p, few, st);
-  if (p.d.D <= 96) return launch_two<T, 96>(p, few, st);
-  return launch_two<T, 128>(p, few, st);
+  if (p.d.D <= 32) return launch_exact<T, 32>(p, few, st);
+  if (p.d.D <= 64) return launch_exact<T, 64>(p, few, st);
+  if (p.d.D <= 96) return launch_exact<T, 96>(p, few, st);
+  return launch_exact<T, 128>(p, few, st);
 }
 
 // few rows: everything that shares a key head fits one 32-row tile
@@ -695,7 +697,7 @@ int so_mha_check(const so_mha_desc* d) {
   const long long s[] = {d->sqb, d->sql, d->sqh, d->skb, d->skl, d->skh, d->svb, d->svl, d->svh};
   for (long long x : s)
     if (x % E) return SO_ERR_ALIGN;
-  if ((((uintptr_t)d->q) | ((uintptr_t)d->k) | ((uintptr_t)d->v) | ((uintptr_t)d->o) | ((uintptr_t)d->o_lo)) & 15) return SO_ERR_ALIGN;
+  if ((((uintptr_t)d->q) | ((uintptr_t)d->k) | ((uintptr_t)d->v) | ((uintptr_t)d->o) | ((uintptr_t)d->o_f32)) & 15) return SO_ERR_ALIGN;
   if (d->bias && (!d->code || (((uintptr_t)d->code) & 15) || d->V != 2 * d->code_max + 1 || d->q_start < 0)) return SO_ERR_SHAPE;
   if (d->bias && !d->linear && (d->width < 1 || d->width > 512)) return SO_ERR_SHAPE;
   if (d->bias && (d->q_start + (long long)d->Lq > d->tokens || d->Lk > d->tokens)) return SO_ERR_SHAPE;

@@ -281,11 +281,11 @@ def qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions=None, start=0, 
 # ------------------------------------------------------------------------------------------------
 class _Desc(ctypes.Structure):
     """so_mha_desc of include/shineon_hip.h."""
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "o", "o_lo", "lse", "bias", "code", "words", "part_o", "part_ml", "dout",
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "o", "o_f32", "lse", "bias", "code", "words", "part_o", "part_ml", "dout",
                                                 "dq", "dk", "dv", "delta", "strips")]
                 + [(n, ctypes.c_longlong) for n in ("sqb", "sql", "sqh", "skb", "skl", "skh", "svb", "svl", "svh")]
                 + [(n, ctypes.c_int) for n in ("dtype", "B", "Hq", "Hk", "Lq", "Lk", "D", "V", "code_max", "tokens", "q_start", "linear",
-                                               "nwords", "two", "width")]
+                                               "nwords", "exact", "width")]
                 + [("scale", ctypes.c_float)])
 
 
@@ -386,7 +386,7 @@ class _AttentionFn(torch.autograd.Function):
         x = _Desc(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr())
         (x.sqb, x.sql, x.sqh), (x.skb, x.skl, x.skh), (x.svb, x.svl, x.svh) = _strides(q), _strides(k), _strides(v)
         x.dtype, x.B, x.Hq, x.Hk, x.Lq, x.Lk, x.D, x.nwords, x.scale = dt, b, hq, hk, lq, lk, d, (lk + 63) // 64, scale
-        words = bias = lse = o_lo = None
+        words = bias = lse = o_f32 = None
         mp = msb = tp = lp = None
         if mask is not None:
             words = torch.empty((b, x.nwords), dtype=torch.int64, device=dev)
@@ -402,9 +402,9 @@ class _AttentionFn(torch.autograd.Function):
             lse = torch.empty((b, hq, lq), dtype=torch.float32, device=dev)
             x.lse = lse.data_ptr()
             if dt == 1:
-                o_lo = torch.empty_like(o)
-                x.o_lo = o_lo.data_ptr()
-                x.two = int(table is not None and ctx.needs_input_grad[3])
+                o_f32 = torch.empty(o.shape, dtype=torch.float32, device=dev)
+                x.o_f32 = o_f32.data_ptr()
+                x.exact = int(table is not None and ctx.needs_input_grad[3])
         at = ctypes.addressof(x)
         parts = L.so_mha_parts(at)
         if parts < 0:
@@ -416,7 +416,7 @@ class _AttentionFn(torch.autograd.Function):
         _launch(dev, L.so_mha_fwd, "mha_fwd", at)
         if train:
             ctx.desc = x      # the backward pass reads the same operands (saved: they stay where they are)
-            ctx.save_for_backward(q, k, v, table, o, o_lo, lse, bias, words)
+            ctx.save_for_backward(q, k, v, table, o, o_f32, lse, bias, words)
         return o if d == d_true else o[..., :d_true].contiguous()
 
     @staticmethod

@@ -208,7 +208,7 @@ def _attention_case(tok, dtype, b, lq, lk, hq, hk, d, shape=None, mask=None, q_s
     o = tok.attention(q, k, v, key_mask=mask, relative=rel, bias_table=table if rel is not None else None, q_start=q_start)
     do = normal(seed + 5, b, lq, hq, d, dtype=dtype)
     want = ref.attention(d64(q), d64(k), d64(v), d ** -0.5, None if mask is None else mask.cpu(), bias, d64(do) if train else None, dtype,
-                         two=rel is not None and train)
+                         exact=rel is not None and train)
     ref.check(o, *want["o"], "o")
     if not train:
         return o

@@ -71,7 +71,7 @@ def pair_buckets(shape, lq, lk, q_start, num, far, both=True):
     return bx if h == 1 else t[(k // w)[None] - (q // w)[:, None] + n - 1] * num + bx
 
 
-def attention(q, k, v, scale, mask=None, bias=None, dout=None, dtype=torch.float32, two=False):
+def attention(q, k, v, scale, mask=None, bias=None, dout=None, dtype=torch.float32, exact=False):
     """64-bit attention and, for every output, a bound on what the kernel's roundings can add up to.  q, k, v, dout: float64 holding the
     exact operand values; bias [H, Lq, Lk].  Returns {name: (value, bound)}."""
     b, lq, hq, d = q.shape
@@ -94,7 +94,7 @@ def attention(q, k, v, scale, mask=None, bias=None, dout=None, dtype=torch.float
     p = e / torch.where(z == 0, 1.0, z)
     o = p @ vh
     u = HALF_STEP[dtype]
-    pu = 0.0 if dtype == torch.float32 else (2.0 ** -16 if two else u)       # rounding of the probabilities as product operands
+    pu = 0.0 if dtype == torch.float32 else (0.0 if exact else u)       # rounding of the probabilities as product operands
     lk = s.shape[-1]
     # absolute error of a score (D products summed, the bias, the subtraction of the maximum), hence relative error of p and of its
     # row's sum; v_exp_f32 and the running rescale add a few steps more; Lk / 8 covers the sequential sums (fp32, worst case / 8)
@@ -109,8 +109,7 @@ def attention(q, k, v, scale, mask=None, bias=None, dout=None, dtype=torch.float
         dp = gh @ vh.transpose(-1, -2)
         dpa = gh.abs() @ vh.abs().transpose(-1, -2)
         delta = (gh * o).sum(-1, keepdim=True)
-        lo = U32 if dtype == torch.float32 else 2.0 ** -16                     # o is kept to this
-        ed = (gh.abs() * (eo + lo * o.abs())).sum(-1, keepdim=True) + U32 * (d + 4) * (gh * o).abs().sum(-1, keepdim=True)
+        ed = (gh.abs() * (eo + U32 * o.abs())).sum(-1, keepdim=True) + U32 * (d + 4) * (gh * o).abs().sum(-1, keepdim=True)
         ds = p * (dp - delta)
         eds = p * (ep * (dpa + delta.abs()) + U32 * (d + 4) * dpa + ed) + U32 * 4 * ds.abs()
         su = 0.0 if dtype == torch.float32 else u
