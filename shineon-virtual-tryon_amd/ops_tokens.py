@@ -8,11 +8,11 @@
 Same contract as ops.py: torch supplies device memory, the current stream and the autograd tape; the arithmetic is in
 libshineon_hip.so, there is no CPU fallback, everything may be captured into a hipGraph.  Two differences: operands may be float32 or
 bfloat16 (arithmetic and statistics are fp32 either way), and every call runs on the device of its operands, on that device's current
-stream, whatever the current device is."""
+stream, whatever the current device is.  Gradients are first order: differentiating them again is refused."""
 import ctypes
-import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._lib import check, lib
 from .ops import _require_cuda
@@ -46,7 +46,7 @@ def _fp32_param(t, shape, device, what):
 
 def _launch(device, fn, what, *args):
     """fn(*args, stream) on `device`'s current stream; launches go to the current device, so that is switched when it is another."""
-    stream = torch.cuda.current_stream(device).cuda_stream
+    stream = torch._C._cuda_getCurrentRawStream(device.index)      # the handle alone: no Stream object (2 us, 5 - 10 in autograd's thread)
     if device.index == torch.cuda.current_device():
         err = fn(*args, stream)
     else:
@@ -54,6 +54,12 @@ def _launch(device, fn, what, *args):
             err = fn(*args, stream)
     if err:
         check(err, what)
+
+
+def _first_order(backward):
+    """once_differentiable, at no cost where no graph of the gradients is asked for."""
+    checked = once_differentiable(backward)
+    return lambda ctx, *grads: (checked if torch.is_grad_enabled() else backward)(ctx, *grads)
 
 
 # ------------------------------------------------------------------------------------------------
@@ -148,6 +154,7 @@ class _DropoutFn(torch.autograd.Function):
         return _dropout_launch(dt, x, p, rng, residual)
 
     @staticmethod
+    @_first_order
     def backward(ctx, dy):
         (rng,) = ctx.saved_tensors
         p, dt = ctx.cfg
@@ -208,6 +215,15 @@ class _QkDesc(ctypes.Structure):
                 + [(n, ctypes.c_int) for n in ("dtype", "Hq", "Hk", "pos64", "B", "L", "D", "R")] + [("eps", ctypes.c_float)])
 
 
+def _qk_desc(q, k, wq, wk, cos, sin, positions, start, eps, dt):
+    (b, n, hq, d), pp, p64, psb, psl = q.shape, None, 0, 0, 0
+    if positions is not None:
+        pp, p64, psl = positions.data_ptr(), int(positions.dtype == torch.int64), positions.stride(-1)
+        psb = positions.stride(0) if positions.dim() == 2 else 0
+    return _QkDesc(q.data_ptr(), k.data_ptr(), wq.data_ptr(), wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), pp, *q.stride()[:3],
+                   *k.stride()[:3], cos.shape[0], psb, psl, start, dt, hq, k.shape[2], p64, b, n, d, 2 * cos.shape[1], eps)
+
+
 class _QkNormRotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, wq, wk, cos, sin, positions, start, eps, dt):
@@ -216,21 +232,20 @@ class _QkNormRotaryFn(torch.autograd.Function):
         yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
         ctx.save_for_backward(q, k, wq, wk, cos, sin, positions)
-        pp, p64, psb, psl = None, 0, 0, 0
-        if positions is not None:
-            pp, p64, psl = positions.data_ptr(), int(positions.dtype == torch.int64), positions.stride(-1)
-            psb = positions.stride(0) if positions.dim() == 2 else 0
-        # what both passes read (the tensors are saved and stay where they are)
-        ctx.desc = _QkDesc(q.data_ptr(), k.data_ptr(), wq.data_ptr(), wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), pp, *q.stride()[:3],
-                           *k.stride()[:3], cos.shape[0], psb, psl, start, dt, hq, k.shape[2], p64, b, n, d, 2 * cos.shape[1], eps)
+        ctx.desc = _qk_desc(q, k, wq, wk, cos, sin, positions, start, eps, dt)
         if b and n:
             _launch(q.device, lib().so_qk_norm_rotary_fwd, "qk_norm_rotary_fwd", ctypes.addressof(ctx.desc), yq.data_ptr(), yk.data_ptr())
         return yq, yk
 
     @staticmethod
+    @_first_order
     def backward(ctx, dyq, dyk):
-        q, k, wq, wk = ctx.saved_tensors[:4]
+        q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
         x = ctx.desc
+        at = tuple(None if t is None else t.data_ptr() for t in (q, k, wq, wk, cos, sin, positions))
+        if at != (x.q, x.k, x.wq, x.wk, x.cosv, x.sinv, x.pos):      # saved tensors may come back elsewhere (hooks, checkpoints)
+            q, k = _heads(q, "q"), _heads(k, "k")
+            x = _qk_desc(q, k, wq, wk, cos, sin, positions, x.start, x.eps, x.dtype)
         dyq, dyk = dyq.contiguous(), dyk.contiguous()
         dq, dk = torch.empty_like(dyq), torch.empty_like(dyk)
         if not (x.B and x.L):
@@ -350,15 +365,16 @@ class RelativePositions:
 
 
 def _rows16(t, what):
-    """[B, L, H, D] as the kernels read it: channels contiguous, everything else a multiple of 16 bytes - zero channels appended to D and
-    a dense copy made where it is not."""
+    """[B, L, H, D] as the kernels read it: channels contiguous, everything else a multiple of 16 bytes, rows less than 2^22 elements apart
+    (128 rows within a 31-bit offset) - zero channels appended to D and a dense copy made where it is not."""
     t = _heads(t, what)
     e = 16 // t.element_size()
     d = t.shape[3]
     if d % e:
         t = torch.nn.functional.pad(t, (0, e - d % e))
     sb, sl, sh, _ = t.stride()
-    if t.data_ptr() % 16 or (sb % e or sl % e or sh % e) and any(s % e for s, n in zip((sb, sl, sh), t.shape) if n > 1):
+    if (t.data_ptr() % 16 or (sl >= 1 << 22 and t.shape[1] > 1)
+            or (sb % e or sl % e or sh % e) and any(s % e for s, n in zip((sb, sl, sh), t.shape) if n > 1)):
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -415,19 +431,31 @@ class _AttentionFn(torch.autograd.Function):
             x.part_ml = x.part_o + 4 * b * hq * lq * parts * d
         _launch(dev, L.so_mha_fwd, "mha_fwd", at)
         if train:
-            ctx.desc = x      # the backward pass reads the same operands (saved: they stay where they are)
+            ctx.desc = x
             ctx.save_for_backward(q, k, v, table, o, o_f32, lse, bias, words)
         return o if d == d_true else o[..., :d_true].contiguous()
 
     @staticmethod
+    @_first_order
     def backward(ctx, dout):
         d_true, rel = ctx.d_true, ctx.rel
         if ctx.desc is None:
             q, k, v, table = ctx.saved_tensors
             return (*(torch.zeros_like(t[..., :d_true]) for t in (q, k, v)), None if table is None else torch.zeros_like(table),
                     None, None, None, None, None, None)
-        q, k, v, table, o = ctx.saved_tensors[:5]
+        q, k, v, table, o, o_f32, lse, bias, words = ctx.saved_tensors
         x = _Desc.from_buffer_copy(ctx.desc)      # a second backward pass of the same graph must not see this one's pointers
+        if q.data_ptr() != x.q or k.data_ptr() != x.k or v.data_ptr() != x.v:      # saved tensors may come back elsewhere (hooks, checkpoints)
+            q, k, v = _rows16(q, "q"), _rows16(k, "k"), _rows16(v, "v")
+            x.q, x.k, x.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+            (x.sqb, x.sql, x.sqh), (x.skb, x.skl, x.skh), (x.svb, x.svl, x.svh) = _strides(q), _strides(k), _strides(v)
+        x.o, x.lse = o.data_ptr(), lse.data_ptr()
+        if o_f32 is not None:
+            x.o_f32 = o_f32.data_ptr()
+        if bias is not None:
+            x.bias = bias.data_ptr() + 512
+        if words is not None:
+            x.words = words.data_ptr()
         b, lq, hq, d = q.shape
         dev, L = q.device, lib()
         if d != d_true:
@@ -467,13 +495,15 @@ def attention(q, k, v, scale=None, key_mask=None, relative=None, bias_table=None
 
     q [B, Lq, Hq, D]; k, v [B, Lk, Hk, D]; Hq a multiple of Hk (query heads h * Hq / Hk .. share key head h); float32 or bfloat16,
     D <= 128.  Any strides: operands whose rows do not start at multiples of 16 bytes, or whose channels are not contiguous, are copied
-    first.  scale: default D^-1/2, must be positive.
+    first.  scale: default D^-1/2, positive.
 
     key_mask: bool [B, Lk], True = visible.  Hidden keys and values may hold anything (inf and NaN included) and get zero gradients; a
     sample without visible keys gives zeros.
 
     relative + bias_table: a RelativePositions plan and its learned table [plan.rows, Hq] (float32).  Key j against query i adds the
     entry of the bucket of token j against token q_start + i.  An entry may be -inf; finite ones beyond +-7.4e8 count as that.
+
+    Training with a table takes scratch for the bias gradient, about Lq Lk / 32 bytes per sample and head, while backward runs.
 
     One or a few queries over long keys (a new token against what came before) are split over the keys.  Returns [B, Lq, Hq, D];
     differentiable in q, k, v and bias_table.  The order of all sums is fixed: the same inputs give the same bits."""
@@ -487,8 +517,8 @@ def attention(q, k, v, scale=None, key_mask=None, relative=None, bias_table=None
     if d < 1 or d > 128:
         raise ValueError(f"head size 1 .. 128 (got {d})")
     scale = d ** -0.5 if scale is None else float(scale)
-    if not (0.0 < scale < math.inf):
-        raise ValueError(f"scale must be positive and finite (got {scale})")
+    if not (1e-20 <= scale <= 1e20):      # the bias is kept divided by it, in fp32
+        raise ValueError(f"scale must be positive, from 1e-20 to 1e20 (got {scale})")
     if key_mask is not None:
         if key_mask.dtype != torch.bool or tuple(key_mask.shape) != (b, lk) or key_mask.device != q.device:
             raise ValueError(f"key_mask: bool of shape ({b}, {lk}) on {q.device} expected, got {key_mask.dtype} {tuple(key_mask.shape)}")

@@ -5,6 +5,7 @@ import math
 import numpy as np
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import tokens_ref as ref
 
@@ -524,8 +525,9 @@ def test_refusals(tok):
         tok.attention(x, x[:, :, :3], x[:, :, :3])
     with pytest.raises(ValueError, match="expected"):
         tok.attention(x, x, x[:, :4])
-    with pytest.raises(ValueError, match="scale"):
-        tok.attention(x, x, x, scale=0.0)
+    for scale in (0.0, -1.0, 1e-30, 1e30, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="scale"):
+            tok.attention(x, x, x, scale=scale)
     with pytest.raises(ValueError, match="key_mask"):
         tok.attention(x, x, x, key_mask=mask.float())
     with pytest.raises(ValueError, match="key_mask"):
@@ -540,6 +542,55 @@ def test_refusals(tok):
         tok.attention(x, x, x, q_start=1)
     with pytest.raises(ValueError, match="plan is on"):
         tok.attention(x, x, x, relative=tok.RelativePositions(5, 8, 20, device="cpu"), bias_table=table)
+
+
+# ------------------------------------------------------------------------------------------------------------------- autograd
+def _taped_leaves(dtype):
+    return [normal(60 + i, *s, dtype=dtype).requires_grad_() for i, s in enumerate(((2, 40, 8, 32), (2, 40, 2, 32), (2, 40, 2, 32)))]
+
+
+def _taped_layer(tok, q, k, v, w, table, plan, rot, mask, positions, rng):
+    q, k, v = q * 1, k * 1, v * 1      # intermediates: nothing but the tape keeps them
+    q, k = tok.qk_norm_rotary(q, k, w * 1, w, *rot, positions=positions)
+    return tok.dropout(tok.attention(q, k, v, key_mask=mask, relative=plan, bias_table=table * 1), 0.3, rng)
+
+
+@TYPES
+@pytest.mark.parametrize("how", ["hooks", "checkpoint"])
+def test_saved_tensors_may_come_back_elsewhere(tok, dtype, how):
+    """Hooks on saved tensors and activation checkpoints hand the backward pass other tensors than the forward pass saved."""
+    leaves = _taped_leaves(dtype)
+    plan, rot = tok.RelativePositions(40, 8, 20), tok.rotary_table(40, 32)
+    w, table = (1 + 0.1 * normal(70, 32)).requires_grad_(), normal(71, plan.rows, 8).requires_grad_()
+    args = (w, table, plan, rot, _mask(2, 40, "ragged"), torch.arange(40, device="cuda").flip(0), tok.rng_state(5, "cuda"))
+    all_leaves, dy = [*leaves, w, table], normal(72, 2, 40, 8, 32, dtype=dtype)
+    want = torch.autograd.grad(_taped_layer(tok, *leaves, *args), all_leaves, dy)
+    if how == "hooks":
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda()):
+            y = _taped_layer(tok, *leaves, *args)
+    else:
+        y = torch.utils.checkpoint.checkpoint(_taped_layer, tok, *leaves, *args, use_reentrant=False)
+    rubbish = [torch.full((n,), float("nan"), device="cuda") for n in (640, 1280, 5120, 10240, 20480, 40960) for _ in range(8)]
+    got = torch.autograd.grad(y, all_leaves, dy)
+    del rubbish
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_second_order_is_refused(tok):
+    x = normal(1, 2, 5, 4, 16).requires_grad_()
+    cos, sin = tok.rotary_table(5, 16)
+    w, rng = torch.ones(16, device="cuda"), tok.rng_state(1, "cuda")
+    for y in (tok.dropout(x, 0.5, rng), tok.qk_norm_rotary(x, x, w, w, cos, sin)[0], tok.attention(x, x, x)):
+        (g,) = torch.autograd.grad((y * y).sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward()
+
+
+def test_attention_rows_far_apart(tok):
+    """Rows so far apart that a tile of them does not fit a 31-bit offset."""
+    q, k = normal(1, 1, 3, 2, 16), torch.zeros(130, 1 << 22, device="cuda")[:, :64].view(1, 130, 4, 16)
+    k.copy_(normal(2, 1, 130, 4, 16))
+    assert torch.equal(tok.attention(q, k[:, :, :2], k[:, :, 2:]), tok.attention(q, k[:, :, :2].contiguous(), k[:, :, 2:].contiguous()))
 
 
 # ------------------------------------------------------------------------------------------------------------------- modules
