@@ -706,12 +706,11 @@ int so_mha_check(const so_mha_desc* d) {
 
 double mha_tiles(int n) { return n / 128 + (n % 128 + 31) / 32 * 0.25; }
 
-int mha_split_parts(double blocks, double block_flop, int dtype, double join_bytes, int most, double gain) {
-  const double us = block_flop / (dtype == SO_F32 ? 0.45e6 : 3.0e6);      // what a CU reaches in these kernels, FLOP per us
+int mha_split_parts(double blocks, double block_us, double join_us, double part_us, int most, double gain) {
   int best = 1;
   double least = 0;
   for (int p = 1; p <= 8 && (p == 1 || p <= most); ++p) {
-    const double t = ceil(blocks * p / 256) / p * us + (p > 1 ? 6.0 + join_bytes * p / 4.0e6 : 0.0);
+    const double t = ceil(blocks * p / 256) / p * block_us + (p > 1 ? join_us + part_us * p : 0.0);
     if (p == 1 || t < gain * least) {
       best = p;
       least = t;
@@ -758,8 +757,11 @@ int so_mha_parts(const void* desc) {
     if (parts > tiles / 2) parts = tiles / 2;
     return parts < 2 ? 1 : (int)(parts > 256 ? 256 : parts);
   }
-  const double rows = (double)d->B * d->Hq * d->Lq;
-  return mha_split_parts((double)d->B * d->Hq * mha_tiles(d->Lq), 4.0 * 128 * d->D * d->Lk, d->dtype, rows * d->D * 8, d->Lk / 128, 0.95);
+  // a map's bias is looked up value by value, whole probabilities are three products for one: 2 x 2304 tokens of a 64 x 36 map, 8 heads of 64,
+  // 288 blocks, training: 116 us whole, 83 + 10 in two parts, 69 + 12 in seven (the join reads from caches)
+  const double rate = (d->exact ? 0.75 : 1.0) * (d->bias && !d->linear ? 0.6 : 1.0), rows = (double)d->B * d->Hq * d->Lq;
+  return mha_split_parts((double)d->B * d->Hq * mha_tiles(d->Lq), mha_us(4.0 * 128 * d->D * d->Lk, d->dtype) / rate, 8.0,
+                         rows * d->D * 8 / 12e6, d->Lk / 128, 0.95);
 }
 
 int so_mha_fwd(const void* desc, void* stream) {
