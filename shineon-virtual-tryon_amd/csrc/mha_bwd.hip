@@ -8,9 +8,10 @@
 // rows of all heads that share them.  7 products instead of the 5 of a single pass whose dq would be added up by atomics.
 //
 // The bias gradient needs dS summed along the diagonals of equal offset.  In mha_dq_k a wave adds the sums of each 32 x 32 piece into
-// rings of its own in LDS, indexed by offset modulo the ring, in a fixed order.  As the walk over the keys moves on, offsets that no later key can reach are summed over the block's rings
-// and written to the block's strip; mha_dvec_k and mha_drow_k add strips over blocks and offsets over buckets.  (LDS float atomics, one
-// ds_add_f32 per register, were the first form: 300 cycles each, two thirds of the whole backward pass.)
+// rings of its own in LDS, indexed by offset modulo the ring, in a fixed order.  As the walk over the keys moves on, offsets that no later
+// key can reach are summed over the block's rings and written to the block's strip; mha_dvec_k and mha_drow_k add strips over blocks and
+// offsets over buckets.  (LDS float atomics, one ds_add_f32 per register, were the first form: 300 cycles each, two thirds of the whole
+// backward pass.)
 #include "mha.h"
 
 using namespace mha;
@@ -143,7 +144,9 @@ __global__ __launch_bounds__(256) void mha_sum_k(const float* part, T* out, long
 
 // BIAS: 0 none, 1 tokens of a sequence (offset = key - query), 2 tokens of a map.  Everything a tile needs travels by LDS-DMA: K, V,
 // the piece of the expanded bias that its offsets lie in and (maps) the keys' codes; nothing in the loop waits for global memory
-// except the one drain per tile.
+// except the one drain per tile.  2 x 4097 tokens, 16 heads on 4 of 128 channels, bf16, with the bias gradient: 475 us, 870 TFLOP/s; fp32,
+// 4 x 2048, 8 heads of 64: 437 us, 118 TFLOP/s (matrix pipes 80 % busy); two 64 x 36 maps, 8 heads of 64, bf16: 154 us, 212 TFLOP/s, bound
+// by the vector instructions of the bias lookup and of map_diagonals.
 template <typename T, int DP, int BIAS>
 __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : DP <= 64 ? 2 : 1)) void mha_dq_k(const BwdP P) {
   typedef Tile<T, DP> TL;
@@ -408,6 +411,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : DP <= 6
     }
 }
 
+// Owns 128 keys, 32 per wave, and walks the 64-row tiles of the query heads that share them.  Scores are computed with keys in the lanes, so
+// P and dS are already operands of dv = P^T do and dk = dS^T q.  Bound by the matrix pipes, with one wave per SIMD above 64 channels: 2 x
+// 4097 tokens, 16 heads on 4 of 128, bf16 695 us, 790 TFLOP/s; fp32, 4 x 2048, 8 heads of 64: 595 us, 115 TFLOP/s (78 % busy).
 template <typename T, int DP, int BIAS>
 __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha_dkv_k(const BwdP P) {
   typedef Tile<T, DP> TL;
@@ -422,7 +428,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
   const Reader<T, DP> rd(sm, lane);
   constexpr int HALF = 32 * TL::kRowBytes;
   // samples and heads in turn: the blocks behind a short sample's last key have nothing to do and are spread over all XCDs
-  const int bh = (int)(blockIdx.x % (unsigned)(D.B * D.Hk)), kp = (int)(blockIdx.x / (unsigned)(D.B * D.Hk)), part = kp / P.ktiles, kt = kp - part * P.ktiles, b = bh / D.Hk, hk = bh - b * D.Hk;
+  const unsigned groups = D.B * D.Hk;
+  const int bh = (int)(blockIdx.x % groups), kp = (int)(blockIdx.x / groups), part = kp / P.ktiles, kt = kp - part * P.ktiles;
+  const int b = bh / D.Hk, hk = bh - b * D.Hk;
   const int key = kt * 128 + 32 * wave + li;
   const unsigned long long* words = D.words ? (const unsigned long long*)D.words + (size_t)b * D.nwords : nullptr;
   const int w0 = 2 * kt;
@@ -448,7 +456,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
   const int mine_k = BIAS == 2 ? D.code[key] - ckf : 32 * wave + li - 16 * half;
 
   const int qt = (D.Lq + BK - 1) / BK, all = (wa | wb) ? G * qt : 0;    // a block without a visible key writes zeros
-  const int each = (all + P.dkv_parts - 1) / P.dkv_parts, from = part * each < all ? part * each : all, n = from + each < all ? from + each : all;
+  const int each = (all + P.dkv_parts - 1) / P.dkv_parts;
+  const int from = part * each < all ? part * each : all, n = from + each < all ? from + each : all;
   const int wave_u = __builtin_amdgcn_readfirstlane(wave);
   const Filler<T, DP, BK, 4> fq(D.D, (unsigned)(D.sql * sizeof(T)), tid), fg(D.D, (unsigned)((size_t)D.Hq * D.D * sizeof(T)), tid);
   auto fetch = [&](int t, int st) {
@@ -487,7 +496,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
   for (int t = from; t < n; ++t) {
     const int st = P.stages == 2 ? (t - from) & 1 : 0;
     const int rows = rd.rows + st * STAGE, cols = rd.cols + st * STAGE;
-    const int stats = opaque(lds_at(sm) + st * STAGE + 2 * TILE + 64 * half), seg = opaque(lds_at(sm) + st * STAGE + 2 * TILE + 8 * BK + 4 * mine_k);
+    const int at = lds_at(sm) + st * STAGE + 2 * TILE, stats = opaque(at + 64 * half), seg = opaque(at + 8 * BK + 4 * mine_k);
     if (P.stages == 2 && t + 1 < n) fetch(t + 1, st ^ 1);
     const int q0 = (t % qt) * BK;
     if (!idle) {
@@ -655,14 +664,15 @@ int make(const so_mha_desc* d, BwdP& p) {
     p.qtiles = (rows * pitch + 127) / 128;
   }
   p.ktiles = (d->Lk + 127) / 128;
-  const double tiles = d->bias && !d->linear ? p.qtiles : mha_tiles(d->Lq), rows = (double)d->B * d->Lq * d->Hq * d->D, keys = (double)d->B * d->Lk * d->Hk * d->D;
+  const double tiles = d->bias && !d->linear ? p.qtiles : mha_tiles(d->Lq);
+  const double rows = (double)d->B * d->Lq * d->Hq * d->D, keys = (double)d->B * d->Lk * d->Hk * d->D;
   // fp32, 2 x 2049 tokens, 8 heads of 64, 272 blocks: mha_dq_k 350 us whole, 221 + 8 us in three parts
-  p.dq_parts = mha_split_parts(d->B * d->Hq * tiles, mha_us(6.0 * 128 * d->D * d->Lk, d->dtype), 6.0, rows * 8 / 4e6, d->Lk / 128, 0.95);
+  p.dq_parts = mha_split_parts((double)d->B * d->Hq * tiles, mha_us(6.0 * 128 * d->D * d->Lk, d->dtype), 6.0, rows * 8 / 4e6, d->Lk / 128, 0.95);
   // (blocks of keys that a mask hides end at once, which the estimate does not know: the rows are only cut for a clear gain.  A training
   // pass whole / cut: bf16, 2 x 4097 tokens, 16 heads on 4, 128 channels 2125 / 1725 us, with a fifth of the keys hidden 1935 / 1530;
   // 9000 tokens, 8 on 4, 64 channels 1127 / 999; fp32, 2 x 2049, 8 of 64 1066 / 870; 1000 tokens, 8 on 1, 128 channels 371 / 164)
   const double q_tiles = (double)d->Lq * (d->Hq / d->Hk) / 128;
-  p.dkv_parts = mha_split_parts(d->B * d->Hk * mha_tiles(d->Lk), mha_us(8.0 * 128 * 128 * d->D * q_tiles, d->dtype), 6.0, keys * 16 / 4e6,
+  p.dkv_parts = mha_split_parts((double)d->B * d->Hk * mha_tiles(d->Lk), mha_us(8.0 * 128 * 128 * d->D * q_tiles, d->dtype), 6.0, keys * 16 / 4e6,
                                 q_tiles < 8 ? (int)q_tiles : 8, 0.7);
   p.dkv_at = p.dq_parts > 1 ? (long long)rows * p.dq_parts : 0;
   p.stages = 2;
@@ -769,7 +779,8 @@ int so_mha_bwd(const void* desc, void* stream) {
   if (!d->q || !d->k || !d->v || !d->o || !d->dout || !d->dq || !d->dk || !d->dv || !d->lse || !d->delta) return SO_ERR_SHAPE;
   if ((((uintptr_t)d->dout) | ((uintptr_t)d->dq) | ((uintptr_t)d->dk) | ((uintptr_t)d->dv)) & 15) return SO_ERR_ALIGN;
   if ((p.dq_parts > 1 || p.dkv_parts > 1) && (!d->part_o || (((uintptr_t)d->part_o) & 15))) return SO_ERR_SHAPE;
-  if ((long long)d->B * d->Hq * p.qtiles * p.dq_parts > 0x7fffffffLL || (long long)d->B * d->Hk * p.ktiles * p.dkv_parts > 0x7fffffffLL) return SO_ERR_SHAPE;
+  const long long dq_blocks = (long long)d->B * d->Hq * p.qtiles * p.dq_parts, dkv_blocks = (long long)d->B * d->Hk * p.ktiles * p.dkv_parts;
+  if (dq_blocks > 0x7fffffffLL || dkv_blocks > 0x7fffffffLL) return SO_ERR_SHAPE;
   return d->dtype == SO_F32 ? launch_d<float>(p, (hipStream_t)stream) : launch_d<__bf16>(p, (hipStream_t)stream);
 }
 

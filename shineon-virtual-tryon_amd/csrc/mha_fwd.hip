@@ -120,7 +120,12 @@ __device__ __forceinline__ void prob_frags(const f32x16& s, typename Elem<T>::fr
 
 // Many rows: a block is 128 rows of one head, 32 per wave, and walks 64-key tiles.  BIAS: 0 none, 1 sequence, 2 map; the piece of the
 // expanded bias that a tile's offsets lie in travels to LDS with the tile.  (Read from global memory by every lane it took 120 of 495 us
-// at 8191 tokens, 16 heads of 64.)  EXACT: the 24 bits of a probability as three bf16 products (rounded to 8 or 16 bits, delta = do . o no longer matches what the backward pass recomputes, and the sums over rows that cancel in the bias gradient show it).
+// at 8191 tokens, 16 heads of 64.)  EXACT: the 24 bits of a probability as three bf16 products (rounded to 8 or 16 bits, delta = do . o
+// no longer matches what the backward pass recomputes, and the sums over rows that cancel in the bias gradient show it).
+//
+// Bound by the matrix pipes in fp32 (80 % busy: 118 TFLOP/s at 4 x 2048 tokens, 8 heads of 64) and at 128 bf16 channels (EXACT, 2 x 4097
+// tokens, 16 heads: 523 us, 1050 TFLOP/s); at 64 bf16 channels by the softmax's vector instructions, of which the matrix instructions hide
+// only a part (8191 tokens, 16 heads: 373 us, 735 TFLOP/s).
 template <typename T, int DP, int BIAS, bool EXACT>
 __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 96 ? 2 : 1))) void mha_fwd_k(const FwdP P) {
   typedef Tile<T, DP> TL;

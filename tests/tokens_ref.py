@@ -1,4 +1,4 @@
-"""Plain 64-bit forms of the token operators (tests are the checker) and the error bounds their tolerances are derived from."""
+"""Plain 64-bit forms of the token operators and the error bounds their tolerances are derived from."""
 import numpy as np
 import torch
 
