@@ -72,7 +72,10 @@ __device__ __forceinline__ void write_row(const FwdP& P, const f32x16 (&o)[NT], 
   if (D.lse && half == 0) D.lse[((size_t)b * D.Hq + head) * D.Lq + qi] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
-// the running softmax of 32 keys per half: s -> probabilities against the new maximum; o and l are rescaled when it moves
+// The running softmax of 32 keys per half: s -> probabilities against the reference m; o and l are rescaled when m moves.  m follows the
+// maximum only when that has grown by more than kSlack (log2 units): probabilities up to 2^kSlack lose nothing in a floating-point type,
+// and after a row's first tiles hardly any tile rescales (following every growth: 380 instead of 366 us at 8191 tokens, 16 heads of 64).
+constexpr float kSlack = 8.f;
 template <int N, int NT>
 __device__ __forceinline__ void softmax_step(f32x16 (&s)[N], f32x16 (&o)[NT], float& m, float& l, float c) {
   float mx = -INFINITY;
@@ -80,24 +83,24 @@ __device__ __forceinline__ void softmax_step(f32x16 (&s)[N], f32x16 (&o)[NT], fl
   for (int u = 0; u < N; ++u)
 #pragma unroll
     for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[u][r]);
-  const float mn = fmaxf(m, half_max(mx) * c), ms = mn == -INFINITY ? 0.f : mn;
-  const float alpha = exp2_(m - ms);
-  m = mn;
-  float sum = 0.f;
-#pragma unroll
-  for (int u = 0; u < N; ++u)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[u][r] = exp2_(__builtin_fmaf(s[u][r], c, -ms));
-      sum += s[u][r];
-    }
-  l = l * alpha + sum;
-  if (__any(alpha != 1.f)) {
+  mx = half_max(mx) * c;
+  if (__any(mx > m + kSlack)) {
+    const float mn = fmaxf(m, mx), alpha = exp2_(m - (mn == -INFINITY ? 0.f : mn));
+    m = mn;
+    l *= alpha;
 #pragma unroll
     for (int v = 0; v < NT; ++v)
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[v][r] *= alpha;
   }
+  const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+  for (int u = 0; u < N; ++u)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[u][r] = exp2_(__builtin_fmaf(s[u][r], c, -ms));
+      l += s[u][r];
+    }
 }
 
 template <typename T, int NCS, bool EXACT>
@@ -125,9 +128,10 @@ __device__ __forceinline__ void prob_frags(const f32x16& s, typename Elem<T>::fr
 //
 // Bound by the matrix pipes in fp32 (80 % busy: 118 TFLOP/s at 4 x 2048 tokens, 8 heads of 64) and at 128 bf16 channels (EXACT, 2 x 4097
 // tokens, 16 heads: 523 us, 1050 TFLOP/s); at 64 bf16 channels by the softmax's vector instructions, of which the matrix instructions hide
-// only a part (8191 tokens, 16 heads: 373 us, 735 TFLOP/s).
+// only a part (8191 tokens, 16 heads: 366 us, 750 TFLOP/s).
+// (Two waves per SIMD in fp32 end at 64 channels: at 96 their registers spill, 4 x 2048 tokens, 8 heads 490 against 455 us.)
 template <typename T, int DP, int BIAS, bool EXACT>
-__global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 96 ? 2 : 1))) void mha_fwd_k(const FwdP P) {
+__global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 64 ? 2 : 1))) void mha_fwd_k(const FwdP P) {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::frag frag;
   constexpr int E = Elem<T>::E, KM = 2 * E, NM = DP / KM, NT = DP / 32, NCS = 32 / KM;
