@@ -331,6 +331,22 @@ def test_attention_hidden_keys_may_hold_anything(tok, dtype, lq, lk):
 
 
 @TYPES
+@pytest.mark.parametrize("lq", [2, 70], ids=["few", "many"])
+@pytest.mark.parametrize("span", [-60.0, 4.0, 60.0, 3000.0])
+def test_attention_scores_that_rise_and_fall(tok, dtype, lq, span):
+    """Scores that climb (or fall) by `span` over the keys: the softmax's reference follows late, in steps, at once or never."""
+    lk, d = 700, 32
+    q, k, v = normal(1, 1, lq, 2, d, dtype=dtype, std=0.1), normal(2, 1, lk, 2, d, dtype=dtype, std=0.1), normal(3, 1, lk, 2, d, dtype=dtype)
+    q[..., 0], k[..., 0] = 1.0, (torch.arange(lk, device="cuda") / lk * span)[None, :, None].to(dtype)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o, do = tok.attention(*leaves, scale=1.0), normal(4, 1, lq, 2, d, dtype=dtype)
+    want = ref.attention(*(d64(t) for t in leaves), 1.0, None, None, d64(do), dtype)
+    ref.check(o, *want["o"], "o")
+    for name, g in zip(("dq", "dk", "dv"), torch.autograd.grad(o, leaves, do)):
+        ref.check(g, *want[name], name)
+
+
+@TYPES
 @pytest.mark.parametrize("d", [1, 3, 20, 33, 72, 100, 127])
 def test_attention_any_head_size(tok, dtype, d):
     _attention_case(tok, dtype, 1, 45, 70, 2, 1, d, shape=70)
