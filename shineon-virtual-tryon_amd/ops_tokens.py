@@ -136,10 +136,11 @@ def _dropout_launch(dt, x, p, rng, residual):
         x, (rows, c, ldx) = _in_order(x)
         if residual is not None:
             residual, (rr, rc, ldr) = _in_order(residual)
-            if rr != rows:      # one of the two is dense, the other has a pitch: both as rows
-                c = c if rows > 1 else rc
-                rows = n // c
-                ldx, ldr = (ldx if ldx < n else c), (ldr if ldr < n else c)
+            if rr != rows:      # one of the two is dense (one row of all elements), the other has a pitch: both as rows
+                if rows == 1:
+                    rows, c, ldx = rr, rc, rc
+                else:
+                    ldr = c
     if n:
         _launch(x.device, lib().so_dropout, "dropout", dt, x.data_ptr(), ldx, None if residual is None else residual.data_ptr(), ldr,
                 y.data_ptr(), c, rows, c, rng.data_ptr(), round(p * 4294967296.0), 1.0 / (1.0 - p) if p < 1.0 else 0.0)

@@ -75,6 +75,19 @@ def test_dropout_reads_slices_in_counting_order(tok, dtype):
 
 
 @TYPES
+def test_dropout_reads_few_rows_of_a_wide_tensor(tok, dtype):
+    """Slices whose pitch is at least their number of elements, beside a dense operand."""
+    p, rng = 0.4, tok.rng_state(7, "cuda", 100)
+    wide = normal(1, 1, 40, 2, 1, dtype=dtype).contiguous(memory_format=torch.channels_last)
+    cases = [normal(2, 2, 100, dtype=dtype)[:, :4], normal(3, 1, 3, 24, dtype=dtype)[..., 8:16], normal(4, 5, 100, dtype=dtype)[:, 7:8], wide[:, :6]]
+    for x in cases:
+        dense = x.clone(memory_format=torch.channels_last if x.dim() == 4 else torch.contiguous_format)
+        want = tok.dropout(dense, p, rng, residual=dense)
+        for a, b in ((x, dense), (dense, x), (x, x)):
+            assert torch.equal(tok.dropout(a, p, rng, residual=b), want)
+
+
+@TYPES
 def test_dropout_limits(tok, dtype):
     rng = tok.rng_state(3, "cuda")
     x = normal(1, 333, dtype=dtype)
