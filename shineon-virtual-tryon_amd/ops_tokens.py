@@ -62,6 +62,12 @@ def _first_order(backward):
     return lambda ctx, *grads: (checked if torch.is_grad_enabled() else backward)(ctx, *grads)
 
 
+def _places(*tensors):
+    """Where operands lie, to tell in the backward pass whether the tape hands back what the forward pass's descriptor describes: saved
+    tensors may come back elsewhere or with other strides (hooks, checkpoints)."""
+    return [None if t is None else (t.data_ptr(), t.stride()) for t in tensors]
+
+
 # ------------------------------------------------------------------------------------------------
 # dropout
 # ------------------------------------------------------------------------------------------------
@@ -233,6 +239,7 @@ class _QkNormRotaryFn(torch.autograd.Function):
         yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
         ctx.save_for_backward(q, k, wq, wk, cos, sin, positions)
+        ctx.places = _places(q, k, wq, wk, cos, sin, positions)
         ctx.desc = _qk_desc(q, k, wq, wk, cos, sin, positions, start, eps, dt)
         if b and n:
             _launch(q.device, lib().so_qk_norm_rotary_fwd, "qk_norm_rotary_fwd", ctypes.addressof(ctx.desc), yq.data_ptr(), yk.data_ptr())
@@ -243,9 +250,9 @@ class _QkNormRotaryFn(torch.autograd.Function):
     def backward(ctx, dyq, dyk):
         q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
         x = ctx.desc
-        at = tuple(None if t is None else t.data_ptr() for t in (q, k, wq, wk, cos, sin, positions))
-        if at != (x.q, x.k, x.wq, x.wk, x.cosv, x.sinv, x.pos):      # saved tensors may come back elsewhere (hooks, checkpoints)
+        if ctx.places != _places(q, k, wq, wk, cos, sin, positions):
             q, k = _heads(q, "q"), _heads(k, "k")
+            wq, wk, cos, sin = (t.contiguous() for t in (wq, wk, cos, sin))
             x = _qk_desc(q, k, wq, wk, cos, sin, positions, x.start, x.eps, x.dtype)
         dyq, dyk = dyq.contiguous(), dyk.contiguous()
         dq, dk = torch.empty_like(dyq), torch.empty_like(dyk)
@@ -432,7 +439,7 @@ class _AttentionFn(torch.autograd.Function):
             x.part_ml = x.part_o + 4 * b * hq * lq * parts * d
         _launch(dev, L.so_mha_fwd, "mha_fwd", at)
         if train:
-            ctx.desc = x
+            ctx.desc, ctx.places = x, _places(q, k, v)
             ctx.save_for_backward(q, k, v, table, o, o_f32, lse, bias, words)
         return o if d == d_true else o[..., :d_true].contiguous()
 
@@ -446,10 +453,11 @@ class _AttentionFn(torch.autograd.Function):
                     None, None, None, None, None, None)
         q, k, v, table, o, o_f32, lse, bias, words = ctx.saved_tensors
         x = _Desc.from_buffer_copy(ctx.desc)      # a second backward pass of the same graph must not see this one's pointers
-        if q.data_ptr() != x.q or k.data_ptr() != x.k or v.data_ptr() != x.v:      # saved tensors may come back elsewhere (hooks, checkpoints)
+        if ctx.places != _places(q, k, v):
             q, k, v = _rows16(q, "q"), _rows16(k, "k"), _rows16(v, "v")
             x.q, x.k, x.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
             (x.sqb, x.sql, x.sqh), (x.skb, x.skl, x.skh), (x.svb, x.svl, x.svh) = _strides(q), _strides(k), _strides(v)
+        o, o_f32, lse, bias, words = (None if t is None else t.contiguous() for t in (o, o_f32, lse, bias, words))
         x.o, x.lse = o.data_ptr(), lse.data_ptr()
         if o_f32 is not None:
             x.o_f32 = o_f32.data_ptr()

@@ -605,6 +605,37 @@ def test_saved_tensors_may_come_back_elsewhere(tok, dtype, how):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def _dense_in_place(t):
+    """What a hook may hand back: the same values at the same address, densely."""
+    if t.is_contiguous():
+        return t
+    dense = t.clone(memory_format=torch.contiguous_format)
+    return t.as_strided(t.shape, dense.stride(), t.storage_offset()).copy_(dense)
+
+
+@TYPES
+def test_saved_tensors_may_come_back_with_other_strides(tok, dtype):
+    """Head-major operands and transposed positions whose saved copies come back dense, at the addresses they had."""
+    def major(i, h):
+        return normal(80 + i, 2, h, 40, 32, dtype=dtype)
+
+    plan, rot, w = tok.RelativePositions(40, 8, 20), tok.rotary_table(40, 32), 1 + 0.1 * normal(70, 32)
+    positions, table = torch.randint(0, 40, (40, 2), generator=torch.Generator().manual_seed(4)).cuda(), normal(71, plan.rows, 8)
+    leaves = [t.requires_grad_() for t in (major(0, 8), major(1, 2), major(2, 2), w, table)]
+    dy = [normal(72 + i, 2, 40, h, 32, dtype=dtype) for i, h in enumerate((8, 8, 2))]
+
+    def run():
+        q, k, v = ((t * 1).transpose(1, 2) for t in leaves[:3])      # [B, L, H, D], strides of [B, H, L, D]
+        yq, yk = tok.qk_norm_rotary((leaves[0] * 1).transpose(1, 2), (leaves[1] * 1).transpose(1, 2), leaves[3] * 1, leaves[3] * 1, *rot,
+                                    positions=(positions * 1).t())
+        return tok.attention(q, k, v, relative=plan, bias_table=leaves[4] * 1), yq, yk
+
+    want = torch.autograd.grad(run(), leaves, dy)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, _dense_in_place):
+        y = run()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, dy), want))
+
+
 def test_second_order_is_refused(tok):
     x = normal(1, 2, 5, 4, 16).requires_grad_()
     cos, sin = tok.rotary_table(5, 16)
