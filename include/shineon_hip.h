@@ -555,7 +555,8 @@ typedef struct so_mha_desc {
   const void *q, *k, *v;
   void* o;
   float* o_f32;                /* bf16, training: the result before its rounding, laid out like o; NULL otherwise */
-  float* lse;                  /* training: [B][Hq][Lq], log2 of the softmax denominators (+inf: empty row); or NULL */
+  float* stats;                /* training: [2][B][Hq][Lq], the softmax's reference m in log2 units (+inf: empty row), then 1 / sum 2^(score - m)
+                                * (0: empty row); or NULL */
   const float* bias;
   const int* code;
   const void* words;

@@ -1,6 +1,6 @@
 // Multi-head attention with a learned relative position bias, backward, gfx950.
 //
-//   P = exp2(c s - lse),  delta_i = sum_c do_ic o_ic,  dS = P (do v^T - delta),
+//   P = exp2(c s - m) / l,  delta_i = sum_c do_ic o_ic,  dS = P (do v^T - delta),
 //   dq = scale dS k,  dk = scale dS^T q,  dv = P^T do,  dtable[r][h] = sum of dS_h over the pairs of bucket r
 //
 // Two passes over the score matrix, each rebuilding P from q, k and the saved row statistics, so that every sum has one owner and a
@@ -153,9 +153,6 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : DP <= 6
   typedef typename Elem<T>::frag frag;
   constexpr int E = Elem<T>::E, KM = 2 * E, NM = DP / KM, NT = DP / 32, NCS = 32 / KM;
   constexpr int TILE = BK * TL::kRowBytes;
-  // start the product do v^T at -delta (sixteen registers that hold it) where that does not spill; else subtract it.  Never in fp32: with
-  // a C operand that outlives the MFMA, hipcc reuses its registers right behind the fp32 form, and dq came out wrong at 128 channels.
-  constexpr bool kInit = sizeof(T) == 2 && DP <= 32;
   extern __shared__ __attribute__((aligned(512))) char sm[];          // [stages][K tile | V tile | bias | codes] | rings
   const so_mha_desc& D = P.d;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
@@ -217,7 +214,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : DP <= 6
     delta = half_sum(delta);
   }
   const size_t stat = ((size_t)b * D.Hq + head) * D.Lq + qi;
-  const float lse = rowv ? D.lse[stat] : INFINITY;
+  const float m_ref = rowv ? D.stats[stat] : INFINITY, inv = rowv ? D.stats[(size_t)D.B * D.Hq * D.Lq + stat] : 0.f, delta_inv = delta * inv;
   if (rowv && half == 0 && part == 0) D.delta[stat] = -delta;
 
   // the first offset of tile t's piece of the bias is code(first key) - code(last query)
@@ -322,7 +319,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : DP <= 6
         for (int r = 0; r < 16; ++r) s[r] = 0.f;
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) dp[r] = kInit ? -delta : 0.f;
+      for (int r = 0; r < 16; ++r) dp[r] = 0.f;
       if (u == 0) {
         const int rb = opaque(rows);
 #pragma unroll
@@ -338,7 +335,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : DP <= 6
         phase(f, [&](int m, const frag& a) { s = mma(a, q[m], s); }, [&](int m) { return rd.col(cb, m % NT, m / NT, HALF * u); });
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = exp2_(__builtin_fmaf(s[r], P.c, -lse)) * (kInit ? dp[r] : dp[r] - delta);      // dS
+      for (int r = 0; r < 16; ++r) s[r] = exp2_(__builtin_fmaf(s[r], P.c, -m_ref)) * __builtin_fmaf(dp[r], inv, -delta_inv);      // dS
       const unsigned w = (unsigned)(w64 >> (32 * u));
       if (w != ~0u) {
         seldom();
@@ -420,7 +417,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
   typedef typename Elem<T>::frag frag;
   constexpr int E = Elem<T>::E, KM = 2 * E, NM = DP / KM, NT = DP / 32, NCS = 32 / KM;
   constexpr int TILE = BK * TL::kRowBytes;
-  extern __shared__ __attribute__((aligned(512))) char sm[];          // [stages][Q tile | dO tile | lse | -delta | bias | codes]
+  extern __shared__ __attribute__((aligned(512))) char sm[];          // [stages][Q tile | dO tile | m | 1 / l | -delta | bias | codes]
   const so_mha_desc& D = P.d;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
   const int G = D.Hq / D.Hk;
@@ -466,16 +463,17 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
     char* qtile = sm + st * STAGE;
     fq.fill(qtile, (const T*)D.q + (size_t)b * D.sqb + (size_t)head * D.sqh + (size_t)q0 * D.sql, rows, 0, wave_u);
     fg.fill(qtile + TILE, (const T*)D.dout + (((size_t)b * D.Lq + q0) * D.Hq + head) * D.D, rows, 0, wave_u);
-    char* stats = qtile + 2 * TILE;      // lse | -delta | bias | codes
+    char* stats = qtile + 2 * TILE;      // m | 1 / l | -delta | bias | codes
     const size_t at = ((size_t)b * D.Hq + head) * D.Lq + q0;
     const unsigned left = D.Lq - q0 < BK ? 4 * (D.Lq - q0) : 4 * BK;
-    fill_dwords<4>(stats, D.lse + at, BK, left, wave_u, lane);
-    fill_dwords<4>(stats + 4 * BK, D.delta + at, BK, left, (wave_u + 1) & 3, lane);
+    fill_dwords<4>(stats, D.stats + at, BK, left, wave_u, lane);
+    fill_dwords<4>(stats + 4 * BK, D.stats + (size_t)D.B * D.Hq * D.Lq + at, BK, left, (wave_u + 1) & 3, lane);
+    fill_dwords<4>(stats + 8 * BK, D.delta + at, BK, left, (wave_u + 2) & 3, lane);
     if constexpr (BIAS != 0) {
       const int* cp = D.code + D.q_start + q0;
       const int cl = BIAS == 2 ? cp[BK - 1] : D.q_start + q0 + BK - 1, n = BIAS == 2 ? ckl - cp[0] - (ckf - cl) + 1 : 128 + BK - 1;
-      fill_dwords<4>(stats + 8 * BK, D.bias + (size_t)head * D.V + D.code_max + ckf - cl, n, 0x7FFFFFFFu, (wave_u + 2) & 3, lane);
-      if constexpr (BIAS == 2) fill_dwords<4>(stats + 8 * BK + 4 * P.seg, cp, BK, 0x7FFFFFFFu, (wave_u + 3) & 3, lane);
+      fill_dwords<4>(stats + 12 * BK, D.bias + (size_t)head * D.V + D.code_max + ckf - cl, n, 0x7FFFFFFFu, (wave_u + 3) & 3, lane);
+      if constexpr (BIAS == 2) fill_dwords<4>(stats + 12 * BK + 4 * P.seg, cp, BK, 0x7FFFFFFFu, wave_u, lane);
     }
   };
 
@@ -496,7 +494,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
   for (int t = from; t < n; ++t) {
     const int st = P.stages == 2 ? (t - from) & 1 : 0;
     const int rows = rd.rows + st * STAGE, cols = rd.cols + st * STAGE;
-    const int at = lds_at(sm) + st * STAGE + 2 * TILE, stats = opaque(at + 64 * half), seg = opaque(at + 8 * BK + 4 * mine_k);
+    const int at = lds_at(sm) + st * STAGE + 2 * TILE, stats = opaque(at + 64 * half), seg = opaque(at + 12 * BK + 4 * mine_k);
     if (P.stages == 2 && t + 1 < n) fetch(t + 1, st ^ 1);
     const int q0 = (t % qt) * BK;
     if (!idle) {
@@ -507,7 +505,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = lds_read<float>(seg + 4 * (BK - 1 - 32 * u - r));
       } else if constexpr (BIAS == 2) {
-        const int codes = lds_at(sm) + st * STAGE + 2 * TILE + 8 * BK + 4 * P.seg, last = seg + 4 * lds_read<int>(codes + 4 * (BK - 1));
+        const int codes = lds_at(sm) + st * STAGE + 2 * TILE + 12 * BK + 4 * P.seg, last = seg + 4 * lds_read<int>(codes + 4 * (BK - 1));
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const i32x4 c = lds_read<i32x4>(codes + 64 * half + 128 * u + 16 * g);
@@ -520,7 +518,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
       }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const f32x4 de = lds_read<f32x4>(stats + 4 * BK + 128 * u + 16 * g);
+        const f32x4 de = lds_read<f32x4>(stats + 8 * BK + 128 * u + 16 * g);
 #pragma unroll
         for (int e = 0; e < 4; ++e) dp[4 * g + e] = de[e];
       }
@@ -547,11 +545,11 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha
       // a hidden key's lane computes like the others (its k and v are zero) and stores zeros at the end
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const f32x4 ls = lds_read<f32x4>(stats + 128 * u + 16 * g);
+        const f32x4 ms = lds_read<f32x4>(stats + 128 * u + 16 * g), inv = lds_read<f32x4>(stats + 4 * BK + 128 * u + 16 * g);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = 4 * g + e;
-          s[r] = exp2_(__builtin_fmaf(s[r], P.c, -ls[e]));
+          s[r] = exp2_(__builtin_fmaf(s[r], P.c, -ms[e])) * inv[e];
           dp[r] *= s[r];
         }
       }
@@ -725,7 +723,7 @@ int launch(BwdP p, hipStream_t st) {
   hipLaunchKernelGGL((mha_dq_k<T, DP, BIAS>), dim3((unsigned)((long long)p.d.B * p.d.Hq * p.qtiles * p.dq_parts)), dim3(256), lds, st, p);
   err = SO_LAUNCH_CHECK();
   if (err) return err;
-  stage = (2 * tile + 2 * BK * 4 + piece + 511) & ~(size_t)511;
+  stage = (2 * tile + 3 * BK * 4 + piece + 511) & ~(size_t)511;
   p.stages = 2 * stage <= kLds ? 2 : 1;
   lds = p.stages * stage;
   p.stage_bytes = (int)stage;
@@ -776,7 +774,7 @@ int so_mha_bwd(const void* desc, void* stream) {
   BwdP p;
   const int err = make(d, p);
   if (err) return err;
-  if (!d->q || !d->k || !d->v || !d->o || !d->dout || !d->dq || !d->dk || !d->dv || !d->lse || !d->delta) return SO_ERR_SHAPE;
+  if (!d->q || !d->k || !d->v || !d->o || !d->dout || !d->dq || !d->dk || !d->dv || !d->stats || !d->delta) return SO_ERR_SHAPE;
   if ((((uintptr_t)d->dout) | ((uintptr_t)d->dq) | ((uintptr_t)d->dk) | ((uintptr_t)d->dv)) & 15) return SO_ERR_ALIGN;
   if ((p.dq_parts > 1 || p.dkv_parts > 1) && (!d->part_o || (((uintptr_t)d->part_o) & 15))) return SO_ERR_SHAPE;
   const long long dq_blocks = (long long)d->B * d->Hq * p.qtiles * p.dq_parts, dkv_blocks = (long long)d->B * d->Hk * p.ktiles * p.dkv_parts;

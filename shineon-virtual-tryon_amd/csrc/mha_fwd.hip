@@ -26,7 +26,15 @@ struct FwdP {
 
 constexpr int kLds = 160 * 1024;
 
-// one row's result: o / l (or o, m, l of a part), its rounding rest and log2 of its sum
+// A row's softmax for the backward pass: reference and 1 / l apart.  Their sum in log2 units would lose l where scores are large (at 2^30 a
+// step of fp32 is 64 to 128), and with it the rounding of m, which is a common factor of the row's probabilities that l carries too.
+__device__ __forceinline__ void write_stats(const so_mha_desc& D, int b, int head, int qi, float m, float l, float inv) {
+  const size_t at = ((size_t)b * D.Hq + head) * D.Lq + qi;
+  D.stats[at] = l == 0.f ? INFINITY : m;
+  D.stats[(size_t)D.B * D.Hq * D.Lq + at] = inv;
+}
+
+// one row's result: o / l (or o, m, l of a part) and its statistics
 template <typename T, int NT>
 __device__ __forceinline__ void write_row(const FwdP& P, const f32x16 (&o)[NT], float m, float l, int b, int hk, int head, int qi, int part, int half) {
   const so_mha_desc& D = P.d;
@@ -69,7 +77,7 @@ __device__ __forceinline__ void write_row(const FwdP& P, const f32x16 (&o)[NT], 
         if (fp) *reinterpret_cast<f32x4*>(fp + c) = x;
       }
     }
-  if (D.lse && half == 0) D.lse[((size_t)b * D.Hq + head) * D.Lq + qi] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+  if (D.stats && half == 0) write_stats(D, b, head, qi, m, l, inv);
 }
 
 // The running softmax of 32 keys per half: s -> probabilities against the reference m; o and l are rescaled when m moves.  m follows the
@@ -512,7 +520,7 @@ __device__ __forceinline__ void write_joined(const so_mha_desc& D, long long at,
   }
   *reinterpret_cast<t4*>((T*)D.o + orow + c) = y;
   if (D.o_f32) *reinterpret_cast<f32x4*>(D.o_f32 + orow + c) = x;
-  if (D.lse && c == 0) D.lse[((size_t)b * D.Hq + head) * D.Lq + qi] = l == 0.f ? INFINITY : mn + __builtin_amdgcn_logf(l);
+  if (D.stats && c == 0) write_stats(D, b, head, qi, mn, l, inv);
 }
 
 // up to kJoin parts: half a wave per row, four channels per lane
@@ -741,7 +749,7 @@ int so_mha_prep(const float* table, const void* lut, int V, int H, float scale, 
   p.bias_blocks = table ? (V + 255) / 256 : 0;
   p.inv_scale = 1.f / scale;
   // Finite entries are kept within +-2^30 in the kernels' log2 units: exp2(fma(acc, c, -m)) sees the rounding of m = max(acc c), at most
-  // 2^-24 of it, as a common factor of a row - at 2^30 that is 2^64, still far from overflow.
+  // 2^-24 of it, as a common factor of a row - at 2^30 that is 2^64, still far from overflow - which the row's sum carries as well.
   p.top = 1073741824.f / (scale * kLog2e);
   const long long mb = mask ? ((long long)B * p.nwords + 3) / 4 : 0;
   if (p.bias_blocks + mb == 0) return 0;

@@ -304,7 +304,7 @@ def qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions=None, start=0, 
 # ------------------------------------------------------------------------------------------------
 class _Desc(ctypes.Structure):
     """so_mha_desc of include/shineon_hip.h."""
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "o", "o_f32", "lse", "bias", "code", "words", "part_o", "part_ml", "dout",
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "o", "o_f32", "stats", "bias", "code", "words", "part_o", "part_ml", "dout",
                                                 "dq", "dk", "dv", "delta", "strips")]
                 + [(n, ctypes.c_longlong) for n in ("sqb", "sql", "sqh", "skb", "skl", "skh", "svb", "svl", "svh")]
                 + [(n, ctypes.c_int) for n in ("dtype", "B", "Hq", "Hk", "Lq", "Lk", "D", "V", "code_max", "tokens", "q_start", "linear",
@@ -410,7 +410,7 @@ class _AttentionFn(torch.autograd.Function):
         x = _Desc(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr())
         (x.sqb, x.sql, x.sqh), (x.skb, x.skl, x.skh), (x.svb, x.svl, x.svh) = _strides(q), _strides(k), _strides(v)
         x.dtype, x.B, x.Hq, x.Hk, x.Lq, x.Lk, x.D, x.nwords, x.scale = dt, b, hq, hk, lq, lk, d, (lk + 63) // 64, scale
-        words = bias = lse = o_f32 = None
+        words = bias = stats = o_f32 = None
         mp = msb = tp = lp = None
         if mask is not None:
             words = torch.empty((b, x.nwords), dtype=torch.int64, device=dev)
@@ -423,8 +423,8 @@ class _AttentionFn(torch.autograd.Function):
         if mp is not None or tp is not None:
             _launch(dev, L.so_mha_prep, "mha_prep", tp, lp, x.V, hq, scale, x.bias, mp, msb or 0, b, lk, x.words)
         if train:
-            lse = torch.empty((b, hq, lq), dtype=torch.float32, device=dev)
-            x.lse = lse.data_ptr()
+            stats = torch.empty((2, b, hq, lq), dtype=torch.float32, device=dev)
+            x.stats = stats.data_ptr()
             if dt == 1:
                 o_f32 = torch.empty(o.shape, dtype=torch.float32, device=dev)
                 x.o_f32 = o_f32.data_ptr()
@@ -440,7 +440,7 @@ class _AttentionFn(torch.autograd.Function):
         _launch(dev, L.so_mha_fwd, "mha_fwd", at)
         if train:
             ctx.desc, ctx.places = x, _places(q, k, v)
-            ctx.save_for_backward(q, k, v, table, o, o_f32, lse, bias, words)
+            ctx.save_for_backward(q, k, v, table, o, o_f32, stats, bias, words)
         return o if d == d_true else o[..., :d_true].contiguous()
 
     @staticmethod
@@ -451,14 +451,14 @@ class _AttentionFn(torch.autograd.Function):
             q, k, v, table = ctx.saved_tensors
             return (*(torch.zeros_like(t[..., :d_true]) for t in (q, k, v)), None if table is None else torch.zeros_like(table),
                     None, None, None, None, None, None)
-        q, k, v, table, o, o_f32, lse, bias, words = ctx.saved_tensors
+        q, k, v, table, o, o_f32, stats, bias, words = ctx.saved_tensors
         x = _Desc.from_buffer_copy(ctx.desc)      # a second backward pass of the same graph must not see this one's pointers
         if ctx.places != _places(q, k, v):
             q, k, v = _rows16(q, "q"), _rows16(k, "k"), _rows16(v, "v")
             x.q, x.k, x.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
             (x.sqb, x.sql, x.sqh), (x.skb, x.skl, x.skh), (x.svb, x.svl, x.svh) = _strides(q), _strides(k), _strides(v)
-        o, o_f32, lse, bias, words = (None if t is None else t.contiguous() for t in (o, o_f32, lse, bias, words))
-        x.o, x.lse = o.data_ptr(), lse.data_ptr()
+        o, o_f32, stats, bias, words = (None if t is None else t.contiguous() for t in (o, o_f32, stats, bias, words))
+        x.o, x.stats = o.data_ptr(), stats.data_ptr()
         if o_f32 is not None:
             x.o_f32 = o_f32.data_ptr()
         if bias is not None:

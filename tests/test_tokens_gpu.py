@@ -323,6 +323,48 @@ def test_attention_blocking_entries(tok, dtype):
         assert (g == 0).all()
 
 
+LOW = [torch.finfo(F32).min, -1e9, -1e8, -1e6, 1e6, 1e9]
+
+
+@TYPES
+@pytest.mark.parametrize("entry", LOW, ids=lambda v: f"{v:.0e}")
+@pytest.mark.parametrize("shape,lq,d", [(50, 50, 32), ((16, 12), 192, 64), (300, 300, 128), (4099, 1, 64)], ids=str)
+def test_attention_gradients_of_rows_with_one_large_entry(tok, dtype, entry, shape, lq, d):
+    """Every pair has the same entry of a great amount: the softmax is the one without it, and so are all gradients.  Queries and keys use
+    different channels, so that every score is the entry itself."""
+    lk = shape if isinstance(shape, int) else shape[0] * shape[1]
+    q, k, v = normal(1, 1, lq, 2, d, dtype=dtype), normal(2, 1, lk, 2, d, dtype=dtype), normal(3, 1, lk, 2, d, dtype=dtype)
+    q[..., d // 2:], k[..., :d // 2] = 0, 0
+    rel = tok.RelativePositions(shape, 8, 20)
+    leaves = [t.requires_grad_() for t in (q, k, v, torch.full((rel.rows, 2), entry, device="cuda"))]
+    o, do = tok.attention(*leaves[:3], relative=rel, bias_table=leaves[3], q_start=lk - lq), normal(4, 1, lq, 2, d, dtype=dtype)
+    want = ref.attention(*(d64(t) for t in leaves[:3]), d ** -0.5, dout=d64(do), dtype=dtype, exact=True)
+    ref.check(o, *want["o"], "o")
+    grads = torch.autograd.grad(o, leaves, do)
+    for name, g in zip(("dq", "dk", "dv"), grads):
+        ref.check(g, *want[name], name)
+    ref.check(grads[3], *ref.table_grad(*want["ds"], ref.pair_buckets(shape, lq, lk, lk - lq, 8, 20), rel.rows), "dtable")
+
+
+@TYPES
+@pytest.mark.parametrize("lq,lk,d", [(130, 200, 64), (3, 700, 128)])
+def test_attention_backward_probabilities_sum_to_one(tok, dtype, lq, lk, d):
+    """Table entries of millions: whatever the scores round to, the probabilities that the backward pass rebuilds add up to one in every
+    row (gradients of the values, for a gradient of ones) and its dS to nothing (gradients of the table)."""
+    q, k, v = normal(1, 1, lq, 1, d, dtype=dtype), normal(2, 1, lk, 1, d, dtype=dtype), normal(3, 1, lk, 1, d, dtype=dtype).requires_grad_()
+    rel = tok.RelativePositions(lk, 32, 128)
+    table = normal(4, rel.rows, 1, std=3e6).requires_grad_()
+    o = tok.attention(q, k, v, relative=rel, bias_table=table)
+    (dv,) = torch.autograd.grad(o, v, torch.ones_like(o), retain_graph=True)
+    # a row's probabilities are rebuilt to 24 + lk / 8 steps and, as operands, rounded to the type; so is their sum over the rows
+    step = ref.U32 * (24 + lk / 8 + lq) + (0 if dtype == F32 else 2 * ref.HALF_STEP[dtype])
+    ref.check(dv.double().sum(1), torch.full((1, 1, d), float(lq), dtype=torch.float64), torch.full((1, 1, d), lq * step, dtype=torch.float64), "dv")
+    do = normal(5, 1, lq, 1, d, dtype=dtype)
+    (dt,) = torch.autograd.grad(o, table, do)
+    size = 2 * (d64(do).abs().sum() * d64(v).abs().max()).item()      # of |P dp| + |P delta| over the rows
+    assert abs(d64(dt).sum().item()) <= ref.U32 * (24 + lk / 8 + d + lq) * size
+
+
 @TYPES
 @pytest.mark.parametrize("lq,lk", [(40, 150), (2, 900)])
 def test_attention_hidden_keys_may_hold_anything(tok, dtype, lq, lk):
