@@ -513,7 +513,8 @@ int so_gan_loss_bwd(const float* x, int ldx, long long rows, int C, int mode, in
 
 /* ---- token operators (csrc/dropout.hip, csrc/qkrope.hip) ----------------------------------------
  * nn.Dropout of the U-Net blocks (models/networks/cpvton/unet.py, use_dropout) and of token blocks, and what an attention over
- * tokens applies to its queries and keys.  Elements are SO_F32 or SO_BF16 (`dtype`), all arithmetic is fp32. */
+ * tokens applies to its queries and keys.  Elements are SO_F32 or SO_BF16 (`dtype`), arithmetic is fp32 between the loads and the
+ * one rounding of a result (attention's backward pass in SO_BF16 rounds operands of its products too: so_mha_bwd). */
 
 /* state = {seed, offset} (int64, device): out <- state, then offset += blocks.  One node per draw: a captured graph replays with
  * new numbers. */
@@ -567,7 +568,6 @@ typedef struct so_mha_desc {
   float* strips;               /* backward, gradient of the bias: so_mha_strip_floats */
   long long sqb, sql, sqh, skb, skl, skh, svb, svl, svh;
   int dtype, B, Hq, Hk, Lq, Lk, D, V, code_max, tokens, q_start, linear, nwords;
-  int exact;                   /* bf16 forward: probabilities as three bf16 products (the bias gradient needs o to fp32 accuracy) */
   int width;                   /* tokens of a map row (a sequence: its length) */
   float scale;
 } so_mha_desc;
@@ -580,7 +580,7 @@ int so_mha_prep(const float* table, const void* lut, int V, int H, float scale, 
 /* parts of the key axis that so_mha_fwd will use for this problem (>= 1), or an error */
 int so_mha_parts(const void* desc);
 int so_mha_fwd(const void* desc, void* stream);
-/* dq, dk, dv from dout; with strips also the per-block sums of the bias gradient over equal offsets, which so_mha_dtable adds up:
+/* dq, dk, dv from dout (SO_BF16: probabilities and their gradients are rounded to bf16 as operands of these three products); with strips also the per-block sums of the bias gradient over equal offsets, which so_mha_dtable adds up:
  * dtable[r][h] = sum over offsets v of row r (order[start[r]] .. order[start[r + 1] - 1]).  dvec: Hq * V floats of scratch. */
 long long so_mha_strip_floats(const void* desc);
 long long so_mha_bwd_floats(const void* desc);      /* part_o of the backward pass; 0: none needed */

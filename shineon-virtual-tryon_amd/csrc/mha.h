@@ -130,7 +130,8 @@ __device__ __forceinline__ void lds_read16(int at, f32x16& v) {
 }
 
 // accumulator registers of step c as a B fragment; bf16 rounds here (half a step, 2^-8 of the value: the products run at the rate of
-// 16-bit operands; sums, statistics and accumulators stay fp32)
+// 16-bit operands; sums, statistics and accumulators stay fp32).  The backward pass takes one fragment, the forward pass as many as the
+// value has bits (kPieces)
 __device__ __forceinline__ void to_frag(const f32x16& a, int c, f32x4& f) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) f[e] = a[4 * c + e];

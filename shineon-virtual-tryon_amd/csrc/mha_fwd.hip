@@ -111,34 +111,36 @@ __device__ __forceinline__ void softmax_step(f32x16 (&s)[N], f32x16 (&o)[NT], fl
     }
 }
 
-template <typename T, int NCS, bool EXACT>
-__device__ __forceinline__ void prob_frags(const f32x16& s, typename Elem<T>::frag (&p)[EXACT ? 3 : 1][NCS]) {
+// Probabilities as operands of the product with v.  bf16: in three pieces, each the 8 bits of what the ones before leave, multiplied one after
+// the other, so that all 24 bits take part.  One piece adds as much error to o as o's own rounding (2.3e-3 instead of 1.7e-3 of its norm), two
+// show in delta = do . o against the probabilities that the backward pass rebuilds: the bias gradient's sums over rows cancel, and it is 2 to
+// 5 times further off.  Pieces by what wants a gradient would make o's bits depend on that.  (8191 tokens, 16 heads of 64: 360, 487, 616 us with
+// one, two, three.)
+template <typename T> constexpr int kPieces = sizeof(T) == 2 ? 3 : 1;
+template <typename T, int NCS>
+__device__ __forceinline__ void prob_frags(const f32x16& s, typename Elem<T>::frag (&p)[kPieces<T>][NCS]) {
   constexpr int E = Elem<T>::E;
 #pragma unroll
   for (int c = 0; c < NCS; ++c) {
     to_frag(s, c, p[0][c]);
-    if constexpr (EXACT) {
-      f32x16 rest;
+    f32x16 rest;
 #pragma unroll
-      for (int i = 1; i < 3; ++i) {
+    for (int i = 1; i < kPieces<T>; ++i) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) rest[E * c + e] = (i == 1 ? s : rest)[E * c + e] - (float)p[i - 1][c][e];
-        to_frag(rest, c, p[i][c]);
-      }
+      for (int e = 0; e < E; ++e) rest[E * c + e] = (i == 1 ? s : rest)[E * c + e] - (float)p[i - 1][c][e];
+      to_frag(rest, c, p[i][c]);
     }
   }
 }
 
 // Many rows: a block is 128 rows of one head, 32 per wave, and walks 64-key tiles.  BIAS: 0 none, 1 sequence, 2 map; the piece of the
 // expanded bias that a tile's offsets lie in travels to LDS with the tile.  (Read from global memory by every lane it took 120 of 495 us
-// at 8191 tokens, 16 heads of 64.)  EXACT: the 24 bits of a probability as three bf16 products (rounded to 8 or 16 bits, delta = do . o
-// no longer matches what the backward pass recomputes, and the sums over rows that cancel in the bias gradient show it).
+// at 8191 tokens, 16 heads of 64.)
 //
-// Bound by the matrix pipes in fp32 (80 % busy: 118 TFLOP/s at 4 x 2048 tokens, 8 heads of 64) and at 128 bf16 channels (EXACT, 2 x 4097
-// tokens, 16 heads: 523 us, 1050 TFLOP/s); at 64 bf16 channels by the softmax's vector instructions, of which the matrix instructions hide
-// only a part (8191 tokens, 16 heads: 366 us, 750 TFLOP/s).
+// Bound by the matrix pipes in fp32 (80 % busy: 118 TFLOP/s at 4 x 2048 tokens, 8 heads of 64) and, with four products for the formula's two,
+// in bf16 (2 x 4097 tokens, 16 heads of 128: 523 us, 1050 TFLOP/s; 8191 tokens, 16 heads of 64: 616 us, 890 TFLOP/s).
 // (Two waves per SIMD in fp32 end at 64 channels: at 96 their registers spill, 4 x 2048 tokens, 8 heads 490 against 455 us.)
-template <typename T, int DP, int BIAS, bool EXACT>
+template <typename T, int DP, int BIAS>
 __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 64 ? 2 : 1))) void mha_fwd_k(const FwdP P) {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::frag frag;
@@ -261,11 +263,11 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
     softmax_step(s, o, m, l, P.c);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      frag p[EXACT ? 3 : 1][NCS];
-      prob_frags<T, NCS, EXACT>(s[u], p);
+      frag p[kPieces<T>][NCS];
+      prob_frags<T, NCS>(s[u], p);
       const auto use = [&](int k, const frag& a) {
 #pragma unroll
-        for (int i = 0; i < (EXACT ? 3 : 1); ++i) o[k % NT] = mma(a, p[i][k / NT], o[k % NT]);
+        for (int i = 0; i < kPieces<T>; ++i) o[k % NT] = mma(a, p[i][k / NT], o[k % NT]);
       };
       if (u == 0) {
         const int cb = opaque(fc);
@@ -302,7 +304,7 @@ struct Few {
   static constexpr int kDepth = kPiece >= 8192 ? 1 : 8192 / kPiece;
   static constexpr int slot(int bias) { return 2 * kPiece + (bias == 1 ? kFewBias * 128 : 0); }
 };
-template <typename T, int DP, int BIAS, bool EXACT>
+template <typename T, int DP, int BIAS>
 __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha_few_k(const FwdP P) {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::frag frag;
@@ -443,8 +445,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
       for (int r = 0; r < 16; ++r) s[0][r] = (seen >> r) & 1 ? s[0][r] : -INFINITY;
     }
     softmax_step(s, o, m, l, P.c);
-    frag p[EXACT ? 3 : 1][NCS];
-    prob_frags<T, NCS, EXACT>(s[0], p);
+    frag p[kPieces<T>][NCS];
+    prob_frags<T, NCS>(s[0], p);
     if (more) arrived<DEPTH * NK + (DEPTH - 1) * NV>();
     else arrived<0>();
     {
@@ -458,7 +460,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void mha
     }
     last_phase(f, [&](int k, const frag& a) {
 #pragma unroll
-      for (int i = 0; i < (EXACT ? 3 : 1); ++i) o[k % NT] = mma(a, p[i][k / NT], o[k % NT]);
+      for (int i = 0; i < kPieces<T>; ++i) o[k % NT] = mma(a, p[i][k / NT], o[k % NT]);
     });
     slot = slot + 1 < DEPTH ? slot + 1 : 0;
   }
@@ -656,7 +658,7 @@ int start(K k, const FwdP& p, size_t lds, long long blocks, hipStream_t st) {
   hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(256), lds, st, p);
   return SO_LAUNCH_CHECK();
 }
-template <typename T, int DP, bool EXACT>
+template <typename T, int DP>
 int launch(FwdP p, bool few, hipStream_t st) {
   constexpr size_t row = Tile<T, DP>::kRowBytes;
   const long long groups = (long long)p.d.B * p.d.Hk;
@@ -664,11 +666,11 @@ int launch(FwdP p, bool few, hipStream_t st) {
     constexpr size_t merge = (256 + 32 * (DP + 1)) * 4;
     typedef Few<T, DP> F;
     const auto lds = [&](int bias) { const size_t n = 4 * F::kDepth * F::slot(bias); return n > merge ? n : merge; };
-    if (!p.d.bias) return start(mha_few_k<T, DP, 0, EXACT>, p, lds(0), groups * p.parts, st);
+    if (!p.d.bias) return start(mha_few_k<T, DP, 0>, p, lds(0), groups * p.parts, st);
     // the expanded bias is addressed with 31 bits
     if (p.d.linear && p.d.Hq / p.d.Hk * p.d.Lq <= kFewBias && 4LL * p.d.Hq * p.d.V < 0x7fffffffLL)
-      return start(mha_few_k<T, DP, 1, EXACT>, p, lds(1), groups * p.parts, st);
-    return start(mha_few_k<T, DP, 2, EXACT>, p, lds(2), groups * p.parts, st);
+      return start(mha_few_k<T, DP, 1>, p, lds(1), groups * p.parts, st);
+    return start(mha_few_k<T, DP, 2>, p, lds(2), groups * p.parts, st);
   }
   const int w = p.d.linear ? 1 : p.d.width;
   p.seg = p.d.bias ? (code_span(128, w) + code_span(64, w) + 1 + 63) / 64 * 64 : 0;
@@ -677,22 +679,15 @@ int launch(FwdP p, bool few, hipStream_t st) {
   p.stages = 2 * stage <= kLds ? 2 : 1;
   const long long blocks = groups * (p.d.Hq / p.d.Hk) * p.row_tiles * p.parts;
   const size_t lds = p.stages * stage;
-  if (!p.d.bias) return start(mha_fwd_k<T, DP, 0, EXACT>, p, lds, blocks, st);
-  return p.d.linear ? start(mha_fwd_k<T, DP, 1, EXACT>, p, lds, blocks, st) : start(mha_fwd_k<T, DP, 2, EXACT>, p, lds, blocks, st);
-}
-template <typename T, int DP>
-int launch_exact(const FwdP& p, bool few, hipStream_t st) {
-  if constexpr (sizeof(T) == 2) {
-    if (p.d.exact) return launch<T, DP, true>(p, few, st);
-  }
-  return launch<T, DP, false>(p, few, st);
+  if (!p.d.bias) return start(mha_fwd_k<T, DP, 0>, p, lds, blocks, st);
+  return p.d.linear ? start(mha_fwd_k<T, DP, 1>, p, lds, blocks, st) : start(mha_fwd_k<T, DP, 2>, p, lds, blocks, st);
 }
 template <typename T>
 int launch_d(const FwdP& p, bool few, hipStream_t st) {
-  if (p.d.D <= 32) return launch_exact<T, 32>(p, few, st);
-  if (p.d.D <= 64) return launch_exact<T, 64>(p, few, st);
-  if (p.d.D <= 96) return launch_exact<T, 96>(p, few, st);
-  return launch_exact<T, 128>(p, few, st);
+  if (p.d.D <= 32) return launch<T, 32>(p, few, st);
+  if (p.d.D <= 64) return launch<T, 64>(p, few, st);
+  if (p.d.D <= 96) return launch<T, 96>(p, few, st);
+  return launch<T, 128>(p, few, st);
 }
 
 // few rows: everything that shares a key head fits one 32-row tile
@@ -774,9 +769,9 @@ int so_mha_parts(const void* desc) {
     if (parts > tiles / 2) parts = tiles / 2;
     return parts < 2 ? 1 : (int)(parts > 256 ? 256 : parts);
   }
-  // a map's bias is looked up value by value, whole probabilities are three products for one: 2 x 2304 tokens of a 64 x 36 map, 8 heads of 64,
+  // a map's bias is looked up value by value, bf16 probabilities are three products for one: 2 x 2304 tokens of a 64 x 36 map, 8 heads of 64,
   // 288 blocks, training: 116 us whole, 83 + 10 in two parts, 69 + 12 in seven (the join reads from caches)
-  const double rate = (d->exact ? 0.75 : 1.0) * (d->bias && !d->linear ? 0.6 : 1.0), rows = (double)d->B * d->Hq * d->Lq;
+  const double rate = (d->dtype == SO_BF16 ? 0.75 : 1.0) * (d->bias && !d->linear ? 0.6 : 1.0), rows = (double)d->B * d->Hq * d->Lq;
   return mha_split_parts((double)d->B * d->Hq * mha_tiles(d->Lq), mha_us(4.0 * 128 * d->D * d->Lk, d->dtype) / rate, 8.0,
                          rows * d->D * 8 / 12e6, d->Lk / 128, 0.95);
 }

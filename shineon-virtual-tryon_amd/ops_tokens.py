@@ -7,7 +7,8 @@
 
 Same contract as ops.py: torch supplies device memory, the current stream and the autograd tape; the arithmetic is in
 libshineon_hip.so, there is no CPU fallback, everything may be captured into a hipGraph.  Two differences: operands may be float32 or
-bfloat16 (arithmetic and statistics are fp32 either way), and every call runs on the device of its operands, on that device's current
+bfloat16 (sums and statistics are fp32 either way; with bfloat16 the backward pass of attention rounds probabilities and score gradients
+to that type before it multiplies them with operands), and every call runs on the device of its operands, on that device's current
 stream, whatever the current device is.  Gradients are first order: differentiating them again is refused."""
 import ctypes
 
@@ -308,7 +309,7 @@ class _Desc(ctypes.Structure):
                                                 "dq", "dk", "dv", "delta", "strips")]
                 + [(n, ctypes.c_longlong) for n in ("sqb", "sql", "sqh", "skb", "skl", "skh", "svb", "svl", "svh")]
                 + [(n, ctypes.c_int) for n in ("dtype", "B", "Hq", "Hk", "Lq", "Lk", "D", "V", "code_max", "tokens", "q_start", "linear",
-                                               "nwords", "exact", "width")]
+                                               "nwords", "width")]
                 + [("scale", ctypes.c_float)])
 
 
@@ -428,7 +429,6 @@ class _AttentionFn(torch.autograd.Function):
             if dt == 1:
                 o_f32 = torch.empty(o.shape, dtype=torch.float32, device=dev)
                 x.o_f32 = o_f32.data_ptr()
-                x.exact = int(table is not None and ctx.needs_input_grad[3])
         at = ctypes.addressof(x)
         parts = L.so_mha_parts(at)
         if parts < 0:
@@ -515,7 +515,12 @@ def attention(q, k, v, scale=None, key_mask=None, relative=None, bias_table=None
     Training with a table takes scratch for the bias gradient, about Lq Lk / 32 bytes per sample and head, while backward runs.
 
     One or a few queries over long keys (a new token against what came before) are split over the keys.  Returns [B, Lq, Hq, D];
-    differentiable in q, k, v and bias_table.  The order of all sums is fixed: the same inputs give the same bits."""
+    differentiable in q, k, v and bias_table.  The order of all sums is fixed: the same inputs give the same bits, whatever wants a
+    gradient.
+
+    bfloat16: probabilities enter the product with v with all their bits, so the result is rounded once.  In the backward pass
+    probabilities (for dv) and score gradients (for dq, dk) are rounded to bfloat16, half a step (2^-8 of a value) each, which adds about
+    as much error to dq, dk and dv as their own rounding; the gradient of bias_table sums unrounded ones."""
     dt = _dtype(q, k, v)
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
         raise ValueError(f"q [B, Lq, Hq, D], k and v [B, Lk, Hk, D] expected, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")

@@ -408,6 +408,41 @@ def test_attention_any_head_size(tok, dtype, d):
 
 
 @TYPES
+@pytest.mark.parametrize("lq,lk", [(90, 90), (300, 300), (1, 900)])
+def test_attention_output_is_the_same_in_every_mode(tok, dtype, lq, lk):
+    """Inference, training with a frozen table and training of everything give the same bits, and the operands' gradients do not depend on
+    whether the table wants one."""
+    q, k, v = normal(1, 1, lq, 2, 64, dtype=dtype), normal(2, 1, lk, 2, 64, dtype=dtype), normal(3, 1, lk, 2, 64, dtype=dtype)
+    rel, table, do = tok.RelativePositions(lk, 8, 20), normal(4, 8, 2), normal(5, 1, lq, 2, 64, dtype=dtype)
+    with torch.no_grad():
+        o = tok.attention(q, k, v, relative=rel, bias_table=table, q_start=lk - lq)
+    grads = []
+    for learned in (False, True):
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        tt = table.clone().requires_grad_(learned)
+        y = tok.attention(*leaves, relative=rel, bias_table=tt, q_start=lk - lq)
+        assert torch.equal(y, o)
+        grads.append(torch.autograd.grad(y, leaves + ([tt] if learned else []), do))
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("hq,hk,d", [(2, 2, 64), (4, 1, 128), (2, 1, 32)])
+@pytest.mark.parametrize("lq,lk", [(300, 300), (1, 4099), (70, 33)])
+def test_attention_bf16_inference_rounds_only_its_output(tok, hq, hk, d, lq, lk):
+    """Probabilities enter the product with v to 2^-16: beside fp32 arithmetic, the rounding of o is the only one."""
+    q, k, v = normal(1, 1, lq, hq, d, dtype=BF16), normal(2, 1, lk, hk, d, dtype=BF16), normal(3, 1, lk, hk, d, dtype=BF16)
+    for table in (None, normal(4, 8, hq)):
+        n = max(lq, lk)
+        rel = None if table is None else tok.RelativePositions(n, 8, 20)
+        bias = None if table is None else d64(table).T[:, ref.pair_buckets(n, lq, lk, n - lq, 8, 20)]
+        o = tok.attention(q, k, v, relative=rel, bias_table=table, q_start=0 if table is None else n - lq)
+        value, bound = ref.attention(d64(q), d64(k), d64(v), d ** -0.5, None, bias, dtype=BF16, exact=True)["o"]
+        sizes = ref.attention(d64(q), d64(k), d64(v).abs(), d ** -0.5, None, bias, dtype=BF16)["o"][0]
+        ref.check(o, value, bound + 2.0 ** -16 * (1 + 2.0 ** -8) * sizes, "o")
+
+
+@TYPES
 def test_attention_strides(tok, dtype):
     """Slices of one projection, head-major tensors, unaligned views, broadcast keys: the same values as dense operands."""
     b, n, h, d = 2, 77, 2, 64
