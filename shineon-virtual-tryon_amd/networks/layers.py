@@ -7,6 +7,7 @@ arithmetic runs in libshineon_hip.so.  Class names keep the substrings `Conv`, `
 (models/networks/__init__.py:52-60).
 """
 import math
+import os
 
 import torch
 from torch import nn
@@ -165,6 +166,13 @@ class FusedReLU(nn.Module):
         return x
 
 
+def _rank():
+    """The data-parallel rank, also before this process has joined its group (train.py builds the model first): the launcher's RANK."""
+    if torch.distributed.is_available() and torch.distributed.is_initialized():
+        return torch.distributed.get_rank()
+    return int(os.environ.get("RANK", "0"))
+
+
 class HipDropout(nn.Module):
     """nn.Dropout(p), with the residual it is added to as an option.  The mask comes from a counter-based generator and is never stored;
     the generator's state lives on the device and moves on with every draw, also in the replays of a captured graph.  The numbers follow
@@ -176,8 +184,7 @@ class HipDropout(nn.Module):
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"dropout probability outside [0, 1]: {p}")
         self.p, self.stream = p, stream
-        rank = torch.distributed.get_rank() if torch.distributed.is_available() and torch.distributed.is_initialized() else 0
-        seed = torch.initial_seed() + 0x9E3779B97F4A7C15 * (65536 * stream + rank + 1)
+        seed = torch.initial_seed() + 0x9E3779B97F4A7C15 * (65536 * stream + _rank() + 1)
         self.register_buffer("rng_state", ops_tokens.rng_state(seed, "cpu"), persistent=False)
 
     def active(self):

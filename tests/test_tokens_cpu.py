@@ -176,3 +176,18 @@ def test_unet_with_relative_attention_and_dropout():
         build(use_self_attn=True, attn_type="none")
     with pytest.raises(ValueError):
         HipDropout(1.5)
+
+
+def test_dropout_ranks_draw_different_masks(monkeypatch):
+    """train.py builds the model before it joins the process group: the launcher's RANK stands for the rank then."""
+    from shineon_virtual_tryon_amd.networks.layers import HipDropout
+
+    states = []
+    for rank in (None, "0", "1", "7"):
+        monkeypatch.delenv("RANK", raising=False)
+        if rank:
+            monkeypatch.setenv("RANK", rank)
+        torch.manual_seed(3)
+        states.append([HipDropout(0.5, stream).rng_state.tolist() for stream in (0, 1)])
+    assert states[0] == states[1]
+    assert len({tuple(s) for pair in states[1:] for s in pair}) == 6
