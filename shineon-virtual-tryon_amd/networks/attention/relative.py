@@ -21,7 +21,7 @@ class RelativeAttention(nn.Module):
     per head); distances from max_distance on share the last bucket.  dropout, stream:
     see HipDropout."""
 
-    def __init__(self, in_dim, activation=None, num_buckets=16, max_distance=32, dropout=0.0, stream=0):
+    def __init__(self, in_dim, activation=None, num_buckets=16, max_distance=32, dropout=0.0, stream=None):
         super().__init__()
         self.head_dim = _head_size(in_dim)
         self.heads = in_dim // self.head_dim

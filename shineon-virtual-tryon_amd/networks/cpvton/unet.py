@@ -64,7 +64,7 @@ class UnetSkipConnectionBlock(nn.Module):
          |-- downsampling -- |submodule| -- upsampling --|"""
 
     def __init__(self, outer_nc, inner_nc, input_nc=None, submodule=None, outermost=False, innermost=False,
-                 norm_layer=HipBatchNorm2d, self_attn=False, use_dropout=False, activation=None, dropout_stream=0):
+                 norm_layer=HipBatchNorm2d, self_attn=False, use_dropout=False, activation=None, dropout_stream=None):
         super().__init__()
         norm_layer = _resolve_norm(norm_layer)
         self.outermost = outermost

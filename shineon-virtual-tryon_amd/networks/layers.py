@@ -176,13 +176,15 @@ def _rank():
 class HipDropout(nn.Module):
     """nn.Dropout(p), with the residual it is added to as an option.  The mask comes from a counter-based generator and is never stored;
     the generator's state lives on the device and moves on with every draw, also in the replays of a captured graph.  The numbers follow
-    from torch's seed, the data-parallel rank and `stream`: modules of one network are given different streams.  The state is not part of
-    the state_dict."""
+    from torch's seed, the data-parallel rank and `stream`, a small number by which the modules of one network differ; without one, a module
+    that drops anything takes one from torch's generator.  The state is not part of the state_dict."""
 
-    def __init__(self, p=0.5, stream=0):
+    def __init__(self, p=0.5, stream=None):
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"dropout probability outside [0, 1]: {p}")
+        if stream is None:      # above all numbers that are given by hand
+            stream = int(torch.randint(1 << 32, 1 << 46, ())) if p > 0.0 else 0
         self.p, self.stream = p, stream
         seed = torch.initial_seed() + 0x9E3779B97F4A7C15 * (65536 * stream + _rank() + 1)
         self.register_buffer("rng_state", ops_tokens.rng_state(seed, "cpu"), persistent=False)

@@ -191,3 +191,24 @@ def test_dropout_ranks_draw_different_masks(monkeypatch):
         states.append([HipDropout(0.5, stream).rng_state.tolist() for stream in (0, 1)])
     assert states[0] == states[1]
     assert len({tuple(s) for pair in states[1:] for s in pair}) == 6
+
+
+def test_dropout_modules_without_a_stream_draw_different_masks():
+    """A module that is not given a stream takes one from torch's generator: others do not share its masks, the seed brings them back, and
+    a module that drops nothing takes nothing."""
+    from shineon_virtual_tryon_amd.networks.attention.relative import RelativeAttention
+    from shineon_virtual_tryon_amd.networks.layers import HipDropout
+
+    def build():
+        torch.manual_seed(3)
+        return [m.rng_state.tolist() for m in (HipDropout(0.5), HipDropout(0.5), RelativeAttention(32, dropout=0.1).dropout,
+                                               RelativeAttention(32, dropout=0.1).dropout, HipDropout(0.5, 0), HipDropout(0.5, 1))]
+
+    states = build()
+    assert len({tuple(s) for s in states}) == 6 and build() == states
+    torch.manual_seed(3)
+    want = torch.rand(3)
+    torch.manual_seed(3)
+    HipDropout(0.0)
+    HipDropout(0.5, 4)
+    assert torch.equal(torch.rand(3), want)
