@@ -177,7 +177,10 @@ class HipDropout(nn.Module):
     """nn.Dropout(p), with the residual it is added to as an option.  The mask comes from a counter-based generator and is never stored;
     the generator's state lives on the device and moves on with every draw, also in the replays of a captured graph.  The numbers follow
     from torch's seed, the data-parallel rank and `stream`, a small number by which the modules of one network differ; without one, a module
-    that drops anything takes one from torch's generator.  The state is not part of the state_dict."""
+    that drops anything takes one from torch's generator.  The state is not part of the state_dict; the trainer's checkpoints hold it beside
+    that (generator_state), so that a resumed run goes on with the masks."""
+
+    _STEP = 0x9E3779B97F4A7C15      # between the seeds of ranks; 65536 times it between streams
 
     def __init__(self, p=0.5, stream=None):
         super().__init__()
@@ -185,9 +188,18 @@ class HipDropout(nn.Module):
             raise ValueError(f"dropout probability outside [0, 1]: {p}")
         if stream is None:      # above all numbers that are given by hand
             stream = int(torch.randint(1 << 32, 1 << 46, ())) if p > 0.0 else 0
-        self.p, self.stream = p, stream
-        seed = torch.initial_seed() + 0x9E3779B97F4A7C15 * (65536 * stream + _rank() + 1)
+        self.p, self.stream, self.rank = p, stream, _rank()
+        seed = torch.initial_seed() + self._STEP * (65536 * stream + self.rank + 1)
         self.register_buffer("rng_state", ops_tokens.rng_state(seed, "cpu"), persistent=False)
+
+    def generator_state(self):
+        """[seed, offset] as rank 0 has them."""
+        seed, offset = self.rng_state.tolist()
+        return ops_tokens.rng_state(seed - self._STEP * self.rank, "cpu", offset).tolist()
+
+    def set_generator_state(self, state):
+        """Goes on from a generator_state(), with this rank's seed."""
+        self.rng_state.copy_(ops_tokens.rng_state(state[0] + self._STEP * self.rank, "cpu", state[1]))
 
     def active(self):
         return self.training and self.p > 0.0

@@ -24,6 +24,7 @@ import torch
 import torch.distributed as dist
 
 from . import ops
+from .networks.layers import HipDropout
 from .options import str2num
 
 logger = logging.getLogger("logger")
@@ -1054,10 +1055,11 @@ class Trainer:
             "lr_schedulers": [sc.state_dict() for sc in self.schedulers],
             "global_step": self.global_step, "epoch": self.current_epoch + (1 if epoch_finished else 0),
             "vgg_pretrained": _vgg_flag(self.model),
+            "dropout_states": {name: m.generator_state() for name, m in _dropouts(self.model)},
         }, path)
 
     def _maybe_resume(self):
-        """Weights, optimizer moments, LR schedule position and counters all come back (train.py:39-54: the reference hands
+        """Weights, optimizer moments, LR schedule position, dropout generators and counters all come back (train.py:39-54: the reference hands
         the same file to load_from_checkpoint and to resume_from_checkpoint)."""
         if not self.resume:
             return
@@ -1068,6 +1070,10 @@ class Trainer:
             # the VGG weights now are the checkpoint's: pretrained unless the checkpoint says it was trained on random ones
             # (reference checkpoints carry no flag and always hold ImageNet weights, models/networks/vgg.py:9)
             vgg.pretrained_loaded = bool(ckpt.get("vgg_pretrained", True))
+        dropped = ckpt.get("dropout_states") or {}
+        for name, m in _dropouts(self.model):
+            if name in dropped:
+                m.set_generator_state(dropped[name])
         self.global_step = int(ckpt.get("global_step", 0))
         self.current_epoch = int(ckpt.get("epoch", 0))
         states, scheds = ckpt.get("optimizer_states") or [], ckpt.get("lr_schedulers") or []
@@ -1242,6 +1248,10 @@ def _vgg_criterion(model):
     """The perceptual-loss module: `criterionVGG` in UnetMaskModel, `criterion_VGG` in SamsModel (the reference's names)."""
     crit = getattr(model, "criterionVGG", None)
     return crit if crit is not None else getattr(model, "criterion_VGG", None)
+
+
+def _dropouts(model):
+    return [(name, m) for name, m in model.named_modules() if isinstance(m, HipDropout)]
 
 
 def _vgg_flag(model):

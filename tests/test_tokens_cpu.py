@@ -212,3 +212,27 @@ def test_dropout_modules_without_a_stream_draw_different_masks():
     HipDropout(0.0)
     HipDropout(0.5, 4)
     assert torch.equal(torch.rand(3), want)
+
+
+def test_dropout_state_travels_between_ranks(monkeypatch):
+    """A checkpoint holds rank 0's state; every rank goes on from it with its own masks."""
+    from shineon_virtual_tryon_amd.networks.layers import HipDropout
+
+    torch.manual_seed(3)
+    mods = []
+    for rank in ("0", "5"):
+        monkeypatch.setenv("RANK", rank)
+        mods.append(HipDropout(0.5, 2))
+    assert mods[0].generator_state() == mods[0].rng_state.tolist() and mods[1].generator_state() == mods[0].generator_state()
+    mods[0].rng_state[1] = 1234
+    state, storage = mods[0].generator_state(), mods[1].rng_state.data_ptr()
+    torch.manual_seed(99)
+    fresh = [mods[1]]
+    for rank in ("0", "5"):
+        monkeypatch.setenv("RANK", rank)
+        fresh.append(HipDropout(0.5, 3))
+        fresh[-1].set_generator_state(state)
+    seed = mods[1].rng_state[0].item()
+    mods[1].set_generator_state(state)
+    assert mods[1].rng_state.tolist() == [seed, 1234] == fresh[2].rng_state.tolist() and mods[1].rng_state.data_ptr() == storage
+    assert fresh[1].rng_state.tolist() == state

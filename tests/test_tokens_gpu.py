@@ -810,3 +810,33 @@ def test_unet_trains_with_relative_attention_and_dropout(tok):
     for name, p in model.unet.named_parameters():
         if any(n in name for n in ("bias_table", "query_norm", "key_norm", "qkv_conv.weight", "out_conv.weight")):
             assert p.grad.isfinite().all() and p.grad.abs().sum() > 0, name
+
+
+def test_resumed_training_goes_on_with_the_masks(tok, tmp_path):
+    """A run that is stopped behind its first epoch and resumed ends with the generator's states and the weights of one that is not."""
+    from shineon_virtual_tryon_amd.networks.layers import HipDropout
+    from shineon_virtual_tryon_amd.options import TrainOptions
+    from shineon_virtual_tryon_amd.trainer import Trainer
+    from shineon_virtual_tryon_amd.unet_mask_model import UnetMaskModel
+
+    def fit(name, epochs, resume=None):
+        root = str(tmp_path / name)
+        opt = TrainOptions().parse(["--model", "tom", "--dataset", "synthetic", "--name", "t", "-b", "1", "--workers", "0", "--synthetic_length", "4",
+                                    "--experiments_dir", root, "--lr", "1e-3", "--use_dropout", "--allow_random_vgg", "--ngf", "8"],
+                                   interactive=False)
+        torch.manual_seed(9)
+        model = UnetMaskModel(opt)
+        Trainer(default_root_dir=root, max_epochs=epochs, limit_train_batches=2, limit_val_batches=1, resume_from_checkpoint=resume).fit(model)
+        ckpt = root + "/checkpoints/final.ckpt"
+        return model, ckpt, torch.load(ckpt, map_location="cpu", weights_only=False)
+
+    model, _, whole = fit("whole", 2)
+    drops = {n: m for n, m in model.named_modules() if isinstance(m, HipDropout)}
+    assert drops and whole["dropout_states"] == {n: m.rng_state.tolist() for n, m in drops.items()}
+    assert all(m.rng_state[1] > 0 for m in drops.values()) and not any("rng_state" in k for k in whole["state_dict"])
+    _, first, half = fit("half", 1)
+    assert half["dropout_states"] != whole["dropout_states"]
+    _, _, resumed = fit("resumed", 2, first)
+    assert resumed["dropout_states"] == whole["dropout_states"] and resumed["global_step"] == whole["global_step"] == 4
+    for k, v in whole["state_dict"].items():
+        assert torch.equal(v, resumed["state_dict"][k]), k
