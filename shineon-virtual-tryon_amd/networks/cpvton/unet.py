@@ -93,7 +93,7 @@ class UnetSkipConnectionBlock(nn.Module):
         if not outermost and not innermost:
             downconv.zero_bias_grad = norm_kind                # downconv -> downnorm
         if self_attn:
-            attention = ATTENTION_TYPES["sagan" if self_attn is True else self_attn]
+            attention = ATTENTION_TYPES[self_attn if isinstance(self_attn, str) else "sagan"]
             down.append(attention(inner_nc, "relu"))
             up.append(attention(outer_nc, "relu"))
         if use_dropout:

@@ -236,3 +236,13 @@ def test_dropout_state_travels_between_ranks(monkeypatch):
     mods[1].set_generator_state(state)
     assert mods[1].rng_state.tolist() == [seed, 1234] == fresh[2].rng_state.tolist() and mods[1].rng_state.data_ptr() == storage
     assert fresh[1].rng_state.tolist() == state
+
+
+@pytest.mark.parametrize("value,name", [(True, "sagan"), (1, "sagan"), ("sagan", "sagan"), ("relative", "relative"), (0, None), (None, None), (False, None)])
+def test_unet_block_takes_any_truth_value_for_attention(value, name):
+    from shineon_virtual_tryon_amd.networks.attention import ATTENTION_TYPES
+    from shineon_virtual_tryon_amd.networks.cpvton.unet import UnetSkipConnectionBlock
+
+    block = UnetSkipConnectionBlock(8, 8, innermost=True, self_attn=value)
+    found = [type(m) for m in block.model if type(m) in ATTENTION_TYPES.values()]
+    assert found == ([ATTENTION_TYPES[name]] * 2 if name else [])
