@@ -261,11 +261,11 @@ class _QkNormRotaryFn(torch.autograd.Function):
             return dq, dk, torch.zeros_like(wq), torch.zeros_like(wk), None, None, None, None, None, None
         d, L = x.D, lib()
         n = L.so_qk_norm_rotary_ws_floats(d)
-        buf = torch.empty((2 + n // d, d), dtype=torch.float32, device=q.device)      # dwq | dwk | scratch
-        at = buf.data_ptr()
+        dw, ws = (torch.empty(m, dtype=torch.float32, device=q.device) for m in ((2, d), n))      # dwq and dwk; scratch
+        at = dw.data_ptr()
         _launch(q.device, L.so_qk_norm_rotary_bwd, "qk_norm_rotary_bwd", ctypes.addressof(x), dyq.data_ptr(), dyk.data_ptr(),
-                dq.data_ptr(), dk.data_ptr(), at, at + 4 * d, at + 8 * d, n)
-        return dq, dk, buf[0], buf[1], None, None, None, None, None, None
+                dq.data_ptr(), dk.data_ptr(), at, at + 4 * d, ws.data_ptr(), n)
+        return dq, dk, dw[0], dw[1], None, None, None, None, None, None
 
 
 def qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions=None, start=0, eps=1e-6):

@@ -196,6 +196,15 @@ def _differences(f, args, grads, step=2.0 ** -6):
         assert abs(slope - g.norm().item()) <= 5e-3 * g.norm().item() + 1e-3, (i, slope, g.norm().item())
 
 
+def test_qk_norm_rotary_gradients_hold_no_scratch(tok):
+    """What stays alive with the weights' gradients is their own size, not the partial sums of the pass."""
+    q, k = normal(1, 2, 300, 4, 128).requires_grad_(), normal(2, 2, 300, 2, 128)
+    wq, wk = (torch.ones(128, device="cuda", requires_grad=True) for _ in range(2))
+    y = tok.qk_norm_rotary(q, k, wq, wk, *tok.rotary_table(300, 128))
+    for g in torch.autograd.grad(y, [q, wq, wk], [torch.ones_like(t) for t in y])[1:]:
+        assert g.untyped_storage().nbytes() <= 2 * 128 * 4
+
+
 @TYPES
 def test_qk_norm_rotary_outside_the_table_is_nan(tok, dtype):
     q, k = normal(1, 2, 3, 2, 16, dtype=dtype), normal(2, 2, 3, 1, 16, dtype=dtype)
