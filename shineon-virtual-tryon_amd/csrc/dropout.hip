@@ -122,6 +122,7 @@ int so_dropout(int dtype, const void* x, long long ldx, const void* residual, lo
   if (threshold < 0 || threshold > (1LL << 32)) return SO_ERR_SHAPE;
   if (C && rows > (1LL << 40) / C) return SO_ERR_SHAPE;      // the grid's 2^31 blocks of 2048 elements
   if (rows == 0 || C == 0) return 0;
+  if (!x || !y || !rng) return SO_ERR_SHAPE;
   DropP p = {};
   p.x = x; p.res = residual; p.y = y; p.rng = (const long long*)rng;
   p.n = rows * C; p.C = C; p.ldx = ldx; p.ldr = ldr; p.ldy = ldy;

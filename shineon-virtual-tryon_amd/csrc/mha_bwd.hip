@@ -754,6 +754,7 @@ int launch_d(const BwdP& p, hipStream_t st) {
 extern "C" {
 
 long long so_mha_strip_floats(const void* desc) {
+  if (!desc) return SO_ERR_SHAPE;
   so_mha_desc d = *(const so_mha_desc*)desc;
   float one;
   d.strips = &one;       // only asked whether it is wanted
@@ -763,6 +764,7 @@ long long so_mha_strip_floats(const void* desc) {
 }
 
 long long so_mha_bwd_floats(const void* desc) {
+  if (!desc) return SO_ERR_SHAPE;
   const so_mha_desc& d = *(const so_mha_desc*)desc;
   BwdP p;
   const int err = make(&d, p);

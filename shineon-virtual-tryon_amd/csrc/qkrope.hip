@@ -221,6 +221,7 @@ int side_blocks(long long rows, int per, int most) {
 int run(QkP& p, int dtype, bool bwd, float* dwq, float* dwk, float* ws, long long ws_floats, hipStream_t st) {
   if (p.B < 1 || p.L < 1 || p.s[0].H < 1 || p.s[1].H < 1 || p.D < 2 || (p.D & 1) || p.D > 128 || p.R < 0 || (p.R & 1) || p.R > p.D)
     return SO_ERR_SHAPE;
+  if (!p.s[0].x || !p.s[1].x || !p.s[0].w || !p.s[1].w || (p.R && (!p.cosv || !p.sinv))) return SO_ERR_SHAPE;      // (an empty table has no address)
   if ((dtype != SO_F32 && dtype != SO_BF16) || (!p.pos && (p.start < 0 || p.start + p.L > p.P))) return SO_ERR_SHAPE;
   const int esize = dtype == SO_F32 ? 4 : 2;
   int V = 16 / esize;
@@ -268,6 +269,7 @@ extern "C" {
 int so_qk_desc_bytes(void) { return (int)sizeof(so_qk_desc); }
 
 int so_qk_norm_rotary_fwd(const void* desc, void* yq, void* yk, void* stream) {
+  if (!desc || !yq || !yk) return SO_ERR_SHAPE;
   const so_qk_desc& d = *(const so_qk_desc*)desc;
   QkP p = make(d);
   p.s[0].y = yq;
@@ -279,6 +281,7 @@ long long so_qk_norm_rotary_ws_floats(int D) { return 2LL * kBlocksBwd * D; }
 
 int so_qk_norm_rotary_bwd(const void* desc, const void* dyq, const void* dyk, void* dq, void* dk, float* dwq, float* dwk, float* ws,
                           long long ws_floats, void* stream) {
+  if (!desc || !dyq || !dyk || !dq || !dk || !dwq || !dwk || !ws) return SO_ERR_SHAPE;
   const so_qk_desc& d = *(const so_qk_desc*)desc;
   QkP p = make(d);
   p.s[0].y = dq; p.s[0].dy = dyq;

@@ -246,3 +246,27 @@ def test_unet_block_takes_any_truth_value_for_attention(value, name):
     block = UnetSkipConnectionBlock(8, 8, innermost=True, self_attn=value)
     found = [type(m) for m in block.model if type(m) in ATTENTION_TYPES.values()]
     assert found == ([ATTENTION_TYPES[name]] * 2 if name else [])
+
+
+def test_c_entry_points_refuse_null_pointers():
+    """A missing descriptor or operand comes back as an error code; nothing is read and nothing is launched."""
+    L, shape = _lib.lib(), -2
+    for fn in (L.so_mha_parts, L.so_mha_strip_floats, L.so_mha_bwd_floats):
+        assert fn(None) == shape
+    assert L.so_mha_fwd(None, None) == L.so_mha_bwd(None, None) == shape
+    assert L.so_mha_dtable(None, 256, 256, 1, 256, 256, None) == shape
+    assert L.so_qk_norm_rotary_fwd(None, 256, 256, None) == shape
+    assert L.so_qk_norm_rotary_bwd(None, 256, 256, 256, 256, 256, 256, 256, 1 << 20, None) == shape
+    base = dict(q=256, k=256, wq=256, wk=256, cosv=256, sinv=256, sqb=320, sql=64, sqh=64, skb=320, skl=64, skh=64, P=8, dtype=0, Hq=1, Hk=1, B=1,
+                L=5, D=64, R=64, eps=1e-6)
+    for name in ("q", "k", "wq", "wk", "cosv", "sinv"):
+        x = tok._QkDesc(**{**base, name: None})
+        assert L.so_qk_norm_rotary_fwd(ctypes.addressof(x), 256, 256, None) == shape, name
+    x = tok._QkDesc(**base)
+    assert L.so_qk_norm_rotary_fwd(ctypes.addressof(x), None, 256, None) == L.so_qk_norm_rotary_fwd(ctypes.addressof(x), 256, None, None) == shape
+    full = [256] * 7
+    for i in range(7):
+        a = [None if j == i else v for j, v in enumerate(full)]
+        assert L.so_qk_norm_rotary_bwd(ctypes.addressof(x), *a, 1 << 20, None) == shape, i
+    for a in ((None, 256, 256), (256, None, 256), (256, 256, None)):
+        assert L.so_dropout(0, a[0], 4, None, 0, a[1], 4, 1, 4, a[2], 0, 1.0, None) == shape
