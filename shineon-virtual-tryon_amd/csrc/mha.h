@@ -348,8 +348,9 @@ int so_mha_check(const so_mha_desc* d);   // shape, type and alignment rules tha
 // 128-row tiles in n rows; the last pays for its 32-row waves only
 double mha_tiles(int n);
 // Parts that the sum axis of a kernel is cut into (at most 8, at most `most`): blocks on one CU share its pipes, so a pass takes as long as
-// the CU with most blocks, ceil(blocks parts / 256) / parts of a whole block's `block_us`; joining costs join_us and part_us per part.  More
+// the CU with most blocks, ceil(blocks parts / 256) / parts of a whole block's `block_us`; joining costs join_us and, for every part, writing and
+// reading `part_bytes` (both counted) at `rate` bytes per us - at most that of a large copy where the parts together outgrow the caches.  More
 // parts are taken when they bring the estimate below `gain` of the last choice.
-int mha_split_parts(double blocks, double block_us, double join_us, double part_us, int most, double gain);
+int mha_split_parts(double blocks, double block_us, double join_us, double part_bytes, double rate, int most, double gain);
 // block_us from a block's FLOP: what a CU reaches in these kernels
 inline double mha_us(double flop, int dtype) { return flop / (dtype == SO_F32 ? 0.45e6 : 3.0e6); }

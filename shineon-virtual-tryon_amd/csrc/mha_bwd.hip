@@ -665,12 +665,12 @@ int make(const so_mha_desc* d, BwdP& p) {
   const double tiles = d->bias && !d->linear ? p.qtiles : mha_tiles(d->Lq);
   const double rows = (double)d->B * d->Lq * d->Hq * d->D, keys = (double)d->B * d->Lk * d->Hk * d->D;
   // fp32, 2 x 2049 tokens, 8 heads of 64, 272 blocks: mha_dq_k 350 us whole, 221 + 8 us in three parts
-  p.dq_parts = mha_split_parts((double)d->B * d->Hq * tiles, mha_us(6.0 * 128 * d->D * d->Lk, d->dtype), 6.0, rows * 8 / 4e6, d->Lk / 128, 0.95);
+  p.dq_parts = mha_split_parts((double)d->B * d->Hq * tiles, mha_us(6.0 * 128 * d->D * d->Lk, d->dtype), 6.0, rows * 8, 4e6, d->Lk / 128, 0.95);
   // (blocks of keys that a mask hides end at once, which the estimate does not know: the rows are only cut for a clear gain.  A training
   // pass whole / cut: bf16, 2 x 4097 tokens, 16 heads on 4, 128 channels 2125 / 1725 us, with a fifth of the keys hidden 1935 / 1530;
   // 9000 tokens, 8 on 4, 64 channels 1127 / 999; fp32, 2 x 2049, 8 of 64 1066 / 870; 1000 tokens, 8 on 1, 128 channels 371 / 164)
   const double q_tiles = (double)d->Lq * (d->Hq / d->Hk) / 128;
-  p.dkv_parts = mha_split_parts((double)d->B * d->Hk * mha_tiles(d->Lk), mha_us(8.0 * 128 * 128 * d->D * q_tiles, d->dtype), 6.0, keys * 16 / 4e6,
+  p.dkv_parts = mha_split_parts((double)d->B * d->Hk * mha_tiles(d->Lk), mha_us(8.0 * 128 * 128 * d->D * q_tiles, d->dtype), 6.0, keys * 16, 4e6,
                                 q_tiles < 8 ? (int)q_tiles : 8, 0.7);
   p.dkv_at = p.dq_parts > 1 ? (long long)rows * p.dq_parts : 0;
   p.stages = 2;

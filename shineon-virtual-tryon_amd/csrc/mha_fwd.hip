@@ -718,11 +718,14 @@ int so_mha_check(const so_mha_desc* d) {
 
 double mha_tiles(int n) { return n / 128 + (n % 128 + 31) / 32 * 0.25; }
 
-int mha_split_parts(double blocks, double block_us, double join_us, double part_us, int most, double gain) {
+int mha_split_parts(double blocks, double block_us, double join_us, double part_bytes, double rate, int most, double gain) {
+  // 66 MB of partial sums (two 64 x 36 maps, 7 parts) were joined at 16 TB/s, 134 MB (2 x 4097 tokens, 16 heads of 128, 2 parts) at 3.9
+  constexpr double kCached = 100e6, kCopy = 4.9e6;
   int best = 1;
   double least = 0;
   for (int p = 1; p <= 8 && (p == 1 || p <= most); ++p) {
-    const double t = ceil(blocks * p / 256) / p * block_us + (p > 1 ? join_us + part_us * p : 0.0);
+    const double bytes = part_bytes * p, at = bytes / 2 > kCached && rate > kCopy ? kCopy : rate;
+    const double t = ceil(blocks * p / 256) / p * block_us + (p > 1 ? join_us + bytes / at : 0.0);
     if (p == 1 || t < gain * least) {
       best = p;
       least = t;
@@ -756,8 +759,9 @@ int so_mha_prep(const float* table, const void* lut, int V, int H, float scale, 
 // Parts of the key axis.  Few rows (bound by reading keys): enough blocks to give every CU two, at least two tiles to a part.  Many rows:
 // blocks that share a CU share its matrix pipes, so the pass takes as long as the CU with most blocks - ceil(blocks parts / 256) / parts
 // of a block's time - and joining costs a launch and 8 bytes per element and part; the cheapest of up to eight parts is taken.  (fp32, 2 x
-// 2049 tokens, 8 heads of 64, 272 blocks: 287, 244, 213, 221 us with 1, 2, 3, 4 parts; bf16, 4 x 600 tokens, 16 heads of 128, 320 blocks: 35,
-// 57, 60, 66 us; one head of 1024: 25, 19, 17, 15 us.)
+// 2049 tokens, 8 heads of 64, 272 blocks: 292, 247, 220, 226 us with 1, 2, 3, 4 parts; bf16, 4 x 600 tokens, 16 heads of 128, 320 blocks: 45,
+// 53, 59, 62 us; one head of 1024: 26, 20, 17, 15 us; 2 x 4097 tokens, 16 heads of 128: 599 and 606 us with 1 and 2 or 3 parts, for 134 MB or
+// more of partial sums.)
 int so_mha_parts(const void* desc) {
   const so_mha_desc* d = (const so_mha_desc*)desc;
   const int err = so_mha_check(d);
@@ -773,7 +777,7 @@ int so_mha_parts(const void* desc) {
   // 288 blocks, training: 116 us whole, 83 + 10 in two parts, 69 + 12 in seven (the join reads from caches)
   const double rate = (d->dtype == SO_BF16 ? 0.75 : 1.0) * (d->bias && !d->linear ? 0.6 : 1.0), rows = (double)d->B * d->Hq * d->Lq;
   return mha_split_parts((double)d->B * d->Hq * mha_tiles(d->Lq), mha_us(4.0 * 128 * d->D * d->Lk, d->dtype) / rate, 8.0,
-                         rows * d->D * 8 / 12e6, d->Lk / 128, 0.95);
+                         rows * d->D * 8, 12e6, d->Lk / 128, 0.95);
 }
 
 int so_mha_fwd(const void* desc, void* stream) {

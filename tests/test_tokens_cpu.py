@@ -270,3 +270,14 @@ def test_c_entry_points_refuse_null_pointers():
         assert L.so_qk_norm_rotary_bwd(ctypes.addressof(x), *a, 1 << 20, None) == shape, i
     for a in ((None, 256, 256), (256, None, 256), (256, 256, None)):
         assert L.so_dropout(0, a[0], 4, None, 0, a[1], 4, 1, 4, a[2], 0, 1.0, None) == shape
+
+
+def test_parts_of_the_keys_weigh_their_partial_sums():
+    """Cut where blocks do not fill the chip, whole where the partial sums outgrow the caches and joining them takes what cutting gains."""
+    def parts(dtype, b, n, hq, hk, d):
+        return _lib.lib().so_mha_parts(ctypes.addressof(_desc(dtype=dtype, B=b, Hq=hq, Hk=hk, Lq=n, Lk=n, D=d, nwords=(n + 63) // 64)))
+
+    assert parts(1, 2, 4097, 16, 4, 128) == 1                # 1032 blocks on 256 CUs, 67 MB a part
+    assert parts(1, 4, 600, 16, 16, 128) == 1                # 304 blocks of 45 us
+    assert parts(0, 2, 2049, 8, 8, 64) > 2                   # 260 blocks of 150 us: two rounds of them whole, 8 MB a part
+    assert parts(1, 1, 1024, 1, 1, 64) > 2                   # 8 blocks
