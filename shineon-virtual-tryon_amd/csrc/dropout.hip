@@ -45,9 +45,10 @@ struct DropP {
   float scale;
 };
 
-// Bound by HBM: the ten rounds take less than the loads.  8 x 4099 x 1024, bf16: 42 us with a residual (4.8 TB/s), 23 us without (5.7).
-// Eight elements (two generator blocks) per thread, so that a bf16 thread moves 16 bytes.  VEC: dense operands, 16-byte aligned; otherwise every element is addressed by
-// its row and column.
+// Bound by HBM: the ten rounds take less than the loads.  8 x 4099 x 1024, bf16: 39-42 us with a residual (4.8-5.1 TB/s), 23 us without (5.7).
+// Eight elements (two generator blocks) per thread, so that a bf16 thread moves 16 bytes.  VEC: dense operands, 16-byte aligned; otherwise every
+// element is addressed by its row and column, and a wave's accesses are 16 or 32 bytes apart: with rows 2048 apart or one element off alignment
+// 112-114 us with a residual (1.8 TB/s), fp32 427 us (0.94 TB/s).
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void dropout_k(const DropP p) {
   const long long e0 = ((long long)blockIdx.x * 256 + threadIdx.x) * 8;

@@ -144,9 +144,10 @@ __global__ __launch_bounds__(256) void mha_sum_k(const float* part, T* out, long
 
 // BIAS: 0 none, 1 tokens of a sequence (offset = key - query), 2 tokens of a map.  Everything a tile needs travels by LDS-DMA: K, V,
 // the piece of the expanded bias that its offsets lie in and (maps) the keys' codes; nothing in the loop waits for global memory
-// except the one drain per tile.  2 x 4097 tokens, 16 heads on 4 of 128 channels, bf16, with the bias gradient: 475 us, 870 TFLOP/s; fp32,
-// 4 x 2048, 8 heads of 64: 437 us, 118 TFLOP/s (matrix pipes 80 % busy); two 64 x 36 maps, 8 heads of 64, bf16: 154 us, 212 TFLOP/s, bound
-// by the vector instructions of the bias lookup and of map_diagonals.
+// except the one drain per tile.  2 x 4097 tokens, 16 heads on 4 of 128 channels, bf16, with the bias gradient: 557 us, 740 TFLOP/s, matrix and
+// vector instructions 41 % of the SIMD cycles each, hardly beside each other; fp32, 4 x 2048, 8 heads of 64: 435 us, 118 TFLOP/s (matrix
+// pipes 80 % busy); two 64 x 36 maps, 8 heads of 64, bf16: 154-160 us, 205-212 TFLOP/s, bound by the vector instructions of the bias lookup
+// and of map_diagonals (at least 44 % of the cycles; matrix 13 %).
 template <typename T, int DP, int BIAS>
 __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : DP <= 64 ? 2 : 1)) void mha_dq_k(const BwdP P) {
   typedef Tile<T, DP> TL;
@@ -409,8 +410,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : DP <= 6
 }
 
 // Owns 128 keys, 32 per wave, and walks the 64-row tiles of the query heads that share them.  Scores are computed with keys in the lanes, so
-// P and dS are already operands of dv = P^T do and dk = dS^T q.  Bound by the matrix pipes, with one wave per SIMD above 64 channels: 2 x
-// 4097 tokens, 16 heads on 4 of 128, bf16 695 us, 790 TFLOP/s; fp32, 4 x 2048, 8 heads of 64: 595 us, 115 TFLOP/s (78 % busy).
+// P and dS are already operands of dv = P^T do and dk = dS^T q.  fp32 is bound by the matrix pipes (4 x 2048, 8 heads of 64: 602 us, 114 TFLOP/s,
+// 78 % busy); bf16 above 64 channels by what one wave per SIMD leaves open (2 x 4097 tokens, 16 heads on 4 of 128: 933 us, 590 TFLOP/s, matrix
+// instructions 31 %, vector instructions 23 % of the SIMD cycles).
 template <typename T, int DP, int BIAS>
 __global__ __launch_bounds__(256, (sizeof(T) == 2 && DP <= 64 ? 2 : 1)) void mha_dkv_k(const BwdP P) {
   typedef Tile<T, DP> TL;

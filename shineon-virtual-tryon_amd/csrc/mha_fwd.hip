@@ -82,7 +82,8 @@ __device__ __forceinline__ void write_row(const FwdP& P, const f32x16 (&o)[NT], 
 
 // The running softmax of 32 keys per half: s -> probabilities against the reference m; o and l are rescaled when m moves.  m follows the
 // maximum only when that has grown by more than kSlack (log2 units): probabilities up to 2^kSlack lose nothing in a floating-point type,
-// and after a row's first tiles hardly any tile rescales (following every growth: 380 instead of 366 us at 8191 tokens, 16 heads of 64).
+// and after a row's first tiles hardly any tile rescales (following every growth: 380 instead of 366 us at 8191 tokens, 16 heads of 64,
+// with probabilities in one piece).
 constexpr float kSlack = 8.f;
 template <int N, int NT>
 __device__ __forceinline__ void softmax_step(f32x16 (&s)[N], f32x16 (&o)[NT], float& m, float& l, float c) {
@@ -114,8 +115,8 @@ __device__ __forceinline__ void softmax_step(f32x16 (&s)[N], f32x16 (&o)[NT], fl
 // Probabilities as operands of the product with v.  bf16: in three pieces, each the 8 bits of what the ones before leave, multiplied one after
 // the other, so that all 24 bits take part.  One piece adds as much error to o as o's own rounding (2.3e-3 instead of 1.7e-3 of its norm), two
 // show in delta = do . o against the probabilities that the backward pass rebuilds: the bias gradient's sums over rows cancel, and it is 2 to
-// 5 times further off.  Pieces by what wants a gradient would make o's bits depend on that.  (8191 tokens, 16 heads of 64: 360, 487, 616 us with
-// one, two, three.)
+// 5 times further off.  Pieces by what wants a gradient would make o's bits depend on that.  (8191 tokens, 16 heads of 64: 354-360, 487,
+// 596-616 us with one, two, three.)
 template <typename T> constexpr int kPieces = sizeof(T) == 2 ? 3 : 1;
 template <typename T, int NCS>
 __device__ __forceinline__ void prob_frags(const f32x16& s, typename Elem<T>::frag (&p)[kPieces<T>][NCS]) {
@@ -137,8 +138,9 @@ __device__ __forceinline__ void prob_frags(const f32x16& s, typename Elem<T>::fr
 // expanded bias that a tile's offsets lie in travels to LDS with the tile.  (Read from global memory by every lane it took 120 of 495 us
 // at 8191 tokens, 16 heads of 64.)
 //
-// Bound by the matrix pipes in fp32 (80 % busy: 118 TFLOP/s at 4 x 2048 tokens, 8 heads of 64) and, with four products for the formula's two,
-// in bf16 (2 x 4097 tokens, 16 heads of 128: 523 us, 1050 TFLOP/s; 8191 tokens, 16 heads of 64: 616 us, 890 TFLOP/s).
+// fp32 is bound by the matrix pipes (80 % busy: 287 us, 120 TFLOP/s at 4 x 2048 tokens, 8 heads of 64).  bf16, four products for the formula's
+// two, by matrix and vector instructions one after the other: at 128 channels 51 and at least 46 % of the SIMD cycles (2 x 4097 tokens, 16 heads:
+// 604 us, 910 TFLOP/s of executed products), at 64 channels 42 and 67 % (8191 tokens, 16 heads: 596-690 us, 800-920 TFLOP/s).
 // (Two waves per SIMD in fp32 end at 64 channels: at 96 their registers spill, 4 x 2048 tokens, 8 heads 490 against 455 us.)
 template <typename T, int DP, int BIAS>
 __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 64 ? 2 : 1))) void mha_fwd_k(const FwdP P) {
@@ -293,7 +295,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? (DP <= 64 ? 3 : 2) : (DP <= 
 // ring of `DEPTH` pieces of keys and of values in LDS: a piece is asked for again as soon as its fragments are in registers, no wave
 // waits for another, and 64 KB per block stay in flight or in use (two blocks a CU).  The four running softmaxes are merged through LDS
 // at the end.  8 rows of 32765 keys (a tenth hidden), 16 heads on 4, 128 channels, bf16, 483 MB: 97 us, 4.95 TB/s, the rate of a large
-// copy (118 us with block-wide tiles of 64 KB, two stages and barriers).
+// copy (118 us with block-wide tiles of 64 KB, two stages and barriers).  fp32, all keys visible, 1.07 GB: 246 us, 4.4 TB/s (132 KB of LDS at 128
+// channels, so one block a CU, and rings of one piece).
 //
 // BIAS: 0 none, 1 a sequence's, at most kFewBias rows: 32 floats per row come with the keys, 2 any other: read into registers, where
 // hipcc's wait for them covers the fills in flight too.

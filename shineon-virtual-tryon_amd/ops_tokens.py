@@ -512,7 +512,10 @@ def attention(q, k, v, scale=None, key_mask=None, relative=None, bias_table=None
     relative + bias_table: a RelativePositions plan and its learned table [plan.rows, Hq] (float32).  Key j against query i adds the
     entry of the bucket of token j against token q_start + i.  An entry may be -inf; finite ones beyond +-7.4e8 count as that.
 
-    Training with a table takes scratch for the bias gradient, about Lq Lk / 32 bytes per sample and head, while backward runs.
+    Training with a table takes scratch for the bias gradient while backward runs, per sample and head 4 bytes for every block of 128
+    queries, part of the keys (1 to 8, more the fewer blocks there are) and offset that the block can meet: Lk + 127 of them in a sequence -
+    Lq Lk / 32 bytes times the parts -, in a map 2 W - 1 for every map row of keys beside those of the queries, whose map rows are padded to
+    multiples of 16 (so_mha_strip_floats; so_mha_bwd_floats says what the parts' sums of dq, dk and dv take besides).
 
     One or a few queries over long keys (a new token against what came before) are split over the keys.  Returns [B, Lq, Hq, D];
     differentiable in q, k, v and bias_table.  The order of all sums is fixed: the same inputs give the same bits, whatever wants a
