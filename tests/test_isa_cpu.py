@@ -12,7 +12,7 @@ import subprocess
 
 import pytest
 
-import shineon_virtual_tryon_amd as pkg
+from shineon_virtual_tryon_amd import _lib
 
 OBJDUMP = shutil.which("llvm-objdump", path=os.pathsep.join(["/opt/rocm/llvm/bin", os.environ.get("PATH", "")]))
 PASSES = {"4x4": 2, "16x16": 8, "32x32": 16}
@@ -74,9 +74,8 @@ def test_the_rule_finds_an_early_overwrite():
 
 @pytest.mark.skipif(OBJDUMP is None, reason="no llvm-objdump")
 def test_no_kernel_overwrites_a_matrix_instructions_operand(tmp_path):
-    path = os.path.join(os.path.dirname(os.path.abspath(pkg.__file__)), "libshineon_hip.so")
     objects, matrix, found = 0, 0, []
-    for i, blob in enumerate(code_objects(path)):
+    for i, blob in enumerate(code_objects(_lib.LIB_PATH)):
         objects += 1
         if b"amdgcn" not in blob[:64] and not blob.startswith(b"\x7fELF"):
             continue
